@@ -332,6 +332,43 @@ typedef struct {
 int pr_adam_max_groups(void);
 int pr_adam_step(const pr_adam_group *groups, int n_groups, void *stream);
 
+/* ---- gradient norm and clipping --------------------------------------------------------------------------------
+ * Replaces torch.nn.utils.clip_grad_norm_ as nerfstudio's Optimizers.optimizer_scaler_step_some calls it for every group
+ * with a max_norm (nerfstudio/engine/optimizers.py:159-172).  Gradients are dense arrays of any of three types; `set`
+ * says which norm a tensor belongs to, and the tensors of a call are ordered by it.  The arrays of tensors, max_norms and
+ * clips are HOST arrays.
+ * pr_grad_norm: norms[s] = norm over all elements of the tensors of set s (0 for an empty set), in float64 until the
+ * last rounding; the same inputs give the same bits; scratch: pr_grad_norm_scratch_bytes (0 for a list it does not
+ * take).  kind: sum of magnitudes, root of the sum of squares, largest
+ * magnitude (a NaN anywhere in the set gives NaN).
+ * pr_grad_scale: g *= min(1, max_norms[s] / (norms[s] + 1e-6)), rounded once to the gradient's type; gradients of a set
+ * whose norm is within bounds are not touched.  Tensors that share memory are refused (PR_EUNSUPPORTED).
+ * pr_adam_step_clipped: pr_adam_step with each group's gradient taken times that factor of clips[i] (norm NULL: 1);
+ * the gradients themselves stay as they are. */
+#define PR_F32 0
+#define PR_F16 1
+#define PR_BF16 2
+#define PR_NORM_1 1
+#define PR_NORM_2 2
+#define PR_NORM_INF 3
+typedef struct {
+  void *grad;      /* device */
+  int64_t numel;
+  int32_t dtype;   /* PR_F32, PR_F16 or PR_BF16 */
+  int32_t set;
+} pr_grad_tensor;
+typedef struct {
+  const float *norm; /* device, may be NULL */
+  double max_norm;
+} pr_grad_clip;
+int pr_grad_norm_max_sets(void);
+size_t pr_grad_norm_scratch_bytes(const pr_grad_tensor *tensors, int n, int n_sets);
+int pr_grad_norm(const pr_grad_tensor *tensors, int n, int n_sets, int kind, void *scratch, size_t scratch_bytes,
+                 float *norms, void *stream);
+int pr_grad_scale(const pr_grad_tensor *tensors, int n, int n_sets, const float *norms, const double *max_norms,
+                  void *stream);
+int pr_adam_step_clipped(const pr_adam_group *groups, const pr_grad_clip *clips, int n_groups, void *stream);
+
 /* ---- fused channel MLP on the rendered feature image ------------------------------------------------------
  * Replaces pogs/pogs.py:516-522 with the module of pogs/pogs.py:153-161: for every pixel
  *   x = alpha > 0 ? feats / max(alpha, 1e-6) : 0            (skipped when alphas is NULL)

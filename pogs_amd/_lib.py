@@ -71,6 +71,11 @@ SIGNATURES = {
     "pr_densify_split_children": (c_int, [c_int64, _P, _P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "pr_adam_max_groups": (c_int, []),
     "pr_adam_step": (c_int, [_P, c_int, _P]),
+    "pr_grad_norm_max_sets": (c_int, []),
+    "pr_grad_norm_scratch_bytes": (c_size_t, [_P, c_int, c_int]),
+    "pr_grad_norm": (c_int, [_P, c_int, c_int, c_int, _P, c_size_t, _P, _P]),
+    "pr_grad_scale": (c_int, [_P, c_int, c_int, _P, _P, _P]),
+    "pr_adam_step_clipped": (c_int, [_P, _P, c_int, _P]),
     "pr_project_fwd_rigid": (c_int, [c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_float, c_float,
                                      c_float, c_float, _P, _P, _P, _P, _P, _P, _P]),
     "pr_project_bwd_rigid": (c_int, [c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_float, _P, _P,
@@ -98,6 +103,11 @@ class AdamGroup(ctypes.Structure):
     _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
                 ("exp_avg_sq", ctypes.c_void_p), ("numel", c_int64), ("step", c_int64), ("lr", ctypes.c_double),
                 ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double)]
+
+
+class GradClip(ctypes.Structure):
+    """pr_grad_clip."""
+    _fields_ = [("norm", ctypes.c_void_p), ("max_norm", ctypes.c_double)]
 
 
 class DensifyRule(ctypes.Structure):

@@ -36,6 +36,15 @@ struct AdamTable {
   unsigned first_block[MAX_GROUPS + 1];
   int n;
 };
+struct ClipTable {  // per group: where its gradient norm is (NULL: not clipped) and the norm it may have
+  const float *norm[MAX_GROUPS];
+  float max_norm[MAX_GROUPS];
+};
+struct NoClip {};
+__device__ __forceinline__ float gradient_factor(const NoClip &, int) { return 1.f; }
+__device__ __forceinline__ float gradient_factor(const ClipTable &c, int gi) {
+  return c.norm[gi] ? clip_coefficient(*c.norm[gi], c.max_norm[gi]) : 1.f;
+}
 
 __device__ __forceinline__ void adam_update(float &p, float g, float &m, float &v, float step_size, float omb1,
                                             float beta2, float omb2, float bias2_sqrt, float eps) {
@@ -45,7 +54,10 @@ __device__ __forceinline__ void adam_update(float &p, float g, float &m, float &
   p = p - step_size * (m / denom);
 }
 
-__global__ void __launch_bounds__(BLOCK) adam_kernel(const AdamTable t) {
+// CLIP = ClipTable: every gradient is taken times its group's factor, which is the same for all of a workgroup's
+// elements.  CLIP = NoClip: the factor is a constant 1 and drops out.
+template <typename CLIP>
+__global__ void __launch_bounds__(BLOCK) adam_kernel(const AdamTable t, const CLIP clip) {
   int gi = 0;
 #pragma unroll 1
   while (gi + 1 < t.n && blockIdx.x >= t.first_block[gi + 1]) ++gi;
@@ -57,13 +69,15 @@ __global__ void __launch_bounds__(BLOCK) adam_kernel(const AdamTable t) {
   const float ss = t.step_size[gi], omb1 = t.one_minus_beta1[gi], b2 = t.beta2[gi], omb2 = t.one_minus_beta2[gi],
               bc = t.bias2_sqrt[gi], eps = t.eps[gi];
   const int64_t base = (int64_t)(blockIdx.x - t.first_block[gi]) * PER_BLOCK;
+  const float factor = gradient_factor(clip, gi);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int64_t i = base + ((int64_t)r * BLOCK + threadIdx.x) * 4;
     if (i + 3 < n) {
       float4 pp = *reinterpret_cast<float4 *>(p + i), mm = *reinterpret_cast<float4 *>(m + i);
       float4 vv = *reinterpret_cast<float4 *>(v + i);
-      const float4 gg = *reinterpret_cast<const float4 *>(g + i);
+      float4 gg = *reinterpret_cast<const float4 *>(g + i);
+      gg.x *= factor, gg.y *= factor, gg.z *= factor, gg.w *= factor;
       adam_update(pp.x, gg.x, mm.x, vv.x, ss, omb1, b2, omb2, bc, eps);
       adam_update(pp.y, gg.y, mm.y, vv.y, ss, omb1, b2, omb2, bc, eps);
       adam_update(pp.z, gg.z, mm.z, vv.z, ss, omb1, b2, omb2, bc, eps);
@@ -74,7 +88,7 @@ __global__ void __launch_bounds__(BLOCK) adam_kernel(const AdamTable t) {
     } else {
       for (int64_t k = i; k < n; ++k) {
         float pk = p[k], mk = m[k], vk = v[k];
-        adam_update(pk, g[k], mk, vk, ss, omb1, b2, omb2, bc, eps);
+        adam_update(pk, g[k] * factor, mk, vk, ss, omb1, b2, omb2, bc, eps);
         p[k] = pk;
         m[k] = mk;
         v[k] = vk;
@@ -88,11 +102,14 @@ __global__ void __launch_bounds__(BLOCK) adam_kernel(const AdamTable t) {
 
 extern "C" int pr_adam_max_groups(void) { return pr::MAX_GROUPS; }
 
-extern "C" int pr_adam_step(const pr_adam_group *groups, int n_groups, void *stream) {
-  if (n_groups < 0 || n_groups > pr::MAX_GROUPS) return PR_EINVAL;
+namespace pr {
+namespace {
+int adam_step(const pr_adam_group *groups, const pr_grad_clip *clips, int n_groups, void *stream) {
+  if (n_groups < 0 || n_groups > MAX_GROUPS) return PR_EINVAL;
   if (n_groups == 0) return PR_OK;
   if (!groups) return PR_EINVAL;
-  pr::AdamTable t;
+  AdamTable t;
+  ClipTable c;
   t.n = 0;
   unsigned blocks = 0;
   for (int i = 0; i < n_groups; ++i) {
@@ -104,7 +121,10 @@ extern "C" int pr_adam_step(const pr_adam_group *groups, int n_groups, void *str
     // 16-byte accesses: torch allocations are; a sliced view might not be
     if ((((uintptr_t)g.param | (uintptr_t)g.grad | (uintptr_t)g.exp_avg | (uintptr_t)g.exp_avg_sq) & 15) != 0)
       return PR_EINVAL;
+    if (clips && clips[i].norm && !(clips[i].max_norm >= 0.0)) return PR_EINVAL;
     const int k = t.n++;
+    c.norm[k] = clips ? clips[i].norm : nullptr;
+    c.max_norm[k] = clips ? (float)clips[i].max_norm : 0.f;
     t.param[k] = g.param;
     t.grad[k] = g.grad;
     t.exp_avg[k] = g.exp_avg;
@@ -120,12 +140,26 @@ extern "C" int pr_adam_step(const pr_adam_group *groups, int n_groups, void *str
     t.bias2_sqrt[k] = (float)sqrt(bias2);
     t.eps[k] = (float)g.eps;
     t.first_block[k] = blocks;
-    const int64_t nb = (g.numel + pr::PER_BLOCK - 1) / pr::PER_BLOCK;
+    const int64_t nb = (g.numel + PER_BLOCK - 1) / PER_BLOCK;
     if (nb + blocks > 0x7fffffffll) return PR_EUNSUPPORTED;
     blocks += (unsigned)nb;
   }
   if (t.n == 0) return PR_OK;
   t.first_block[t.n] = blocks;
-  hipLaunchKernelGGL(pr::adam_kernel, dim3(blocks), dim3(pr::BLOCK), 0, (hipStream_t)stream, t);
-  return pr::check_launch("pr_adam_step");
+  if (clips)
+    hipLaunchKernelGGL(adam_kernel<ClipTable>, dim3(blocks), dim3(BLOCK), 0, (hipStream_t)stream, t, c);
+  else
+    hipLaunchKernelGGL(adam_kernel<NoClip>, dim3(blocks), dim3(BLOCK), 0, (hipStream_t)stream, t, NoClip{});
+  return check_launch("pr_adam_step");
+}
+}  // namespace
+}  // namespace pr
+
+extern "C" int pr_adam_step(const pr_adam_group *groups, int n_groups, void *stream) {
+  return pr::adam_step(groups, nullptr, n_groups, stream);
+}
+
+extern "C" int pr_adam_step_clipped(const pr_adam_group *groups, const pr_grad_clip *clips, int n_groups, void *stream) {
+  if (n_groups > 0 && !clips) return PR_EINVAL;
+  return pr::adam_step(groups, clips, n_groups, stream);
 }

@@ -1,0 +1,385 @@
+// Norm of the gradients of many tensors and their scaling to at most a given norm (pr_grad_norm / pr_grad_scale).
+//
+// Stands in for torch.nn.utils.clip_grad_norm_, which nerfstudio's Optimizers.optimizer_scaler_step_some calls for every
+// parameter group with a max_norm (nerfstudio/engine/optimizers.py:159-172).
+//   norm_s = sqrt(sum over the tensors of set s of g^2)        (or sum |g|, or max |g|)
+//   g     <- g * min(1, max_norm_s / (norm_s + 1e-6))
+//
+// HBM-bound: the norm reads every gradient once, the scaling reads and writes it once.  The tensors of a launch are laid
+// end to end in one index space, each rounded up to 64 elements, and every workgroup takes an equal range of it: the
+// number of workgroups follows the number of elements and not of tensors, and a range starts on a 64-element boundary of
+// its tensor, so that 16-byte accesses stay aligned wherever the tensor is.  A set of tensors (one norm) starts on a
+// workgroup boundary; all sets share the launch.  Sums are kept in float64 from the first
+// element on (float32 gradients of 1e30 square to a finite value, and the order of the sum does not show in float32);
+// partials go to memory, one per workgroup and set, and are added in one fixed order: the result does not depend on the
+// order in which workgroups run.
+#include <math.h>
+#include <stdlib.h>
+
+#include <algorithm>
+
+#include "common.h"
+
+namespace pr {
+namespace {
+
+constexpr int MAX_TENSORS = 128;  // per launch: the table travels in the kernel argument (at most 4 KB)
+constexpr int MAX_SETS = 32;
+constexpr int BLOCK = 256;
+constexpr int64_t UNIT = 64;        // elements a tensor is rounded up to in the launch's index space
+constexpr int64_t MIN_RANGE = 8192;  // elements per workgroup at least
+constexpr int MAX_BLOCKS = 2048;     // per launch: eight workgroups for each CU
+
+struct Table {
+  void *grad[MAX_TENSORS];
+  int64_t numel[MAX_TENSORS];
+  unsigned first_unit[MAX_TENSORS + 1];
+  unsigned char dtype[MAX_TENSORS], set[MAX_TENSORS];
+  unsigned units_per_block;
+  int n;
+};
+
+struct SetRanges {  // partials of set s: [first[s], first[s + 1])
+  unsigned first[MAX_SETS + 1];
+};
+
+struct MaxNorms {
+  float of[MAX_SETS];
+};
+
+__device__ __forceinline__ float from_bits16(unsigned short b, int dtype) {
+  if (dtype == PR_F16) return (float)__builtin_bit_cast(_Float16, b);
+  return __builtin_bit_cast(float, (unsigned)b << 16);
+}
+__device__ __forceinline__ unsigned short to_bits16(float v, int dtype) {
+  if (dtype == PR_F16) return __builtin_bit_cast(unsigned short, (_Float16)v);
+  return __builtin_bit_cast(unsigned short, (__bf16)v);
+}
+
+template <int KIND>
+__device__ __forceinline__ double combine(double a, double b) {
+  if (KIND != PR_NORM_INF) return a + b;
+  return (a > b || a != a) ? a : b;  // max that keeps NaN
+}
+template <int KIND>
+__device__ __forceinline__ void take(double &acc, float g) {
+  if (KIND == PR_NORM_2) acc = fma((double)g, (double)g, acc);
+  else acc = combine<KIND>(acc, (double)fabsf(g));
+}
+
+template <int KIND>
+__device__ __forceinline__ double block_combine(double v) {
+  __shared__ double part[BLOCK / 64];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v = combine<KIND>(v, __shfl_xor(v, d));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = part[0];
+#pragma unroll
+  for (int i = 1; i < BLOCK / 64; ++i) v = combine<KIND>(v, part[i]);
+  return v;
+}
+
+// The tensor whose units hold `unit`.
+__device__ __forceinline__ int find_tensor(const Table &t, unsigned unit) {
+  int lo = 0, hi = t.n - 1;
+#pragma unroll 1
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first_unit[mid] <= unit) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <int KIND>
+__device__ __forceinline__ double range_norm(const void *grad, int dtype, int64_t lo, int64_t hi) {
+  double acc[4] = {0., 0., 0., 0.};
+  if (dtype == PR_F32) {
+    const float *g = (const float *)grad;
+    const bool vec = ((uintptr_t)g & 15) == 0;
+    int64_t i = lo + 4 * threadIdx.x;
+    if (vec) {
+      for (; i + 3 * 4 * BLOCK + 3 < hi; i += 4 * 4 * BLOCK) {
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const float4 *>(g + i + u * 4 * BLOCK);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          take<KIND>(acc[0], v[u].x), take<KIND>(acc[1], v[u].y);
+          take<KIND>(acc[2], v[u].z), take<KIND>(acc[3], v[u].w);
+        }
+      }
+    }
+    for (; i < hi; i += 4 * BLOCK)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < hi) take<KIND>(acc[k], g[i + k]);
+  } else {
+    const unsigned short *g = (const unsigned short *)grad;
+    const bool vec = ((uintptr_t)g & 15) == 0;
+    int64_t i = lo + 8 * threadIdx.x;
+    if (vec) {
+      for (; i + 8 * BLOCK + 7 < hi; i += 2 * 8 * BLOCK) {
+        uint4 v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) v[u] = *reinterpret_cast<const uint4 *>(g + i + u * 8 * BLOCK);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            take<KIND>(acc[k], from_bits16((unsigned short)(w[k] & 0xffffu), dtype));
+            take<KIND>(acc[k], from_bits16((unsigned short)(w[k] >> 16), dtype));
+          }
+        }
+      }
+    }
+    for (; i < hi; i += 8 * BLOCK)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i + k < hi) take<KIND>(acc[k & 3], from_bits16(g[i + k], dtype));
+  }
+  return combine<KIND>(combine<KIND>(acc[0], acc[1]), combine<KIND>(acc[2], acc[3]));
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(BLOCK) grad_norm_kernel(const Table t, double *__restrict__ partials) {
+  unsigned unit = blockIdx.x * t.units_per_block;
+  const unsigned end = min(unit + t.units_per_block, t.first_unit[t.n]);
+  double acc = 0.;
+  int k = find_tensor(t, unit);
+#pragma unroll 1
+  while (unit < end) {
+    const unsigned stop = min(end, t.first_unit[k + 1]);
+    const int64_t lo = (int64_t)(unit - t.first_unit[k]) * UNIT;
+    const int64_t hi = min((int64_t)(stop - t.first_unit[k]) * UNIT, t.numel[k]);
+    acc = combine<KIND>(acc, range_norm<KIND>(t.grad[k], t.dtype[k], lo, hi));
+    unit = stop;
+    ++k;
+  }
+  acc = block_combine<KIND>(acc);
+  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(BLOCK) grad_norm_finish_kernel(const SetRanges sets, const double *__restrict__ partials,
+                                                                 float *__restrict__ norms) {
+  const int s = blockIdx.x;
+  double acc = 0.;
+  for (unsigned i = sets.first[s] + threadIdx.x; i < sets.first[s + 1]; i += BLOCK) acc = combine<KIND>(acc, partials[i]);
+  acc = block_combine<KIND>(acc);
+  if (threadIdx.x == 0) norms[s] = (float)(KIND == PR_NORM_2 ? sqrt(acc) : acc);
+}
+
+__device__ __forceinline__ void range_scale(void *grad, int dtype, int64_t lo, int64_t hi, float c) {
+  if (dtype == PR_F32) {
+    float *g = (float *)grad;
+    int64_t i = lo + 4 * threadIdx.x;
+    if (((uintptr_t)g & 15) == 0) {
+      for (; i + 4 * BLOCK + 3 < hi; i += 2 * 4 * BLOCK) {
+        float4 a = *reinterpret_cast<float4 *>(g + i), b = *reinterpret_cast<float4 *>(g + i + 4 * BLOCK);
+        a.x *= c, a.y *= c, a.z *= c, a.w *= c;
+        b.x *= c, b.y *= c, b.z *= c, b.w *= c;
+        *reinterpret_cast<float4 *>(g + i) = a;
+        *reinterpret_cast<float4 *>(g + i + 4 * BLOCK) = b;
+      }
+    }
+    for (; i < hi; i += 4 * BLOCK)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < hi) g[i + k] *= c;
+  } else {
+    unsigned short *g = (unsigned short *)grad;
+    int64_t i = lo + 8 * threadIdx.x;
+    if (((uintptr_t)g & 15) == 0) {
+      for (; i + 7 < hi; i += 8 * BLOCK) {
+        uint4 v = *reinterpret_cast<uint4 *>(g + i);
+        unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const unsigned a = to_bits16(from_bits16((unsigned short)(w[k] & 0xffffu), dtype) * c, dtype);
+          const unsigned b = to_bits16(from_bits16((unsigned short)(w[k] >> 16), dtype) * c, dtype);
+          w[k] = a | (b << 16);
+        }
+        *reinterpret_cast<uint4 *>(g + i) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    for (; i < hi; i += 8 * BLOCK)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i + k < hi) g[i + k] = to_bits16(from_bits16(g[i + k], dtype) * c, dtype);
+  }
+}
+
+__global__ void __launch_bounds__(BLOCK) grad_scale_kernel(const Table t, const float *__restrict__ norms,
+                                                           const MaxNorms max_norms) {
+  unsigned unit = blockIdx.x * t.units_per_block;
+  const unsigned end = min(unit + t.units_per_block, t.first_unit[t.n]);
+  int k = find_tensor(t, unit);
+  const float c = clip_coefficient(norms[t.set[k]], max_norms.of[t.set[k]]);
+  // a norm within bounds leaves every value as it is: nothing to read or write (NaN is no such norm)
+  if (c == 1.f) return;
+#pragma unroll 1
+  while (unit < end) {
+    const unsigned stop = min(end, t.first_unit[k + 1]);
+    const int64_t lo = (int64_t)(unit - t.first_unit[k]) * UNIT;
+    const int64_t hi = min((int64_t)(stop - t.first_unit[k]) * UNIT, t.numel[k]);
+    range_scale(t.grad[k], t.dtype[k], lo, hi, c);
+    unit = stop;
+    ++k;
+  }
+}
+
+// Cuts the host's list into launches of at most MAX_TENSORS tensors.  next() fills the table (n == 0 at the end).
+struct Launches {
+  const pr_grad_tensor *tensors;
+  int n, at = 0;
+  Table t;
+  unsigned blocks = 0;
+  unsigned set_blocks[MAX_SETS];  // workgroups of each set in this launch
+  Launches(const pr_grad_tensor *tensors_, int n_) : tensors(tensors_), n(n_) {}
+  int next() {
+    t.n = 0;
+    blocks = 0;
+    std::fill(set_blocks, set_blocks + MAX_SETS, 0u);
+    int64_t total = 0;
+    for (; at < n && t.n < MAX_TENSORS; ++at) {
+      const pr_grad_tensor &g = tensors[at];
+      if (g.numel == 0) continue;
+      const int64_t u = (g.numel + UNIT - 1) / UNIT;
+      if (total + u > 0x3fffffffll) {
+        if (t.n == 0) return PR_EUNSUPPORTED;
+        break;
+      }
+      t.grad[t.n] = g.grad;
+      t.numel[t.n] = g.numel;
+      t.dtype[t.n] = (unsigned char)g.dtype;
+      t.set[t.n] = (unsigned char)g.set;
+      total += u;
+      ++t.n;
+    }
+    const int64_t per = std::max<int64_t>((total + MAX_BLOCKS - 1) / MAX_BLOCKS, MIN_RANGE / UNIT);
+    t.units_per_block = (unsigned)per;
+    // total <= 2^30 and at most MAX_SETS roundings to per < 2^20: below 2^32
+    int64_t units = 0;
+    auto close = [&](int set) {  // the set's last workgroup keeps the rest of its range
+      const int64_t b = (units + per - 1) / per;
+      set_blocks[set] = (unsigned)(b - blocks);
+      blocks = (unsigned)b;
+      units = b * per;
+    };
+    for (int k = 0; k < t.n; ++k) {
+      if (k > 0 && t.set[k] != t.set[k - 1]) close(t.set[k - 1]);
+      t.first_unit[k] = (unsigned)units;
+      units += (t.numel[k] + UNIT - 1) / UNIT;
+    }
+    if (t.n > 0) close(t.set[t.n - 1]);
+    t.first_unit[t.n] = (unsigned)units;
+    return PR_OK;
+  }
+};
+
+int check_tensors(const pr_grad_tensor *tensors, int n, int n_sets) {
+  if (n < 0 || n_sets < 1 || n_sets > MAX_SETS || (n > 0 && !tensors)) return PR_EINVAL;
+  for (int i = 0; i < n; ++i) {
+    const pr_grad_tensor &g = tensors[i];
+    if (g.numel < 0 || (g.numel > 0 && !g.grad) || g.dtype < PR_F32 || g.dtype > PR_BF16) return PR_EINVAL;
+    if (((uintptr_t)g.grad & (g.dtype == PR_F32 ? 3 : 1)) != 0) return PR_EINVAL;
+    if (g.set < 0 || g.set >= n_sets || (i > 0 && g.set < tensors[i - 1].set)) return PR_EINVAL;
+  }
+  return PR_OK;
+}
+
+// Whether no two tensors share memory (scaling them in one launch would race).
+int check_apart(const pr_grad_tensor *tensors, int n) {
+  struct Span {
+    uintptr_t lo, hi;
+  };
+  Span *s = (Span *)malloc(sizeof(Span) * (size_t)std::max(n, 1));
+  if (!s) return PR_ESCRATCH;
+  int m = 0;
+  for (int i = 0; i < n; ++i) {
+    const uintptr_t lo = (uintptr_t)tensors[i].grad;
+    if (tensors[i].numel > 0) s[m++] = Span{lo, lo + (uintptr_t)tensors[i].numel * (tensors[i].dtype == PR_F32 ? 4 : 2)};
+  }
+  std::sort(s, s + m, [](const Span &a, const Span &b) { return a.lo < b.lo; });
+  bool apart = true;
+  for (int i = 1; i < m; ++i) apart &= s[i - 1].hi <= s[i].lo;
+  free(s);
+  if (apart) return PR_OK;
+  set_error_text("pr_grad_scale: two gradients share memory");
+  return PR_EUNSUPPORTED;
+}
+
+}  // namespace
+}  // namespace pr
+
+extern "C" int pr_grad_norm_max_sets(void) { return pr::MAX_SETS; }
+
+extern "C" size_t pr_grad_norm_scratch_bytes(const pr_grad_tensor *tensors, int n, int n_sets) {
+  if (pr::check_tensors(tensors, n, n_sets) != PR_OK) return 0;
+  pr::Launches l(tensors, n);
+  size_t blocks = 0;
+  do {
+    if (l.next() != PR_OK) return 0;
+    blocks += l.blocks;
+  } while (l.t.n > 0);
+  return std::max<size_t>(blocks, 1) * sizeof(double);
+}
+
+extern "C" int pr_grad_norm(const pr_grad_tensor *tensors, int n, int n_sets, int kind, void *scratch,
+                            size_t scratch_bytes, float *norms, void *stream) {
+  int rc = pr::check_tensors(tensors, n, n_sets);
+  if (rc != PR_OK) return rc;
+  if (kind < PR_NORM_1 || kind > PR_NORM_INF || !norms || !scratch || ((uintptr_t)scratch & 7)) return PR_EINVAL;
+  hipStream_t st = (hipStream_t)stream;
+  double *partials = (double *)scratch;
+  size_t used = 0;
+  pr::SetRanges sets;
+  unsigned set_partials[pr::MAX_SETS] = {};
+  for (pr::Launches l(tensors, n);;) {
+    rc = l.next();
+    if (rc != PR_OK) return rc;
+    if (l.t.n == 0) break;
+    if ((used + l.blocks) * sizeof(double) > scratch_bytes) return PR_ESCRATCH;
+    const dim3 grid(l.blocks), block(pr::BLOCK);
+    if (kind == PR_NORM_2) hipLaunchKernelGGL(pr::grad_norm_kernel<PR_NORM_2>, grid, block, 0, st, l.t, partials + used);
+    else if (kind == PR_NORM_1) hipLaunchKernelGGL(pr::grad_norm_kernel<PR_NORM_1>, grid, block, 0, st, l.t, partials + used);
+    else hipLaunchKernelGGL(pr::grad_norm_kernel<PR_NORM_INF>, grid, block, 0, st, l.t, partials + used);
+    rc = pr::check_launch("pr_grad_norm");
+    if (rc != PR_OK) return rc;
+    used += l.blocks;
+    for (int s = 0; s < n_sets; ++s) set_partials[s] += l.set_blocks[s];
+  }
+  // tensors are ordered by set: a set's partials are consecutive, over launches too
+  sets.first[0] = 0;
+  for (int s = 0; s < n_sets; ++s) sets.first[s + 1] = sets.first[s] + set_partials[s];
+  const dim3 grid(n_sets), block(pr::BLOCK);
+  if (kind == PR_NORM_2) hipLaunchKernelGGL(pr::grad_norm_finish_kernel<PR_NORM_2>, grid, block, 0, st, sets, partials, norms);
+  else if (kind == PR_NORM_1) hipLaunchKernelGGL(pr::grad_norm_finish_kernel<PR_NORM_1>, grid, block, 0, st, sets, partials, norms);
+  else hipLaunchKernelGGL(pr::grad_norm_finish_kernel<PR_NORM_INF>, grid, block, 0, st, sets, partials, norms);
+  return pr::check_launch("pr_grad_norm");
+}
+
+extern "C" int pr_grad_scale(const pr_grad_tensor *tensors, int n, int n_sets, const float *norms, const double *max_norms,
+                             void *stream) {
+  int rc = pr::check_tensors(tensors, n, n_sets);
+  if (rc != PR_OK) return rc;
+  if (!norms || !max_norms) return PR_EINVAL;
+  rc = pr::check_apart(tensors, n);
+  if (rc != PR_OK) return rc;
+  pr::MaxNorms m{};
+  for (int s = 0; s < n_sets; ++s) {
+    if (!(max_norms[s] >= 0.0)) return PR_EINVAL;
+    m.of[s] = (float)max_norms[s];
+  }
+  for (pr::Launches l(tensors, n);;) {
+    rc = l.next();
+    if (rc != PR_OK) return rc;
+    if (l.t.n == 0) return PR_OK;
+    hipLaunchKernelGGL(pr::grad_scale_kernel, dim3(l.blocks), dim3(pr::BLOCK), 0, (hipStream_t)stream, l.t, norms, m);
+    rc = pr::check_launch("pr_grad_scale");
+    if (rc != PR_OK) return rc;
+  }
+}

@@ -447,9 +447,14 @@ class ShardAdam:
     """``update`` callback of ``ShardedExchange``: Adam (``torch.optim.Adam`` arithmetic, no weight decay) on this
     rank's slices, all slices of a bucket in ONE ``pr_adam_step`` launch.  ``config``: {name: {"lr": float,
     "eps": 1e-15, "betas": (0.9, 0.999)}}, the per-group settings of ``pogs/pogs_config.py:38-85``; ``lr`` may be
-    changed between steps (schedulers).  Moments are kept per (parameter, slice) and created on first use."""
+    changed between steps (schedulers).  Moments are kept per (parameter, slice) and created on first use.
+    A group's ``max_norm`` is refused: a bucket's shard is stepped before the other gradients have arrived, so the norm
+    it would be clipped by is not known there (``FlatGrads`` with ``pogs_amd.optim.Optimizers`` clips)."""
 
     def __init__(self, config: Dict[str, dict]):
+        for name, cfg in config.items():
+            if cfg.get("max_norm") is not None:
+                raise ValueError(f"ShardAdam cannot clip group '{name}' to max_norm: shards are stepped bucket by bucket")
         self.config = config
         self.state: Dict[tuple, dict] = {}
 

@@ -7,19 +7,135 @@ optional exponential-decay schedule per group (``nerfstudio/engine/schedulers.py
 gradient-accumulation periods.  Same method names and meaning; the difference is that all groups due in an
 iteration are updated by ONE kernel launch (``pr_adam_step``).  No PyTorch fallback.
 
+Gradient clipping (``OptimizerConfig.max_norm``, applied in ``optimizers.py:159-172`` through
+``torch.nn.utils.clip_grad_norm_``): a group whose config has ``max_norm`` is clipped to that norm in its step, by a factor
+that the Adam kernel takes from device memory, so clipping costs one pass over the gradients and no host
+synchronisation.  ``grad_norm`` and ``clip_grad_norm_`` are the same kernels for callers with an optimiser of their own.
+
 State is kept in torch's own layout, so ``state_dict()[name]`` loads into ``torch.optim.Adam`` and back.
 """
 from __future__ import annotations
 
 import ctypes
 import math
-from typing import Dict, List, Optional
+from array import array
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
 
 from . import _lib
 from .rendering import _call, _stream
+
+
+_GRAD_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}        # PR_F32, PR_F16, PR_BF16
+_NORM_KINDS = {1.0: 1, 2.0: 2, math.inf: 3}                                   # PR_NORM_1, PR_NORM_2, PR_NORM_INF
+
+
+def _one_block(t: Tensor) -> bool:
+    """Whether the elements of ``t`` fill one block of memory, in any order of dimensions."""
+    want = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _grad_table(grads: Sequence[Tensor], sets: Sequence[int]) -> array:
+    """The grads as an array of ``pr_grad_tensor``: pointer, elements, type and set (the upper half word)."""
+    words = array("q")
+    for g, s in zip(grads, sets):
+        words.extend((g.data_ptr(), g.numel(), _GRAD_TYPES[g.dtype] | s << 32))
+    return words
+
+
+def _address(a: array) -> ctypes.c_void_p:
+    return ctypes.c_void_p(a.buffer_info()[0])
+
+
+def _set_norms(grads: Sequence[Tensor], sets: Sequence[int], n_sets: int, kind: int) -> Tuple[array, Tensor]:
+    """``norms [n_sets]`` (float32, on the device) of gradients ordered by set, and their table.  Runs on the current
+    stream of the current device."""
+    lib = _lib.load()
+    table = _grad_table(grads, sets)
+    at, n = _address(table), len(grads)
+    nbytes = lib.pr_grad_norm_scratch_bytes(at, n, n_sets)
+    scratch = torch.empty(max(nbytes // 8, 1), dtype=torch.float64, device=grads[0].device)
+    norms = torch.empty(n_sets, dtype=torch.float32, device=grads[0].device)
+    _call("pr_grad_norm", at, n, n_sets, kind, scratch.data_ptr(), nbytes, norms.data_ptr(), _stream())
+    return table, norms
+
+
+def _check_grads(grads: Sequence[Tensor]) -> None:
+    dev = grads[0].device
+    for g in grads:
+        if g.is_sparse or not g.is_cuda:
+            raise RuntimeError("pogs_amd.optim needs dense gradients on a HIP device (no CPU fallback)")
+        if g.dtype not in _GRAD_TYPES:
+            raise TypeError(f"gradients must be float32, float16 or bfloat16, got {g.dtype}")
+        if g.device != dev:
+            raise RuntimeError(f"gradients are on different devices: {dev} and {g.device}")
+
+
+def _norm_kind(norm_type: float) -> int:
+    kind = _NORM_KINDS.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type}")
+    return kind
+
+
+def _max_norm(value) -> float:
+    value = float(value)
+    if not value >= 0.0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {value}")
+    return value
+
+
+def grad_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
+    """Norm over all elements of all ``tensors`` (gradients; float32, float16 or bfloat16 in any mix and layout) as a
+    0-d float32 tensor on their device.  Counterpart of ``torch.nn.utils.get_total_norm`` for ``norm_type`` 1, 2 and inf.
+    Sums are kept in float64, in an order that depends on the sizes alone: equal inputs give equal bits.  No host
+    synchronisation; safe in a captured graph.  An empty list has norm 0 (on the CPU, as in torch)."""
+    kind = _norm_kind(norm_type)
+    grads = [tensors] if isinstance(tensors, Tensor) else list(tensors)
+    if not grads:
+        return torch.tensor(0.0)
+    _check_grads(grads)
+    with torch.no_grad(), torch.cuda.device(grads[0].device):
+        flat = [g if g.is_contiguous() or _one_block(g) else g.contiguous() for g in grads]
+        return _set_norms(flat, [0] * len(flat), 1, kind)[1][0]
+
+
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> Tensor:
+    """``torch.nn.utils.clip_grad_norm_``: multiplies the ``.grad`` of every parameter that has one by
+    ``min(1, max_norm / (norm + 1e-6))``, in place, and returns the norm over all of them before that (0-d float32).
+
+    Gradients may be float32, float16 or bfloat16, of any layout, all on one device and in memory of their own: two
+    gradients that share memory (a parameter listed twice) are refused, as scaling them at once is a race.  Each value is
+    rounded once, to its own type.  Where the norm is within bounds no gradient is written.  A norm that is not finite
+    gives what torch gives: factor 0 for an infinite norm, NaN for a NaN one; ``error_if_nonfinite`` raises instead, and
+    only then does the host wait for the device."""
+    kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
+    params = [parameters] if isinstance(parameters, Tensor) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    _check_grads(grads)
+    with torch.no_grad(), torch.cuda.device(grads[0].device):
+        flat = [g if g.is_contiguous() or _one_block(g) else g.contiguous() for g in grads]
+        table, norms = _set_norms(flat, [0] * len(flat), 1, kind)
+        if error_if_nonfinite and not math.isfinite(norms.item()):
+            raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is "
+                               "non-finite, so it cannot be clipped. To disable this error and scale the gradients by "
+                               "the non-finite norm anyway, set `error_if_nonfinite=False`")
+        limit = ctypes.c_double(max_norm)
+        _call("pr_grad_scale", _address(table), len(flat), 1, norms.data_ptr(), ctypes.addressof(limit), _stream())
+        for g, f in zip(grads, flat):
+            if f is not g:
+                g.copy_(f)
+        return norms[0]
 
 
 class ExponentialDecay:
@@ -44,13 +160,18 @@ class ExponentialDecay:
 
 class Optimizers:
     """config: ``{group: {"lr": float, "eps": float = 1e-15, "betas": (0.9, 0.999), "scheduler": ExponentialDecay
-    or None}}``; param_groups: ``{group: [parameters]}`` (float32 HIP tensors)."""
+    or None, "max_norm": float or None}}``; param_groups: ``{group: [parameters]}`` (float32 HIP tensors).
+
+    ``max_norm``: the group's gradient, over all its parameters, is clipped to that 2-norm in every step, as by
+    ``clip_grad_norm_``; the parameters' ``.grad`` keep their values.  ``grad_norms`` holds the norms that the last step
+    clipped by, one 0-d device tensor a group."""
 
     def __init__(self, config: Dict[str, dict], param_groups: Dict[str, List[Tensor]]):
         _lib.load()
         self.config, self.parameters = config, {}
         self._state: Dict[str, List[dict]] = {}
         self._sched_steps: Dict[str, int] = {}
+        self.grad_norms: Dict[str, Tensor] = {}
         for name, params in param_groups.items():
             if name not in config:
                 raise RuntimeError(f"Optimizer config for '{name}' not found in config file. Provided configs "
@@ -59,6 +180,8 @@ class Optimizers:
                 if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
                     raise RuntimeError("pogs_amd.optim needs contiguous float32 parameters on a HIP device "
                                        "(no CPU fallback)")
+            if config[name].get("max_norm") is not None:
+                _max_norm(config[name]["max_norm"])
             self.parameters[name] = list(params)
             self._state[name] = [{} for _ in params]
             self._sched_steps[name] = 0
@@ -90,14 +213,21 @@ class Optimizers:
     def optimizer_step(self, param_group_name: str) -> None:
         self.optimizer_step_some([param_group_name])
 
-    def optimizer_step_all(self) -> None:
-        self.optimizer_step_some(list(self.parameters))
+    def optimizer_step_all(self, max_norm: Optional[float] = None) -> None:
+        self.optimizer_step_some(list(self.parameters), max_norm)
 
-    def optimizer_step_some(self, param_groups: List[str]) -> None:
+    def optimizer_step_some(self, param_groups: List[str], max_norm: Optional[float] = None) -> None:
         """One Adam update of every parameter (that has a gradient) of the named groups, in one launch per
-        ``pr_adam_max_groups()`` tensors."""
-        entries, keep = [], []
-        for name in param_groups:
+        ``pr_adam_max_groups()`` tensors.  Groups with a ``max_norm`` of their own are clipped one by one; ``max_norm``
+        given here clips the gradient of all the named groups together to one norm instead, and then none of them may
+        have its own."""
+        limits = [self.config[name].get("max_norm") for name in param_groups]
+        if max_norm is not None:
+            max_norm = _max_norm(max_norm)
+            if any(m is not None for m in limits):
+                raise ValueError("a max_norm over all groups and a max_norm of a group's own exclude each other")
+        entries, keep, clipped = [], [], []      # clipped: (group or None for all, limit, entry's index)
+        for name, limit in zip(param_groups, limits):
             cfg = self.config[name]
             b1, b2 = cfg.get("betas", (0.9, 0.999))
             lr, eps = self.lr(name), cfg.get("eps", 1e-15)
@@ -112,20 +242,53 @@ class Optimizers:
                     st["exp_avg"] = torch.zeros_like(p)
                     st["exp_avg_sq"] = torch.zeros_like(p)
                 st["step"] += 1
+                if max_norm is not None:
+                    clipped.append((None, max_norm, len(entries)))
+                elif limit is not None:
+                    clipped.append((name, _max_norm(limit), len(entries)))
                 keep.append(g)
                 entries.append(_lib.AdamGroup(p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(),
                                               st["exp_avg_sq"].data_ptr(), p.numel(), st["step"], lr, b1, b2, eps))
+        self.grad_norms = {}
         if not entries:
             return
         lib = _lib.load()
         chunk = lib.pr_adam_max_groups()
         dev = keep[0].device
         with torch.cuda.device(dev), torch.no_grad():
+            clips = self._clips(clipped, keep, param_groups, len(entries)) if clipped else None
             for i in range(0, len(entries), chunk):
                 part = entries[i:i + chunk]
                 arr = (_lib.AdamGroup * len(part))(*part)
-                _call("pr_adam_step", ctypes.cast(arr, ctypes.c_void_p), len(part), _stream())
+                if clips is None:
+                    _call("pr_adam_step", ctypes.cast(arr, ctypes.c_void_p), len(part), _stream())
+                else:
+                    by = (_lib.GradClip * len(part))(*clips[i:i + chunk])
+                    _call("pr_adam_step_clipped", ctypes.cast(arr, ctypes.c_void_p), ctypes.cast(by, ctypes.c_void_p),
+                          len(part), _stream())
         del keep
+
+    def _clips(self, clipped, grads: List[Tensor], param_groups: List[str], n: int) -> List[_lib.GradClip]:
+        """``pr_grad_clip`` of every entry of a step, the norms on their way on the current stream."""
+        clips = [_lib.GradClip(None, 0.0)] * n
+        names = list(dict.fromkeys(name for name, _, _ in clipped))
+        most = _lib.load().pr_grad_norm_max_sets()
+        for lo in range(0, len(names), most):
+            of = {name: i for i, name in enumerate(names[lo:lo + most])}
+            mine = [c for c in clipped if c[0] in of]
+            _, norms = _set_norms([grads[k] for _, _, k in mine], [of[name] for name, _, _ in mine], len(of), 2)
+            each = norms.unbind()
+            for name, limit, k in mine:
+                clips[k] = _lib.GradClip(each[of[name]].data_ptr(), limit)
+            for name, i in of.items():      # these hold the storage that the step's kernel reads
+                for group in (param_groups if name is None else [name]):
+                    self.grad_norms[group] = each[i]
+        return clips
+
+    def state(self, name: str, index: int = 0) -> dict:
+        """The Adam state of one parameter of a group (``step``, ``exp_avg``, ``exp_avg_sq``; empty before its first
+        step).  The tensors are the live ones."""
+        return self._state[name][index]
 
     # the trainer's per-iteration bookkeeping (trainer.py:494-510)
     @staticmethod
