@@ -34,6 +34,11 @@ extern "C" {
 #define PR_ESCRATCH (-3)    /* scratch buffer too small */
 #define PR_EHIP (-4)        /* a HIP runtime call or launch failed; hipGetLastError text via pr_last_hip_error */
 
+/* Element types, where an entry point takes more than float32. */
+#define PR_F32 0
+#define PR_F16 1
+#define PR_BF16 2
+
 /* Library/ABI version, (major<<16)|minor. */
 int pr_version(void);
 const char *pr_error_string(int code);
@@ -345,9 +350,6 @@ int pr_adam_step(const pr_adam_group *groups, int n_groups, void *stream);
  * whose norm is within bounds are not touched.  Tensors that share memory are refused (PR_EUNSUPPORTED).
  * pr_adam_step_clipped: pr_adam_step with each group's gradient taken times that factor of clips[i] (norm NULL: 1);
  * the gradients themselves stay as they are. */
-#define PR_F32 0
-#define PR_F16 1
-#define PR_BF16 2
 #define PR_NORM_1 1
 #define PR_NORM_2 2
 #define PR_NORM_INF 3
@@ -471,6 +473,31 @@ int pr_densify_split_children(int64_t n_out, const int32_t *map_src, const int32
                               const float *means, const float *scales, const float *quats, const float *opacities,
                               const float *noise, float *means_out, float *scales_out, float *opacities_out,
                               void *stream);
+
+/* ---- softmax cross entropy over a large vocabulary of embeddings ------------------------------------------------
+ * For feature rows x[P,D] (the clip head's outputs, pogs/fields/gaussian_field.py:194-204) and embeddings w[V,D] of the
+ * same type (PR_F32, PR_F16, PR_BF16; any strides, in elements): z = scale <x_p, w_v>, lse_p = log sum_v exp z_pv,
+ * row_loss_p = lse_p - z_p,label; logits and gradients of logits are never held for more than a piece of the vocabulary.
+ * The reference has no such loss; this is torch.nn.functional.cross_entropy(scale * x @ w.T, labels) and its gradients.
+ * A row whose label is ignore_index has row_loss 0, lse 0 and no gradient, whatever its features hold; any other label
+ * outside 0..V-1 makes the row's loss NaN and, through it, its gradients.
+ * pr_vocab_ce_fwd: P >= 1.  row_loss[P]; lse[P] and loss[1] may be NULL; loss = sum of row_loss, or (mean != 0) their mean
+ * over the rows not ignored (NaN if there are none).  kept: what pr_vocab_ce_bwd reads (packed operands, row statistics).
+ * pr_vocab_ce_bwd: dx[P,D] and dw[V,D] (contiguous, 16-byte aligned, the inputs' type, either may be NULL) from the
+ * gradient g_loss of row_loss (per_row != 0: [P]) or of loss (one value) and g_lse[P] of lse; a NULL one is 0.  kept is
+ * read only: several calls may share it.  Products take float16 operands (float32 input: two planes, 2^-22) and add in
+ * float32; sums run in a fixed order, so equal inputs give equal bits. */
+size_t pr_vocab_ce_kept_bytes(int dtype, int64_t P, int64_t V, int64_t D);
+size_t pr_vocab_ce_fwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D);
+size_t pr_vocab_ce_bwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D, int want_dx, int want_dw);
+int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const void *x, int64_t ldx_row, int64_t ldx_col,
+                    const void *w, int64_t ldw_row, int64_t ldw_col, const int64_t *labels, int64_t ignore_index,
+                    float scale, int mean, void *kept, size_t kept_bytes, void *scratch, size_t scratch_bytes,
+                    float *row_loss, float *lse, float *loss, void *stream);
+int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const void *x, int64_t ldx_row, int64_t ldx_col,
+                    const void *w, int64_t ldw_row, int64_t ldw_col, const int64_t *labels, int64_t ignore_index,
+                    float scale, int mean, int per_row, const void *kept, size_t kept_bytes, const float *g_loss,
+                    const float *g_lse, void *scratch, size_t scratch_bytes, void *dx, void *dw, void *stream);
 
 #ifdef __cplusplus
 }

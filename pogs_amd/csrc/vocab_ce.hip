@@ -1,0 +1,865 @@
+// Softmax cross entropy of feature rows over a large vocabulary of embeddings, without keeping the logits
+// (pr_vocab_ce_fwd / pr_vocab_ce_bwd).
+//
+//   z_pv  = scale <x_p, w_v>          p < P rows, v < V words, contraction over D features
+//   lse_p = log sum_v exp z_pv        loss_p = lse_p - z_p,label(p)
+//   with upstream gradients u_p of loss_p and l_p of lse_p, a_p = u_p + l_p, b_p = u_p:
+//   G_pv  = a_p exp(z_pv - lse_p) - b_p [v = label(p)],   dX = scale G W,   dW = scale G^T X
+//
+// All products run on the matrix cores as v_mfma_f32_32x32x16_f16 with float32 accumulators.  Operands are packed once
+// per call into fragment order, 1 KB blocks [32 rows][16 of the contraction] with lane l's eight values consecutive, so
+// that a block moves memory -> LDS by one direct 16-byte-a-lane load and LDS -> registers by one conflict-free
+// ds_read_b128.  Packing scales each tensor by one power of two that brings its largest magnitude to 2^13..2^14: a
+// bfloat16 value keeps all its bits down to 2^-31 of the largest, and a float32 value becomes two float16 planes (head
+// and residual, 22 bits down to 2^-17 of the largest) whose products head*head + head*residual + residual*head lose 2^-22.
+// float16 input is packed as it is.  Values that are not finite stay so; rows with the ignored label are packed as zeros,
+// whatever they hold.
+//
+// One product kernel with four epilogues:
+//   STATS  256 words x 128 rows: the row of X is on the lane, so the running maximum and sum over the words are taken in
+//          registers; one (max, sum) pair per row and 128 words leaves, in the log2 domain
+//   GRAD   the same product again for a piece of the vocabulary, turned into G in float16 (scaled by a power of two).  A
+//          lane's eight accumulators are eight consecutive slots of the contraction of dX = G W as they stand, if W's
+//          packed copy uses the same slot order; for dW = G^T X the tile is transposed by two products with the
+//          identity, which are exact
+//   DX     dX partials in float32, one plane per split of the contraction over words, added to over the pieces
+//   DW     dW rows of the piece, contraction over all rows, written in the output type
+// G of one piece is all that is ever held of the P x V logits.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.h"
+
+namespace pr {
+namespace {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef unsigned u4v __attribute__((ext_vector_type(4)));
+
+constexpr int TILE_V = 256;  // words per workgroup of STATS and GRAD; words of the packed copies are padded to it
+constexpr int TILE_P = 128;  // rows per workgroup
+constexpr int TOP_EXP = 13;  // packed magnitudes are below 2^(TOP_EXP + 1)
+constexpr float MAX_FLOOR = -3.0e38f;  // a maximum over nothing: exp2 of anything minus it is 0, not NaN
+constexpr float LN2F = 0.69314718055994531f;
+constexpr int AMAX_BLOCKS = 512;  // partial maxima per tensor
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  return (float)v;
+}
+
+struct Matrix {  // rows x cols with any strides (elements)
+  const void *data;
+  int64_t rows, cols, ld_row, ld_col;
+};
+
+struct Scalars {  // per call, on the device
+  int exp_x, exp_w;  // packed = value * 2^exp
+  float n_valid;     // rows whose label is not the ignored one
+};
+
+__device__ __forceinline__ bool row_in(const int64_t *labels, int64_t ignore, int64_t p) {
+  return !labels || labels[p] != ignore;
+}
+
+// ---- packing --------------------------------------------------------------------------------------------------------
+// Largest finite magnitude of W (workgroups 0..nb-1) and of X's rows that count (nb..2nb-1), one partial each.
+template <typename T>
+__global__ void __launch_bounds__(256) vce_amax_kernel(Matrix w, Matrix x, const int64_t *labels, int64_t ignore,
+                                                       float *__restrict__ partial) {
+  const int nb = gridDim.x / 2;
+  const bool is_x = (int)blockIdx.x >= nb;
+  const Matrix m = is_x ? x : w;
+  const T *src = (const T *)m.data;
+  const int lane = threadIdx.x & 63;
+  float top = 0.f;
+  for (int64_t r = ((int64_t)(blockIdx.x % nb) * 4 + (threadIdx.x >> 6)); r < m.rows; r += (int64_t)nb * 4) {
+    if (is_x && !row_in(labels, ignore, r)) continue;
+    for (int64_t c = lane; c < m.cols; c += 64) {
+      const float v = fabsf(to_f32(src[r * m.ld_row + c * m.ld_col]));
+      if (v < INFINITY) top = fmaxf(top, v);
+    }
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  __shared__ float part[4];
+  if (lane == 0) part[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+
+__device__ __forceinline__ int top_exponent(float amax) { return amax > 0.f ? TOP_EXP - ilogbf(amax) : 0; }
+
+// Exponents from the partial maxima (float16 input: none are taken, exponent 0).
+__global__ void __launch_bounds__(256) vce_exponents_kernel(const float *__restrict__ partial, int nb, Scalars *s) {
+  __shared__ float part[2][4];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    float top = 0.f;
+    for (int i = threadIdx.x; i < nb; i += 256) top = fmaxf(top, partial[t * nb + i]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if ((threadIdx.x & 63) == 0) part[t][threadIdx.x >> 6] = top;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    const float *q = part[threadIdx.x];
+    const int e = nb ? top_exponent(fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]))) : 0;
+    (threadIdx.x == 0 ? s->exp_w : s->exp_x) = e;
+  }
+}
+
+template <int NP>
+__device__ __forceinline__ void put_block(const float (&v)[8], u4v *dst, int64_t plane) {
+  h8v hi, lo;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    hi[i] = (_Float16)v[i];
+    if (NP == 2) lo[i] = (_Float16)(v[i] - (float)hi[i]);
+  }
+  dst[0] = __builtin_bit_cast(u4v, hi);
+  if (NP == 2) dst[plane] = __builtin_bit_cast(u4v, lo);
+}
+
+struct PackJob {
+  Matrix m;
+  const int64_t *labels;  // rows with the ignored label are zeros (NULL: all count)
+  int64_t ignore;
+  u4v *dst;
+  int64_t plane;    // 16-byte units between the head and the residual plane
+  int64_t blocks;   // 1 KB blocks of one plane
+  int kblocks;      // 16-wide blocks of the contraction per 32-row tile
+  float sign;
+  int is_x;
+};
+
+// Contraction over the columns: block (tile t, k step s), lane (m, h): row 32 t + m, columns 16 s + 8 h + 0..7.
+template <typename T, int NP>
+__global__ void __launch_bounds__(256) vce_pack_kernel(PackJob a, PackJob b, int64_t groups_a, const Scalars *s) {
+  const bool first = blockIdx.x < groups_a;
+  const PackJob &j = first ? a : b;
+  const int lane = threadIdx.x & 63;
+  const int64_t blk = ((int64_t)blockIdx.x - (first ? 0 : groups_a)) * 4 + (threadIdx.x >> 6);
+  if (blk >= j.blocks) return;
+  const int64_t row = blk / j.kblocks * 32 + (lane & 31);
+  const int64_t k0 = blk % j.kblocks * 16 + 8 * (lane >> 5);
+  const int e = j.is_x ? s->exp_x : s->exp_w;
+  float v[8];
+  const bool live = row < j.m.rows && row_in(j.labels, j.ignore, row);
+  const T *src = (const T *)j.m.data + (live ? row * j.m.ld_row : 0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = live && k0 + i < j.m.cols ? ldexpf(to_f32(src[(k0 + i) * j.m.ld_col]), e) * j.sign : 0.f;
+  put_block<NP>(v, j.dst + blk * 64 + lane, j.plane);
+}
+
+// Place of slot i of lane half h in k step s of a 32-wide piece of the contraction, for operands that meet a transposed
+// or accumulator-order factor: the order in which a 32x32 accumulator tile holds its rows.
+__device__ __forceinline__ constexpr int slot_place(int s, int h, int i) { return 16 * s + 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// Contraction over the rows: block (column tile t, k step s), lane (m, h): column 32 t + m, rows in slot order.
+template <typename T, int NP>
+__global__ void __launch_bounds__(256) vce_pack_t_kernel(PackJob a, PackJob b, int64_t groups_a, const Scalars *s) {
+  const bool first = blockIdx.x < groups_a;
+  const PackJob &j = first ? a : b;
+  const int lane = threadIdx.x & 63;
+  const int64_t blk = ((int64_t)blockIdx.x - (first ? 0 : groups_a)) * 4 + (threadIdx.x >> 6);
+  if (blk >= j.blocks) return;
+  const int64_t col = blk / j.kblocks * 32 + (lane & 31);
+  const int64_t kb = blk % j.kblocks;
+  const int e = j.is_x ? s->exp_x : s->exp_w;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = kb / 2 * 32 + slot_place((int)(kb & 1), lane >> 5, i);
+    const bool live = col < j.m.cols && row < j.m.rows && row_in(j.labels, j.ignore, row);
+    v[i] = live ? ldexpf(to_f32(((const T *)j.m.data)[row * j.m.ld_row + col * j.m.ld_col]), e) : 0.f;
+  }
+  put_block<NP>(v, j.dst + blk * 64 + lane, j.plane);
+}
+
+// ---- products -------------------------------------------------------------------------------------------------------
+enum { STATS, GRAD, DX, DW };
+
+struct GemmArgs {
+  const u4v *A, *B;            // operand blocks, already at the first block of the contraction
+  int64_t plane_a, plane_b;    // 16-byte units between planes
+  int64_t ld_a, ld_b;          // blocks per 32-row tile
+  int a_tiles;                 // 32-row tiles A has (tiles past them repeat the last one; their results are not used)
+  int kblocks, k_split;        // blocks of the contraction, and of each split of it (the last one may have fewer)
+  int m_tiles, n_tiles, splits;
+  const Scalars *scal;
+  const int *exp_g;            // DW: packed gradient = G * 2^exp_g
+  float scale;
+  // STATS, GRAD
+  int64_t P, V, v0;            // v0: first word of the piece
+  const int64_t *labels;
+  float2 *partial;             // STATS: [pair][Pp]
+  float *target;               // STATS: [Pp], the label's logit in the log2 domain
+  int64_t Pp;
+  const float *lse2;           // GRAD
+  const float *coef_a, *coef_b;
+  u4v *gx, *gw;                // GRAD: G as the operand of DX and of DW (either may be NULL)
+  int64_t plane_gx, plane_gw, ld_gx, ld_gw;
+  // DX
+  float *acc;                  // [split][Pp][ld_acc]
+  int64_t ld_acc;
+  int add;
+  // DW
+  void *out;                   // [V][D], contiguous
+  int64_t D;
+};
+
+typedef __attribute__((address_space(1))) const void *global_ptr;
+typedef __attribute__((address_space(3))) void *lds_ptr;
+
+template <typename T>
+__device__ __forceinline__ void store4(T *dst, float a, float b, float c, float d) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<t4 *>(dst) = t4{(T)a, (T)b, (T)c, (T)d};
+}
+
+// Workgroup of four wavefronts, 64 MT x 128 of the product: wavefront (wm, wn) holds MT x 2 accumulator tiles.  Three
+// LDS stages of 16 (two planes) or 32 (one plane) of the contraction, filled by direct loads two stages ahead; one
+// barrier a stage.
+template <int NP, int MT, int MODE, typename T>
+__global__ void __launch_bounds__(256, 2) vce_gemm_kernel(const GemmArgs g) {
+  extern __shared__ u4v lds[];
+  constexpr int KB = NP == 1 ? 2 : 1;
+  constexpr int A_BLOCKS = 2 * MT * KB * NP, B_BLOCKS = 4 * KB * NP, STAGE = A_BLOCKS + B_BLOCKS, LOADS = STAGE / 4;
+  static_assert(STAGE % 4 == 0, "every wavefront fills the same share of a stage");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+
+  // Workgroups go to the eight XCDs in turn: each XCD takes a run of consecutive tiles, ordered as bands of eight
+  // M tiles walked along N, so that its L2 holds the operands of the tiles it works on together.
+  const unsigned tiles = (unsigned)g.m_tiles * g.n_tiles * g.splits;
+  const unsigned per_xcd = (tiles + 7) / 8;
+  unsigned t = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per_xcd || t >= tiles) return;
+  const unsigned split = t / ((unsigned)g.m_tiles * g.n_tiles);
+  t -= split * (unsigned)g.m_tiles * g.n_tiles;
+  const unsigned band = t / (8u * g.n_tiles), in_band = t - band * 8u * g.n_tiles;
+  const unsigned band_m = min(8u, (unsigned)g.m_tiles - band * 8u);
+  const int m_tile = (int)(band * 8u + in_band % band_m), n_tile = (int)(in_band / band_m);
+
+  // this wavefront's LOADS blocks of a stage
+  const u4v *src[LOADS];
+#pragma unroll
+  for (int l = 0; l < LOADS; ++l) {
+    const int j = wave * LOADS + l;
+    const bool is_a = j < A_BLOCKS;
+    const int q = is_a ? j : j - A_BLOCKS;
+    const int per = is_a ? 2 * MT : 4;      // tiles of the operand; blocks are ordered [plane][k block][tile]
+    const int tile = q % per, kb = q / per % KB, plane = q / per / KB;
+    const int64_t row = is_a ? min(m_tile * 2 * MT + tile, g.a_tiles - 1) : (int64_t)n_tile * 4 + tile;
+    const u4v *base = is_a ? g.A + plane * g.plane_a + row * g.ld_a * 64 : g.B + plane * g.plane_b + row * g.ld_b * 64;
+    src[l] = base + ((int64_t)split * g.k_split + kb) * 64 + lane;
+  }
+  const int stages = min(g.k_split, g.kblocks - (int)split * g.k_split) / KB;
+  auto fill = [&](int buf) {
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) {
+      __builtin_amdgcn_global_load_lds((global_ptr)src[l], (lds_ptr)(lds + (buf * STAGE + wave * LOADS + l) * 64), 16, 0, 0);
+      src[l] += KB * 64;
+    }
+  };
+  f16v acc[MT][2];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][n][r] = 0.f;
+
+  fill(0);
+  if (stages > 1) fill(1);
+  int buf = 0;
+  for (int st = 0; st < stages; ++st) {
+    // this wavefront's loads of the stage have arrived (the next stage's LOADS may be in flight) and its reads of the
+    // stage before are done; after the barrier both hold for all four
+    if (st + 1 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (st + 2 < stages) fill(buf == 0 ? 2 : buf - 1);
+    const u4v *sa = lds + buf * STAGE * 64 + (wm * MT) * 64 + lane;
+    const u4v *sb = lds + (buf * STAGE + A_BLOCKS + wn * 2) * 64 + lane;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      h8v a[NP][MT], b[NP][2];
+#pragma unroll
+      for (int pl = 0; pl < NP; ++pl) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) b[pl][n] = __builtin_bit_cast(h8v, sb[((pl * KB + kb) * 4 + n) * 64]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) a[pl][i] = __builtin_bit_cast(h8v, sa[((pl * KB + kb) * 2 * MT + i) * 64]);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][n], acc[i][n], 0, 0, 0);
+          if (NP == 2) {
+            acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[NP - 1][i], b[0][n], acc[i][n], 0, 0, 0);
+            acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[NP - 1][n], acc[i][n], 0, 0, 0);
+          }
+        }
+    }
+    buf = buf == 2 ? 0 : buf + 1;
+  }
+
+  const int h = lane >> 5;
+  const int m0 = m_tile * 64 * MT + wm * 32 * MT;                      // first row of A of this wavefront
+  const int64_t n0 = (int64_t)n_tile * 128 + wn * 64 + (lane & 31);    // this lane's row of B, tile 0
+  // accumulator register r of tile (i, n): row m0 + 32 i + (r & 3) + 8 (r >> 2) + 4 h of A, row n0 + 32 n of B
+
+  if (MODE == STATS || MODE == GRAD) {
+    const float c = ldexpf(fabsf(g.scale) * LOG2E, -(g.scal->exp_x + g.scal->exp_w));
+    const int64_t left = g.V - (g.v0 + m0);      // words of this wavefront that exist
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int64_t p = n0 + 32 * n;
+      const int64_t label = p < g.P ? g.labels[p] : -1;
+      const int64_t rel = label - (g.v0 + m0);
+      const int at = rel >= 0 && rel < 32 * MT ? (int)rel : -1;        // the label's place among this wavefront's words
+      const bool here = __any(at >= 0);
+      if (MODE == STATS) {
+        if (here) {
+          float z = 0.f;
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z = at == 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h ? acc[i][n][r] * c : z;
+          if (at >= 0 && ((at >> 2) & 1) == h) g.target[p] = z;
+        }
+        if (left < 32 * MT) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (32 * i + (r & 3) + 8 * (r >> 2) + 4 * h >= left) acc[i][n][r] = -INFINITY;
+        }
+        float top = acc[0][n][0];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][n][r]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        top = fmaxf(top * c, MAX_FLOOR);
+        float sum = 0.f;
+        if (left >= 32 * MT) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -top));
+        } else {  // (the selection and not the infinity keeps the others out: c may have underflowed to 0)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              sum += 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h >= left
+                         ? 0.f : __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -top));
+        }
+        sum += __shfl_xor(sum, 32);
+        if (h == 0) g.partial[(int64_t)(m_tile * 2 + wm) * g.Pp + p] = make_float2(top, sum);
+      } else {
+        const float l2 = g.lse2[p], ca = g.coef_a[p], cb = g.coef_b[p];
+        h8v ident[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ident[s][i] = slot_place(s, h, i) == (lane & 31) ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          float v[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) v[r] = ca * __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -l2));
+          if (here) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] -= at == 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h ? cb : 0.f;
+          }
+          if (left < 32 * MT) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (32 * i + (r & 3) + 8 * (r >> 2) + 4 * h >= left) v[r] = 0.f;
+          }
+          h8v f[NP][2];
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              f[0][s][k] = (_Float16)v[8 * s + k];
+              if (NP == 2) f[NP - 1][s][k] = (_Float16)(v[8 * s + k] - (float)f[0][s][k]);
+            }
+          const int64_t pt = (int64_t)n_tile * 4 + wn * 2 + n, vt = m0 / 32 + i;
+#pragma unroll
+          for (int pl = 0; pl < NP; ++pl) {
+            if (g.gx) {
+              u4v *dst = g.gx + pl * g.plane_gx + (pt * g.ld_gx + vt * 2) * 64 + lane;
+#pragma unroll
+              for (int s = 0; s < 2; ++s) dst[s * 64] = __builtin_bit_cast(u4v, f[pl][s]);
+            }
+            if (g.gw) {
+              f16v tr;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) tr[r] = 0.f;
+#pragma unroll
+              for (int s = 0; s < 2; ++s) tr = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[pl][s], ident[s], tr, 0, 0, 0);
+              u4v *dst = g.gw + pl * g.plane_gw + (vt * g.ld_gw + pt * 2) * 64 + lane;
+#pragma unroll
+              for (int s = 0; s < 2; ++s) {
+                h8v o;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) o[k] = (_Float16)tr[8 * s + k];
+                dst[s * 64] = __builtin_bit_cast(u4v, o);
+              }
+            }
+          }
+        }
+      }
+    }
+  } else if (MODE == DX) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int d = m0 + 32 * i + 8 * q + 4 * h;
+          if (d >= g.ld_acc) continue;
+          float4 *dst = reinterpret_cast<float4 *>(g.acc + ((int64_t)split * g.Pp + n0 + 32 * n) * g.ld_acc + d);
+          float4 v = make_float4(acc[i][n][4 * q], acc[i][n][4 * q + 1], acc[i][n][4 * q + 2], acc[i][n][4 * q + 3]);
+          if (g.add) {
+            const float4 o = *dst;
+            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+          }
+          *dst = v;
+        }
+  } else {
+    const int e = -(*g.exp_g + g.scal->exp_x);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int64_t v = g.v0 + n0 + 32 * n;
+      if (v >= g.V) continue;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int d = m0 + 32 * i + 8 * q + 4 * h;
+          float x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] = ldexpf(acc[i][n][4 * q + k] * g.scale, e);
+          T *dst = (T *)g.out + v * g.D + d;
+          if ((g.D & 3) == 0) {
+            if (d < g.D) store4<T>(dst, x[0], x[1], x[2], x[3]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (d + k < g.D) dst[k] = (T)x[k];
+          }
+        }
+    }
+  }
+}
+
+// ---- rows -----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void merge(float &m, float &s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  s = s * __builtin_amdgcn_exp2f(m - top) + s2 * __builtin_amdgcn_exp2f(m2 - top);
+  m = top;
+}
+
+// Joins a row's (max, sum) pairs: 8 rows x 32 lanes per workgroup.
+__global__ void __launch_bounds__(256) vce_join_kernel(int64_t P, int64_t V, int64_t Pp, int pairs,
+                                                       const float2 *__restrict__ partial, const float *__restrict__ target,
+                                                       const int64_t *__restrict__ labels, int64_t ignore,
+                                                       float *__restrict__ lse2, float *__restrict__ lse,
+                                                       float *__restrict__ row_loss) {
+  const int row = threadIdx.x & 7, lane = threadIdx.x >> 3;
+  const int64_t p = (int64_t)blockIdx.x * 8 + row;
+  float m = MAX_FLOOR, s = 0.f;
+  for (int j = lane; j < pairs; j += 32) {
+    const float2 q = partial[(int64_t)j * Pp + p];
+    merge(m, s, q.x, q.y);
+  }
+  __shared__ float2 part[32][8];
+  part[lane][row] = make_float2(m, s);
+  __syncthreads();
+  for (int d = 16; d > 0; d >>= 1) {
+    if (lane < d) {
+      const float2 q = part[lane + d][row];
+      merge(m, s, q.x, q.y);
+      part[lane][row] = make_float2(m, s);
+    }
+    __syncthreads();
+  }
+  if (lane != 0) return;
+  const float l2 = m + log2f(s);
+  lse2[p] = p < P ? l2 : 0.f;
+  if (p >= P) return;
+  const int64_t label = labels[p];
+  const bool in = label != ignore;
+  if (lse) lse[p] = in ? l2 * LN2F : 0.f;
+  // a label outside the vocabulary has no logit: the row's loss is NaN
+  row_loss[p] = !in ? 0.f : label < 0 || label >= V ? NAN : (l2 - target[p]) * LN2F;
+}
+
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[16];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.;
+  for (int i = 0; i < (int)blockDim.x / 64; ++i) v += part[i];
+  return v;
+}
+
+__global__ void __launch_bounds__(1024) vce_reduce_kernel(int64_t P, const float *__restrict__ row_loss,
+                                                          const int64_t *__restrict__ labels, int64_t ignore, int mean,
+                                                          float *__restrict__ loss, Scalars *s) {
+  double sum = 0., n = 0.;
+  for (int64_t p = threadIdx.x; p < P; p += 1024) {
+    sum += (double)row_loss[p];
+    n += labels[p] != ignore ? 1. : 0.;
+  }
+  sum = block_sum(sum);
+  n = block_sum(n);
+  if (threadIdx.x == 0) {
+    s->n_valid = (float)n;
+    if (loss) *loss = (float)(mean ? sum / n : sum);
+  }
+}
+
+// Row factors of G, scaled by the power of two that brings the largest to 2^12..2^13 (|G| <= |a| + |b|).
+__global__ void __launch_bounds__(1024) vce_coef_kernel(int64_t P, int64_t Pp, int64_t V, const float *__restrict__ g_loss,
+                                                        int per_row, int mean, const float *__restrict__ g_lse,
+                                                        const int64_t *__restrict__ labels, int64_t ignore,
+                                                        const Scalars *s, int *__restrict__ exp_g,
+                                                        float *__restrict__ coef_a, float *__restrict__ coef_b) {
+  const float inv = mean ? 1.f / s->n_valid : 1.f;
+  auto row = [&](int64_t p, float &a, float &b) {
+    a = b = 0.f;
+    if (p >= P || labels[p] == ignore) return;
+    b = g_loss ? g_loss[per_row ? p : 0] * inv : 0.f;
+    a = b + (g_lse ? g_lse[p] : 0.f);
+    if (g_loss && (labels[p] < 0 || labels[p] >= V)) a = NAN;   // no such word: the row's loss is NaN
+  };
+  float top = 0.f;
+  for (int64_t p = threadIdx.x; p < P; p += 1024) {
+    float a, b;
+    row(p, a, b);
+    a = fabsf(a), b = fabsf(b);
+    if (a < INFINITY) top = fmaxf(top, a);
+    if (b < INFINITY) top = fmaxf(top, b);
+  }
+  __shared__ float part[16];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = part[0];
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, part[i]);
+  const int e = top > 0.f ? TOP_EXP - 1 - ilogbf(top) : 0;
+  if (threadIdx.x == 0) *exp_g = e;
+  for (int64_t p = threadIdx.x; p < Pp; p += 1024) {
+    float a, b;
+    row(p, a, b);
+    coef_a[p] = ldexpf(a, e);
+    coef_b[p] = ldexpf(b, e);
+  }
+}
+
+// dX = sum of the splits, scaled, in the output type.
+template <typename T>
+__global__ void __launch_bounds__(256) vce_dx_kernel(int64_t P, int64_t D, int64_t Pp, int64_t ld, int splits, float scale,
+                                                     const float *__restrict__ acc, const Scalars *s,
+                                                     const int *__restrict__ exp_g, T *__restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= P * D) return;
+  const int64_t p = i / D, d = i - p * D;
+  float v = 0.f;
+  for (int k = 0; k < splits; ++k) v += acc[((int64_t)k * Pp + p) * ld + d];
+  out[i] = (T)ldexpf(v * scale, -(*exp_g + s->exp_w));
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+struct Shape {
+  int64_t P, V, D, Pp, Vp, Dk;
+  int np;
+  Shape(int dtype, int64_t P_, int64_t V_, int64_t D_)
+      : P(P_), V(V_), D(D_), Pp(round_up(P_, TILE_P)), Vp(round_up(V_, TILE_V)), Dk(round_up(D_, 32)),
+        np(dtype == PR_F32 ? 2 : 1) {}
+  int64_t plane(int64_t rows) const { return rows * Dk / 8; }   // 16-byte units of one packed plane
+};
+
+bool valid_shape(int dtype, int64_t P, int64_t V, int64_t D) {
+  return dtype >= PR_F32 && dtype <= PR_BF16 && P >= 0 && V >= 1 && D >= 1 && P < (1ll << 30) && V < (1ll << 30) &&
+         D < (1ll << 20) && P * D < (1ll << 38) && V * D < (1ll << 38);
+}
+
+struct Carve {  // consecutive 256-byte-aligned pieces of a buffer
+  char *at;
+  size_t used = 0;
+  explicit Carve(void *base) : at((char *)base) {}
+  template <typename T>
+  T *take(int64_t n) {
+    T *p = (T *)(at ? at + used : nullptr);
+    used += (size_t)round_up((int64_t)sizeof(T) * n, 256);
+    return p;
+  }
+};
+
+struct Kept {  // what the forward pass leaves for the backward pass
+  Scalars *scal;
+  float *lse2;
+  u4v *xf, *wf;
+  Kept(Carve &c, const Shape &s) {
+    scal = c.take<Scalars>(1);
+    lse2 = c.take<float>(s.Pp);
+    xf = c.take<u4v>(s.np * s.plane(s.Pp));
+    wf = c.take<u4v>(s.np * s.plane(s.Vp));
+  }
+};
+
+struct FwdScratch {
+  float *amax, *target;
+  float2 *partial;
+  int pairs;
+  FwdScratch(Carve &c, const Shape &s) {
+    pairs = (int)(s.Vp / TILE_V * 2);
+    amax = c.take<float>(2 * AMAX_BLOCKS);
+    target = c.take<float>(s.Pp);
+    partial = c.take<float2>((int64_t)pairs * s.Pp);
+  }
+};
+
+constexpr int64_t PIECE_BYTES = 512ll << 20;  // G of one piece of the vocabulary, all copies and planes
+
+struct BwdScratch {
+  int *exp_g;
+  float *coef_a, *coef_b, *acc;
+  u4v *xt, *wt, *gx, *gw;
+  int64_t piece;  // words
+  int splits, kper;  // splits of a full piece's words, blocks of the contraction each
+  BwdScratch(Carve &c, const Shape &s, bool dx, bool dw) {
+    const int64_t per_word = s.Pp * 2 * s.np * (int(dx) + int(dw));
+    piece = std::min(s.Vp, std::max<int64_t>(PIECE_BYTES / per_word / TILE_V, 1) * TILE_V);
+    const int64_t pieces = (s.Vp + piece - 1) / piece;
+    piece = round_up((s.Vp + pieces - 1) / pieces, TILE_V);   // of equal size
+    // enough workgroups for every CU to hold two, at least 16 stages each
+    const int64_t tiles = std::max<int64_t>(1, (s.Dk + 255) / 256 * (s.Pp / TILE_P));
+    const int64_t want = std::min<int64_t>(16, std::max<int64_t>(1, 512 / tiles));
+    const int64_t k = piece / 16;
+    kper = (int)round_up((k + want - 1) / want, 32);
+    splits = (int)((k + kper - 1) / kper);
+    exp_g = c.take<int>(1);
+    coef_a = c.take<float>(s.Pp);
+    coef_b = c.take<float>(s.Pp);
+    acc = c.take<float>(dx ? splits * s.Pp * s.Dk : 0);
+    wt = c.take<u4v>(dx ? s.np * s.plane(s.Vp) : 0);
+    xt = c.take<u4v>(dw ? s.np * s.plane(s.Pp) : 0);
+    gx = c.take<u4v>(dx ? s.np * s.Pp * piece / 8 : 0);
+    gw = c.take<u4v>(dw ? s.np * s.Pp * piece / 8 : 0);
+  }
+};
+
+template <int NP, int MT, int MODE, typename T>
+int launch_gemm(const GemmArgs &g, hipStream_t st) {
+  constexpr int KB = NP == 1 ? 2 : 1;
+  const size_t bytes = (size_t)3 * (2 * MT + 4) * KB * NP * 1024;
+  const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles * g.splits;
+  if (tiles > (1ll << 30)) {
+    set_error_text("pr_vocab_ce: too many tiles for one launch");
+    return PR_EUNSUPPORTED;
+  }
+  PR_HIP(hipFuncSetAttribute((const void *)vce_gemm_kernel<NP, MT, MODE, T>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)bytes));
+  hipLaunchKernelGGL((vce_gemm_kernel<NP, MT, MODE, T>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), bytes, st, g);
+  return check_launch("pr_vocab_ce");
+}
+
+template <typename T, int NP>
+int pack(bool transposed, const PackJob &a, const PackJob &b, const Scalars *s, hipStream_t st) {
+  const int64_t ga = (a.blocks + 3) / 4, gb = (b.blocks + 3) / 4;
+  if (ga + gb == 0) return PR_OK;
+  if (ga + gb > 0x7fffffffll) return PR_EUNSUPPORTED;
+  if (transposed)
+    hipLaunchKernelGGL((vce_pack_t_kernel<T, NP>), dim3((unsigned)(ga + gb)), dim3(256), 0, st, a, b, ga, s);
+  else
+    hipLaunchKernelGGL((vce_pack_kernel<T, NP>), dim3((unsigned)(ga + gb)), dim3(256), 0, st, a, b, ga, s);
+  return check_launch("pr_vocab_ce");
+}
+
+struct Call {
+  int dtype;
+  int64_t P, V, D;
+  Matrix x, w;
+  const int64_t *labels;
+  int64_t ignore;
+  float scale;
+};
+
+#define PR_TRY(e)                  \
+  do {                             \
+    const int _rc = (e);           \
+    if (_rc != PR_OK) return _rc;  \
+  } while (0)
+
+template <typename T, int NP>
+int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, float *lse, float *loss, hipStream_t st) {
+  const Shape s(c.dtype, c.P, c.V, c.D);
+  const bool scaled = c.dtype != PR_F16;
+  if (scaled) {
+    hipLaunchKernelGGL((vce_amax_kernel<T>), dim3(2 * AMAX_BLOCKS), dim3(256), 0, st, c.w, c.x, c.labels, c.ignore, f.amax);
+    PR_TRY(check_launch("pr_vocab_ce"));
+  }
+  hipLaunchKernelGGL(vce_exponents_kernel, dim3(1), dim3(256), 0, st, f.amax, scaled ? AMAX_BLOCKS : 0, k.scal);
+  PR_TRY(check_launch("pr_vocab_ce"));
+  const int kb = (int)(s.Dk / 16);
+  const PackJob jw{c.w, nullptr, 0, k.wf, s.plane(s.Vp), s.Vp / 32 * kb, kb, 1.f, 0};
+  const PackJob jx{c.x, c.labels, c.ignore, k.xf, s.plane(s.Pp), s.Pp / 32 * kb, kb, c.scale < 0.f ? -1.f : 1.f, 1};
+  PR_TRY((pack<T, NP>(false, jw, jx, k.scal, st)));
+  GemmArgs g{};
+  g.A = k.wf, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
+  g.a_tiles = (int)(s.Vp / 32), g.kblocks = g.k_split = kb, g.m_tiles = (int)(s.Vp / TILE_V), g.n_tiles = (int)(s.Pp / TILE_P), g.splits = 1;
+  g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.labels = c.labels;
+  g.partial = f.partial, g.target = f.target, g.Pp = s.Pp;
+  PR_TRY((launch_gemm<NP, 4, STATS, T>(g, st)));
+  hipLaunchKernelGGL(vce_join_kernel, dim3((unsigned)(s.Pp / 8)), dim3(256), 0, st, c.P, c.V, s.Pp, f.pairs, f.partial,
+                     f.target, c.labels, c.ignore, k.lse2, lse, row_loss);
+  PR_TRY(check_launch("pr_vocab_ce"));
+  hipLaunchKernelGGL(vce_reduce_kernel, dim3(1), dim3(1024), 0, st, c.P, row_loss, c.labels, c.ignore, mean, loss, k.scal);
+  return check_launch("pr_vocab_ce");
+}
+
+template <typename T, int NP>
+int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b, const float *g_loss, const float *g_lse, T *dx,
+             T *dw, hipStream_t st) {
+  const Shape s(c.dtype, c.P, c.V, c.D);
+  hipLaunchKernelGGL(vce_coef_kernel, dim3(1), dim3(1024), 0, st, c.P, s.Pp, c.V, g_loss, per_row, mean, g_lse, c.labels,
+                     c.ignore, k.scal, b.exp_g, b.coef_a, b.coef_b);
+  PR_TRY(check_launch("pr_vocab_ce"));
+  const int kb = (int)(s.Dk / 16), kv = (int)(s.Vp / 16), kp = (int)(s.Pp / 16);
+  const PackJob jw{c.w, nullptr, 0, b.wt, s.plane(s.Vp), dx ? s.Dk / 32 * kv : 0, kv, 1.f, 0};
+  const PackJob jx{c.x, c.labels, c.ignore, b.xt, s.plane(s.Pp), dw ? s.Dk / 32 * kp : 0, kp, 1.f, 1};
+  PR_TRY((pack<T, NP>(true, jw, jx, k.scal, st)));
+  // 256 features per workgroup unless 128 leave fewer of them unused
+  const bool narrow = round_up(s.Dk, 128) * 8 < round_up(s.Dk, 256) * 7;
+  const int d_tiles = (int)(narrow ? round_up(s.Dk, 128) / 128 : round_up(s.Dk, 256) / 256);
+  for (int64_t v0 = 0; v0 < s.Vp; v0 += b.piece) {
+    const int64_t words = std::min(b.piece, s.Vp - v0);
+    GemmArgs g{};
+    g.A = k.wf + v0 / 32 * kb * 64, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
+    g.a_tiles = (int)(words / 32), g.kblocks = g.k_split = kb, g.m_tiles = (int)(words / TILE_V), g.n_tiles = (int)(s.Pp / TILE_P);
+    g.splits = 1, g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.v0 = v0, g.labels = c.labels, g.Pp = s.Pp;
+    g.lse2 = k.lse2, g.coef_a = b.coef_a, g.coef_b = b.coef_b;
+    g.gx = dx ? b.gx : nullptr, g.gw = dw ? b.gw : nullptr;
+    g.plane_gx = g.plane_gw = s.Pp * b.piece / 8, g.ld_gx = b.piece / 16, g.ld_gw = kp;
+    PR_TRY((launch_gemm<NP, 4, GRAD, T>(g, st)));
+    if (dx) {
+      GemmArgs x{};
+      x.A = b.wt + v0 / 16 * 64, x.B = b.gx, x.plane_a = s.plane(s.Vp), x.plane_b = g.plane_gx, x.ld_a = kv, x.ld_b = g.ld_gx;
+      x.a_tiles = (int)(s.Dk / 32), x.m_tiles = d_tiles, x.n_tiles = (int)(s.Pp / TILE_P), x.scal = k.scal;
+      x.acc = b.acc, x.Pp = s.Pp, x.ld_acc = s.Dk, x.add = v0 > 0;
+      // the splits of a full piece; a shorter last piece leaves the rest of them as they are
+      x.kblocks = (int)(words / 16), x.k_split = b.kper, x.splits = (x.kblocks + b.kper - 1) / b.kper;
+      PR_TRY(narrow ? (launch_gemm<NP, 2, DX, T>(x, st)) : (launch_gemm<NP, 4, DX, T>(x, st)));
+    }
+    if (dw) {
+      GemmArgs w{};
+      w.A = b.xt, w.B = b.gw, w.plane_a = s.plane(s.Pp), w.plane_b = g.plane_gw, w.ld_a = w.ld_b = kp;
+      w.a_tiles = (int)(s.Dk / 32), w.kblocks = w.k_split = kp, w.m_tiles = d_tiles, w.n_tiles = (int)(words / 128), w.splits = 1;
+      w.scal = k.scal, w.exp_g = b.exp_g, w.scale = c.scale, w.V = c.V, w.v0 = v0, w.out = dw, w.D = c.D;
+      PR_TRY(narrow ? (launch_gemm<NP, 2, DW, T>(w, st)) : (launch_gemm<NP, 4, DW, T>(w, st)));
+    }
+  }
+  if (dx && c.P > 0) {
+    hipLaunchKernelGGL((vce_dx_kernel<T>), dim3((unsigned)((c.P * c.D + 255) / 256)), dim3(256), 0, st, c.P, c.D, s.Pp, s.Dk,
+                       b.splits, c.scale, b.acc, k.scal, b.exp_g, dx);
+    PR_TRY(check_launch("pr_vocab_ce"));
+  }
+  return PR_OK;
+}
+
+int check_call(const Call &c) {
+  if (!valid_shape(c.dtype, c.P, c.V, c.D) || !(fabsf(c.scale) < INFINITY)) return PR_EINVAL;
+  if (c.P < 1 || !c.x.data || !c.w.data || !c.labels) return PR_EINVAL;
+  const uintptr_t mask = c.dtype == PR_F32 ? 3 : 1;
+  if (((uintptr_t)c.x.data & mask) || ((uintptr_t)c.w.data & mask) || ((uintptr_t)c.labels & 7)) return PR_EINVAL;
+  if (c.x.ld_row < 0 || c.x.ld_col < 0 || c.w.ld_row < 0 || c.w.ld_col < 0) return PR_EINVAL;
+  return PR_OK;
+}
+
+}  // namespace
+}  // namespace pr
+
+extern "C" size_t pr_vocab_ce_kept_bytes(int dtype, int64_t P, int64_t V, int64_t D) {
+  if (!pr::valid_shape(dtype, P, V, D)) return 0;
+  pr::Carve c(nullptr);
+  pr::Kept k(c, pr::Shape(dtype, P, V, D));
+  return c.used;
+}
+
+extern "C" size_t pr_vocab_ce_fwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D) {
+  if (!pr::valid_shape(dtype, P, V, D)) return 0;
+  pr::Carve c(nullptr);
+  pr::FwdScratch f(c, pr::Shape(dtype, P, V, D));
+  return c.used;
+}
+
+extern "C" size_t pr_vocab_ce_bwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D, int want_dx, int want_dw) {
+  if (!pr::valid_shape(dtype, P, V, D) || P < 1 || (!want_dx && !want_dw)) return 0;
+  pr::Carve c(nullptr);
+  pr::BwdScratch b(c, pr::Shape(dtype, P, V, D), want_dx, want_dw);
+  return c.used;
+}
+
+extern "C" int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const void *x, int64_t ldx_row, int64_t ldx_col,
+                               const void *w, int64_t ldw_row, int64_t ldw_col, const int64_t *labels, int64_t ignore_index,
+                               float scale, int mean, void *kept, size_t kept_bytes, void *scratch, size_t scratch_bytes,
+                               float *row_loss, float *lse, float *loss, void *stream) {
+  const pr::Call c{dtype, P, V, D, {x, P, D, ldx_row, ldx_col}, {w, V, D, ldw_row, ldw_col}, labels, ignore_index, scale};
+  PR_TRY(pr::check_call(c));
+  if (!kept || !scratch || !row_loss || ((uintptr_t)kept & 15) || ((uintptr_t)scratch & 15)) return PR_EINVAL;
+  if (kept_bytes < pr_vocab_ce_kept_bytes(dtype, P, V, D) ||
+      scratch_bytes < pr_vocab_ce_fwd_scratch_bytes(dtype, P, V, D))
+    return PR_ESCRATCH;
+  const pr::Shape s(dtype, P, V, D);
+  pr::Carve ck(kept), cs(scratch);
+  pr::Kept k(ck, s);
+  pr::FwdScratch f(cs, s);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == PR_F32) return pr::forward<float, 2>(c, mean, k, f, row_loss, lse, loss, st);
+  if (dtype == PR_F16) return pr::forward<_Float16, 1>(c, mean, k, f, row_loss, lse, loss, st);
+  return pr::forward<__bf16, 1>(c, mean, k, f, row_loss, lse, loss, st);
+}
+
+extern "C" int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const void *x, int64_t ldx_row, int64_t ldx_col,
+                               const void *w, int64_t ldw_row, int64_t ldw_col, const int64_t *labels, int64_t ignore_index,
+                               float scale, int mean, int per_row, const void *kept, size_t kept_bytes, const float *g_loss,
+                               const float *g_lse, void *scratch, size_t scratch_bytes, void *dx, void *dw, void *stream) {
+  const pr::Call c{dtype, P, V, D, {x, P, D, ldx_row, ldx_col}, {w, V, D, ldw_row, ldw_col}, labels, ignore_index, scale};
+  PR_TRY(pr::check_call(c));
+  if (!dx && !dw) return PR_OK;
+  if (!kept || !scratch || ((uintptr_t)kept & 15) || ((uintptr_t)scratch & 15)) return PR_EINVAL;
+  if (((uintptr_t)dx & 15) || ((uintptr_t)dw & 15)) return PR_EINVAL;
+  if (kept_bytes < pr_vocab_ce_kept_bytes(dtype, P, V, D) ||
+      scratch_bytes < pr_vocab_ce_bwd_scratch_bytes(dtype, P, V, D, dx != nullptr, dw != nullptr))
+    return PR_ESCRATCH;
+  const pr::Shape s(dtype, P, V, D);
+  pr::Carve ck(const_cast<void *>(kept)), cs(scratch);
+  pr::Kept k(ck, s);
+  pr::BwdScratch b(cs, s, dx != nullptr, dw != nullptr);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == PR_F32) return pr::backward<float, 2>(c, per_row, mean, k, b, g_loss, g_lse, (float *)dx, (float *)dw, st);
+  if (dtype == PR_F16)
+    return pr::backward<_Float16, 1>(c, per_row, mean, k, b, g_loss, g_lse, (_Float16 *)dx, (_Float16 *)dw, st);
+  return pr::backward<__bf16, 1>(c, per_row, mean, k, b, g_loss, g_lse, (__bf16 *)dx, (__bf16 *)dw, st);
+}

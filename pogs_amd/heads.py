@@ -23,6 +23,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
+from .vocabulary import vocabulary_cross_entropy
 
 
 class HeadNames(Enum):
@@ -184,6 +185,14 @@ class FieldHeads(torch.nn.Module):
     def get_clip_outputs_from_feature(self, features: torch.Tensor, clip_scale: torch.Tensor) -> torch.Tensor:
         x = torch.cat([features, clip_scale.view(-1, 1).to(features.dtype)], dim=-1)   # gaussian_field.py:184,202
         return self.clip_net(x, norm_eps=0.0)
+
+    def get_vocabulary_loss_from_feature(self, features: torch.Tensor, clip_scale: torch.Tensor,
+                                         vocabulary: torch.Tensor, labels: torch.Tensor, logit_scale: float = 100.0,
+                                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+        """Cross entropy of the rows' clip features over a table of phrase embeddings ``[V, clip_n_dims]`` (float32,
+        usually of unit rows), ``logit_scale`` times their products as logits: ``vocabulary_cross_entropy``."""
+        clip = self.get_clip_outputs_from_feature(features, clip_scale)
+        return vocabulary_cross_entropy(clip, vocabulary, labels.reshape(-1), logit_scale, ignore_index, reduction)
 
     def get_instance_outputs_from_feature(self, features: torch.Tensor) -> torch.Tensor:
         return self.instance_net(features, norm_eps=self.INSTANCE_EPS)

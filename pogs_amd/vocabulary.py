@@ -1,0 +1,146 @@
+"""Cross entropy of feature rows over a large vocabulary of embeddings (MI355X matrix cores).
+
+What the clip head's unit features (``FieldHeads.get_clip_outputs_from_feature``, ``pogs/fields/gaussian_field.py:194-204``)
+are trained and scored on when every pixel has a label in a table of phrase embeddings.  The value and the gradients of
+``torch.nn.functional.cross_entropy(scale * features @ vocabulary.T, labels)``, without the ``[rows, words]`` logits: the
+forward pass keeps one maximum and sum a row, the backward pass makes the products again for one piece of the vocabulary
+at a time.  Products take float16 operands scaled by powers of two and add in float32; float32 inputs are split into two
+float16 planes (2^-22 a product), so float32 stays float32 in accuracy.  Results do not depend on the order in which
+workgroups run.  HIP kernels only (``pr_vocab_ce_fwd``, ``pr_vocab_ce_bwd``); there is no CPU path.
+"""
+from __future__ import annotations
+
+import math
+from typing import Tuple, Union
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+from torch.autograd.graph import get_gradient_edge
+
+from . import _lib
+from .rendering import _call, _ptr, _stream
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # PR_F32, PR_F16, PR_BF16
+_REDUCTIONS = ("none", "sum", "mean")
+
+
+def _scratch(nbytes: int, device) -> Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+class _VocabularyCrossEntropy(torch.autograd.Function):
+    """``x [P, D]``, ``w [V, D]``, ``labels [P]`` int64 -> (loss, lse): loss ``[P]`` or 0-d, lse ``[P]``."""
+
+    @staticmethod
+    def forward(ctx, x, w, labels, scale, ignore_index, reduction):
+        ctx.set_materialize_grads(False)
+        ctx.args = scale, ignore_index, reduction
+        (P, D), V, dev = x.shape, w.shape[0], x.device
+        row_loss = torch.empty(P, dtype=torch.float32, device=dev)
+        lse = torch.empty(P, dtype=torch.float32, device=dev)
+        if P == 0:
+            ctx.save_for_backward(x, w, labels, None)
+            total = {"none": row_loss, "sum": row_loss.new_zeros(()), "mean": row_loss.new_full((), math.nan)}
+            return total[reduction], lse
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        lib, t = _lib.load(), _TYPES[x.dtype]
+        with torch.cuda.device(dev):
+            kept = _scratch(lib.pr_vocab_ce_kept_bytes(t, P, V, D), dev)
+            scratch = _scratch(lib.pr_vocab_ce_fwd_scratch_bytes(t, P, V, D), dev)
+            _call("pr_vocab_ce_fwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index,
+                  scale, int(reduction == "mean"), _ptr(kept), kept.numel(), _ptr(scratch), scratch.numel(),
+                  _ptr(row_loss), _ptr(lse), _ptr(loss), _stream())
+        ctx.save_for_backward(x, w, labels, kept)
+        return (row_loss if reduction == "none" else loss), lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_loss, g_lse):
+        x, w, labels, kept = ctx.saved_tensors
+        scale, ignore_index, reduction = ctx.args
+        (P, D), V, dev = x.shape, w.shape[0], x.device
+        want_x, want_w = ctx.needs_input_grad[:2]
+        if P == 0 or (g_loss is None and g_lse is None):
+            return (torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None) + (None,) * 4
+        g_loss = None if g_loss is None else g_loss.float().contiguous()
+        g_lse = None if g_lse is None else g_lse.float().contiguous()
+        dx = torch.empty(P, D, dtype=x.dtype, device=dev) if want_x else None
+        dw = torch.empty(V, D, dtype=w.dtype, device=dev) if want_w else None
+        lib, t = _lib.load(), _TYPES[x.dtype]
+        with torch.cuda.device(dev):
+            scratch = _scratch(lib.pr_vocab_ce_bwd_scratch_bytes(t, P, V, D, int(want_x), int(want_w)), dev)
+            _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index,
+                  scale, int(reduction == "mean"), int(reduction == "none"), _ptr(kept), kept.numel(), _ptr(g_loss),
+                  _ptr(g_lse), _ptr(scratch), scratch.numel(), _ptr(dx), _ptr(dw), _stream())
+        return dx, dw, None, None, None, None
+
+
+_STREAM_KEY = "pogs_amd.stream"
+
+
+def _leaf_nodes(*tensors: Tensor) -> list:
+    """The gradient nodes of the leaves among ``tensors``, marked with the stream they came up on.  A leaf's node lives as
+    long as any graph of it does and keeps its first stream; a backward pass captured on another stream would make that
+    one part of the capture, which ends the process.  So the call that would lead there is refused."""
+    nodes = []
+    for t in tensors:
+        if torch.is_grad_enabled() and t.is_leaf and t.requires_grad:
+            node = get_gradient_edge(t).node
+            stream = torch.cuda.current_stream(t.device).cuda_stream
+            if node.metadata.setdefault(_STREAM_KEY, stream) != stream and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a graph of the same features or vocabulary, made outside the capture, is still alive: "
+                                   "its backward pass cannot be captured; drop that graph's outputs first")
+            nodes.append(node)
+    return nodes
+
+
+def _check(features: Tensor, vocabulary: Tensor, labels: Tensor, scale: float, reduction: str) -> float:
+    if vocabulary.dim() != 2 or 0 in vocabulary.shape:
+        raise ValueError(f"the vocabulary must be [words, dims] and not empty, got {tuple(vocabulary.shape)}")
+    if features.dim() < 1 or features.shape[-1] != vocabulary.shape[1]:
+        raise ValueError(f"features {tuple(features.shape)} do not end in the vocabulary's {vocabulary.shape[1]} dims")
+    if labels.shape != features.shape[:-1]:
+        raise ValueError(f"labels must be {tuple(features.shape[:-1])}, one a feature row, got {tuple(labels.shape)}")
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"labels must be int64 or int32, got {labels.dtype}")
+    if features.dtype != vocabulary.dtype or features.dtype not in _TYPES:
+        raise TypeError("features and vocabulary must both be float32, float16 or bfloat16, got "
+                        f"{features.dtype} and {vocabulary.dtype}")
+    if isinstance(scale, Tensor):
+        raise TypeError("scale is a plain number; multiply the features by a learned one")
+    if not math.isfinite(scale) or abs(scale) > 3e38:
+        raise ValueError(f"scale must be finite, got {scale}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
+    if not (features.is_cuda and vocabulary.is_cuda and labels.is_cuda):
+        raise RuntimeError("pogs_amd.vocabulary runs on a HIP device only (no CPU fallback)")
+    if not features.device == vocabulary.device == labels.device:
+        raise RuntimeError("features, vocabulary and labels are on different devices")
+    return float(scale)
+
+
+def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tensor, scale: float = 1.0,
+                             ignore_index: int = -100, reduction: str = "mean",
+                             return_lse: bool = False) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+    """Cross entropy of ``scale * features @ vocabulary.T`` against ``labels``, logits never stored.
+
+    ``features``: ``[..., D]`` and ``vocabulary``: ``[V, D]``, both float32, float16 or bfloat16, any strides;
+    ``labels``: ``[...]`` int64 or int32.  Returns float32: the mean over the rows whose label is not ``ignore_index``
+    (NaN if there are none, as in torch), their ``"sum"``, or with ``"none"`` one value a row (0 for an ignored one);
+    with ``return_lse`` also every row's ``log sum_v exp(scale <x, w_v>)`` (0 for an ignored row).  Differentiable in
+    features and vocabulary, through the loss and the log-sum (gradients in the inputs' type, from the formula; not
+    twice).  Ignored rows contribute nothing, even if their features are not finite.  A label that is neither in
+    ``0..V-1`` nor ``ignore_index`` makes its row's loss NaN and the gradients with it: nothing is read out of range,
+    and the host does not wait to look.  Safe in a captured graph, gradients included, as long as no graph of the same
+    leaves made outside the capture is alive (refused where one of this function is)."""
+    scale = _check(features, vocabulary, labels, scale, reduction)
+    nodes = _leaf_nodes(features, vocabulary)    # held until the new graph holds them
+    D = features.shape[-1]
+    x = features.reshape(-1, D)
+    flat = labels.reshape(-1).to(torch.int64).contiguous()
+    loss, lse = _VocabularyCrossEntropy.apply(x, vocabulary, flat, scale, int(ignore_index), reduction)
+    del nodes
+    if reduction == "none":
+        loss = loss.reshape(labels.shape)
+    return (loss, lse.reshape(labels.shape)) if return_lse else loss
