@@ -481,12 +481,15 @@ int pr_densify_split_children(int64_t n_out, const int32_t *map_src, const int32
  * The reference has no such loss; this is torch.nn.functional.cross_entropy(scale * x @ w.T, labels) and its gradients.
  * A row whose label is ignore_index has row_loss 0, lse 0 and no gradient, whatever its features hold; any other label
  * outside 0..V-1 makes the row's loss NaN and, through it, its gradients.
- * pr_vocab_ce_fwd: P >= 1.  row_loss[P]; lse[P] and loss[1] may be NULL; loss = sum of row_loss, or (mean != 0) their mean
- * over the rows not ignored (NaN if there are none).  kept: what pr_vocab_ce_bwd reads (packed operands, row statistics).
+ * pr_vocab_ce_fwd: P >= 1.  row_loss[P]; lse[P] and loss[1] may be NULL (a backward pass with mean != 0
+ * needs the loss); loss = sum of row_loss, or (mean != 0) their mean
+ * over the rows not ignored (NaN if there are none).  kept: what pr_vocab_ce_bwd reads (packed operands, row statistics);
+ * NULL, for at most pr_vocab_ce_score_rows() rows and no backward pass: the vocabulary is read once and not packed.
  * pr_vocab_ce_bwd: dx[P,D] and dw[V,D] (contiguous, 16-byte aligned, the inputs' type, either may be NULL) from the
  * gradient g_loss of row_loss (per_row != 0: [P]) or of loss (one value) and g_lse[P] of lse; a NULL one is 0.  kept is
  * read only: several calls may share it.  Products take float16 operands (float32 input: two planes, 2^-22) and add in
  * float32; sums run in a fixed order, so equal inputs give equal bits. */
+int pr_vocab_ce_score_rows(void);
 size_t pr_vocab_ce_kept_bytes(int dtype, int64_t P, int64_t V, int64_t D);
 size_t pr_vocab_ce_fwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D);
 size_t pr_vocab_ce_bwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D, int want_dx, int want_dw);

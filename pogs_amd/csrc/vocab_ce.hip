@@ -12,8 +12,8 @@
 // ds_read_b128.  Packing scales each tensor by one power of two that brings its largest magnitude to 2^13..2^14: a
 // bfloat16 value keeps all its bits down to 2^-31 of the largest, and a float32 value becomes two float16 planes (head
 // and residual, 22 bits down to 2^-17 of the largest) whose products head*head + head*residual + residual*head lose 2^-22.
-// float16 input is packed as it is.  Values that are not finite stay so; rows with the ignored label are packed as zeros,
-// whatever they hold.
+// float16 input is packed as it is.  X takes the scale's sign.  Values that are not finite stay so; rows with the ignored
+// label are packed as zeros, whatever they hold.
 //
 // One product kernel with four epilogues:
 //   STATS  256 words x 128 rows: the row of X is on the lane, so the running maximum and sum over the words are taken in
@@ -43,12 +43,9 @@ constexpr int TILE_P = 128;  // rows per workgroup
 constexpr int TOP_EXP = 13;  // packed magnitudes are below 2^(TOP_EXP + 1)
 constexpr float MAX_FLOOR = -3.0e38f;  // a maximum over nothing: exp2 of anything minus it is 0, not NaN
 constexpr float LN2F = 0.69314718055994531f;
-constexpr int AMAX_BLOCKS = 512;  // partial maxima per tensor
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) {
-  return (float)v;
-}
+constexpr int SCORE_ROWS = 64;      // rows that the forward pass without packing takes at most
+constexpr int SCORE_BLOCKS = 1024;  // its workgroups: four per CU
+constexpr int AMAX_BLOCKS = 1024;  // partial maxima per tensor at most
 
 struct Matrix {  // rows x cols with any strides (elements)
   const void *data;
@@ -60,67 +57,111 @@ struct Scalars {  // per call, on the device
   float n_valid;     // rows whose label is not the ignored one
 };
 
-__device__ __forceinline__ bool row_in(const int64_t *labels, int64_t ignore, int64_t p) {
-  return !labels || labels[p] != ignore;
+// ---- packing --------------------------------------------------------------------------------------------------------
+template <typename T>
+struct Eight;  // eight consecutive elements as one or two 16-byte accesses
+template <>
+struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float *p) {
+    a = reinterpret_cast<const float4 *>(p)[0];
+    b = reinterpret_cast<const float4 *>(p)[1];
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+};
+template <typename T>
+struct Eight {
+  u4v a;
+  __device__ __forceinline__ void load(const T *p) { a = *reinterpret_cast<const u4v *>(p); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    const t8 t = __builtin_bit_cast(t8, a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+  }
+};
+
+// Whether eight consecutive elements of a row can be read by 16-byte accesses: unit column stride, aligned rows.
+template <typename T>
+__device__ __forceinline__ bool wide_rows(const Matrix &m) {
+  return m.ld_col == 1 && (((uintptr_t)m.data | (uintptr_t)(m.ld_row * (int64_t)sizeof(T))) & 15) == 0;
 }
 
-// ---- packing --------------------------------------------------------------------------------------------------------
-// Largest finite magnitude of W (workgroups 0..nb-1) and of X's rows that count (nb..2nb-1), one partial each.
 template <typename T>
-__global__ void __launch_bounds__(256) vce_amax_kernel(Matrix w, Matrix x, const int64_t *labels, int64_t ignore,
-                                                       float *__restrict__ partial) {
-  const int nb = gridDim.x / 2;
-  const bool is_x = (int)blockIdx.x >= nb;
-  const Matrix m = is_x ? x : w;
-  const T *src = (const T *)m.data;
-  const int lane = threadIdx.x & 63;
-  float top = 0.f;
-  for (int64_t r = ((int64_t)(blockIdx.x % nb) * 4 + (threadIdx.x >> 6)); r < m.rows; r += (int64_t)nb * 4) {
-    if (is_x && !row_in(labels, ignore, r)) continue;
-    for (int64_t c = lane; c < m.cols; c += 64) {
-      const float v = fabsf(to_f32(src[r * m.ld_row + c * m.ld_col]));
-      if (v < INFINITY) top = fmaxf(top, v);
-    }
+__device__ __forceinline__ void load8(const Matrix &m, bool wide, int64_t row, int64_t k, float (&v)[8]) {
+  const T *src = (const T *)m.data + row * m.ld_row;
+  if (wide && k + 8 <= m.cols) {
+    Eight<T> e;
+    e.load(src + k);
+    e.get(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < m.cols ? (float)src[(k + i) * m.ld_col] : 0.f;
   }
+}
+
+struct AmaxJob {
+  Matrix m;
+  const int64_t *labels;  // rows with the ignored label do not count (NULL: all do)
+  int64_t ignore;
+  int blocks;             // workgroups, one partial each
+};
+
+__device__ __forceinline__ float block_max(float top) {
+  __shared__ float part[4];
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  __shared__ float part[4];
-  if (lane == 0) part[threadIdx.x >> 6] = top;
   __syncthreads();
-  if (threadIdx.x == 0) partial[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+  __syncthreads();
+  return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
 }
 
-__device__ __forceinline__ int top_exponent(float amax) { return amax > 0.f ? TOP_EXP - ilogbf(amax) : 0; }
-
-// Exponents from the partial maxima (float16 input: none are taken, exponent 0).
-__global__ void __launch_bounds__(256) vce_exponents_kernel(const float *__restrict__ partial, int nb, Scalars *s) {
-  __shared__ float part[2][4];
+// Largest finite magnitude of W, then of X.  A unit is eight elements of a row; units are dealt out over the workgroups.
+template <typename T>
+__global__ void __launch_bounds__(256) vce_amax_kernel(AmaxJob w, AmaxJob x, float *__restrict__ partial) {
+  const bool first = (int)blockIdx.x < w.blocks;
+  const AmaxJob &j = first ? w : x;
+  const bool wide = wide_rows<T>(j.m);
+  const int64_t per_row = (j.m.cols + 7) / 8, units = j.m.rows * per_row, step = (int64_t)j.blocks * 256;
+  float top = 0.f;
+  auto take = [&](const float (&v)[8]) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    float top = 0.f;
-    for (int i = threadIdx.x; i < nb; i += 256) top = fmaxf(top, partial[t * nb + i]);
+    for (int k = 0; k < 8; ++k) top = fabsf(v[k]) < INFINITY ? fmaxf(top, fabsf(v[k])) : top;
+  };
+  int64_t u = (int64_t)(blockIdx.x - (first ? 0 : w.blocks)) * 256 + threadIdx.x;
+  if (!j.labels && wide && j.m.ld_row == j.m.cols && (j.m.cols & 7) == 0) {
+    const T *src = (const T *)j.m.data;      // one run of memory: four units in flight
+    for (; u + 3 * step < units; u += 4 * step) {
+      Eight<T> e[4];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if ((threadIdx.x & 63) == 0) part[t][threadIdx.x >> 6] = top;
+      for (int q = 0; q < 4; ++q) e[q].load(src + (u + q * step) * 8);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[8];
+        e[q].get(v);
+        take(v);
+      }
+    }
   }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    const float *q = part[threadIdx.x];
-    const int e = nb ? top_exponent(fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]))) : 0;
-    (threadIdx.x == 0 ? s->exp_w : s->exp_x) = e;
+  for (; u < units; u += step) {
+    const int64_t row = u / per_row;
+    if (j.labels && j.labels[row] == j.ignore) continue;
+    float v[8];
+    load8<T>(j.m, wide, row, (u - row * per_row) * 8, v);
+    take(v);
   }
+  top = block_max(top);
+  if (threadIdx.x == 0) partial[blockIdx.x] = top;
 }
 
-template <int NP>
-__device__ __forceinline__ void put_block(const float (&v)[8], u4v *dst, int64_t plane) {
-  h8v hi, lo;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    hi[i] = (_Float16)v[i];
-    if (NP == 2) lo[i] = (_Float16)(v[i] - (float)hi[i]);
-  }
-  dst[0] = __builtin_bit_cast(u4v, hi);
-  if (NP == 2) dst[plane] = __builtin_bit_cast(u4v, lo);
+__device__ __forceinline__ int top_exponent(const float *partial, int n) {
+  float top = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, partial[i]);
+  top = block_max(top);
+  return top > 0.f ? TOP_EXP - ilogbf(top) : 0;
 }
 
 struct PackJob {
@@ -129,55 +170,96 @@ struct PackJob {
   int64_t ignore;
   u4v *dst;
   int64_t plane;    // 16-byte units between the head and the residual plane
-  int64_t blocks;   // 1 KB blocks of one plane
+  int64_t units;    // (32-row tile, 64 columns) pairs
   int kblocks;      // 16-wide blocks of the contraction per 32-row tile
+  int partials;     // of the largest magnitude
   float sign;
-  int is_x;
 };
 
-// Contraction over the columns: block (tile t, k step s), lane (m, h): row 32 t + m, columns 16 s + 8 h + 0..7.
+// A wavefront takes 32 rows x 64 columns: eight lanes read 128 (float32: 256) consecutive bytes of a row and store them
+// to the four blocks' places, 128 consecutive bytes for eight rows.
+// Block (tile t, k step s), lane (m, h): row 32 t + m, columns 16 s + 8 h + 0..7.
 template <typename T, int NP>
-__global__ void __launch_bounds__(256) vce_pack_kernel(PackJob a, PackJob b, int64_t groups_a, const Scalars *s) {
-  const bool first = blockIdx.x < groups_a;
-  const PackJob &j = first ? a : b;
-  const int lane = threadIdx.x & 63;
-  const int64_t blk = ((int64_t)blockIdx.x - (first ? 0 : groups_a)) * 4 + (threadIdx.x >> 6);
-  if (blk >= j.blocks) return;
-  const int64_t row = blk / j.kblocks * 32 + (lane & 31);
-  const int64_t k0 = blk % j.kblocks * 16 + 8 * (lane >> 5);
-  const int e = j.is_x ? s->exp_x : s->exp_w;
-  float v[8];
-  const bool live = row < j.m.rows && row_in(j.labels, j.ignore, row);
-  const T *src = (const T *)j.m.data + (live ? row * j.m.ld_row : 0);
+__global__ void __launch_bounds__(256) vce_pack_kernel(PackJob w, PackJob x, const float *__restrict__ partial,
+                                                       Scalars *__restrict__ s) {
+  const int ew = top_exponent(partial, w.partials), ex = top_exponent(partial + w.partials, x.partials);
+  if (blockIdx.x == 0 && threadIdx.x == 0) s->exp_w = ew, s->exp_x = ex;
+  const bool wide_w = wide_rows<T>(w.m), wide_x = wide_rows<T>(x.m);
+  const int lane = threadIdx.x & 63, piece = lane & 7;
+  for (int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); u < w.units + x.units; u += (int64_t)gridDim.x * 4) {
+    const bool first = u < w.units;
+    const PackJob &j = first ? w : x;
+    const int groups = (j.kblocks + 3) / 4, e = first ? ew : ex;
+    const int64_t v = first ? u : u - w.units, tile = v / groups;
+    const int64_t kb = (v - tile * groups) * 4 + piece / 2, k = kb * 16 + (piece & 1) * 8;
+    if (kb >= j.kblocks) continue;
+    u4v *dst = j.dst + (tile * j.kblocks + kb) * 64 + (piece & 1) * 32 + lane / 8;
+    float val[4][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    v[i] = live && k0 + i < j.m.cols ? ldexpf(to_f32(src[(k0 + i) * j.m.ld_col]), e) * j.sign : 0.f;
-  put_block<NP>(v, j.dst + blk * 64 + lane, j.plane);
+    for (int q = 0; q < 4; ++q) {
+      const int64_t row = tile * 32 + q * 8 + lane / 8;
+      const bool live = row < j.m.rows && k < j.m.cols && !(j.labels && j.labels[row] == j.ignore);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) val[q][i] = 0.f;
+      if (live) load8<T>(j.m, first ? wide_w : wide_x, row, k, val[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      h8v hi, lo;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = ldexpf(val[q][i], e) * j.sign;
+        hi[i] = (_Float16)f;
+        if (NP == 2) lo[i] = (_Float16)(f - (float)hi[i]);
+      }
+      dst[q * 8] = __builtin_bit_cast(u4v, hi);
+      if (NP == 2) dst[q * 8 + j.plane] = __builtin_bit_cast(u4v, lo);
+    }
+  }
 }
 
-// Place of slot i of lane half h in k step s of a 32-wide piece of the contraction, for operands that meet a transposed
-// or accumulator-order factor: the order in which a 32x32 accumulator tile holds its rows.
+// Place of slot i of lane half h in k step s of a 32-wide piece of the contraction, for operands that come out of (or
+// meet one that comes out of) an accumulator: the order in which a 32x32 accumulator tile holds its rows.
 __device__ __forceinline__ constexpr int slot_place(int s, int h, int i) { return 16 * s + 8 * (i >> 2) + 4 * h + (i & 3); }
 
-// Contraction over the rows: block (column tile t, k step s), lane (m, h): column 32 t + m, rows in slot order.
-template <typename T, int NP>
-__global__ void __launch_bounds__(256) vce_pack_t_kernel(PackJob a, PackJob b, int64_t groups_a, const Scalars *s) {
-  const bool first = blockIdx.x < groups_a;
-  const PackJob &j = first ? a : b;
-  const int lane = threadIdx.x & 63;
-  const int64_t blk = ((int64_t)blockIdx.x - (first ? 0 : groups_a)) * 4 + (threadIdx.x >> 6);
-  if (blk >= j.blocks) return;
-  const int64_t col = blk / j.kblocks * 32 + (lane & 31);
-  const int64_t kb = blk % j.kblocks;
-  const int e = j.is_x ? s->exp_x : s->exp_w;
-  float v[8];
+struct TransposeJob {
+  const u4v *src;     // [32-row tile][k block], contraction over the columns
+  u4v *dst;           // [32-column tile][row block], contraction over the rows, in slot order
+  int64_t plane;      // of both: they hold the same number of blocks
+  int64_t row_tiles, col_tiles;
+};
+
+// The packed copies for the contraction over rows, from those over columns: one 32x32 tile and plane per wavefront, as
+// two products with the identity.  Each value passes the matrix core as itself times one: exact.
+__global__ void __launch_bounds__(256) vce_transpose_kernel(TransposeJob w, TransposeJob x, int planes) {
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int64_t nw = w.row_tiles * w.col_tiles, nx = x.row_tiles * x.col_tiles;
+  h8v ident[2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t row = kb / 2 * 32 + slot_place((int)(kb & 1), lane >> 5, i);
-    const bool live = col < j.m.cols && row < j.m.rows && row_in(j.labels, j.ignore, row);
-    v[i] = live ? ldexpf(to_f32(((const T *)j.m.data)[row * j.m.ld_row + col * j.m.ld_col]), e) : 0.f;
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ident[s][i] = 16 * s + 8 * h + i == (lane & 31) ? (_Float16)1.f : (_Float16)0.f;
+  for (int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); u < (nw + nx) * planes; u += (int64_t)gridDim.x * 4) {
+    const int64_t pl = u / (nw + nx), v = u - pl * (nw + nx);
+    const bool first = v < nw;
+    const TransposeJob &j = first ? w : x;
+    const int64_t q = first ? v : v - nw, rt = q / j.col_tiles, ct = q - rt * j.col_tiles;
+    const u4v *src = j.src + pl * j.plane + (rt * j.col_tiles + ct) * 128 + lane;
+    f16v tr;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) tr[r] = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      tr = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, src[s * 64]), ident[s], tr, 0, 0, 0);
+    u4v *dst = j.dst + pl * j.plane + (ct * j.row_tiles + rt) * 128 + lane;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      h8v o;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k] = (_Float16)tr[8 * s + k];
+      dst[s * 64] = __builtin_bit_cast(u4v, o);
+    }
   }
-  put_block<NP>(v, j.dst + blk * 64 + lane, j.plane);
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------
@@ -451,7 +533,7 @@ __global__ void __launch_bounds__(256, 2) vce_gemm_kernel(const GemmArgs g) {
           const int d = m0 + 32 * i + 8 * q + 4 * h;
           float x[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = ldexpf(acc[i][n][4 * q + k] * g.scale, e);
+          for (int k = 0; k < 4; ++k) x[k] = ldexpf(acc[i][n][4 * q + k] * fabsf(g.scale), e);  // X's copy has its sign
           T *dst = (T *)g.out + v * g.D + d;
           if ((g.D & 3) == 0) {
             if (d < g.D) store4<T>(dst, x[0], x[1], x[2], x[3]);
@@ -465,22 +547,217 @@ __global__ void __launch_bounds__(256, 2) vce_gemm_kernel(const GemmArgs g) {
   }
 }
 
-// ---- rows -----------------------------------------------------------------------------------------------------------
+// ---- few rows -------------------------------------------------------------------------------------------------------
+// Forward alone for at most 32 NB rows: the vocabulary is read once, as it is, and nothing is packed.  16-bit operands go
+// to the matrix cores in their own type; a float32 value is cut into three bfloat16 pieces that hold all its 24 bits (by
+// truncation, so the largest values do not overflow), six products of which leave out less than 2^-21 of a product.
+// A workgroup takes 32 words at a time; its four wavefronts take the 64-wide pieces of the contraction in turn, add
+// their tiles through LDS, and each keeps the running maximum and sum over a quarter of the words.
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+
+template <typename T>
+struct Operand;  // the pieces of eight consecutive values, ready for the matrix cores
+template <>
+struct Operand<float> {
+  u4v piece[3];
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned a[3], b[3];
+      cut(v[2 * i], a), cut(v[2 * i + 1], b);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) piece[k][i] = __builtin_amdgcn_perm(b[k], a[k], 0x07060302);  // the upper halves
+    }
+  }
+  static __device__ __forceinline__ void cut(float v, unsigned (&p)[3]) {
+    p[0] = __builtin_bit_cast(unsigned, v) & 0xffff0000u;
+    v -= __builtin_bit_cast(float, p[0]);
+    p[1] = __builtin_bit_cast(unsigned, v) & 0xffff0000u;
+    p[2] = __builtin_bit_cast(unsigned, v - __builtin_bit_cast(float, p[1]));
+  }
+  static __device__ __forceinline__ f16v product(const Operand &a, const Operand &b, f16v acc) {
+#pragma unroll
+    for (int n = 2; n >= 0; --n)     // smallest first
+#pragma unroll
+      for (int k = 0; k <= n; ++k)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a.piece[k]),
+                                                      __builtin_bit_cast(b8v, b.piece[n - k]), acc, 0, 0, 0);
+    return acc;
+  }
+};
+template <>
+struct Operand<_Float16> {
+  u4v piece[1];
+  static __device__ __forceinline__ f16v product(const Operand &a, const Operand &b, f16v acc) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a.piece[0]), __builtin_bit_cast(h8v, b.piece[0]),
+                                                  acc, 0, 0, 0);
+  }
+};
+template <>
+struct Operand<__bf16> {
+  u4v piece[1];
+  static __device__ __forceinline__ f16v product(const Operand &a, const Operand &b, f16v acc) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a.piece[0]), __builtin_bit_cast(b8v, b.piece[0]),
+                                                   acc, 0, 0, 0);
+  }
+};
+
+// Elements k..k+7 of a row as they are (16 or 32 bytes).  WIDE: 16-byte accesses (wide_rows, and the row's length is a
+// multiple of eight).  Past the end of the row its last elements are read again: the other factor is zero there.
+template <typename T, bool WIDE>
+__device__ __forceinline__ Eight<T> fetch8(const Matrix &m, int64_t row, int64_t k) {
+  const T *src = (const T *)m.data + row * m.ld_row;
+  if (WIDE) {
+    Eight<T> e;
+    e.load(src + min(k, m.cols - 8));
+    return e;
+  }
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  t8 z;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = src[min(k + i, m.cols - 1) * m.ld_col];
+  return __builtin_bit_cast(Eight<T>, z);
+}
+template <typename T>
+__device__ __forceinline__ void zero_past(Eight<T> &e, int64_t left) {  // keeps the first `left` elements
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  t8 z = __builtin_bit_cast(t8, e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = i < left ? z[i] : (T)0.f;
+  e = __builtin_bit_cast(Eight<T>, z);
+}
+__device__ __forceinline__ Operand<float> operand(const Eight<float> &e) {
+  float v[8];
+  e.get(v);
+  Operand<float> o;
+  o.set(v);
+  return o;
+}
+template <typename T>
+__device__ __forceinline__ Operand<T> operand(const Eight<T> &e) {
+  return Operand<T>{{e.a}};
+}
+
 __device__ __forceinline__ void merge(float &m, float &s, float m2, float s2) {
   const float top = fmaxf(m, m2);
   s = s * __builtin_amdgcn_exp2f(m - top) + s2 * __builtin_amdgcn_exp2f(m2 - top);
   m = top;
 }
 
-// Joins a row's (max, sum) pairs: 8 rows x 32 lanes per workgroup.
-__global__ void __launch_bounds__(256) vce_join_kernel(int64_t P, int64_t V, int64_t Pp, int pairs,
-                                                       const float2 *__restrict__ partial, const float *__restrict__ target,
-                                                       const int64_t *__restrict__ labels, int64_t ignore,
-                                                       float *__restrict__ lse2, float *__restrict__ lse,
-                                                       float *__restrict__ row_loss) {
+template <typename T, int NB, bool WIDE>
+__global__ void __launch_bounds__(256, 2) vce_score_kernel(Matrix w, Matrix x, const int64_t *__restrict__ labels,
+                                                        int64_t ignore, float scale, float2 *__restrict__ partial,
+                                                        float *__restrict__ target) {
+  __shared__ float sum[4][NB][16][64];
+  __shared__ float2 join[4][NB][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const float c = scale * LOG2E;
+  int64_t label[NB], xrow[NB], xlen[NB];   // a row that does not count has length 0
+  float top[NB], tot[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int64_t p = 32 * n + (lane & 31);
+    label[n] = p < x.rows ? labels[p] : ignore;
+    xrow[n] = min(p, x.rows - 1);
+    xlen[n] = label[n] != ignore ? x.cols : 0;
+    top[n] = MAX_FLOOR, tot[n] = 0.f;
+  }
+  const int64_t tiles = (w.rows + 31) / 32;
+  const int groups = (int)((w.cols + 63) / 64);
+  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int64_t v = t * 32 + (lane & 31);
+    f16v acc[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
+    auto words = [&](int g, Eight<T> (&a)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) a[q] = fetch8<T, WIDE>(w, min(v, w.rows - 1), (int64_t)g * 64 + 16 * q + 8 * h);
+    };
+    Eight<T> a[4], next[4];
+    if (wave < groups) words(wave, a);
+    for (int g = wave; g < groups; g += 4) {
+      if (g + 4 < groups) words(g + 4, next);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const Operand<T> oa = operand(a[q]);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const int64_t k = (int64_t)g * 64 + 16 * q + 8 * h;
+          Eight<T> b = fetch8<T, WIDE>(x, xrow[n], k);
+          zero_past(b, WIDE ? (k < xlen[n] ? 8 : 0) : xlen[n] - k);
+          acc[n] = Operand<T>::product(oa, operand(b), acc[n]);
+        }
+        a[q] = next[q];
+      }
+    }
+    __syncthreads();  // the tile before has been read
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[wave][n][r][lane] = acc[n][r];
+    __syncthreads();
+    // this wavefront's registers 4 wave..4 wave + 3: words 8 wave + 4 h + 0..3 of the tile
+    const int64_t v0 = t * 32 + 8 * wave + 4 * h;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float z[4], most = MAX_FLOOR;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 4 * wave + k;
+        z[k] = ((sum[0][n][r][lane] + sum[1][n][r][lane]) + (sum[2][n][r][lane] + sum[3][n][r][lane])) * c;
+        if (label[n] == v0 + k) target[32 * n + (lane & 31)] = z[k];
+        if (v0 + k < w.rows) most = fmaxf(most, z[k]);
+      }
+      float add = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) add += v0 + k < w.rows ? __builtin_amdgcn_exp2f(z[k] - most) : 0.f;
+      merge(top[n], tot[n], most, add);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    merge(top[n], tot[n], __shfl_xor(top[n], 32), __shfl_xor(tot[n], 32));
+    if (h == 0) join[wave][n][lane] = make_float2(top[n], tot[n]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * NB; i += 256) {
+    float2 q = join[0][i / 32][i & 31];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+      const float2 o = join[k][i / 32][i & 31];
+      merge(q.x, q.y, o.x, o.y);
+    }
+    if (i < x.rows) partial[(int64_t)i * gridDim.x + blockIdx.x] = q;
+  }
+}
+
+// ---- rows -----------------------------------------------------------------------------------------------------------
+struct RowsOut {
+  int64_t P, V, ignore;
+  const int64_t *labels;
+  const float *target;
+  float *lse2, *lse, *row_loss;  // lse2 and lse may be NULL
+};
+
+__device__ __forceinline__ void finish_row(const RowsOut &o, int64_t p, float m, float s) {
+  const float l2 = m + log2f(s);
+  if (o.lse2) o.lse2[p] = p < o.P ? l2 : 0.f;
+  if (p >= o.P) return;
+  const int64_t label = o.labels[p];
+  const bool in = label != o.ignore;
+  if (o.lse) o.lse[p] = in ? l2 * LN2F : 0.f;
+  // a label outside the vocabulary has no logit: the row's loss is NaN
+  o.row_loss[p] = !in ? 0.f : label < 0 || label >= o.V ? NAN : (l2 - o.target[p]) * LN2F;
+}
+
+// Joins the (max, sum) pairs of the rows, [pair][Pp]: 8 rows x 32 lanes per workgroup.
+__global__ void __launch_bounds__(256) vce_join_kernel(RowsOut o, int64_t Pp, int pairs, const float2 *__restrict__ partial) {
   const int row = threadIdx.x & 7, lane = threadIdx.x >> 3;
   const int64_t p = (int64_t)blockIdx.x * 8 + row;
   float m = MAX_FLOOR, s = 0.f;
+#pragma unroll 4
   for (int j = lane; j < pairs; j += 32) {
     const float2 q = partial[(int64_t)j * Pp + p];
     merge(m, s, q.x, q.y);
@@ -496,15 +773,25 @@ __global__ void __launch_bounds__(256) vce_join_kernel(int64_t P, int64_t V, int
     }
     __syncthreads();
   }
-  if (lane != 0) return;
-  const float l2 = m + log2f(s);
-  lse2[p] = p < P ? l2 : 0.f;
-  if (p >= P) return;
-  const int64_t label = labels[p];
-  const bool in = label != ignore;
-  if (lse) lse[p] = in ? l2 * LN2F : 0.f;
-  // a label outside the vocabulary has no logit: the row's loss is NaN
-  row_loss[p] = !in ? 0.f : label < 0 || label >= V ? NAN : (l2 - target[p]) * LN2F;
+  if (lane == 0) finish_row(o, p, m, s);
+}
+
+// The same for [row][pair], one row per workgroup.
+__global__ void __launch_bounds__(256) vce_join_row_kernel(RowsOut o, int pairs, const float2 *__restrict__ partial) {
+  const float2 *src = partial + (int64_t)blockIdx.x * pairs;
+  float m = MAX_FLOOR, s = 0.f;
+#pragma unroll 4
+  for (int j = threadIdx.x; j < pairs; j += 256) merge(m, s, src[j].x, src[j].y);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) merge(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
+  __shared__ float2 part[4];
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  m = part[0].x, s = part[0].y;
+#pragma unroll
+  for (int k = 1; k < 4; ++k) merge(m, s, part[k].x, part[k].y);
+  finish_row(o, blockIdx.x, m, s);
 }
 
 __device__ __forceinline__ double block_sum(double v) {
@@ -530,8 +817,8 @@ __global__ void __launch_bounds__(1024) vce_reduce_kernel(int64_t P, const float
   sum = block_sum(sum);
   n = block_sum(n);
   if (threadIdx.x == 0) {
-    s->n_valid = (float)n;
-    if (loss) *loss = (float)(mean ? sum / n : sum);
+    if (s) s->n_valid = (float)n;
+    *loss = (float)(mean ? sum / n : sum);
   }
 }
 
@@ -685,18 +972,6 @@ int launch_gemm(const GemmArgs &g, hipStream_t st) {
   return check_launch("pr_vocab_ce");
 }
 
-template <typename T, int NP>
-int pack(bool transposed, const PackJob &a, const PackJob &b, const Scalars *s, hipStream_t st) {
-  const int64_t ga = (a.blocks + 3) / 4, gb = (b.blocks + 3) / 4;
-  if (ga + gb == 0) return PR_OK;
-  if (ga + gb > 0x7fffffffll) return PR_EUNSUPPORTED;
-  if (transposed)
-    hipLaunchKernelGGL((vce_pack_t_kernel<T, NP>), dim3((unsigned)(ga + gb)), dim3(256), 0, st, a, b, ga, s);
-  else
-    hipLaunchKernelGGL((vce_pack_kernel<T, NP>), dim3((unsigned)(ga + gb)), dim3(256), 0, st, a, b, ga, s);
-  return check_launch("pr_vocab_ce");
-}
-
 struct Call {
   int dtype;
   int64_t P, V, D;
@@ -716,26 +991,65 @@ template <typename T, int NP>
 int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, float *lse, float *loss, hipStream_t st) {
   const Shape s(c.dtype, c.P, c.V, c.D);
   const bool scaled = c.dtype != PR_F16;
+  auto amax_blocks = [&](const Matrix &m) {  // at least 32 units a thread
+    return scaled ? (int)std::min<int64_t>(AMAX_BLOCKS, (m.rows * ((m.cols + 7) / 8) + 8191) / 8192) : 0;
+  };
+  const AmaxJob aw{c.w, nullptr, 0, amax_blocks(c.w)}, ax{c.x, c.labels, c.ignore, amax_blocks(c.x)};
   if (scaled) {
-    hipLaunchKernelGGL((vce_amax_kernel<T>), dim3(2 * AMAX_BLOCKS), dim3(256), 0, st, c.w, c.x, c.labels, c.ignore, f.amax);
+    hipLaunchKernelGGL((vce_amax_kernel<T>), dim3(aw.blocks + ax.blocks), dim3(256), 0, st, aw, ax, f.amax);
     PR_TRY(check_launch("pr_vocab_ce"));
   }
-  hipLaunchKernelGGL(vce_exponents_kernel, dim3(1), dim3(256), 0, st, f.amax, scaled ? AMAX_BLOCKS : 0, k.scal);
-  PR_TRY(check_launch("pr_vocab_ce"));
   const int kb = (int)(s.Dk / 16);
-  const PackJob jw{c.w, nullptr, 0, k.wf, s.plane(s.Vp), s.Vp / 32 * kb, kb, 1.f, 0};
-  const PackJob jx{c.x, c.labels, c.ignore, k.xf, s.plane(s.Pp), s.Pp / 32 * kb, kb, c.scale < 0.f ? -1.f : 1.f, 1};
-  PR_TRY((pack<T, NP>(false, jw, jx, k.scal, st)));
+  const PackJob jw{c.w, nullptr, 0, k.wf, s.plane(s.Vp), s.Vp / 32 * ((kb + 3) / 4), kb, aw.blocks, 1.f};
+  const PackJob jx{c.x, c.labels, c.ignore, k.xf, s.plane(s.Pp), s.Pp / 32 * ((kb + 3) / 4), kb, ax.blocks,
+                   c.scale < 0.f ? -1.f : 1.f};
+  const int64_t pack_blocks = std::min<int64_t>(2048, (jw.units + jx.units + 3) / 4);
+  hipLaunchKernelGGL((vce_pack_kernel<T, NP>), dim3((unsigned)pack_blocks), dim3(256), 0, st, jw, jx, f.amax, k.scal);
+  PR_TRY(check_launch("pr_vocab_ce"));
   GemmArgs g{};
   g.A = k.wf, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
   g.a_tiles = (int)(s.Vp / 32), g.kblocks = g.k_split = kb, g.m_tiles = (int)(s.Vp / TILE_V), g.n_tiles = (int)(s.Pp / TILE_P), g.splits = 1;
   g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.labels = c.labels;
   g.partial = f.partial, g.target = f.target, g.Pp = s.Pp;
   PR_TRY((launch_gemm<NP, 4, STATS, T>(g, st)));
-  hipLaunchKernelGGL(vce_join_kernel, dim3((unsigned)(s.Pp / 8)), dim3(256), 0, st, c.P, c.V, s.Pp, f.pairs, f.partial,
-                     f.target, c.labels, c.ignore, k.lse2, lse, row_loss);
+  const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k.lse2, lse, row_loss};
+  hipLaunchKernelGGL(vce_join_kernel, dim3((unsigned)(s.Pp / 8)), dim3(256), 0, st, rows, s.Pp, f.pairs, f.partial);
   PR_TRY(check_launch("pr_vocab_ce"));
+  if (!loss) return PR_OK;
   hipLaunchKernelGGL(vce_reduce_kernel, dim3(1), dim3(1024), 0, st, c.P, row_loss, c.labels, c.ignore, mean, loss, k.scal);
+  return check_launch("pr_vocab_ce");
+}
+
+struct ScoreScratch {  // of the forward pass for few rows
+  float *target;
+  float2 *partial;
+  int blocks;
+  ScoreScratch(Carve &c, const Shape &s) {
+    blocks = (int)std::min<int64_t>(SCORE_BLOCKS, (s.V + 31) / 32);
+    target = c.take<float>(SCORE_ROWS);
+    partial = c.take<float2>((int64_t)blocks * SCORE_ROWS);
+  }
+};
+
+template <typename T>
+int score(const Call &c, int mean, ScoreScratch &f, float *row_loss, float *lse, float *loss, hipStream_t st) {
+  const dim3 grid(f.blocks), block(256);
+  auto aligned = [](const Matrix &m) {
+    return m.ld_col == 1 && ((uintptr_t)m.data & 15) == 0 && (m.ld_row * (int64_t)sizeof(T)) % 16 == 0 && m.cols % 8 == 0;
+  };
+  const bool wide = aligned(c.w) && aligned(c.x);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, block, 0, st, c.w, c.x, c.labels, c.ignore, c.scale, f.partial, f.target);
+  };
+  if (c.P <= 32) wide ? launch(vce_score_kernel<T, 1, true>) : launch(vce_score_kernel<T, 1, false>);
+  else wide ? launch(vce_score_kernel<T, 2, true>) : launch(vce_score_kernel<T, 2, false>);
+  PR_TRY(check_launch("pr_vocab_ce"));
+  const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, nullptr, lse, row_loss};
+  hipLaunchKernelGGL(vce_join_row_kernel, dim3((unsigned)c.P), block, 0, st, rows, f.blocks, f.partial);
+  PR_TRY(check_launch("pr_vocab_ce"));
+  if (!loss) return PR_OK;
+  hipLaunchKernelGGL(vce_reduce_kernel, dim3(1), dim3(1024), 0, st, c.P, row_loss, c.labels, c.ignore, mean, loss,
+                     (Scalars *)nullptr);
   return check_launch("pr_vocab_ce");
 }
 
@@ -747,9 +1061,11 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
                      c.ignore, k.scal, b.exp_g, b.coef_a, b.coef_b);
   PR_TRY(check_launch("pr_vocab_ce"));
   const int kb = (int)(s.Dk / 16), kv = (int)(s.Vp / 16), kp = (int)(s.Pp / 16);
-  const PackJob jw{c.w, nullptr, 0, b.wt, s.plane(s.Vp), dx ? s.Dk / 32 * kv : 0, kv, 1.f, 0};
-  const PackJob jx{c.x, c.labels, c.ignore, b.xt, s.plane(s.Pp), dw ? s.Dk / 32 * kp : 0, kp, 1.f, 1};
-  PR_TRY((pack<T, NP>(true, jw, jx, k.scal, st)));
+  const TransposeJob tw{k.wf, b.wt, s.plane(s.Vp), dx ? s.Vp / 32 : 0, s.Dk / 32};
+  const TransposeJob tx{k.xf, b.xt, s.plane(s.Pp), dw ? s.Pp / 32 : 0, s.Dk / 32};
+  const int64_t turns = ((tw.row_tiles + tx.row_tiles) * (s.Dk / 32) * NP + 3) / 4;
+  hipLaunchKernelGGL(vce_transpose_kernel, dim3((unsigned)std::min<int64_t>(4096, turns)), dim3(256), 0, st, tw, tx, NP);
+  PR_TRY(check_launch("pr_vocab_ce"));
   // 256 features per workgroup unless 128 leave fewer of them unused
   const bool narrow = round_up(s.Dk, 128) * 8 < round_up(s.Dk, 256) * 7;
   const int d_tiles = (int)(narrow ? round_up(s.Dk, 128) / 128 : round_up(s.Dk, 256) / 256);
@@ -807,11 +1123,15 @@ extern "C" size_t pr_vocab_ce_kept_bytes(int dtype, int64_t P, int64_t V, int64_
   return c.used;
 }
 
+extern "C" int pr_vocab_ce_score_rows(void) { return pr::SCORE_ROWS; }
+
 extern "C" size_t pr_vocab_ce_fwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D) {
   if (!pr::valid_shape(dtype, P, V, D)) return 0;
-  pr::Carve c(nullptr);
-  pr::FwdScratch f(c, pr::Shape(dtype, P, V, D));
-  return c.used;
+  const pr::Shape s(dtype, P, V, D);
+  pr::Carve packed(nullptr), plain(nullptr);
+  pr::FwdScratch f(packed, s);
+  pr::ScoreScratch g(plain, s);
+  return P <= pr::SCORE_ROWS ? std::max(packed.used, plain.used) : packed.used;
 }
 
 extern "C" size_t pr_vocab_ce_bwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D, int want_dx, int want_dw) {
@@ -827,15 +1147,22 @@ extern "C" int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const
                                float *row_loss, float *lse, float *loss, void *stream) {
   const pr::Call c{dtype, P, V, D, {x, P, D, ldx_row, ldx_col}, {w, V, D, ldw_row, ldw_col}, labels, ignore_index, scale};
   PR_TRY(pr::check_call(c));
-  if (!kept || !scratch || !row_loss || ((uintptr_t)kept & 15) || ((uintptr_t)scratch & 15)) return PR_EINVAL;
-  if (kept_bytes < pr_vocab_ce_kept_bytes(dtype, P, V, D) ||
+  if ((!kept && P > pr::SCORE_ROWS) || !scratch || !row_loss || ((uintptr_t)kept & 15) || ((uintptr_t)scratch & 15))
+    return PR_EINVAL;
+  if ((kept && kept_bytes < pr_vocab_ce_kept_bytes(dtype, P, V, D)) ||
       scratch_bytes < pr_vocab_ce_fwd_scratch_bytes(dtype, P, V, D))
     return PR_ESCRATCH;
   const pr::Shape s(dtype, P, V, D);
+  hipStream_t st = (hipStream_t)stream;
   pr::Carve ck(kept), cs(scratch);
+  if (!kept) {
+    pr::ScoreScratch f(cs, s);
+    if (dtype == PR_F32) return pr::score<float>(c, mean, f, row_loss, lse, loss, st);
+    if (dtype == PR_F16) return pr::score<_Float16>(c, mean, f, row_loss, lse, loss, st);
+    return pr::score<__bf16>(c, mean, f, row_loss, lse, loss, st);
+  }
   pr::Kept k(ck, s);
   pr::FwdScratch f(cs, s);
-  hipStream_t st = (hipStream_t)stream;
   if (dtype == PR_F32) return pr::forward<float, 2>(c, mean, k, f, row_loss, lse, loss, st);
   if (dtype == PR_F16) return pr::forward<_Float16, 1>(c, mean, k, f, row_loss, lse, loss, st);
   return pr::forward<__bf16, 1>(c, mean, k, f, row_loss, lse, loss, st);

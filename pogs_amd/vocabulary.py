@@ -33,7 +33,7 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
     """``x [P, D]``, ``w [V, D]``, ``labels [P]`` int64 -> (loss, lse): loss ``[P]`` or 0-d, lse ``[P]``."""
 
     @staticmethod
-    def forward(ctx, x, w, labels, scale, ignore_index, reduction):
+    def forward(ctx, x, w, labels, scale, ignore_index, reduction, with_grad):
         ctx.set_materialize_grads(False)
         ctx.args = scale, ignore_index, reduction
         (P, D), V, dev = x.shape, w.shape[0], x.device
@@ -43,14 +43,16 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
             ctx.save_for_backward(x, w, labels, None)
             total = {"none": row_loss, "sum": row_loss.new_zeros(()), "mean": row_loss.new_full((), math.nan)}
             return total[reduction], lse
-        loss = torch.empty((), dtype=torch.float32, device=dev)
+        loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
         lib, t = _lib.load(), _TYPES[x.dtype]
         with torch.cuda.device(dev):
-            kept = _scratch(lib.pr_vocab_ce_kept_bytes(t, P, V, D), dev)
+            # few rows and no gradient to come: nothing is packed and nothing kept
+            plain = not with_grad and P <= lib.pr_vocab_ce_score_rows()
+            kept = _scratch(0 if plain else lib.pr_vocab_ce_kept_bytes(t, P, V, D), dev)
             scratch = _scratch(lib.pr_vocab_ce_fwd_scratch_bytes(t, P, V, D), dev)
             _call("pr_vocab_ce_fwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index,
-                  scale, int(reduction == "mean"), _ptr(kept), kept.numel(), _ptr(scratch), scratch.numel(),
-                  _ptr(row_loss), _ptr(lse), _ptr(loss), _stream())
+                  scale, int(reduction == "mean"), None if plain else _ptr(kept), kept.numel(), _ptr(scratch),
+                  scratch.numel(), _ptr(row_loss), _ptr(lse), _ptr(loss), _stream())
         ctx.save_for_backward(x, w, labels, kept)
         return (row_loss if reduction == "none" else loss), lse
 
@@ -62,7 +64,7 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
         (P, D), V, dev = x.shape, w.shape[0], x.device
         want_x, want_w = ctx.needs_input_grad[:2]
         if P == 0 or (g_loss is None and g_lse is None):
-            return (torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None) + (None,) * 4
+            return (torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None) + (None,) * 5
         g_loss = None if g_loss is None else g_loss.float().contiguous()
         g_lse = None if g_lse is None else g_lse.float().contiguous()
         dx = torch.empty(P, D, dtype=x.dtype, device=dev) if want_x else None
@@ -73,7 +75,7 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
             _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index,
                   scale, int(reduction == "mean"), int(reduction == "none"), _ptr(kept), kept.numel(), _ptr(g_loss),
                   _ptr(g_lse), _ptr(scratch), scratch.numel(), _ptr(dx), _ptr(dw), _stream())
-        return dx, dw, None, None, None, None
+        return (dx, dw) + (None,) * 5
 
 
 _STREAM_KEY = "pogs_amd.stream"
@@ -139,7 +141,8 @@ def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tenso
     D = features.shape[-1]
     x = features.reshape(-1, D)
     flat = labels.reshape(-1).to(torch.int64).contiguous()
-    loss, lse = _VocabularyCrossEntropy.apply(x, vocabulary, flat, scale, int(ignore_index), reduction)
+    with_grad = torch.is_grad_enabled() and (x.requires_grad or vocabulary.requires_grad)
+    loss, lse = _VocabularyCrossEntropy.apply(x, vocabulary, flat, scale, int(ignore_index), reduction, with_grad)
     del nodes
     if reduction == "none":
         loss = loss.reshape(labels.shape)

@@ -24,10 +24,11 @@ HALF = {torch.float32: U, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 IGN = -100
 
 
-def reference(x, w, labels, scale, g_loss, g_lse, ignore=IGN, dtype=None):
+def reference(x, w, labels, scale, g_loss, g_lse, ignore=IGN, dtype=None, n3=None):
     """Values and bounds in float64; g_loss, g_lse: [P] gradients of the row losses and of the log-sums."""
     dtype = dtype or x.dtype
-    n3, rho = (3, 3 * 2.0 ** -22) if NP[dtype] == 2 else (1, 0.0)
+    n3 = n3 or (3 if NP[dtype] == 2 else 1)
+    rho = 3 * 2.0 ** -22 if NP[dtype] == 2 else 0.0
     P, D = x.shape
     V = w.shape[0]
     keep = labels != ignore
@@ -141,9 +142,11 @@ def test_entry_points_validate_without_a_gpu():
                                    None, None)
 
     for kw in (dict(dtype=3), dict(P=0), dict(V=0), dict(D=0), dict(x=None), dict(w=None), dict(labels=None), dict(x=odd),
-               dict(labels=odd), dict(ld=(-1, 1)), dict(scale=math.nan), dict(scale=math.inf), dict(kept=None),
-               dict(scratch=None), dict(row=None), dict(kept=odd), dict(scratch=odd)):
+               dict(labels=odd), dict(ld=(-1, 1)), dict(scale=math.nan), dict(scale=math.inf), dict(kept=None, P=0),
+               dict(scratch=None), dict(row=None), dict(kept=odd), dict(scratch=odd),
+               dict(kept=None, P=lib.pr_vocab_ce_score_rows() + 1), dict(kept=None, scratch=None)):
         assert fwd(**kw) == -1, kw
+    assert fwd(kept=None, sb=16) == -3
     assert fwd(kb=16) == -3 and fwd(sb=16) == -3
 
     def bwd(dx=ok, dw=ok, kept=ok, kb=1 << 30, scratch=ok, sb=1 << 30, P=4):
@@ -284,10 +287,13 @@ def test_labels_outside_the_vocabulary():
     from pogs_amd.vocabulary import vocabulary_cross_entropy
 
     x, w, y = inputs(60, 100, 24, torch.float32, seed=3)
-    good = vocabulary_cross_entropy(x, w, y, reduction="none")
+    plain = vocabulary_cross_entropy(x, w, y, reduction="none")        # few rows without gradients: kernels of their own
+    good = vocabulary_cross_entropy(x.clone().requires_grad_(True), w, y, reduction="none")
     for bad in (100, -1, 1 << 40, -(1 << 40), 256, 127):
         lab = y.clone()
         lab[17] = bad
+        loss = vocabulary_cross_entropy(x, w, lab, reduction="none")
+        assert math.isnan(loss[17].item()) and torch.equal(loss[:17], plain[:17]) and torch.equal(loss[18:], plain[18:])
         xr = x.clone().requires_grad_(True)
         loss = vocabulary_cross_entropy(xr, w, lab, reduction="none")
         assert math.isnan(loss[17].item())
@@ -337,6 +343,37 @@ def test_large_logits_and_mixed_row_sizes():
     x = x * torch.logspace(-6, 3, 64, device="cuda")[:, None]
     check(x, w, y, reduction="none")
     check(x, w, y, reduction="sum")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("P,V,D", [(1, 1, 1), (1, 33, 64), (1, 40_000, 512), (5, 31, 7), (31, 257, 65), (32, 1000, 130),
+                                   (33, 999, 256), (63, 64, 1030), (64, 5000, 100), (65, 300, 72), (24, 33_000, 96)])
+def test_scoring_without_gradients(P, V, D, dtype):
+    """Few rows and no gradient to come: the vocabulary is read as it is.  float32 values are cut into three pieces of
+    eight bits by truncation; the products left out are below 2 * 2^-7 * 2^-15 + 2^-30 of their product (inside rho), and
+    six passes are added (n3)."""
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    x, w, y = inputs(P, V, D, dtype, seed=P + V, ignored=0.2 if P > 4 else 0.0)
+    z = torch.zeros(P, device="cuda", dtype=torch.float64)
+    wide = torch.full((P, D + 24), float("nan"), dtype=dtype, device="cuda")
+    for scale, layout in ((1.0, 0), (-7.0, 1), (30.0, 2)):
+        xs, ws = x, w
+        if layout == 1:
+            xs, ws = wide[:, 8:D + 8].copy_(x), w.t().contiguous().t()
+        elif layout == 2:
+            xs, ws = wide[:, 3:D + 3].copy_(x), torch.cat([w, w], 1)[:, :D]
+        ref = reference(x, w, y, scale, z, z, n3=6 if dtype == torch.float32 else 1)
+        with torch.no_grad():
+            loss, lse = vocabulary_cross_entropy(xs, ws.requires_grad_(layout == 0), y, scale, reduction="none", return_lse=True)
+            total = vocabulary_cross_entropy(xs, ws, y, scale, reduction="sum")
+        w.requires_grad_(False)
+        close(loss, ref["loss"], "loss")
+        close(lse, ref["lse"], "lse")
+        close(total, (ref["loss"][0].sum(), ref["loss"][1].sum() + 2 * U * ref["loss"][0].sum().abs()), "sum")
+        again = vocabulary_cross_entropy(xs, ws, y, scale, reduction="none")
+        assert torch.equal(again, loss)
 
 
 @pytest.mark.gpu
