@@ -269,7 +269,7 @@ struct GemmArgs {
   const u4v *A, *B;            // operand blocks, already at the first block of the contraction
   int64_t plane_a, plane_b;    // 16-byte units between planes
   int64_t ld_a, ld_b;          // blocks per 32-row tile
-  int a_tiles;                 // 32-row tiles A has (tiles past them repeat the last one; their results are not used)
+  int a_tiles, b_tiles;        // 32-row tiles A and B have (tiles past them repeat the last one; results are not used)
   int kblocks, k_split;        // blocks of the contraction, and of each split of it (the last one may have fewer)
   int m_tiles, n_tiles, splits;
   const Scalars *scal;
@@ -303,17 +303,21 @@ __device__ __forceinline__ void store4(T *dst, float a, float b, float c, float 
   *reinterpret_cast<t4 *>(dst) = t4{(T)a, (T)b, (T)c, (T)d};
 }
 
-// Workgroup of four wavefronts, 64 MT x 128 of the product: wavefront (wm, wn) holds MT x 2 accumulator tiles.  Three
-// LDS stages of 16 (two planes) or 32 (one plane) of the contraction, filled by direct loads two stages ahead; one
-// barrier a stage.
-template <int NP, int MT, int MODE, typename T>
-__global__ void __launch_bounds__(256, 2) vce_gemm_kernel(const GemmArgs g) {
+// WM x WN wavefronts of MT x NT accumulator tiles each: 32 WM MT rows of A by 32 WN NT rows of B.  LDS holds three stages
+// of 16 (two planes) or 32 (one plane) of the contraction, filled by direct loads two or three stages ahead.
+// Four wavefronts (two workgroups share a CU, one does its epilogue while the other multiplies): a stage has two halves,
+// and while the matrix cores work on one the next comes from LDS.
+// Eight wavefronts (one workgroup to a CU, half the loads per product): two groups of four, one wavefront of each on every
+// SIMD, take turns between barriers, one reading its next stage while the other multiplies.
+template <int NP, int WM, int WN, int MT, int NT, int MODE, typename T>
+__global__ void __launch_bounds__(WM *WN * 64, 2) vce_gemm_kernel(const GemmArgs g) {
   extern __shared__ u4v lds[];
-  constexpr int KB = NP == 1 ? 2 : 1;
-  constexpr int A_BLOCKS = 2 * MT * KB * NP, B_BLOCKS = 4 * KB * NP, STAGE = A_BLOCKS + B_BLOCKS, LOADS = STAGE / 4;
-  static_assert(STAGE % 4 == 0, "every wavefront fills the same share of a stage");
+  constexpr int WAVES = WM * WN, KB = NP == 1 ? 2 : 1;
+  constexpr int A_TILES = WM * MT, B_TILES = WN * NT;
+  constexpr int STAGE = (A_TILES + B_TILES) * 2, LOADS = STAGE / WAVES;
+  static_assert((WAVES == 4 || WAVES == 8) && STAGE % WAVES == 0, "every wavefront fills the same share of a stage");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / WN, wn = wave % WN;
 
   // Workgroups go to the eight XCDs in turn: each XCD takes a run of consecutive tiles, ordered as bands of eight
   // M tiles walked along N, so that its L2 holds the operands of the tiles it works on together.
@@ -327,82 +331,144 @@ __global__ void __launch_bounds__(256, 2) vce_gemm_kernel(const GemmArgs g) {
   const unsigned band_m = min(8u, (unsigned)g.m_tiles - band * 8u);
   const int m_tile = (int)(band * 8u + in_band % band_m), n_tile = (int)(in_band / band_m);
 
-  // this wavefront's LOADS blocks of a stage
+  // this wavefront's LOADS blocks of a stage, ordered [half: k block or plane][tile] for A, then for B
   const u4v *src[LOADS];
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) {
     const int j = wave * LOADS + l;
-    const bool is_a = j < A_BLOCKS;
-    const int q = is_a ? j : j - A_BLOCKS;
-    const int per = is_a ? 2 * MT : 4;      // tiles of the operand; blocks are ordered [plane][k block][tile]
-    const int tile = q % per, kb = q / per % KB, plane = q / per / KB;
-    const int64_t row = is_a ? min(m_tile * 2 * MT + tile, g.a_tiles - 1) : (int64_t)n_tile * 4 + tile;
+    const bool is_a = j < 2 * A_TILES;
+    const int q = is_a ? j : j - 2 * A_TILES, per = is_a ? A_TILES : B_TILES;
+    const int tile = q % per, half = q / per;
+    const int kb = NP == 1 ? half : 0, plane = NP == 1 ? 0 : half;
+    const int64_t row = is_a ? min(m_tile * A_TILES + tile, g.a_tiles - 1) : min(n_tile * B_TILES + tile, g.b_tiles - 1);
     const u4v *base = is_a ? g.A + plane * g.plane_a + row * g.ld_a * 64 : g.B + plane * g.plane_b + row * g.ld_b * 64;
-    src[l] = base + ((int64_t)split * g.k_split + kb) * 64 + lane;
+    src[l] = base + ((int64_t)split * g.k_split + kb) * 64;
   }
   const int stages = min(g.k_split, g.kblocks - (int)split * g.k_split) / KB;
   auto fill = [&](int buf) {
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) {
-      __builtin_amdgcn_global_load_lds((global_ptr)src[l], (lds_ptr)(lds + (buf * STAGE + wave * LOADS + l) * 64), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_ptr)(src[l] + lane), (lds_ptr)(lds + (buf * STAGE + wave * LOADS + l) * 64), 16, 0,
+                                       0);
       src[l] += KB * 64;
     }
   };
-  f16v acc[MT][2];
+  f16v acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][n][r] = 0.f;
 
-  fill(0);
-  if (stages > 1) fill(1);
-  int buf = 0;
-  for (int st = 0; st < stages; ++st) {
-    // this wavefront's loads of the stage have arrived (the next stage's LOADS may be in flight) and its reads of the
-    // stage before are done; after the barrier both hold for all four
-    if (st + 1 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+  struct Half {  // one k block, or one plane, of a stage
+    h8v a[MT], b[NT];
+  };
+  auto read = [&](int buf, int half, Half &f) {
+    const u4v *sa = lds + (buf * STAGE + half * A_TILES + wm * MT) * 64 + lane;
+    const u4v *sb = lds + (buf * STAGE + 2 * A_TILES + half * B_TILES + wn * NT) * 64 + lane;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) f.b[n] = __builtin_bit_cast(h8v, sb[n * 64]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) f.a[i] = __builtin_bit_cast(h8v, sa[i * 64]);
+  };
+  auto multiply = [&](const Half &fa, const Half &fb) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa.a[i], fb.b[n], acc[i][n], 0, 0, 0);
+  };
+  // the second half's products; for two planes the mixed ones (residual times residual is left out)
+  auto multiply_second = [&](const Half &first, const Half &second) {
+    if (NP == 1) {
+      multiply(second, second);
+    } else {
+      multiply(second, first);
+      multiply(first, second);
+    }
+  };
+  // Waits for all but the youngest `n` fills of this wavefront and for its own LDS reads; after the barrier both hold for
+  // all wavefronts.
+  auto arrive = [&](int n) {
+    if (n == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
+    else if (n == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (st + 2 < stages) fill(buf == 0 ? 2 : buf - 1);
-    const u4v *sa = lds + buf * STAGE * 64 + (wm * MT) * 64 + lane;
-    const u4v *sb = lds + (buf * STAGE + A_BLOCKS + wn * 2) * 64 + lane;
+  };
+  int buf = 0;
+  if (WAVES == 4) {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      h8v a[NP][MT], b[NP][2];
-#pragma unroll
-      for (int pl = 0; pl < NP; ++pl) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) b[pl][n] = __builtin_bit_cast(h8v, sb[((pl * KB + kb) * 4 + n) * 64]);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) a[pl][i] = __builtin_bit_cast(h8v, sa[((pl * KB + kb) * 2 * MT + i) * 64]);
+    for (int st = 0; st < 3; ++st)
+      if (st < stages) fill(st);
+    arrive(stages > 2 ? 2 : stages > 1 ? 1 : 0);
+    Half first, second;
+    read(0, 0, first);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    for (int st = 0; st < stages; ++st) {
+      const int next = buf == 2 ? 0 : buf + 1;
+      read(buf, 1, second);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      multiply(first, first);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      Half ahead = first;
+      if (st + 1 < stages) {
+        arrive(st + 2 < stages ? 1 : 0);
+        if (st + 3 < stages) fill(buf);       // every wavefront has read this stage
+        read(next, 0, ahead);
       }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][n], acc[i][n], 0, 0, 0);
-          if (NP == 2) {
-            acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[NP - 1][i], b[0][n], acc[i][n], 0, 0, 0);
-            acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[NP - 1][n], acc[i][n], 0, 0, 0);
-          }
-        }
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      multiply_second(first, second);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      // lgkmcnt(0): the next half has come while the matrix cores were fed.  As an instruction that the compiler knows,
+      // or it would wait in front of the next products for the reads issued just before them
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      first = ahead;
+      buf = next;
     }
-    buf = buf == 2 ? 0 : buf + 1;
+  } else {
+    fill(0);
+    if (stages > 1) fill(1);
+    arrive(stages > 1 ? 1 : 0);
+    const bool late = wave >= WAVES / 2;
+    if (late) __builtin_amdgcn_s_barrier();    // the second group is one barrier behind
+    for (int st = 0; st < stages; ++st) {
+      Half first, second;
+      read(buf, 0, first);
+      read(buf, 1, second);
+      // the stage before this one: this group has read it two barriers ago, the other one barrier ago
+      if (st + 2 < stages) fill(buf == 0 ? 2 : buf - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      // the stage after this one: this group reads it two barriers from now, and the other group's loads of it are waited
+      // for one barrier from now
+      arrive(st + 2 < stages ? 1 : 0);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      multiply(first, first);
+      multiply_second(first, second);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      buf = buf == 2 ? 0 : buf + 1;
+    }
+    if (!late) __builtin_amdgcn_s_barrier();
   }
 
   const int h = lane >> 5;
-  const int m0 = m_tile * 64 * MT + wm * 32 * MT;                      // first row of A of this wavefront
-  const int64_t n0 = (int64_t)n_tile * 128 + wn * 64 + (lane & 31);    // this lane's row of B, tile 0
+  const int m0 = (m_tile * WM + wm) * 32 * MT;                                     // first row of A of this wavefront
+  const int64_t n0 = ((int64_t)n_tile * WN + wn) * 32 * NT + (lane & 31);          // this lane's row of B, tile 0
   // accumulator register r of tile (i, n): row m0 + 32 i + (r & 3) + 8 (r >> 2) + 4 h of A, row n0 + 32 n of B
 
   if (MODE == STATS || MODE == GRAD) {
     const float c = ldexpf(fabsf(g.scale) * LOG2E, -(g.scal->exp_x + g.scal->exp_w));
     const int64_t left = g.V - (g.v0 + m0);      // words of this wavefront that exist
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < NT; ++n) {
       const int64_t p = n0 + 32 * n;
       const int64_t label = p < g.P ? g.labels[p] : -1;
       const int64_t rel = label - (g.v0 + m0);
@@ -446,7 +512,7 @@ __global__ void __launch_bounds__(256, 2) vce_gemm_kernel(const GemmArgs g) {
                          ? 0.f : __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -top));
         }
         sum += __shfl_xor(sum, 32);
-        if (h == 0) g.partial[(int64_t)(m_tile * 2 + wm) * g.Pp + p] = make_float2(top, sum);
+        if (h == 0) g.partial[(int64_t)(m_tile * WM + wm) * g.Pp + p] = make_float2(top, sum);
       } else {
         const float l2 = g.lse2[p], ca = g.coef_a[p], cb = g.coef_b[p];
         h8v ident[2];
@@ -476,7 +542,7 @@ __global__ void __launch_bounds__(256, 2) vce_gemm_kernel(const GemmArgs g) {
               f[0][s][k] = (_Float16)v[8 * s + k];
               if (NP == 2) f[NP - 1][s][k] = (_Float16)(v[8 * s + k] - (float)f[0][s][k]);
             }
-          const int64_t pt = (int64_t)n_tile * 4 + wn * 2 + n, vt = m0 / 32 + i;
+          const int64_t pt = ((int64_t)n_tile * WN + wn) * NT + n, vt = m0 / 32 + i;
 #pragma unroll
           for (int pl = 0; pl < NP; ++pl) {
             if (g.gx) {
@@ -505,7 +571,8 @@ __global__ void __launch_bounds__(256, 2) vce_gemm_kernel(const GemmArgs g) {
     }
   } else if (MODE == DX) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n) {
+      if (n0 + 32 * n >= g.Pp) continue;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -520,10 +587,11 @@ __global__ void __launch_bounds__(256, 2) vce_gemm_kernel(const GemmArgs g) {
           }
           *dst = v;
         }
+    }
   } else {
     const int e = -(*g.exp_g + g.scal->exp_x);
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < NT; ++n) {
       const int64_t v = g.v0 + n0 + 32 * n;
       if (v >= g.V) continue;
 #pragma unroll
@@ -920,7 +988,7 @@ struct FwdScratch {
   float2 *partial;
   int pairs;
   FwdScratch(Carve &c, const Shape &s) {
-    pairs = (int)(s.Vp / TILE_V * 2);
+    pairs = (int)(s.Vp / 128);   // a wavefront's words
     amax = c.take<float>(2 * AMAX_BLOCKS);
     target = c.take<float>(s.Pp);
     partial = c.take<float2>((int64_t)pairs * s.Pp);
@@ -940,11 +1008,17 @@ struct BwdScratch {
     piece = std::min(s.Vp, std::max<int64_t>(PIECE_BYTES / per_word / TILE_V, 1) * TILE_V);
     const int64_t pieces = (s.Vp + piece - 1) / piece;
     piece = round_up((s.Vp + pieces - 1) / pieces, TILE_V);   // of equal size
-    // enough workgroups for every CU to hold two, at least 16 stages each
-    const int64_t tiles = std::max<int64_t>(1, (s.Dk + 255) / 256 * (s.Pp / TILE_P));
-    const int64_t want = std::min<int64_t>(16, std::max<int64_t>(1, 512 / tiles));
+    // splits of the words' contraction: the number up to 16 that leaves the fewest of the 256 CUs without work, at least
+    // 16 stages each
+    const int64_t tiles = round_up(s.Dk, 256) / 256 * ((s.Pp + 255) / 256);
     const int64_t k = piece / 16;
-    kper = (int)round_up((k + want - 1) / want, 32);
+    int want = 1;
+    double best = 0.;
+    for (int n = 1; n <= 16 && k / n >= 32; ++n) {
+      const double used = (double)(tiles * n) / (double)round_up(tiles * n, 256);
+      if (used > best + 0.02) best = used, want = n;
+    }
+    kper = (int)round_up((k + want - 1) / want, 2);
     splits = (int)((k + kper - 1) / kper);
     exp_g = c.take<int>(1);
     coef_a = c.take<float>(s.Pp);
@@ -957,19 +1031,29 @@ struct BwdScratch {
   }
 };
 
-template <int NP, int MT, int MODE, typename T>
-int launch_gemm(const GemmArgs &g, hipStream_t st) {
-  constexpr int KB = NP == 1 ? 2 : 1;
-  const size_t bytes = (size_t)3 * (2 * MT + 4) * KB * NP * 1024;
+template <int NP, int WM, int WN, int MT, int NT, int MODE, typename T>
+int launch_tiles(GemmArgs g, int64_t m_rows, int64_t n_rows, hipStream_t st) {
+  const size_t bytes = (size_t)3 * (WM * MT + WN * NT) * 2 * 1024;
+  g.m_tiles = (int)((m_rows + WM * MT * 32 - 1) / (WM * MT * 32));
+  g.n_tiles = (int)((n_rows + WN * NT * 32 - 1) / (WN * NT * 32));
+  g.a_tiles = (int)(m_rows / 32), g.b_tiles = (int)(n_rows / 32);
   const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles * g.splits;
   if (tiles > (1ll << 30)) {
     set_error_text("pr_vocab_ce: too many tiles for one launch");
     return PR_EUNSUPPORTED;
   }
-  PR_HIP(hipFuncSetAttribute((const void *)vce_gemm_kernel<NP, MT, MODE, T>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)bytes));
-  hipLaunchKernelGGL((vce_gemm_kernel<NP, MT, MODE, T>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), bytes, st, g);
+  const auto kernel = vce_gemm_kernel<NP, WM, WN, MT, NT, MODE, T>;
+  PR_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(WM * WN * 64), bytes, st, g);
   return check_launch("pr_vocab_ce");
+}
+
+// Products whose M rows are features: 256 of them per workgroup unless 128 leave fewer unused.
+bool narrow_features(int64_t Dk) { return round_up(Dk, 128) * 8 < round_up(Dk, 256) * 7; }
+template <int NP, int MODE, typename T>
+int launch_features(const GemmArgs &g, int64_t Dk, int64_t n_rows, hipStream_t st) {
+  return narrow_features(Dk) ? launch_tiles<NP, 2, 4, 2, 2, MODE, T>(g, Dk, n_rows, st)
+                             : launch_tiles<NP, 2, 4, 4, 2, MODE, T>(g, Dk, n_rows, st);
 }
 
 struct Call {
@@ -1008,10 +1092,10 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
   PR_TRY(check_launch("pr_vocab_ce"));
   GemmArgs g{};
   g.A = k.wf, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
-  g.a_tiles = (int)(s.Vp / 32), g.kblocks = g.k_split = kb, g.m_tiles = (int)(s.Vp / TILE_V), g.n_tiles = (int)(s.Pp / TILE_P), g.splits = 1;
+  g.kblocks = g.k_split = kb, g.splits = 1;
   g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.labels = c.labels;
   g.partial = f.partial, g.target = f.target, g.Pp = s.Pp;
-  PR_TRY((launch_gemm<NP, 4, STATS, T>(g, st)));
+  PR_TRY((launch_tiles<NP, 2, 2, 4, 2, STATS, T>(g, s.Vp, s.Pp, st)));
   const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k.lse2, lse, row_loss};
   hipLaunchKernelGGL(vce_join_kernel, dim3((unsigned)(s.Pp / 8)), dim3(256), 0, st, rows, s.Pp, f.pairs, f.partial);
   PR_TRY(check_launch("pr_vocab_ce"));
@@ -1066,34 +1150,29 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
   const int64_t turns = ((tw.row_tiles + tx.row_tiles) * (s.Dk / 32) * NP + 3) / 4;
   hipLaunchKernelGGL(vce_transpose_kernel, dim3((unsigned)std::min<int64_t>(4096, turns)), dim3(256), 0, st, tw, tx, NP);
   PR_TRY(check_launch("pr_vocab_ce"));
-  // 256 features per workgroup unless 128 leave fewer of them unused
-  const bool narrow = round_up(s.Dk, 128) * 8 < round_up(s.Dk, 256) * 7;
-  const int d_tiles = (int)(narrow ? round_up(s.Dk, 128) / 128 : round_up(s.Dk, 256) / 256);
   for (int64_t v0 = 0; v0 < s.Vp; v0 += b.piece) {
     const int64_t words = std::min(b.piece, s.Vp - v0);
     GemmArgs g{};
     g.A = k.wf + v0 / 32 * kb * 64, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
-    g.a_tiles = (int)(words / 32), g.kblocks = g.k_split = kb, g.m_tiles = (int)(words / TILE_V), g.n_tiles = (int)(s.Pp / TILE_P);
-    g.splits = 1, g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.v0 = v0, g.labels = c.labels, g.Pp = s.Pp;
+    g.kblocks = g.k_split = kb, g.splits = 1, g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.v0 = v0, g.labels = c.labels, g.Pp = s.Pp;
     g.lse2 = k.lse2, g.coef_a = b.coef_a, g.coef_b = b.coef_b;
     g.gx = dx ? b.gx : nullptr, g.gw = dw ? b.gw : nullptr;
     g.plane_gx = g.plane_gw = s.Pp * b.piece / 8, g.ld_gx = b.piece / 16, g.ld_gw = kp;
-    PR_TRY((launch_gemm<NP, 4, GRAD, T>(g, st)));
+    PR_TRY((launch_tiles<NP, 2, 2, 4, 2, GRAD, T>(g, words, s.Pp, st)));
     if (dx) {
       GemmArgs x{};
       x.A = b.wt + v0 / 16 * 64, x.B = b.gx, x.plane_a = s.plane(s.Vp), x.plane_b = g.plane_gx, x.ld_a = kv, x.ld_b = g.ld_gx;
-      x.a_tiles = (int)(s.Dk / 32), x.m_tiles = d_tiles, x.n_tiles = (int)(s.Pp / TILE_P), x.scal = k.scal;
-      x.acc = b.acc, x.Pp = s.Pp, x.ld_acc = s.Dk, x.add = v0 > 0;
+      x.scal = k.scal, x.acc = b.acc, x.Pp = s.Pp, x.ld_acc = s.Dk, x.add = v0 > 0;
       // the splits of a full piece; a shorter last piece leaves the rest of them as they are
       x.kblocks = (int)(words / 16), x.k_split = b.kper, x.splits = (x.kblocks + b.kper - 1) / b.kper;
-      PR_TRY(narrow ? (launch_gemm<NP, 2, DX, T>(x, st)) : (launch_gemm<NP, 4, DX, T>(x, st)));
+      PR_TRY((launch_features<NP, DX, T>(x, s.Dk, s.Pp, st)));
     }
     if (dw) {
       GemmArgs w{};
       w.A = b.xt, w.B = b.gw, w.plane_a = s.plane(s.Pp), w.plane_b = g.plane_gw, w.ld_a = w.ld_b = kp;
-      w.a_tiles = (int)(s.Dk / 32), w.kblocks = w.k_split = kp, w.m_tiles = d_tiles, w.n_tiles = (int)(words / 128), w.splits = 1;
+      w.kblocks = w.k_split = kp, w.splits = 1;
       w.scal = k.scal, w.exp_g = b.exp_g, w.scale = c.scale, w.V = c.V, w.v0 = v0, w.out = dw, w.D = c.D;
-      PR_TRY(narrow ? (launch_gemm<NP, 2, DW, T>(w, st)) : (launch_gemm<NP, 4, DW, T>(w, st)));
+      PR_TRY((launch_features<NP, DW, T>(w, s.Dk, words, st)));
     }
   }
   if (dx && c.P > 0) {
