@@ -28,6 +28,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.h"
 
@@ -38,8 +39,9 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef unsigned u4v __attribute__((ext_vector_type(4)));
 
-constexpr int TILE_V = 256;  // words per workgroup of STATS and GRAD; words of the packed copies are padded to it
-constexpr int TILE_P = 128;  // rows per workgroup
+constexpr int TILE_V = 256;  // words of the packed copies are padded to it
+constexpr int TILE_P = 256;  // rows per workgroup; rows of the packed copies are padded to it
+constexpr int CUS = 256;
 constexpr int TOP_EXP = 13;  // packed magnitudes are below 2^(TOP_EXP + 1)
 constexpr float MAX_FLOOR = -3.0e38f;  // a maximum over nothing: exp2 of anything minus it is 0, not NaN
 constexpr float LN2F = 0.69314718055994531f;
@@ -119,21 +121,22 @@ __device__ __forceinline__ float block_max(float top) {
   return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
 }
 
-// Largest finite magnitude of W, then of X.  A unit is eight elements of a row; units are dealt out over the workgroups.
+// Largest finite magnitude of W, then of X.  One run of memory is read as such; otherwise a wavefront takes four rows.
 template <typename T>
 __global__ void __launch_bounds__(256) vce_amax_kernel(AmaxJob w, AmaxJob x, float *__restrict__ partial) {
   const bool first = (int)blockIdx.x < w.blocks;
   const AmaxJob &j = first ? w : x;
   const bool wide = wide_rows<T>(j.m);
-  const int64_t per_row = (j.m.cols + 7) / 8, units = j.m.rows * per_row, step = (int64_t)j.blocks * 256;
+  const int block = (int)blockIdx.x - (first ? 0 : w.blocks);
   float top = 0.f;
   auto take = [&](const float (&v)[8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) top = fabsf(v[k]) < INFINITY ? fmaxf(top, fabsf(v[k])) : top;
   };
-  int64_t u = (int64_t)(blockIdx.x - (first ? 0 : w.blocks)) * 256 + threadIdx.x;
   if (!j.labels && wide && j.m.ld_row == j.m.cols && (j.m.cols & 7) == 0) {
-    const T *src = (const T *)j.m.data;      // one run of memory: four units in flight
+    const T *src = (const T *)j.m.data;
+    const int64_t units = j.m.rows * (j.m.cols / 8), step = (int64_t)j.blocks * 256;
+    int64_t u = (int64_t)block * 256 + threadIdx.x;
     for (; u + 3 * step < units; u += 4 * step) {
       Eight<T> e[4];
 #pragma unroll
@@ -145,13 +148,27 @@ __global__ void __launch_bounds__(256) vce_amax_kernel(AmaxJob w, AmaxJob x, flo
         take(v);
       }
     }
-  }
-  for (; u < units; u += step) {
-    const int64_t row = u / per_row;
-    if (j.labels && j.labels[row] == j.ignore) continue;
-    float v[8];
-    load8<T>(j.m, wide, row, (u - row * per_row) * 8, v);
-    take(v);
+    for (; u < units; u += step) {
+      Eight<T> e;
+      e.load(src + u * 8);
+      float v[8];
+      e.get(v);
+      take(v);
+    }
+  } else {
+    for (int64_t r0 = ((int64_t)block * 4 + (threadIdx.x >> 6)) * 4; r0 < j.m.rows; r0 += (int64_t)j.blocks * 16)
+      for (int64_t k = (threadIdx.x & 63) * 8; k < j.m.cols; k += 512) {
+        float v[4][8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[q][i] = 0.f;
+          const int64_t row = r0 + q;
+          if (row < j.m.rows && !(j.labels && j.labels[row] == j.ignore)) load8<T>(j.m, wide, row, k, v[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) take(v[q]);
+      }
   }
   top = block_max(top);
   if (threadIdx.x == 0) partial[blockIdx.x] = top;
@@ -189,9 +206,9 @@ __global__ void __launch_bounds__(256) vce_pack_kernel(PackJob w, PackJob x, con
   for (int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); u < w.units + x.units; u += (int64_t)gridDim.x * 4) {
     const bool first = u < w.units;
     const PackJob &j = first ? w : x;
-    const int groups = (j.kblocks + 3) / 4, e = first ? ew : ex;
-    const int64_t v = first ? u : u - w.units, tile = v / groups;
-    const int64_t kb = (v - tile * groups) * 4 + piece / 2, k = kb * 16 + (piece & 1) * 8;
+    const int e = first ? ew : ex;
+    const unsigned groups = (j.kblocks + 3) / 4, v = (unsigned)(first ? u : u - w.units), at = v / groups;  // units < 2^31
+    const int64_t tile = at, kb = (v - at * groups) * 4 + piece / 2, k = kb * 16 + (piece & 1) * 8;
     if (kb >= j.kblocks) continue;
     u4v *dst = j.dst + (tile * j.kblocks + kb) * 64 + (piece & 1) * 32 + lane / 8;
     float val[4][8];
@@ -240,10 +257,11 @@ __global__ void __launch_bounds__(256) vce_transpose_kernel(TransposeJob w, Tran
 #pragma unroll
     for (int i = 0; i < 8; ++i) ident[s][i] = 16 * s + 8 * h + i == (lane & 31) ? (_Float16)1.f : (_Float16)0.f;
   for (int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); u < (nw + nx) * planes; u += (int64_t)gridDim.x * 4) {
-    const int64_t pl = u / (nw + nx), v = u - pl * (nw + nx);
+    const int64_t pl = u >= nw + nx, v = pl ? u - (nw + nx) : u;
     const bool first = v < nw;
     const TransposeJob &j = first ? w : x;
-    const int64_t q = first ? v : v - nw, rt = q / j.col_tiles, ct = q - rt * j.col_tiles;
+    const unsigned q = (unsigned)(first ? v : v - nw), by = q / (unsigned)j.col_tiles;                 // tiles < 2^31
+    const int64_t rt = by, ct = q - by * (unsigned)j.col_tiles;
     const u4v *src = j.src + pl * j.plane + (rt * j.col_tiles + ct) * 128 + lane;
     f16v tr;
 #pragma unroll
@@ -303,64 +321,57 @@ __device__ __forceinline__ void store4(T *dst, float a, float b, float c, float 
   *reinterpret_cast<t4 *>(dst) = t4{(T)a, (T)b, (T)c, (T)d};
 }
 
-// WM x WN wavefronts of MT x NT accumulator tiles each: 32 WM MT rows of A by 32 WN NT rows of B.  LDS holds three stages
-// of 16 (two planes) or 32 (one plane) of the contraction, filled by direct loads two or three stages ahead.
-// Four wavefronts (two workgroups share a CU, one does its epilogue while the other multiplies): a stage has two halves,
-// and while the matrix cores work on one the next comes from LDS.
-// Eight wavefronts (one workgroup to a CU, half the loads per product): two groups of four, one wavefront of each on every
-// SIMD, take turns between barriers, one reading its next stage while the other multiplies.
-template <int NP, int WM, int WN, int MT, int NT, int MODE, typename T>
-__global__ void __launch_bounds__(WM *WN * 64, 2) vce_gemm_kernel(const GemmArgs g) {
+// Eight wavefronts, 2 x 4, of MT x 2 accumulator tiles each: 64 MT rows of A by 256 rows of B.  LDS holds three stages of
+// 16 (two planes) or 32 (one plane) of the contraction, filled by direct loads two stages ahead.  The wavefronts form two
+// groups, one wavefront of each on every SIMD, that take turns between barriers: one reads its next stage from LDS while
+// the other multiplies.  One workgroup a CU, which takes tile after tile and starts the next one's loads before it turns
+// to the epilogue.
+template <int NP, int MT, int MODE, typename T>
+__global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g) {
   extern __shared__ u4v lds[];
-  constexpr int WAVES = WM * WN, KB = NP == 1 ? 2 : 1;
+  constexpr int WM = 2, WN = 4, NT = 2, WAVES = WM * WN, KB = NP == 1 ? 2 : 1;
   constexpr int A_TILES = WM * MT, B_TILES = WN * NT;
-  constexpr int STAGE = (A_TILES + B_TILES) * 2, LOADS = STAGE / WAVES;
-  static_assert((WAVES == 4 || WAVES == 8) && STAGE % WAVES == 0, "every wavefront fills the same share of a stage");
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int STAGE = (A_TILES + B_TILES) * 2, LOADS = (STAGE + WAVES - 1) / WAVES;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
+  const bool late = wave >= WAVES / 2;
 
   // Workgroups go to the eight XCDs in turn: each XCD takes a run of consecutive tiles, ordered as bands of eight
   // M tiles walked along N, so that its L2 holds the operands of the tiles it works on together.
-  const unsigned tiles = (unsigned)g.m_tiles * g.n_tiles * g.splits;
-  const unsigned per_xcd = (tiles + 7) / 8;
-  unsigned t = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per_xcd || t >= tiles) return;
-  const unsigned split = t / ((unsigned)g.m_tiles * g.n_tiles);
-  t -= split * (unsigned)g.m_tiles * g.n_tiles;
-  const unsigned band = t / (8u * g.n_tiles), in_band = t - band * 8u * g.n_tiles;
-  const unsigned band_m = min(8u, (unsigned)g.m_tiles - band * 8u);
-  const int m_tile = (int)(band * 8u + in_band % band_m), n_tile = (int)(in_band / band_m);
+  const unsigned tiles = (unsigned)g.m_tiles * g.n_tiles * g.splits, per_xcd = (tiles + 7) / 8;
+  const unsigned lo = (blockIdx.x & 7) * per_xcd, hi = min(lo + per_xcd, tiles);
+  unsigned tile = lo + (blockIdx.x >> 3);
+  if (tile >= hi) return;
 
-  // this wavefront's LOADS blocks of a stage, ordered [half: k block or plane][tile] for A, then for B
-  const u4v *src[LOADS];
+  int m_tile, n_tile, split, stages;
+  const u4v *src[LOADS];  // this wavefront's blocks of a stage, ordered [half: k block or plane][tile] for A, then for B
+  auto place = [&](unsigned t) {
+    split = (int)(t / ((unsigned)g.m_tiles * g.n_tiles));
+    t -= split * (unsigned)g.m_tiles * g.n_tiles;
+    const unsigned band = t / (8u * g.n_tiles), in_band = t - band * 8u * g.n_tiles;
+    const unsigned band_m = min(8u, (unsigned)g.m_tiles - band * 8u);
+    m_tile = (int)(band * 8u + in_band % band_m), n_tile = (int)(in_band / band_m);
+    stages = min(g.k_split, g.kblocks - split * g.k_split) / KB;
 #pragma unroll
-  for (int l = 0; l < LOADS; ++l) {
-    const int j = wave * LOADS + l;
-    const bool is_a = j < 2 * A_TILES;
-    const int q = is_a ? j : j - 2 * A_TILES, per = is_a ? A_TILES : B_TILES;
-    const int tile = q % per, half = q / per;
-    const int kb = NP == 1 ? half : 0, plane = NP == 1 ? 0 : half;
-    const int64_t row = is_a ? min(m_tile * A_TILES + tile, g.a_tiles - 1) : min(n_tile * B_TILES + tile, g.b_tiles - 1);
-    const u4v *base = is_a ? g.A + plane * g.plane_a + row * g.ld_a * 64 : g.B + plane * g.plane_b + row * g.ld_b * 64;
-    src[l] = base + ((int64_t)split * g.k_split + kb) * 64;
-  }
-  const int stages = min(g.k_split, g.kblocks - (int)split * g.k_split) / KB;
+    for (int l = 0; l < LOADS; ++l) {
+      const int j = min(wave * LOADS + l, STAGE - 1);  // (a share past the end repeats the last block, into its own place)
+      const bool is_a = j < 2 * A_TILES;
+      const int q = is_a ? j : j - 2 * A_TILES, per = is_a ? A_TILES : B_TILES;
+      const int at = q % per, half = q / per;
+      const int kb = NP == 1 ? half : 0, plane = NP == 1 ? 0 : half;
+      const int64_t row = is_a ? min(m_tile * A_TILES + at, g.a_tiles - 1) : min(n_tile * B_TILES + at, g.b_tiles - 1);
+      const u4v *base = is_a ? g.A + plane * g.plane_a + row * g.ld_a * 64 : g.B + plane * g.plane_b + row * g.ld_b * 64;
+      src[l] = base + ((int64_t)split * g.k_split + kb) * 64;
+    }
+  };
   auto fill = [&](int buf) {
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) {
-      __builtin_amdgcn_global_load_lds((global_ptr)(src[l] + lane), (lds_ptr)(lds + (buf * STAGE + wave * LOADS + l) * 64), 16, 0,
-                                       0);
+      const int j = min(wave * LOADS + l, STAGE - 1);
+      __builtin_amdgcn_global_load_lds((global_ptr)(src[l] + lane), (lds_ptr)(lds + (buf * STAGE + j) * 64), 16, 0, 0);
       src[l] += KB * 64;
     }
   };
-  f16v acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][n][r] = 0.f;
-
   struct Half {  // one k block, or one plane, of a stage
     h8v a[MT], b[NT];
   };
@@ -372,246 +383,236 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) vce_gemm_kernel(const GemmArgs
 #pragma unroll
     for (int i = 0; i < MT; ++i) f.a[i] = __builtin_bit_cast(h8v, sa[i * 64]);
   };
+  f16v acc[MT][NT];
   auto multiply = [&](const Half &fa, const Half &fb) {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa.a[i], fb.b[n], acc[i][n], 0, 0, 0);
   };
-  // the second half's products; for two planes the mixed ones (residual times residual is left out)
-  auto multiply_second = [&](const Half &first, const Half &second) {
-    if (NP == 1) {
-      multiply(second, second);
-    } else {
-      multiply(second, first);
-      multiply(first, second);
-    }
-  };
-  // Waits for all but the youngest `n` fills of this wavefront and for its own LDS reads; after the barrier both hold for
-  // all wavefronts.
-  auto arrive = [&](int n) {
-    if (n == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
-    else if (n == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+  // Waits for all but the youngest fill of this wavefront (`more`: there is one) and for its own LDS reads; after the
+  // barrier both hold for all wavefronts that have come to it.
+  auto arrive = [&](bool more) {
+    if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  int buf = 0;
-  if (WAVES == 4) {
+
+  place(tile);
+  fill(0);
+  if (stages > 1) fill(1);
+  for (;;) {
 #pragma unroll
-    for (int st = 0; st < 3; ++st)
-      if (st < stages) fill(st);
-    arrive(stages > 2 ? 2 : stages > 1 ? 1 : 0);
-    Half first, second;
-    read(0, 0, first);
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-    for (int st = 0; st < stages; ++st) {
-      const int next = buf == 2 ? 0 : buf + 1;
-      read(buf, 1, second);
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_setprio(1);
-      multiply(first, first);
-      __builtin_amdgcn_s_setprio(0);
-      __builtin_amdgcn_sched_barrier(0);
-      Half ahead = first;
-      if (st + 1 < stages) {
-        arrive(st + 2 < stages ? 1 : 0);
-        if (st + 3 < stages) fill(buf);       // every wavefront has read this stage
-        read(next, 0, ahead);
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][n][r] = 0.f;
+    const int m0 = (m_tile * WM + wm) * 32 * MT;                                   // first row of A of this wavefront
+    const int64_t n0 = ((int64_t)n_tile * WN + wn) * 32 * NT + (lane & 31);        // this lane's row of B, tile 0
+    const int of_split = split, of_m = m_tile, of_n = n_tile;
+    // what the epilogue needs of its rows, ahead of the loads that it would wait for otherwise
+    int place_of[NT];             // the label's place among this wavefront's words, or something out of their range
+    float lse2[NT], coef_a[NT], coef_b[NT];
+    if constexpr (MODE == STATS || MODE == GRAD) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int64_t p = n0 + 32 * n, rel = (p < g.P ? g.labels[p] : -1) - (g.v0 + m0);
+        place_of[n] = rel >= 0 && rel < 32 * MT ? (int)rel : -32;
+        if constexpr (MODE == GRAD) lse2[n] = g.lse2[p], coef_a[n] = g.coef_a[p], coef_b[n] = g.coef_b[p];
       }
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_setprio(1);
-      multiply_second(first, second);
-      __builtin_amdgcn_s_setprio(0);
-      __builtin_amdgcn_sched_barrier(0);
-      // lgkmcnt(0): the next half has come while the matrix cores were fed.  As an instruction that the compiler knows,
-      // or it would wait in front of the next products for the reads issued just before them
-      __builtin_amdgcn_s_waitcnt(0xc07f);
-      first = ahead;
-      buf = next;
     }
-  } else {
-    fill(0);
-    if (stages > 1) fill(1);
-    arrive(stages > 1 ? 1 : 0);
-    const bool late = wave >= WAVES / 2;
+    arrive(stages > 1);
     if (late) __builtin_amdgcn_s_barrier();    // the second group is one barrier behind
+    int buf = 0;
     for (int st = 0; st < stages; ++st) {
       Half first, second;
       read(buf, 0, first);
       read(buf, 1, second);
-      // the stage before this one: this group has read it two barriers ago, the other one barrier ago
+      // into the stage before this one: this group has read it two barriers ago, the other one barrier ago
       if (st + 2 < stages) fill(buf == 0 ? 2 : buf - 1);
       __builtin_amdgcn_sched_barrier(0);
-      // the stage after this one: this group reads it two barriers from now, and the other group's loads of it are waited
-      // for one barrier from now
-      arrive(st + 2 < stages ? 1 : 0);
+      // the stage after this one: this group reads it two barriers from now, and the other group waits for its loads of
+      // it before the barrier in between
+      arrive(st + 2 < stages);
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
       multiply(first, first);
-      multiply_second(first, second);
+      if (NP == 1) {
+        multiply(second, second);
+      } else {  // head by residual and residual by head; residual by residual is left out
+        multiply(second, first);
+        multiply(first, second);
+      }
       __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       buf = buf == 2 ? 0 : buf + 1;
     }
-    if (!late) __builtin_amdgcn_s_barrier();
-  }
+    if (!late) __builtin_amdgcn_s_barrier();   // in step again: every wavefront has read the last stage
 
-  const int h = lane >> 5;
-  const int m0 = (m_tile * WM + wm) * 32 * MT;                                     // first row of A of this wavefront
-  const int64_t n0 = ((int64_t)n_tile * WN + wn) * 32 * NT + (lane & 31);          // this lane's row of B, tile 0
-  // accumulator register r of tile (i, n): row m0 + 32 i + (r & 3) + 8 (r >> 2) + 4 h of A, row n0 + 32 n of B
+    tile += gridDim.x >> 3;
+    const bool again = tile < hi;
+    if (again) {
+      place(tile);
+      fill(0);
+      if (stages > 1) fill(1);
+    }
+    // accumulator register r of tile (i, n): row m0 + 32 i + (r & 3) + 8 (r >> 2) + 4 h of A, row n0 + 32 n of B
 
-  if (MODE == STATS || MODE == GRAD) {
-    const float c = ldexpf(fabsf(g.scale) * LOG2E, -(g.scal->exp_x + g.scal->exp_w));
-    const int64_t left = g.V - (g.v0 + m0);      // words of this wavefront that exist
+    if constexpr (MODE == STATS || MODE == GRAD) {
+      const float c = ldexpf(fabsf(g.scale) * LOG2E, -(g.scal->exp_x + g.scal->exp_w));
+      // words of this wavefront that exist, from this lane's first one on: compared with constants below
+      const int left = (int)min(g.V - (g.v0 + m0), (int64_t)(32 * MT)) - 4 * h;
+      const bool whole = g.V - (g.v0 + m0) >= 32 * MT;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int64_t p = n0 + 32 * n;
-      const int64_t label = p < g.P ? g.labels[p] : -1;
-      const int64_t rel = label - (g.v0 + m0);
-      const int at = rel >= 0 && rel < 32 * MT ? (int)rel : -1;        // the label's place among this wavefront's words
-      const bool here = __any(at >= 0);
-      if (MODE == STATS) {
-        if (here) {
-          float z = 0.f;
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) z = at == 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h ? acc[i][n][r] * c : z;
-          if (at >= 0 && ((at >> 2) & 1) == h) g.target[p] = z;
-        }
-        if (left < 32 * MT) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (32 * i + (r & 3) + 8 * (r >> 2) + 4 * h >= left) acc[i][n][r] = -INFINITY;
-        }
-        float top = acc[0][n][0];
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][n][r]);
-        top = fmaxf(top, __shfl_xor(top, 32));
-        top = fmaxf(top * c, MAX_FLOOR);
-        float sum = 0.f;
-        if (left >= 32 * MT) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -top));
-        } else {  // (the selection and not the infinity keeps the others out: c may have underflowed to 0)
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              sum += 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h >= left
-                         ? 0.f : __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -top));
-        }
-        sum += __shfl_xor(sum, 32);
-        if (h == 0) g.partial[(int64_t)(m_tile * WM + wm) * g.Pp + p] = make_float2(top, sum);
-      } else {
-        const float l2 = g.lse2[p], ca = g.coef_a[p], cb = g.coef_b[p];
-        h8v ident[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ident[s][i] = slot_place(s, h, i) == (lane & 31) ? (_Float16)1.f : (_Float16)0.f;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          float v[16];
-#pragma unroll
-          for (int r = 0; r < 16; ++r) v[r] = ca * __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -l2));
+      for (int n = 0; n < NT; ++n) {
+        const int64_t p = n0 + 32 * n;
+        const bool mine = place_of[n] >= 0;
+        const int at = place_of[n] - 4 * h;    // from this lane's first word on; the other half's places match no constant
+        const bool here = __any(mine);
+        if constexpr (MODE == STATS) {
           if (here) {
+            float z = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) v[r] -= at == 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h ? cb : 0.f;
-          }
-          if (left < 32 * MT) {
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (32 * i + (r & 3) + 8 * (r >> 2) + 4 * h >= left) v[r] = 0.f;
+              for (int r = 0; r < 16; ++r) z = at == 32 * i + (r & 3) + 8 * (r >> 2) ? acc[i][n][r] * c : z;
+            if (mine && (at & 4) == 0) g.target[p] = z;
           }
-          h8v f[NP][2];
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+                if (32 * i + (r & 3) + 8 * (r >> 2) >= left) acc[i][n][r] = -INFINITY;
+          }
+          float top = acc[0][n][0];
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][n][r]);
+          top = fmaxf(top, __shfl_xor(top, 32));
+          top = fmaxf(top * c, MAX_FLOOR);
+          float sum = 0.f;
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -top));
+          } else {  // (the selection and not the infinity keeps the others out: c may have underflowed to 0)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+                sum += 32 * i + (r & 3) + 8 * (r >> 2) >= left
+                           ? 0.f : __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -top));
+          }
+          sum += __shfl_xor(sum, 32);
+          if (h == 0) g.partial[(int64_t)(of_m * WM + wm) * g.Pp + p] = make_float2(top, sum);
+        } else {
+          const float l2 = lse2[n], ca = coef_a[n], cb = coef_b[n];
+          h8v ident[2];
 #pragma unroll
           for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              f[0][s][k] = (_Float16)v[8 * s + k];
-              if (NP == 2) f[NP - 1][s][k] = (_Float16)(v[8 * s + k] - (float)f[0][s][k]);
+            for (int i = 0; i < 8; ++i) ident[s][i] = slot_place(s, h, i) == (lane & 31) ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            float v[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] = ca * __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -l2));
+            if (here) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) v[r] -= at == 32 * i + (r & 3) + 8 * (r >> 2) ? cb : 0.f;
             }
-          const int64_t pt = ((int64_t)n_tile * WN + wn) * NT + n, vt = m0 / 32 + i;
+            if (!whole) {
 #pragma unroll
-          for (int pl = 0; pl < NP; ++pl) {
-            if (g.gx) {
-              u4v *dst = g.gx + pl * g.plane_gx + (pt * g.ld_gx + vt * 2) * 64 + lane;
-#pragma unroll
-              for (int s = 0; s < 2; ++s) dst[s * 64] = __builtin_bit_cast(u4v, f[pl][s]);
+              for (int r = 0; r < 16; ++r)
+                if (32 * i + (r & 3) + 8 * (r >> 2) >= left) v[r] = 0.f;
             }
-            if (g.gw) {
-              f16v tr;
+            h8v f[NP][2];
 #pragma unroll
-              for (int r = 0; r < 16; ++r) tr[r] = 0.f;
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-              for (int s = 0; s < 2; ++s) tr = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[pl][s], ident[s], tr, 0, 0, 0);
-              u4v *dst = g.gw + pl * g.plane_gw + (vt * g.ld_gw + pt * 2) * 64 + lane;
+              for (int k = 0; k < 8; ++k) {
+                f[0][s][k] = (_Float16)v[8 * s + k];
+                if (NP == 2) f[NP - 1][s][k] = (_Float16)(v[8 * s + k] - (float)f[0][s][k]);
+              }
+            const int64_t pt = ((int64_t)of_n * WN + wn) * NT + n, vt = m0 / 32 + i;
+            if (vt >= g.a_tiles) continue;     // past the piece
 #pragma unroll
-              for (int s = 0; s < 2; ++s) {
-                h8v o;
+            for (int pl = 0; pl < NP; ++pl) {
+              if (g.gx) {
+                u4v *dst = g.gx + pl * g.plane_gx + (pt * g.ld_gx + vt * 2) * 64 + lane;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] = (_Float16)tr[8 * s + k];
-                dst[s * 64] = __builtin_bit_cast(u4v, o);
+                for (int s = 0; s < 2; ++s) dst[s * 64] = __builtin_bit_cast(u4v, f[pl][s]);
+              }
+              if (g.gw) {
+                f16v tr;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) tr[r] = 0.f;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) tr = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[pl][s], ident[s], tr, 0, 0, 0);
+                u4v *dst = g.gw + pl * g.plane_gw + (vt * g.ld_gw + pt * 2) * 64 + lane;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                  h8v o;
+#pragma unroll
+                  for (int k = 0; k < 8; ++k) o[k] = (_Float16)tr[8 * s + k];
+                  dst[s * 64] = __builtin_bit_cast(u4v, o);
+                }
               }
             }
           }
         }
       }
-    }
-  } else if (MODE == DX) {
+    } else if constexpr (MODE == DX) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (n0 + 32 * n >= g.Pp) continue;
+      for (int n = 0; n < NT; ++n) {
+  #pragma unroll
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int d = m0 + 32 * i + 8 * q + 4 * h;
-          if (d >= g.ld_acc) continue;
-          float4 *dst = reinterpret_cast<float4 *>(g.acc + ((int64_t)split * g.Pp + n0 + 32 * n) * g.ld_acc + d);
-          float4 v = make_float4(acc[i][n][4 * q], acc[i][n][4 * q + 1], acc[i][n][4 * q + 2], acc[i][n][4 * q + 3]);
-          if (g.add) {
-            const float4 o = *dst;
-            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+          for (int q = 0; q < 4; ++q) {
+            const int d = m0 + 32 * i + 8 * q + 4 * h;
+            if (d >= g.ld_acc) continue;
+            float4 *dst = reinterpret_cast<float4 *>(g.acc + ((int64_t)of_split * g.Pp + n0 + 32 * n) * g.ld_acc + d);
+            float4 v = make_float4(acc[i][n][4 * q], acc[i][n][4 * q + 1], acc[i][n][4 * q + 2], acc[i][n][4 * q + 3]);
+            if (g.add) {
+              const float4 o = *dst;
+              v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+            }
+            *dst = v;
           }
-          *dst = v;
-        }
-    }
-  } else {
-    const int e = -(*g.exp_g + g.scal->exp_x);
+      }
+    } else {
+      const int e = -(*g.exp_g + g.scal->exp_x);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int64_t v = g.v0 + n0 + 32 * n;
-      if (v >= g.V) continue;
+      for (int n = 0; n < NT; ++n) {
+        const int64_t v = g.v0 + n0 + 32 * n;
+        if (v >= g.V) continue;
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int d = m0 + 32 * i + 8 * q + 4 * h;
-          float x[4];
+          for (int q = 0; q < 4; ++q) {
+            const int d = m0 + 32 * i + 8 * q + 4 * h;
+            float x[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = ldexpf(acc[i][n][4 * q + k] * fabsf(g.scale), e);  // X's copy has its sign
-          T *dst = (T *)g.out + v * g.D + d;
-          if ((g.D & 3) == 0) {
-            if (d < g.D) store4<T>(dst, x[0], x[1], x[2], x[3]);
-          } else {
+            for (int k = 0; k < 4; ++k) x[k] = ldexpf(acc[i][n][4 * q + k] * fabsf(g.scale), e);  // X's copy has its sign
+            T *dst = (T *)g.out + v * g.D + d;
+            if ((g.D & 3) == 0) {
+              if (d < g.D) store4<T>(dst, x[0], x[1], x[2], x[3]);
+            } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (d + k < g.D) dst[k] = (T)x[k];
+              for (int k = 0; k < 4; ++k)
+                if (d + k < g.D) dst[k] = (T)x[k];
+            }
           }
-        }
+      }
     }
+    if (!again) return;
   }
 }
 
@@ -929,17 +930,33 @@ __global__ void __launch_bounds__(1024) vce_coef_kernel(int64_t P, int64_t Pp, i
   }
 }
 
-// dX = sum of the splits, scaled, in the output type.
+// Rows of a gradient = sum of the splits, scaled, in the output type: a row per wavefront, four features per lane.
 template <typename T>
-__global__ void __launch_bounds__(256) vce_dx_kernel(int64_t P, int64_t D, int64_t Pp, int64_t ld, int splits, float scale,
-                                                     const float *__restrict__ acc, const Scalars *s,
-                                                     const int *__restrict__ exp_g, T *__restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= P * D) return;
-  const int64_t p = i / D, d = i - p * D;
-  float v = 0.f;
-  for (int k = 0; k < splits; ++k) v += acc[((int64_t)k * Pp + p) * ld + d];
-  out[i] = (T)ldexpf(v * scale, -(*exp_g + s->exp_w));
+__global__ void __launch_bounds__(256) vce_finish_kernel(int64_t P, int64_t D, int64_t Pp, int64_t ld, int splits, float scale,
+                                                     const float *__restrict__ acc,
+                                                         const int *__restrict__ exp_other, const int *__restrict__ exp_g,
+                                                         T *__restrict__ out) {
+  const int64_t p = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (p >= P) return;
+  const int e = -(*exp_g + *exp_other);
+  for (int64_t d = (threadIdx.x & 63) * 4; d < D; d += 256) {
+    const float *src = acc + p * ld + d;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const float4 a = *reinterpret_cast<const float4 *>(src + k * Pp * ld);
+      v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+    }
+    const float x[4] = {ldexpf(v.x * scale, e), ldexpf(v.y * scale, e), ldexpf(v.z * scale, e), ldexpf(v.w * scale, e)};
+    T *dst = out + p * D + d;
+    if ((D & 3) == 0) {
+      store4<T>(dst, x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (d + k < D) dst[k] = (T)x[k];
+    }
+  }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
@@ -983,12 +1000,15 @@ struct Kept {  // what the forward pass leaves for the backward pass
   }
 };
 
+int word_units(int64_t words, int64_t rows);
+
 struct FwdScratch {
   float *amax, *target;
   float2 *partial;
   int pairs;
   FwdScratch(Carve &c, const Shape &s) {
-    pairs = (int)(s.Vp / 128);   // a wavefront's words
+    const int64_t words = 64 * word_units(s.Vp, s.Pp);
+    pairs = (int)((s.Vp + words - 1) / words * 2);   // a wavefront's words each
     amax = c.take<float>(2 * AMAX_BLOCKS);
     target = c.take<float>(s.Pp);
     partial = c.take<float2>((int64_t)pairs * s.Pp);
@@ -997,33 +1017,41 @@ struct FwdScratch {
 
 constexpr int64_t PIECE_BYTES = 512ll << 20;  // G of one piece of the vocabulary, all copies and planes
 
+// Splits of a contraction of `k` blocks: the number up to 16 that leaves the fewest of the CUs without work (fewer if
+// that is within 2 %: each split writes and reads its own partial result), at least four blocks each.
+struct Splits {
+  int n, blocks;  // blocks of each but the last
+};
+Splits choose_splits(int64_t Dk, int64_t n_rows, int64_t k) {
+  const int64_t tiles = round_up(Dk, 256) / 256 * ((n_rows + 255) / 256);
+  int want = 1;
+  double best = 0.;
+  for (int n = 1; n <= 16 && k / n >= 4; ++n) {
+    const double used = (double)(tiles * n) / (double)round_up(tiles * n, CUS);
+    if (used > best + 0.02) best = used, want = n;
+  }
+  const int blocks = (int)round_up((k + want - 1) / want, 2);
+  return Splits{(int)((k + blocks - 1) / blocks), blocks};
+}
+
 struct BwdScratch {
   int *exp_g;
-  float *coef_a, *coef_b, *acc;
+  float *coef_a, *coef_b, *acc, *acc_w;
   u4v *xt, *wt, *gx, *gw;
   int64_t piece;  // words
-  int splits, kper;  // splits of a full piece's words, blocks of the contraction each
+  Splits split_words, split_rows;  // of the contractions of dX (a full piece's words) and of dW
   BwdScratch(Carve &c, const Shape &s, bool dx, bool dw) {
     const int64_t per_word = s.Pp * 2 * s.np * (int(dx) + int(dw));
     piece = std::min(s.Vp, std::max<int64_t>(PIECE_BYTES / per_word / TILE_V, 1) * TILE_V);
     const int64_t pieces = (s.Vp + piece - 1) / piece;
     piece = round_up((s.Vp + pieces - 1) / pieces, TILE_V);   // of equal size
-    // splits of the words' contraction: the number up to 16 that leaves the fewest of the 256 CUs without work, at least
-    // 16 stages each
-    const int64_t tiles = round_up(s.Dk, 256) / 256 * ((s.Pp + 255) / 256);
-    const int64_t k = piece / 16;
-    int want = 1;
-    double best = 0.;
-    for (int n = 1; n <= 16 && k / n >= 32; ++n) {
-      const double used = (double)(tiles * n) / (double)round_up(tiles * n, 256);
-      if (used > best + 0.02) best = used, want = n;
-    }
-    kper = (int)round_up((k + want - 1) / want, 2);
-    splits = (int)((k + kper - 1) / kper);
+    split_words = choose_splits(s.Dk, s.Pp, piece / 16);
+    split_rows = choose_splits(s.Dk, piece, s.Pp / 16);
     exp_g = c.take<int>(1);
     coef_a = c.take<float>(s.Pp);
     coef_b = c.take<float>(s.Pp);
-    acc = c.take<float>(dx ? splits * s.Pp * s.Dk : 0);
+    acc = c.take<float>(dx ? split_words.n * s.Pp * s.Dk : 0);
+    acc_w = c.take<float>(dw && split_rows.n > 1 ? split_rows.n * piece * s.Dk : 0);
     wt = c.take<u4v>(dx ? s.np * s.plane(s.Vp) : 0);
     xt = c.take<u4v>(dw ? s.np * s.plane(s.Pp) : 0);
     gx = c.take<u4v>(dx ? s.np * s.Pp * piece / 8 : 0);
@@ -1031,29 +1059,65 @@ struct BwdScratch {
   }
 };
 
-template <int NP, int WM, int WN, int MT, int NT, int MODE, typename T>
+template <int NP, int MT, int MODE, typename T>
 int launch_tiles(GemmArgs g, int64_t m_rows, int64_t n_rows, hipStream_t st) {
-  const size_t bytes = (size_t)3 * (WM * MT + WN * NT) * 2 * 1024;
-  g.m_tiles = (int)((m_rows + WM * MT * 32 - 1) / (WM * MT * 32));
-  g.n_tiles = (int)((n_rows + WN * NT * 32 - 1) / (WN * NT * 32));
+  const size_t bytes = (size_t)3 * (2 * MT + 8) * 2 * 1024;
+  g.m_tiles = (int)((m_rows + 64 * MT - 1) / (64 * MT)), g.n_tiles = (int)((n_rows + 255) / 256);
   g.a_tiles = (int)(m_rows / 32), g.b_tiles = (int)(n_rows / 32);
   const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles * g.splits;
   if (tiles > (1ll << 30)) {
     set_error_text("pr_vocab_ce: too many tiles for one launch");
     return PR_EUNSUPPORTED;
   }
-  const auto kernel = vce_gemm_kernel<NP, WM, WN, MT, NT, MODE, T>;
-  PR_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(WM * WN * 64), bytes, st, g);
+  const auto kernel = vce_gemm_kernel<NP, MT, MODE, T>;
+  static std::atomic<uint64_t> known{0};   // devices that know the kernel's LDS size
+  int device = 0;
+  PR_HIP(hipGetDevice(&device));
+  const uint64_t bit = 1ull << (device & 63);
+  if (device > 63 || !(known.load(std::memory_order_acquire) & bit)) {
+    PR_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    known.fetch_or(bit, std::memory_order_release);
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(CUS, (tiles + 7) / 8 * 8)), dim3(512), bytes, st, g);
   return check_launch("pr_vocab_ce");
 }
 
-// Products whose M rows are features: 256 of them per workgroup unless 128 leave fewer unused.
-bool narrow_features(int64_t Dk) { return round_up(Dk, 128) * 8 < round_up(Dk, 256) * 7; }
+// Words per workgroup of STATS and GRAD, in units of 64: the number whose rounds over the CUs take the least time, a
+// tile taking its share of products plus what does not shrink with it.
+int word_units(int64_t words, int64_t rows) {
+  int best = 1;
+  double least = 1e300;
+  for (int mt = 1; mt <= 5; ++mt) {
+    const int64_t tiles = (words + 64 * mt - 1) / (64 * mt) * ((rows + 255) / 256);
+    const double time = (double)((tiles + CUS - 1) / CUS) * (mt + 0.6);
+    if (time < least) least = time, best = mt;
+  }
+  return best;
+}
+template <int NP, int MODE>
+int launch_words(const GemmArgs &g, int64_t words, int64_t rows, hipStream_t st) {
+  switch (word_units(words, rows)) {
+    case 1: return launch_tiles<NP, 1, MODE, float>(g, words, rows, st);
+    case 2: return launch_tiles<NP, 2, MODE, float>(g, words, rows, st);
+    case 3: return launch_tiles<NP, 3, MODE, float>(g, words, rows, st);
+    case 4: return launch_tiles<NP, 4, MODE, float>(g, words, rows, st);
+    default: return launch_tiles<NP, 5, MODE, float>(g, words, rows, st);
+  }
+}
+
+// The same for the products whose M rows are features, `n_rows` by `splits` of them.
 template <int NP, int MODE, typename T>
 int launch_features(const GemmArgs &g, int64_t Dk, int64_t n_rows, hipStream_t st) {
-  return narrow_features(Dk) ? launch_tiles<NP, 2, 4, 2, 2, MODE, T>(g, Dk, n_rows, st)
-                             : launch_tiles<NP, 2, 4, 4, 2, MODE, T>(g, Dk, n_rows, st);
+  int best = 4;
+  double least = 1e300;
+  for (int mt = 4; mt >= 1; mt /= 2) {
+    const int64_t tiles = (Dk + 64 * mt - 1) / (64 * mt) * ((n_rows + 255) / 256) * g.splits;
+    const double time = (double)((tiles + CUS - 1) / CUS) * (mt + 0.6);
+    if (time < least) least = time, best = mt;
+  }
+  if (best == 4) return launch_tiles<NP, 4, MODE, T>(g, Dk, n_rows, st);
+  if (best == 2) return launch_tiles<NP, 2, MODE, T>(g, Dk, n_rows, st);
+  return launch_tiles<NP, 1, MODE, T>(g, Dk, n_rows, st);
 }
 
 struct Call {
@@ -1075,10 +1139,10 @@ template <typename T, int NP>
 int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, float *lse, float *loss, hipStream_t st) {
   const Shape s(c.dtype, c.P, c.V, c.D);
   const bool scaled = c.dtype != PR_F16;
-  auto amax_blocks = [&](const Matrix &m) {  // at least 32 units a thread
-    return scaled ? (int)std::min<int64_t>(AMAX_BLOCKS, (m.rows * ((m.cols + 7) / 8) + 8191) / 8192) : 0;
-  };
-  const AmaxJob aw{c.w, nullptr, 0, amax_blocks(c.w)}, ax{c.x, c.labels, c.ignore, amax_blocks(c.x)};
+  // 64 elements a thread, or four rows a wavefront, until the chip is full
+  auto amax_blocks = [&](int64_t n) { return scaled ? (int)std::min<int64_t>(AMAX_BLOCKS, n) : 0; };
+  const AmaxJob aw{c.w, nullptr, 0, amax_blocks((c.V * ((c.D + 7) / 8) + 2047) / 2048)};
+  const AmaxJob ax{c.x, c.labels, c.ignore, amax_blocks((c.P + 15) / 16)};
   if (scaled) {
     hipLaunchKernelGGL((vce_amax_kernel<T>), dim3(aw.blocks + ax.blocks), dim3(256), 0, st, aw, ax, f.amax);
     PR_TRY(check_launch("pr_vocab_ce"));
@@ -1095,7 +1159,7 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
   g.kblocks = g.k_split = kb, g.splits = 1;
   g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.labels = c.labels;
   g.partial = f.partial, g.target = f.target, g.Pp = s.Pp;
-  PR_TRY((launch_tiles<NP, 2, 2, 4, 2, STATS, T>(g, s.Vp, s.Pp, st)));
+  PR_TRY((launch_words<NP, STATS>(g, s.Vp, s.Pp, st)));
   const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k.lse2, lse, row_loss};
   hipLaunchKernelGGL(vce_join_kernel, dim3((unsigned)(s.Pp / 8)), dim3(256), 0, st, rows, s.Pp, f.pairs, f.partial);
   PR_TRY(check_launch("pr_vocab_ce"));
@@ -1158,26 +1222,36 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
     g.lse2 = k.lse2, g.coef_a = b.coef_a, g.coef_b = b.coef_b;
     g.gx = dx ? b.gx : nullptr, g.gw = dw ? b.gw : nullptr;
     g.plane_gx = g.plane_gw = s.Pp * b.piece / 8, g.ld_gx = b.piece / 16, g.ld_gw = kp;
-    PR_TRY((launch_tiles<NP, 2, 2, 4, 2, GRAD, T>(g, words, s.Pp, st)));
+    PR_TRY((launch_words<NP, GRAD>(g, words, s.Pp, st)));
     if (dx) {
       GemmArgs x{};
       x.A = b.wt + v0 / 16 * 64, x.B = b.gx, x.plane_a = s.plane(s.Vp), x.plane_b = g.plane_gx, x.ld_a = kv, x.ld_b = g.ld_gx;
       x.scal = k.scal, x.acc = b.acc, x.Pp = s.Pp, x.ld_acc = s.Dk, x.add = v0 > 0;
       // the splits of a full piece; a shorter last piece leaves the rest of them as they are
-      x.kblocks = (int)(words / 16), x.k_split = b.kper, x.splits = (x.kblocks + b.kper - 1) / b.kper;
-      PR_TRY((launch_features<NP, DX, T>(x, s.Dk, s.Pp, st)));
+      x.kblocks = (int)(words / 16), x.k_split = b.split_words.blocks;
+      x.splits = (x.kblocks + x.k_split - 1) / x.k_split;
+      PR_TRY((launch_features<NP, DX, float>(x, s.Dk, s.Pp, st)));
     }
     if (dw) {
       GemmArgs w{};
       w.A = b.xt, w.B = b.gw, w.plane_a = s.plane(s.Pp), w.plane_b = g.plane_gw, w.ld_a = w.ld_b = kp;
-      w.kblocks = w.k_split = kp, w.splits = 1;
+      w.kblocks = kp, w.k_split = b.split_rows.blocks, w.splits = b.split_rows.n;
       w.scal = k.scal, w.exp_g = b.exp_g, w.scale = c.scale, w.V = c.V, w.v0 = v0, w.out = dw, w.D = c.D;
-      PR_TRY((launch_features<NP, DW, T>(w, s.Dk, words, st)));
+      if (w.splits == 1) {
+        PR_TRY((launch_features<NP, DW, T>(w, s.Dk, words, st)));
+      } else {
+        w.acc = b.acc_w, w.Pp = words, w.ld_acc = s.Dk;
+        PR_TRY((launch_features<NP, DX, float>(w, s.Dk, words, st)));
+        const int64_t rows = std::min(words, c.V - v0);
+        hipLaunchKernelGGL((vce_finish_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, rows, c.D, words, s.Dk,
+                           w.splits, fabsf(c.scale), b.acc_w, &k.scal->exp_x, b.exp_g, dw + v0 * c.D);
+        PR_TRY(check_launch("pr_vocab_ce"));
+      }
     }
   }
   if (dx && c.P > 0) {
-    hipLaunchKernelGGL((vce_dx_kernel<T>), dim3((unsigned)((c.P * c.D + 255) / 256)), dim3(256), 0, st, c.P, c.D, s.Pp, s.Dk,
-                       b.splits, c.scale, b.acc, k.scal, b.exp_g, dx);
+    hipLaunchKernelGGL((vce_finish_kernel<T>), dim3((unsigned)((c.P + 3) / 4)), dim3(256), 0, st, c.P, c.D, s.Pp, s.Dk,
+                       b.split_words.n, c.scale, b.acc, &k.scal->exp_w, b.exp_g, dx);
     PR_TRY(check_launch("pr_vocab_ce"));
   }
   return PR_OK;
