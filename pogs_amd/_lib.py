@@ -113,6 +113,7 @@ class AdamGroup(ctypes.Structure):
                 ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double)]
 
 
+
 class GradClip(ctypes.Structure):
     """pr_grad_clip."""
     _fields_ = [("norm", ctypes.c_void_p), ("max_norm", ctypes.c_double)]

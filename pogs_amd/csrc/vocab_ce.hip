@@ -248,7 +248,8 @@ struct TransposeJob {
 
 // The packed copies for the contraction over rows, from those over columns: one 32x32 tile and plane per wavefront, as
 // two products with the identity.  Each value passes the matrix core as itself times one: exact.
-__global__ void __launch_bounds__(256) vce_transpose_kernel(TransposeJob w, TransposeJob x, int planes) {
+__device__ __forceinline__ void transpose_tiles(const TransposeJob &w, const TransposeJob &x, int planes, int64_t u,
+                                                int64_t step) {
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const int64_t nw = w.row_tiles * w.col_tiles, nx = x.row_tiles * x.col_tiles;
   h8v ident[2];
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(256) vce_transpose_kernel(TransposeJob w, Tran
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int i = 0; i < 8; ++i) ident[s][i] = 16 * s + 8 * h + i == (lane & 31) ? (_Float16)1.f : (_Float16)0.f;
-  for (int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); u < (nw + nx) * planes; u += (int64_t)gridDim.x * 4) {
+  for (; u < (nw + nx) * planes; u += step) {
     const int64_t pl = u >= nw + nx, v = pl ? u - (nw + nx) : u;
     const bool first = v < nw;
     const TransposeJob &j = first ? w : x;
@@ -278,6 +279,69 @@ __global__ void __launch_bounds__(256) vce_transpose_kernel(TransposeJob w, Tran
       dst[s * 64] = __builtin_bit_cast(u4v, o);
     }
   }
+}
+
+struct CoefJob {
+  int64_t P, Pp, V, ignore;
+  const int64_t *labels;
+  const float *g_loss, *g_lse;  // either may be NULL
+  int per_row, mean;
+  const Scalars *s;
+  int *exp_g;
+  float *a, *b;
+  __device__ __forceinline__ void row(int64_t p, float one, float &ra, float &rb) const {
+    ra = rb = 0.f;
+    if (p >= P || labels[p] == ignore) return;
+    rb = !g_loss ? 0.f : per_row ? g_loss[p] : one;
+    ra = rb + (g_lse ? g_lse[p] : 0.f);
+    if (g_loss && (labels[p] < 0 || labels[p] >= V)) ra = NAN;   // no such word: the row's loss is NaN
+  }
+};
+
+constexpr int COEF_ROWS = 4096;  // rows whose factors one workgroup writes
+
+// Row factors of G, scaled by the power of two that brings the largest to 2^12..2^13 (|G| <= |a| + |b|).  Every
+// workgroup looks for the largest itself; with one gradient for all rows there is nothing to look for.
+__device__ __forceinline__ void row_factors(const CoefJob &c, int block) {
+  const float one = c.g_loss && !c.per_row ? *c.g_loss * (c.mean ? 1.f / c.s->n_valid : 1.f) : 0.f;
+  float top = fabsf(one) < INFINITY ? fabsf(one) : 0.f;
+  if (c.per_row || c.g_lse) {
+    for (int64_t p = threadIdx.x; p < c.P; p += 1024) {
+      float a, b;
+      c.row(p, one, a, b);
+      a = fabsf(a), b = fabsf(b);
+      if (a < INFINITY) top = fmaxf(top, a);
+      if (b < INFINITY) top = fmaxf(top, b);
+    }
+    __shared__ float part[16];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = part[0];
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, part[i]);
+  }
+  const int e = top > 0.f ? TOP_EXP - 1 - ilogbf(top) : 0;
+  if (block == 0 && threadIdx.x == 0) *c.exp_g = e;
+  const int64_t end = min((int64_t)(block + 1) * COEF_ROWS, c.Pp);
+  for (int64_t p = (int64_t)block * COEF_ROWS + threadIdx.x; p < end; p += 1024) {
+    float a, b;
+    c.row(p, one, a, b);
+    c.a[p] = ldexpf(a, e);
+    c.b[p] = ldexpf(b, e);
+  }
+}
+
+// What the gradients' products need besides the packed operands, in one launch: the first workgroups write the row
+// factors, the others the transposed copies.
+__global__ void __launch_bounds__(1024) vce_prepare_kernel(CoefJob c, TransposeJob w, TransposeJob x, int planes) {
+  const int coef_blocks = (int)((c.Pp + COEF_ROWS - 1) / COEF_ROWS);
+  if ((int)blockIdx.x < coef_blocks) {
+    row_factors(c, blockIdx.x);
+    return;
+  }
+  transpose_tiles(w, x, planes, (int64_t)(blockIdx.x - coef_blocks) * 16 + (threadIdx.x >> 6),
+                  (int64_t)(gridDim.x - coef_blocks) * 16);
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------
@@ -891,45 +955,6 @@ __global__ void __launch_bounds__(1024) vce_reduce_kernel(int64_t P, const float
   }
 }
 
-// Row factors of G, scaled by the power of two that brings the largest to 2^12..2^13 (|G| <= |a| + |b|).
-__global__ void __launch_bounds__(1024) vce_coef_kernel(int64_t P, int64_t Pp, int64_t V, const float *__restrict__ g_loss,
-                                                        int per_row, int mean, const float *__restrict__ g_lse,
-                                                        const int64_t *__restrict__ labels, int64_t ignore,
-                                                        const Scalars *s, int *__restrict__ exp_g,
-                                                        float *__restrict__ coef_a, float *__restrict__ coef_b) {
-  const float inv = mean ? 1.f / s->n_valid : 1.f;
-  auto row = [&](int64_t p, float &a, float &b) {
-    a = b = 0.f;
-    if (p >= P || labels[p] == ignore) return;
-    b = g_loss ? g_loss[per_row ? p : 0] * inv : 0.f;
-    a = b + (g_lse ? g_lse[p] : 0.f);
-    if (g_loss && (labels[p] < 0 || labels[p] >= V)) a = NAN;   // no such word: the row's loss is NaN
-  };
-  float top = 0.f;
-  for (int64_t p = threadIdx.x; p < P; p += 1024) {
-    float a, b;
-    row(p, a, b);
-    a = fabsf(a), b = fabsf(b);
-    if (a < INFINITY) top = fmaxf(top, a);
-    if (b < INFINITY) top = fmaxf(top, b);
-  }
-  __shared__ float part[16];
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-  __syncthreads();
-  top = part[0];
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, part[i]);
-  const int e = top > 0.f ? TOP_EXP - 1 - ilogbf(top) : 0;
-  if (threadIdx.x == 0) *exp_g = e;
-  for (int64_t p = threadIdx.x; p < Pp; p += 1024) {
-    float a, b;
-    row(p, a, b);
-    coef_a[p] = ldexpf(a, e);
-    coef_b[p] = ldexpf(b, e);
-  }
-}
-
 // Rows of a gradient = sum of the splits, scaled, in the output type: a row per wavefront, four features per lane.
 template <typename T>
 __global__ void __launch_bounds__(256) vce_finish_kernel(int64_t P, int64_t D, int64_t Pp, int64_t ld, int splits, float scale,
@@ -1205,14 +1230,13 @@ template <typename T, int NP>
 int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b, const float *g_loss, const float *g_lse, T *dx,
              T *dw, hipStream_t st) {
   const Shape s(c.dtype, c.P, c.V, c.D);
-  hipLaunchKernelGGL(vce_coef_kernel, dim3(1), dim3(1024), 0, st, c.P, s.Pp, c.V, g_loss, per_row, mean, g_lse, c.labels,
-                     c.ignore, k.scal, b.exp_g, b.coef_a, b.coef_b);
-  PR_TRY(check_launch("pr_vocab_ce"));
   const int kb = (int)(s.Dk / 16), kv = (int)(s.Vp / 16), kp = (int)(s.Pp / 16);
+  const CoefJob coef{c.P, s.Pp, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, b.exp_g, b.coef_a, b.coef_b};
   const TransposeJob tw{k.wf, b.wt, s.plane(s.Vp), dx ? s.Vp / 32 : 0, s.Dk / 32};
   const TransposeJob tx{k.xf, b.xt, s.plane(s.Pp), dw ? s.Pp / 32 : 0, s.Dk / 32};
-  const int64_t turns = ((tw.row_tiles + tx.row_tiles) * (s.Dk / 32) * NP + 3) / 4;
-  hipLaunchKernelGGL(vce_transpose_kernel, dim3((unsigned)std::min<int64_t>(4096, turns)), dim3(256), 0, st, tw, tx, NP);
+  const int64_t turns = ((tw.row_tiles + tx.row_tiles) * (s.Dk / 32) * NP + 15) / 16;
+  hipLaunchKernelGGL(vce_prepare_kernel, dim3((unsigned)((s.Pp + COEF_ROWS - 1) / COEF_ROWS + std::min<int64_t>(1024, turns))),
+                     dim3(1024), 0, st, coef, tw, tx, NP);
   PR_TRY(check_launch("pr_vocab_ce"));
   for (int64_t v0 = 0; v0 < s.Vp; v0 += b.piece) {
     const int64_t words = std::min(b.piece, s.Vp - v0);

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from array import array
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
@@ -25,9 +26,11 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .rendering import _call, _stream
+from .rendering import _call, _on, _stream
 
 
+_ADAM_GROUP = struct.Struct("=4Q2q4d")     # pr_adam_group
+_GRAD_CLIP = struct.Struct("=Qd")           # pr_grad_clip
 _GRAD_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}        # PR_F32, PR_F16, PR_BF16
 _NORM_KINDS = {1.0: 1, 2.0: 2, math.inf: 3}                                   # PR_NORM_1, PR_NORM_2, PR_NORM_INF
 
@@ -42,11 +45,11 @@ def _one_block(t: Tensor) -> bool:
     return True
 
 
-def _grad_table(grads: Sequence[Tensor], sets: Sequence[int]) -> array:
+def _grad_table(grads: Sequence[Tensor], sets: Optional[Sequence[int]] = None) -> array:
     """The grads as an array of ``pr_grad_tensor``: pointer, elements, type and set (the upper half word)."""
     words = array("q")
-    for g, s in zip(grads, sets):
-        words.extend((g.data_ptr(), g.numel(), _GRAD_TYPES[g.dtype] | s << 32))
+    for i, g in enumerate(grads):
+        words.extend((g.data_ptr(), g.numel(), _GRAD_TYPES[g.dtype] | (sets[i] << 32 if sets else 0)))
     return words
 
 
@@ -54,20 +57,18 @@ def _address(a: array) -> ctypes.c_void_p:
     return ctypes.c_void_p(a.buffer_info()[0])
 
 
-def _set_norms(grads: Sequence[Tensor], sets: Sequence[int], n_sets: int, kind: int) -> Tuple[array, Tensor]:
-    """``norms [n_sets]`` (float32, on the device) of gradients ordered by set, and their table.  Runs on the current
-    stream of the current device."""
+def _set_norms(table: array, shape: tuple, kind: int, device, stream: int) -> Tensor:
+    """The norms (float32, on the device) of the sets of a table of gradients ordered by set: ``()`` or ``(sets,)``."""
     lib = _lib.load()
-    table = _grad_table(grads, sets)
-    at, n = _address(table), len(grads)
+    at, n, n_sets = _address(table), len(table) // 3, shape[0] if shape else 1
     nbytes = lib.pr_grad_norm_scratch_bytes(at, n, n_sets)
-    scratch = torch.empty(max(nbytes // 8, 1), dtype=torch.float64, device=grads[0].device)
-    norms = torch.empty(n_sets, dtype=torch.float32, device=grads[0].device)
-    _call("pr_grad_norm", at, n, n_sets, kind, scratch.data_ptr(), nbytes, norms.data_ptr(), _stream())
-    return table, norms
+    scratch = torch.empty(max(nbytes // 8, 1), dtype=torch.float64, device=device)
+    norms = torch.empty(shape, dtype=torch.float32, device=device)
+    _call("pr_grad_norm", at, n, n_sets, kind, scratch.data_ptr(), nbytes, norms.data_ptr(), stream)
+    return norms
 
 
-def _check_grads(grads: Sequence[Tensor]) -> None:
+def _check_grads(grads: Sequence[Tensor]) -> torch.device:
     dev = grads[0].device
     for g in grads:
         if g.is_sparse or not g.is_cuda:
@@ -76,6 +77,7 @@ def _check_grads(grads: Sequence[Tensor]) -> None:
             raise TypeError(f"gradients must be float32, float16 or bfloat16, got {g.dtype}")
         if g.device != dev:
             raise RuntimeError(f"gradients are on different devices: {dev} and {g.device}")
+    return dev
 
 
 def _norm_kind(norm_type: float) -> int:
@@ -101,10 +103,10 @@ def grad_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) 
     grads = [tensors] if isinstance(tensors, Tensor) else list(tensors)
     if not grads:
         return torch.tensor(0.0)
-    _check_grads(grads)
-    with torch.no_grad(), torch.cuda.device(grads[0].device):
-        flat = [g if g.is_contiguous() or _one_block(g) else g.contiguous() for g in grads]
-        return _set_norms(flat, [0] * len(flat), 1, kind)[1][0]
+    dev = _check_grads(grads)
+    with _on(dev):
+        flat = [g if g.is_contiguous() or _one_block(g) else g.detach().contiguous() for g in grads]
+        return _set_norms(_grad_table(flat), (), kind, dev, _stream())
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -122,20 +124,22 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     grads = [p.grad for p in params if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
-    _check_grads(grads)
-    with torch.no_grad(), torch.cuda.device(grads[0].device):
-        flat = [g if g.is_contiguous() or _one_block(g) else g.contiguous() for g in grads]
-        table, norms = _set_norms(flat, [0] * len(flat), 1, kind)
+    dev = _check_grads(grads)
+    with _on(dev):
+        flat = [g if g.is_contiguous() or _one_block(g) else g.detach().contiguous() for g in grads]
+        table, stream = _grad_table(flat), _stream()
+        norms = _set_norms(table, (), kind, dev, stream)
         if error_if_nonfinite and not math.isfinite(norms.item()):
             raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is "
                                "non-finite, so it cannot be clipped. To disable this error and scale the gradients by "
                                "the non-finite norm anyway, set `error_if_nonfinite=False`")
         limit = ctypes.c_double(max_norm)
-        _call("pr_grad_scale", _address(table), len(flat), 1, norms.data_ptr(), ctypes.addressof(limit), _stream())
+        _call("pr_grad_scale", _address(table), len(flat), 1, norms.data_ptr(), ctypes.addressof(limit), stream)
         for g, f in zip(grads, flat):
             if f is not g:
-                g.copy_(f)
-        return norms[0]
+                with torch.no_grad():
+                    g.copy_(f)
+        return norms
 
 
 class ExponentialDecay:
@@ -164,14 +168,14 @@ class Optimizers:
 
     ``max_norm``: the group's gradient, over all its parameters, is clipped to that 2-norm in every step, as by
     ``clip_grad_norm_``; the parameters' ``.grad`` keep their values.  ``grad_norms`` holds the norms that the last step
-    clipped by, one 0-d device tensor a group."""
+    clipped by."""
 
     def __init__(self, config: Dict[str, dict], param_groups: Dict[str, List[Tensor]]):
         _lib.load()
         self.config, self.parameters = config, {}
         self._state: Dict[str, List[dict]] = {}
         self._sched_steps: Dict[str, int] = {}
-        self.grad_norms: Dict[str, Tensor] = {}
+        self._norms: List[Tuple[Tensor, Dict[str, int]]] = []
         for name, params in param_groups.items():
             if name not in config:
                 raise RuntimeError(f"Optimizer config for '{name}' not found in config file. Provided configs "
@@ -247,43 +251,49 @@ class Optimizers:
                 elif limit is not None:
                     clipped.append((name, _max_norm(limit), len(entries)))
                 keep.append(g)
-                entries.append(_lib.AdamGroup(p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(),
-                                              st["exp_avg_sq"].data_ptr(), p.numel(), st["step"], lr, b1, b2, eps))
-        self.grad_norms = {}
+                entries.append(_ADAM_GROUP.pack(p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(),
+                                                st["exp_avg_sq"].data_ptr(), p.numel(), st["step"], lr, b1, b2, eps))
+        self._norms = []
         if not entries:
             return
         lib = _lib.load()
         chunk = lib.pr_adam_max_groups()
-        dev = keep[0].device
-        with torch.cuda.device(dev), torch.no_grad():
-            clips = self._clips(clipped, keep, param_groups, len(entries)) if clipped else None
+        with _on(keep[0].device):
+            stream = _stream()
+            clips = self._clips(clipped, keep, param_groups, len(entries), stream) if clipped else None
             for i in range(0, len(entries), chunk):
                 part = entries[i:i + chunk]
-                arr = (_lib.AdamGroup * len(part))(*part)
                 if clips is None:
-                    _call("pr_adam_step", ctypes.cast(arr, ctypes.c_void_p), len(part), _stream())
+                    _call("pr_adam_step", b"".join(part), len(part), stream)
                 else:
-                    by = (_lib.GradClip * len(part))(*clips[i:i + chunk])
-                    _call("pr_adam_step_clipped", ctypes.cast(arr, ctypes.c_void_p), ctypes.cast(by, ctypes.c_void_p),
-                          len(part), _stream())
+                    _call("pr_adam_step_clipped", b"".join(part), b"".join(clips[i:i + chunk]), len(part), stream)
         del keep
 
-    def _clips(self, clipped, grads: List[Tensor], param_groups: List[str], n: int) -> List[_lib.GradClip]:
-        """``pr_grad_clip`` of every entry of a step, the norms on their way on the current stream."""
-        clips = [_lib.GradClip(None, 0.0)] * n
+    def _clips(self, clipped, grads: List[Tensor], param_groups: List[str], n: int, stream: int) -> List[bytes]:
+        """``pr_grad_clip`` of every entry of a step, the norms on their way on the given stream."""
+        clips = [_GRAD_CLIP.pack(0, 0.0)] * n
         names = list(dict.fromkeys(name for name, _, _ in clipped))
         most = _lib.load().pr_grad_norm_max_sets()
         for lo in range(0, len(names), most):
             of = {name: i for i, name in enumerate(names[lo:lo + most])}
             mine = [c for c in clipped if c[0] in of]
-            _, norms = _set_norms([grads[k] for _, _, k in mine], [of[name] for name, _, _ in mine], len(of), 2)
-            each = norms.unbind()
+            table = _grad_table([grads[k] for _, _, k in mine], [of[name] for name, _, _ in mine])
+            norms = _set_norms(table, (len(of),), 2, grads[0].device, stream)
+            at = norms.data_ptr()
             for name, limit, k in mine:
-                clips[k] = _lib.GradClip(each[of[name]].data_ptr(), limit)
-            for name, i in of.items():      # these hold the storage that the step's kernel reads
-                for group in (param_groups if name is None else [name]):
-                    self.grad_norms[group] = each[i]
+                clips[k] = _GRAD_CLIP.pack(at + 4 * of[name], limit)
+            # (this holds the storage that the step's kernel reads)
+            self._norms.append((norms, {g: 0 for g in param_groups} if None in of else of))
         return clips
+
+    @property
+    def grad_norms(self) -> Dict[str, Tensor]:
+        """The norms that the last step clipped by, one 0-d tensor on the device for each group."""
+        out = {}
+        for norms, of in self._norms:
+            each = norms.unbind()
+            out.update((name, each[i]) for name, i in of.items())
+        return out
 
     def state(self, name: str, index: int = 0) -> dict:
         """The Adam state of one parameter of a group (``step``, ``exp_avg``, ``exp_avg_sq``; empty before its first

@@ -13,6 +13,7 @@ costs one projection, one binning and one walk over the tile lists instead of tw
 """
 from __future__ import annotations
 
+import contextlib
 import math
 import os
 import threading
@@ -32,6 +33,14 @@ def _ptr(t: Optional[Tensor]):
 
 def _stream():
     return torch.cuda.current_stream().cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Context in which ``device`` is the current one: nothing to do where it already is (the change costs 3 us)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 class StageTimer:

@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 from torch.autograd.graph import get_gradient_edge
 
 from . import _lib
-from .rendering import _call, _ptr, _stream
+from .rendering import _call, _on, _ptr, _stream
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # PR_F32, PR_F16, PR_BF16
 _REDUCTIONS = ("none", "sum", "mean")
@@ -29,32 +29,35 @@ def _scratch(nbytes: int, device) -> Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
-class _VocabularyCrossEntropy(torch.autograd.Function):
-    """``x [P, D]``, ``w [V, D]``, ``labels [P]`` int64 -> (loss, lse): loss ``[P]`` or 0-d, lse ``[P]``."""
+def _forward(x, w, labels, scale, ignore_index, reduction, want_lse, with_grad):
+    """``x [P, D]``, ``w [V, D]``, ``labels [P]`` int64 -> loss (``[P]`` or 0-d), lse ``[P]`` or None, what backward keeps."""
+    (P, D), V, dev = x.shape, w.shape[0], x.device
+    row_loss = torch.empty(P, dtype=torch.float32, device=dev)
+    lse = torch.empty(P, dtype=torch.float32, device=dev) if want_lse else None
+    if P == 0:
+        total = {"none": row_loss, "sum": row_loss.new_zeros(()), "mean": row_loss.new_full((), math.nan)}
+        return total[reduction], lse, None
+    loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
+    lib, t = _lib.load(), _TYPES[x.dtype]
+    # few rows and no gradient to come: nothing is packed and nothing kept
+    plain = not with_grad and P <= lib.pr_vocab_ce_score_rows()
+    kept = None if plain else _scratch(lib.pr_vocab_ce_kept_bytes(t, P, V, D), dev)
+    scratch = _scratch(lib.pr_vocab_ce_fwd_scratch_bytes(t, P, V, D), dev)
+    with _on(dev):
+        _call("pr_vocab_ce_fwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index, scale,
+              int(reduction == "mean"), _ptr(kept), 0 if plain else kept.numel(), _ptr(scratch), scratch.numel(),
+              _ptr(row_loss), _ptr(lse), _ptr(loss), _stream())
+    return (row_loss if loss is None else loss), lse, kept
 
+
+class _VocabularyCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, labels, scale, ignore_index, reduction, with_grad):
+    def forward(ctx, x, w, labels, scale, ignore_index, reduction, want_lse):
         ctx.set_materialize_grads(False)
         ctx.args = scale, ignore_index, reduction
-        (P, D), V, dev = x.shape, w.shape[0], x.device
-        row_loss = torch.empty(P, dtype=torch.float32, device=dev)
-        lse = torch.empty(P, dtype=torch.float32, device=dev)
-        if P == 0:
-            ctx.save_for_backward(x, w, labels, None)
-            total = {"none": row_loss, "sum": row_loss.new_zeros(()), "mean": row_loss.new_full((), math.nan)}
-            return total[reduction], lse
-        loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
-        lib, t = _lib.load(), _TYPES[x.dtype]
-        with torch.cuda.device(dev):
-            # few rows and no gradient to come: nothing is packed and nothing kept
-            plain = not with_grad and P <= lib.pr_vocab_ce_score_rows()
-            kept = _scratch(0 if plain else lib.pr_vocab_ce_kept_bytes(t, P, V, D), dev)
-            scratch = _scratch(lib.pr_vocab_ce_fwd_scratch_bytes(t, P, V, D), dev)
-            _call("pr_vocab_ce_fwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index,
-                  scale, int(reduction == "mean"), None if plain else _ptr(kept), kept.numel(), _ptr(scratch),
-                  scratch.numel(), _ptr(row_loss), _ptr(lse), _ptr(loss), _stream())
+        loss, lse, kept = _forward(x, w, labels, scale, ignore_index, reduction, want_lse, True)
         ctx.save_for_backward(x, w, labels, kept)
-        return (row_loss if reduction == "none" else loss), lse
+        return loss, lse
 
     @staticmethod
     @once_differentiable
@@ -70,8 +73,8 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
         dx = torch.empty(P, D, dtype=x.dtype, device=dev) if want_x else None
         dw = torch.empty(V, D, dtype=w.dtype, device=dev) if want_w else None
         lib, t = _lib.load(), _TYPES[x.dtype]
-        with torch.cuda.device(dev):
-            scratch = _scratch(lib.pr_vocab_ce_bwd_scratch_bytes(t, P, V, D, int(want_x), int(want_w)), dev)
+        scratch = _scratch(lib.pr_vocab_ce_bwd_scratch_bytes(t, P, V, D, int(want_x), int(want_w)), dev)
+        with _on(dev):
             _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index,
                   scale, int(reduction == "mean"), int(reduction == "none"), _ptr(kept), kept.numel(), _ptr(g_loss),
                   _ptr(g_lse), _ptr(scratch), scratch.numel(), _ptr(dx), _ptr(dw), _stream())
@@ -87,7 +90,7 @@ def _leaf_nodes(*tensors: Tensor) -> list:
     one part of the capture, which ends the process.  So the call that would lead there is refused."""
     nodes = []
     for t in tensors:
-        if torch.is_grad_enabled() and t.is_leaf and t.requires_grad:
+        if t.is_leaf and t.requires_grad:
             node = get_gradient_edge(t).node
             stream = torch.cuda.current_stream(t.device).cuda_stream
             if node.metadata.setdefault(_STREAM_KEY, stream) != stream and torch.cuda.is_current_stream_capturing():
@@ -137,13 +140,17 @@ def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tenso
     and the host does not wait to look.  Safe in a captured graph, gradients included, as long as no graph of the same
     leaves made outside the capture is alive (refused where one of this function is)."""
     scale = _check(features, vocabulary, labels, scale, reduction)
-    nodes = _leaf_nodes(features, vocabulary)    # held until the new graph holds them
     D = features.shape[-1]
-    x = features.reshape(-1, D)
-    flat = labels.reshape(-1).to(torch.int64).contiguous()
-    with_grad = torch.is_grad_enabled() and (x.requires_grad or vocabulary.requires_grad)
-    loss, lse = _VocabularyCrossEntropy.apply(x, vocabulary, flat, scale, int(ignore_index), reduction, with_grad)
-    del nodes
-    if reduction == "none":
+    x = features if features.dim() == 2 else features.reshape(-1, D)
+    flat = labels if labels.dim() == 1 else labels.reshape(-1)
+    if flat.dtype != torch.int64 or not flat.is_contiguous():
+        flat = flat.to(torch.int64).contiguous()
+    if torch.is_grad_enabled() and (features.requires_grad or vocabulary.requires_grad):
+        nodes = _leaf_nodes(features, vocabulary)    # held until the new graph holds them
+        loss, lse = _VocabularyCrossEntropy.apply(x, vocabulary, flat, scale, int(ignore_index), reduction, return_lse)
+        del nodes
+    else:
+        loss, lse, _ = _forward(x, vocabulary, flat, scale, int(ignore_index), reduction, return_lse, False)
+    if reduction == "none" and labels.dim() != 1:
         loss = loss.reshape(labels.shape)
     return (loss, lse.reshape(labels.shape)) if return_lse else loss
