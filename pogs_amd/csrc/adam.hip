@@ -41,6 +41,9 @@ struct ClipTable {  // per group: where its gradient norm is (NULL: not clipped)
   float max_norm[MAX_GROUPS];
 };
 struct NoClip {};
+// From the last element to the first where a norm has been taken just before: the end of the gradients is still cached.
+__device__ __forceinline__ unsigned block_of(const NoClip &) { return blockIdx.x; }
+__device__ __forceinline__ unsigned block_of(const ClipTable &) { return gridDim.x - 1 - blockIdx.x; }
 __device__ __forceinline__ float gradient_factor(const NoClip &, int) { return 1.f; }
 __device__ __forceinline__ float gradient_factor(const ClipTable &c, int gi) {
   return c.norm[gi] ? clip_coefficient(*c.norm[gi], c.max_norm[gi]) : 1.f;
@@ -58,9 +61,10 @@ __device__ __forceinline__ void adam_update(float &p, float g, float &m, float &
 // elements.  CLIP = NoClip: the factor is a constant 1 and drops out.
 template <typename CLIP>
 __global__ void __launch_bounds__(BLOCK) adam_kernel(const AdamTable t, const CLIP clip) {
+  const unsigned block = block_of(clip);
   int gi = 0;
 #pragma unroll 1
-  while (gi + 1 < t.n && blockIdx.x >= t.first_block[gi + 1]) ++gi;
+  while (gi + 1 < t.n && block >= t.first_block[gi + 1]) ++gi;
   const int64_t n = t.numel[gi];
   float *__restrict__ p = t.param[gi];
   const float *__restrict__ g = t.grad[gi];
@@ -68,7 +72,7 @@ __global__ void __launch_bounds__(BLOCK) adam_kernel(const AdamTable t, const CL
   float *__restrict__ v = t.exp_avg_sq[gi];
   const float ss = t.step_size[gi], omb1 = t.one_minus_beta1[gi], b2 = t.beta2[gi], omb2 = t.one_minus_beta2[gi],
               bc = t.bias2_sqrt[gi], eps = t.eps[gi];
-  const int64_t base = (int64_t)(blockIdx.x - t.first_block[gi]) * PER_BLOCK;
+  const int64_t base = (int64_t)(block - t.first_block[gi]) * PER_BLOCK;
   const float factor = gradient_factor(clip, gi);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {

@@ -5,11 +5,11 @@
 //   norm_s = sqrt(sum over the tensors of set s of g^2)        (or sum |g|, or max |g|)
 //   g     <- g * min(1, max_norm_s / (norm_s + 1e-6))
 //
-// HBM-bound: the norm reads every gradient once, the scaling reads and writes it once.  The tensors of a launch are laid
-// end to end in one index space, each rounded up to 64 elements, and every workgroup takes an equal range of it: the
-// number of workgroups follows the number of elements and not of tensors, and a range starts on a 64-element boundary of
-// its tensor, so that 16-byte accesses stay aligned wherever the tensor is.  A set of tensors (one norm) starts on a
-// workgroup boundary; all sets share the launch.  Sums are kept in float64 from the first
+// HBM-bound: the norm reads every gradient once, the scaling reads and writes it once.  Every tensor of a launch gets
+// workgroups by its size, at least one (a workgroup that went through several small tensors would wait out the memory
+// latency of each: 26 against 5 us for 56 tensors of 1 to 2 M elements), and they take its chunks of 4096 elements in
+// turn, so that the chip reads one run of memory at a time.  The scaling goes through the chunks from the last to the
+// first: the last ones read for the norm are still in the 256 MB cache behind HBM.  Sums are kept in float64 from the first
 // element on (float32 gradients of 1e30 square to a finite value, and the order of the sum does not show in float32);
 // partials go to memory, one per workgroup and set, and are added in one fixed order: the result does not depend on the
 // order in which workgroups run.
@@ -26,16 +26,14 @@ namespace {
 constexpr int MAX_TENSORS = 128;  // per launch: the table travels in the kernel argument (at most 4 KB)
 constexpr int MAX_SETS = 32;
 constexpr int BLOCK = 256;
-constexpr int64_t UNIT = 64;        // elements a tensor is rounded up to in the launch's index space
-constexpr int64_t MIN_RANGE = 8192;  // elements per workgroup at least
-constexpr int MAX_BLOCKS = 2048;     // per launch: eight workgroups for each CU
+constexpr int64_t CHUNK = 4096;  // elements a workgroup takes at a time: 16 each, in 16-byte accesses
+constexpr int MAX_BLOCKS = 2048;  // per launch, besides one for each tensor: eight workgroups for each CU
 
 struct Table {
   void *grad[MAX_TENSORS];
   int64_t numel[MAX_TENSORS];
-  unsigned first_unit[MAX_TENSORS + 1];
+  unsigned first_block[MAX_TENSORS + 1];
   unsigned char dtype[MAX_TENSORS], set[MAX_TENSORS];
-  unsigned units_per_block;
   int n;
 };
 
@@ -80,86 +78,69 @@ __device__ __forceinline__ double block_combine(double v) {
   return v;
 }
 
-// The tensor whose units hold `unit`.
-__device__ __forceinline__ int find_tensor(const Table &t, unsigned unit) {
+// The tensor that a workgroup belongs to.
+__device__ __forceinline__ int find_tensor(const Table &t, unsigned block) {
   int lo = 0, hi = t.n - 1;
 #pragma unroll 1
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (t.first_unit[mid] <= unit) lo = mid;
+    if (t.first_block[mid] <= block) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
 
-template <int KIND>
-__device__ __forceinline__ double range_norm(const void *grad, int dtype, int64_t lo, int64_t hi) {
-  double acc[4] = {0., 0., 0., 0.};
+__device__ __forceinline__ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// f(value) for this thread's elements of a chunk that starts at `lo` and has `left` elements (more than CHUNK: a whole one)
+template <typename F>
+__device__ __forceinline__ void each_of_chunk(const void *grad, int dtype, int64_t lo, int64_t left, F f) {
   if (dtype == PR_F32) {
-    const float *g = (const float *)grad;
-    const bool vec = ((uintptr_t)g & 15) == 0;
-    int64_t i = lo + 4 * threadIdx.x;
-    if (vec) {
-      for (; i + 3 * 4 * BLOCK + 3 < hi; i += 4 * 4 * BLOCK) {
-        float4 v[4];
+    const float *g = (const float *)grad + lo;
+    if (left >= CHUNK && aligned16(g)) {
+      float4 v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const float4 *>(g + i + u * 4 * BLOCK);
+      for (int u = 0; u < 4; ++u) v[u] = reinterpret_cast<const float4 *>(g)[u * BLOCK + threadIdx.x];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          take<KIND>(acc[0], v[u].x), take<KIND>(acc[1], v[u].y);
-          take<KIND>(acc[2], v[u].z), take<KIND>(acc[3], v[u].w);
-        }
-      }
+      for (int u = 0; u < 4; ++u) f(v[u].x, 0), f(v[u].y, 1), f(v[u].z, 2), f(v[u].w, 3);
+    } else {
+#pragma unroll 8
+      for (int u = 0; u < 16; ++u)
+        if (u * BLOCK + (int)threadIdx.x < left) f(g[u * BLOCK + threadIdx.x], u & 3);
     }
-    for (; i < hi; i += 4 * BLOCK)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (i + k < hi) take<KIND>(acc[k], g[i + k]);
   } else {
-    const unsigned short *g = (const unsigned short *)grad;
-    const bool vec = ((uintptr_t)g & 15) == 0;
-    int64_t i = lo + 8 * threadIdx.x;
-    if (vec) {
-      for (; i + 8 * BLOCK + 7 < hi; i += 2 * 8 * BLOCK) {
-        uint4 v[2];
+    const unsigned short *g = (const unsigned short *)grad + lo;
+    if (left >= CHUNK && aligned16(g)) {
+      uint4 v[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) v[u] = *reinterpret_cast<const uint4 *>(g + i + u * 8 * BLOCK);
+      for (int u = 0; u < 2; ++u) v[u] = reinterpret_cast<const uint4 *>(g)[u * BLOCK + threadIdx.x];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      for (int u = 0; u < 2; ++u) {
+        const unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            take<KIND>(acc[k], from_bits16((unsigned short)(w[k] & 0xffffu), dtype));
-            take<KIND>(acc[k], from_bits16((unsigned short)(w[k] >> 16), dtype));
-          }
+        for (int k = 0; k < 4; ++k) {
+          f(from_bits16((unsigned short)(w[k] & 0xffffu), dtype), k);
+          f(from_bits16((unsigned short)(w[k] >> 16), dtype), k);
         }
       }
+    } else {
+#pragma unroll 8
+      for (int u = 0; u < 16; ++u)
+        if (u * BLOCK + (int)threadIdx.x < left) f(from_bits16(g[u * BLOCK + threadIdx.x], dtype), u & 3);
     }
-    for (; i < hi; i += 8 * BLOCK)
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (i + k < hi) take<KIND>(acc[k & 3], from_bits16(g[i + k], dtype));
   }
-  return combine<KIND>(combine<KIND>(acc[0], acc[1]), combine<KIND>(acc[2], acc[3]));
 }
 
 template <int KIND>
 __global__ void __launch_bounds__(BLOCK) grad_norm_kernel(const Table t, double *__restrict__ partials) {
-  unsigned unit = blockIdx.x * t.units_per_block;
-  const unsigned end = min(unit + t.units_per_block, t.first_unit[t.n]);
-  double acc = 0.;
-  int k = find_tensor(t, unit);
-#pragma unroll 1
-  while (unit < end) {
-    const unsigned stop = min(end, t.first_unit[k + 1]);
-    const int64_t lo = (int64_t)(unit - t.first_unit[k]) * UNIT;
-    const int64_t hi = min((int64_t)(stop - t.first_unit[k]) * UNIT, t.numel[k]);
-    acc = combine<KIND>(acc, range_norm<KIND>(t.grad[k], t.dtype[k], lo, hi));
-    unit = stop;
-    ++k;
-  }
-  acc = block_combine<KIND>(acc);
-  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+  const int k = find_tensor(t, blockIdx.x);
+  const unsigned first = t.first_block[k], blocks = t.first_block[k + 1] - first;
+  const int64_t n = t.numel[k];
+  double acc[4] = {0., 0., 0., 0.};
+  for (int64_t lo = (int64_t)(blockIdx.x - first) * CHUNK; lo < n; lo += (int64_t)blocks * CHUNK)
+    each_of_chunk(t.grad[k], t.dtype[k], lo, n - lo, [&](float g, int at) { take<KIND>(acc[at], g); });
+  const double all = block_combine<KIND>(combine<KIND>(combine<KIND>(acc[0], acc[1]), combine<KIND>(acc[2], acc[3])));
+  if (threadIdx.x == 0) partials[blockIdx.x] = all;
 }
 
 template <int KIND>
@@ -172,63 +153,59 @@ __global__ void __launch_bounds__(BLOCK) grad_norm_finish_kernel(const SetRanges
   if (threadIdx.x == 0) norms[s] = (float)(KIND == PR_NORM_2 ? sqrt(acc) : acc);
 }
 
-__device__ __forceinline__ void range_scale(void *grad, int dtype, int64_t lo, int64_t hi, float c) {
+__device__ __forceinline__ void scale_chunk(void *grad, int dtype, int64_t lo, int64_t left, float c) {
   if (dtype == PR_F32) {
-    float *g = (float *)grad;
-    int64_t i = lo + 4 * threadIdx.x;
-    if (((uintptr_t)g & 15) == 0) {
-      for (; i + 4 * BLOCK + 3 < hi; i += 2 * 4 * BLOCK) {
-        float4 a = *reinterpret_cast<float4 *>(g + i), b = *reinterpret_cast<float4 *>(g + i + 4 * BLOCK);
-        a.x *= c, a.y *= c, a.z *= c, a.w *= c;
-        b.x *= c, b.y *= c, b.z *= c, b.w *= c;
-        *reinterpret_cast<float4 *>(g + i) = a;
-        *reinterpret_cast<float4 *>(g + i + 4 * BLOCK) = b;
-      }
-    }
-    for (; i < hi; i += 4 * BLOCK)
+    float *g = (float *)grad + lo;
+    if (left >= CHUNK && aligned16(g)) {
+      float4 v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (i + k < hi) g[i + k] *= c;
+      for (int u = 0; u < 4; ++u) v[u] = reinterpret_cast<float4 *>(g)[u * BLOCK + threadIdx.x];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        reinterpret_cast<float4 *>(g)[u * BLOCK + threadIdx.x] = make_float4(v[u].x * c, v[u].y * c, v[u].z * c, v[u].w * c);
+    } else {
+#pragma unroll 8
+      for (int u = 0; u < 16; ++u)
+        if (u * BLOCK + (int)threadIdx.x < left) g[u * BLOCK + threadIdx.x] *= c;
+    }
   } else {
-    unsigned short *g = (unsigned short *)grad;
-    int64_t i = lo + 8 * threadIdx.x;
-    if (((uintptr_t)g & 15) == 0) {
-      for (; i + 7 < hi; i += 8 * BLOCK) {
-        uint4 v = *reinterpret_cast<uint4 *>(g + i);
-        unsigned w[4] = {v.x, v.y, v.z, v.w};
+    unsigned short *g = (unsigned short *)grad + lo;
+    if (left >= CHUNK && aligned16(g)) {
+      uint4 v[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) v[u] = reinterpret_cast<uint4 *>(g)[u * BLOCK + threadIdx.x];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const unsigned a = to_bits16(from_bits16((unsigned short)(w[k] & 0xffffu), dtype) * c, dtype);
           const unsigned b = to_bits16(from_bits16((unsigned short)(w[k] >> 16), dtype) * c, dtype);
           w[k] = a | (b << 16);
         }
-        *reinterpret_cast<uint4 *>(g + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4 *>(g)[u * BLOCK + threadIdx.x] = make_uint4(w[0], w[1], w[2], w[3]);
       }
+    } else {
+#pragma unroll 8
+      for (int u = 0; u < 16; ++u)
+        if (u * BLOCK + (int)threadIdx.x < left)
+          g[u * BLOCK + threadIdx.x] = to_bits16(from_bits16(g[u * BLOCK + threadIdx.x], dtype) * c, dtype);
     }
-    for (; i < hi; i += 8 * BLOCK)
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (i + k < hi) g[i + k] = to_bits16(from_bits16(g[i + k], dtype) * c, dtype);
   }
 }
 
 __global__ void __launch_bounds__(BLOCK) grad_scale_kernel(const Table t, const float *__restrict__ norms,
                                                            const MaxNorms max_norms) {
-  unsigned unit = blockIdx.x * t.units_per_block;
-  const unsigned end = min(unit + t.units_per_block, t.first_unit[t.n]);
-  int k = find_tensor(t, unit);
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const int k = find_tensor(t, block);
   const float c = clip_coefficient(norms[t.set[k]], max_norms.of[t.set[k]]);
   // a norm within bounds leaves every value as it is: nothing to read or write (NaN is no such norm)
   if (c == 1.f) return;
-#pragma unroll 1
-  while (unit < end) {
-    const unsigned stop = min(end, t.first_unit[k + 1]);
-    const int64_t lo = (int64_t)(unit - t.first_unit[k]) * UNIT;
-    const int64_t hi = min((int64_t)(stop - t.first_unit[k]) * UNIT, t.numel[k]);
-    range_scale(t.grad[k], t.dtype[k], lo, hi, c);
-    unit = stop;
-    ++k;
-  }
+  const unsigned first = t.first_block[k], blocks = t.first_block[k + 1] - first;
+  const int64_t n = t.numel[k], chunks = (n + CHUNK - 1) / CHUNK;
+  // this workgroup's chunks, the last one first
+  int64_t i = block - first;
+  for (i += (chunks - 1 - i) / blocks * blocks; i >= 0; i -= blocks) scale_chunk(t.grad[k], t.dtype[k], i * CHUNK, n - i * CHUNK, c);
 }
 
 // Cuts the host's list into launches of at most MAX_TENSORS tensors.  next() fills the table (n == 0 at the end).
@@ -243,39 +220,27 @@ struct Launches {
     t.n = 0;
     blocks = 0;
     std::fill(set_blocks, set_blocks + MAX_SETS, 0u);
-    int64_t total = 0;
+    int64_t chunks = 0;
     for (; at < n && t.n < MAX_TENSORS; ++at) {
       const pr_grad_tensor &g = tensors[at];
       if (g.numel == 0) continue;
-      const int64_t u = (g.numel + UNIT - 1) / UNIT;
-      if (total + u > 0x3fffffffll) {
-        if (t.n == 0) return PR_EUNSUPPORTED;
-        break;
-      }
       t.grad[t.n] = g.grad;
       t.numel[t.n] = g.numel;
       t.dtype[t.n] = (unsigned char)g.dtype;
       t.set[t.n] = (unsigned char)g.set;
-      total += u;
+      chunks += (g.numel + CHUNK - 1) / CHUNK;
       ++t.n;
     }
-    const int64_t per = std::max<int64_t>((total + MAX_BLOCKS - 1) / MAX_BLOCKS, MIN_RANGE / UNIT);
-    t.units_per_block = (unsigned)per;
-    // total <= 2^30 and at most MAX_SETS roundings to per < 2^20: below 2^32
-    int64_t units = 0;
-    auto close = [&](int set) {  // the set's last workgroup keeps the rest of its range
-      const int64_t b = (units + per - 1) / per;
-      set_blocks[set] = (unsigned)(b - blocks);
-      blocks = (unsigned)b;
-      units = b * per;
-    };
+    // two chunks a workgroup at least, more where that would be too many workgroups
+    const int64_t per = std::max<int64_t>((chunks + MAX_BLOCKS - 1) / MAX_BLOCKS, 2);
     for (int k = 0; k < t.n; ++k) {
-      if (k > 0 && t.set[k] != t.set[k - 1]) close(t.set[k - 1]);
-      t.first_unit[k] = (unsigned)units;
-      units += (t.numel[k] + UNIT - 1) / UNIT;
+      const int64_t c = (t.numel[k] + CHUNK - 1) / CHUNK;
+      const unsigned b = (unsigned)((c + per - 1) / per);
+      t.first_block[k] = blocks;
+      blocks += b;
+      set_blocks[t.set[k]] += b;
     }
-    if (t.n > 0) close(t.set[t.n - 1]);
-    t.first_unit[t.n] = (unsigned)units;
+    t.first_block[t.n] = blocks;
     return PR_OK;
   }
 };
@@ -284,7 +249,7 @@ int check_tensors(const pr_grad_tensor *tensors, int n, int n_sets) {
   if (n < 0 || n_sets < 1 || n_sets > MAX_SETS || (n > 0 && !tensors)) return PR_EINVAL;
   for (int i = 0; i < n; ++i) {
     const pr_grad_tensor &g = tensors[i];
-    if (g.numel < 0 || (g.numel > 0 && !g.grad) || g.dtype < PR_F32 || g.dtype > PR_BF16) return PR_EINVAL;
+    if (g.numel < 0 || g.numel > (1ll << 38) || (g.numel > 0 && !g.grad) || g.dtype < PR_F32 || g.dtype > PR_BF16) return PR_EINVAL;
     if (((uintptr_t)g.grad & (g.dtype == PR_F32 ? 3 : 1)) != 0) return PR_EINVAL;
     if (g.set < 0 || g.set >= n_sets || (i > 0 && g.set < tensors[i - 1].set)) return PR_EINVAL;
   }
