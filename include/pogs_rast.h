@@ -344,12 +344,13 @@ int pr_adam_step(const pr_adam_group *groups, int n_groups, void *stream);
  * clips are HOST arrays.
  * pr_grad_norm: norms[s] = norm over all elements of the tensors of set s (0 for an empty set), in float64 until the
  * last rounding; the same inputs give the same bits; scratch: pr_grad_norm_scratch_bytes (0 for a list it does not
- * take).  kind: sum of magnitudes, root of the sum of squares, largest
- * magnitude (a NaN anywhere in the set gives NaN).
- * pr_grad_scale: g *= min(1, max_norms[s] / (norms[s] + 1e-6)), rounded once to the gradient's type; gradients of a set
- * whose norm is within bounds are not touched.  Tensors that share memory are refused (PR_EUNSUPPORTED).
- * pr_adam_step_clipped: pr_adam_step with each group's gradient taken times that factor of clips[i] (norm NULL: 1);
- * the gradients themselves stay as they are. */
+ * take).  kind: sum of magnitudes, root of the sum of squares, largest magnitude (a NaN anywhere in the set gives NaN).
+ * pr_grad_clip: the norms, and then g *= min(1, max_norms[s] / (norms[s] + 1e-6)), rounded once to the gradient's type;
+ * gradients of a set whose norm is within bounds are not touched.  Tensors that share memory are refused
+ * (PR_EUNSUPPORTED).
+ * pr_adam_step_clipped: pr_adam_step (of any number of groups) with each gradient taken times that factor for its set's
+ * 2-norm and clips[i].max_norm (set -1: taken as it is); norms[s] are written, the gradients stay as they are.  Groups of
+ * a set follow one another, sets in ascending order; scratch: pr_adam_clip_scratch_bytes. */
 #define PR_NORM_1 1
 #define PR_NORM_2 2
 #define PR_NORM_INF 3
@@ -360,16 +361,19 @@ typedef struct {
   int32_t set;
 } pr_grad_tensor;
 typedef struct {
-  const float *norm; /* device, may be NULL */
+  int32_t set;
+  int32_t reserved;
   double max_norm;
-} pr_grad_clip;
+} pr_clip_rule;
 int pr_grad_norm_max_sets(void);
 size_t pr_grad_norm_scratch_bytes(const pr_grad_tensor *tensors, int n, int n_sets);
 int pr_grad_norm(const pr_grad_tensor *tensors, int n, int n_sets, int kind, void *scratch, size_t scratch_bytes,
                  float *norms, void *stream);
-int pr_grad_scale(const pr_grad_tensor *tensors, int n, int n_sets, const float *norms, const double *max_norms,
-                  void *stream);
-int pr_adam_step_clipped(const pr_adam_group *groups, const pr_grad_clip *clips, int n_groups, void *stream);
+int pr_grad_clip(const pr_grad_tensor *tensors, int n, int n_sets, int kind, const double *max_norms, void *scratch,
+                 size_t scratch_bytes, float *norms, void *stream);
+size_t pr_adam_clip_scratch_bytes(const pr_adam_group *groups, const pr_clip_rule *clips, int n_groups, int n_sets);
+int pr_adam_step_clipped(const pr_adam_group *groups, const pr_clip_rule *clips, int n_groups, int n_sets, void *scratch,
+                         size_t scratch_bytes, float *norms, void *stream);
 
 /* ---- fused channel MLP on the rendered feature image ------------------------------------------------------
  * Replaces pogs/pogs.py:516-522 with the module of pogs/pogs.py:153-161: for every pixel

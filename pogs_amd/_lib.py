@@ -82,8 +82,9 @@ SIGNATURES = {
     "pr_grad_norm_max_sets": (c_int, []),
     "pr_grad_norm_scratch_bytes": (c_size_t, [_P, c_int, c_int]),
     "pr_grad_norm": (c_int, [_P, c_int, c_int, c_int, _P, c_size_t, _P, _P]),
-    "pr_grad_scale": (c_int, [_P, c_int, c_int, _P, _P, _P]),
-    "pr_adam_step_clipped": (c_int, [_P, _P, c_int, _P]),
+    "pr_grad_clip": (c_int, [_P, c_int, c_int, c_int, _P, _P, c_size_t, _P, _P]),
+    "pr_adam_clip_scratch_bytes": (c_size_t, [_P, _P, c_int, c_int]),
+    "pr_adam_step_clipped": (c_int, [_P, _P, c_int, c_int, _P, c_size_t, _P, _P]),
     "pr_project_fwd_rigid": (c_int, [c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_float, c_float,
                                      c_float, c_float, _P, _P, _P, _P, _P, _P, _P]),
     "pr_project_bwd_rigid": (c_int, [c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_float, _P, _P,
@@ -114,9 +115,9 @@ class AdamGroup(ctypes.Structure):
 
 
 
-class GradClip(ctypes.Structure):
-    """pr_grad_clip."""
-    _fields_ = [("norm", ctypes.c_void_p), ("max_norm", ctypes.c_double)]
+class ClipRule(ctypes.Structure):
+    """pr_clip_rule."""
+    _fields_ = [("set", ctypes.c_int32), ("reserved", ctypes.c_int32), ("max_norm", ctypes.c_double)]
 
 
 class DensifyRule(ctypes.Structure):

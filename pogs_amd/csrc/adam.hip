@@ -16,7 +16,9 @@
 // grid; each lane handles four consecutive elements with 16-byte accesses.
 #include <math.h>
 
-#include "common.h"
+#include <stdlib.h>
+
+#include "grad_norm.h"
 
 namespace pr {
 namespace {
@@ -36,17 +38,23 @@ struct AdamTable {
   unsigned first_block[MAX_GROUPS + 1];
   int n;
 };
-struct ClipTable {  // per group: where its gradient norm is (NULL: not clipped) and the norm it may have
-  const float *norm[MAX_GROUPS];
+struct ClipTable {  // per group: the set whose norm its gradient is clipped by (-1: not clipped) and what it may be
+  NormSets sets;
+  int set[MAX_GROUPS];
   float max_norm[MAX_GROUPS];
+  float *norms;
 };
 struct NoClip {};
 // From the last element to the first where a norm has been taken just before: the end of the gradients is still cached.
 __device__ __forceinline__ unsigned block_of(const NoClip &) { return blockIdx.x; }
 __device__ __forceinline__ unsigned block_of(const ClipTable &) { return gridDim.x - 1 - blockIdx.x; }
-__device__ __forceinline__ float gradient_factor(const NoClip &, int) { return 1.f; }
-__device__ __forceinline__ float gradient_factor(const ClipTable &c, int gi) {
-  return c.norm[gi] ? clip_coefficient(*c.norm[gi], c.max_norm[gi]) : 1.f;
+__device__ __forceinline__ float gradient_factor(const NoClip &, int, bool) { return 1.f; }
+__device__ __forceinline__ float gradient_factor(const ClipTable &c, int gi, bool first) {
+  const int s = c.set[gi];
+  if (s < 0) return 1.f;
+  const float norm = norm_of_set<PR_NORM_2>(c.sets, s);
+  if (first && threadIdx.x == 0) c.norms[s] = norm;   // (every group of the set writes the same)
+  return clip_coefficient(norm, c.max_norm[gi]);
 }
 
 __device__ __forceinline__ void adam_update(float &p, float g, float &m, float &v, float step_size, float omb1,
@@ -73,7 +81,7 @@ __global__ void __launch_bounds__(BLOCK) adam_kernel(const AdamTable t, const CL
   const float ss = t.step_size[gi], omb1 = t.one_minus_beta1[gi], b2 = t.beta2[gi], omb2 = t.one_minus_beta2[gi],
               bc = t.bias2_sqrt[gi], eps = t.eps[gi];
   const int64_t base = (int64_t)(block - t.first_block[gi]) * PER_BLOCK;
-  const float factor = gradient_factor(clip, gi);
+  const float factor = gradient_factor(clip, gi, base == 0);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int64_t i = base + ((int64_t)r * BLOCK + threadIdx.x) * 4;
@@ -108,14 +116,7 @@ extern "C" int pr_adam_max_groups(void) { return pr::MAX_GROUPS; }
 
 namespace pr {
 namespace {
-int adam_step(const pr_adam_group *groups, const pr_grad_clip *clips, int n_groups, void *stream) {
-  if (n_groups < 0 || n_groups > MAX_GROUPS) return PR_EINVAL;
-  if (n_groups == 0) return PR_OK;
-  if (!groups) return PR_EINVAL;
-  AdamTable t;
-  ClipTable c;
-  t.n = 0;
-  unsigned blocks = 0;
+int check_groups(const pr_adam_group *groups, int n_groups) {
   for (int i = 0; i < n_groups; ++i) {
     const pr_adam_group &g = groups[i];
     if (g.numel < 0 || g.step < 1 || !(g.beta1 >= 0.0 && g.beta1 < 1.0) || !(g.beta2 >= 0.0 && g.beta2 < 1.0))
@@ -125,9 +126,22 @@ int adam_step(const pr_adam_group *groups, const pr_grad_clip *clips, int n_grou
     // 16-byte accesses: torch allocations are; a sliced view might not be
     if ((((uintptr_t)g.param | (uintptr_t)g.grad | (uintptr_t)g.exp_avg | (uintptr_t)g.exp_avg_sq) & 15) != 0)
       return PR_EINVAL;
-    if (clips && clips[i].norm && !(clips[i].max_norm >= 0.0)) return PR_EINVAL;
+  }
+  return PR_OK;
+}
+
+// Arguments checked.  clips and sets NULL: not clipped.
+int adam_launch(const pr_adam_group *groups, const pr_clip_rule *clips, const NormSets *sets, float *norms, int n_groups,
+                hipStream_t st) {
+  AdamTable t;
+  ClipTable c;
+  t.n = 0;
+  unsigned blocks = 0;
+  for (int i = 0; i < n_groups; ++i) {
+    const pr_adam_group &g = groups[i];
+    if (g.numel == 0) continue;
     const int k = t.n++;
-    c.norm[k] = clips ? clips[i].norm : nullptr;
+    c.set[k] = clips ? clips[i].set : -1;
     c.max_norm[k] = clips ? (float)clips[i].max_norm : 0.f;
     t.param[k] = g.param;
     t.grad[k] = g.grad;
@@ -150,20 +164,70 @@ int adam_step(const pr_adam_group *groups, const pr_grad_clip *clips, int n_grou
   }
   if (t.n == 0) return PR_OK;
   t.first_block[t.n] = blocks;
-  if (clips)
-    hipLaunchKernelGGL(adam_kernel<ClipTable>, dim3(blocks), dim3(BLOCK), 0, (hipStream_t)stream, t, c);
-  else
-    hipLaunchKernelGGL(adam_kernel<NoClip>, dim3(blocks), dim3(BLOCK), 0, (hipStream_t)stream, t, NoClip{});
-  return check_launch("pr_adam_step");
+  if (!clips) {
+    hipLaunchKernelGGL(adam_kernel<NoClip>, dim3(blocks), dim3(BLOCK), 0, st, t, NoClip{});
+    return check_launch("pr_adam_step");
+  }
+  c.sets = *sets;
+  c.norms = norms;
+  hipLaunchKernelGGL(adam_kernel<ClipTable>, dim3(blocks), dim3(BLOCK), 0, st, t, c);
+  return check_launch("pr_adam_step_clipped");
 }
+
+// The clipped groups' gradients as tensors, ordered by set; -1 where the arguments are not valid.
+int clipped_tensors(const pr_adam_group *groups, const pr_clip_rule *clips, int n_groups, int n_sets, pr_grad_tensor *out) {
+  int m = 0;
+  for (int i = 0; i < n_groups; ++i) {
+    if (clips[i].set < 0) continue;
+    if (!(clips[i].max_norm >= 0.0)) return -1;
+    out[m++] = pr_grad_tensor{const_cast<float *>(groups[i].grad), groups[i].numel, PR_F32, clips[i].set};
+  }
+  return check_grad_tensors(out, m, n_sets) == PR_OK ? m : -1;
+}
+
+struct Tensors {  // freed at the end of a call
+  pr_grad_tensor *p;
+  explicit Tensors(int n) : p((pr_grad_tensor *)malloc(sizeof(pr_grad_tensor) * (size_t)(n > 0 ? n : 1))) {}
+  ~Tensors() { free(p); }
+};
 }  // namespace
 }  // namespace pr
 
 extern "C" int pr_adam_step(const pr_adam_group *groups, int n_groups, void *stream) {
-  return pr::adam_step(groups, nullptr, n_groups, stream);
+  if (n_groups < 0 || n_groups > pr::MAX_GROUPS) return PR_EINVAL;
+  if (n_groups == 0) return PR_OK;
+  if (!groups) return PR_EINVAL;
+  const int rc = pr::check_groups(groups, n_groups);
+  if (rc != PR_OK) return rc;
+  return pr::adam_launch(groups, nullptr, nullptr, nullptr, n_groups, (hipStream_t)stream);
 }
 
-extern "C" int pr_adam_step_clipped(const pr_adam_group *groups, const pr_grad_clip *clips, int n_groups, void *stream) {
-  if (n_groups > 0 && !clips) return PR_EINVAL;
-  return pr::adam_step(groups, clips, n_groups, stream);
+extern "C" size_t pr_adam_clip_scratch_bytes(const pr_adam_group *groups, const pr_clip_rule *clips, int n_groups, int n_sets) {
+  if (n_groups < 0 || !groups || !clips) return 0;
+  pr::Tensors t(n_groups);
+  if (!t.p) return 0;
+  const int n = pr::clipped_tensors(groups, clips, n_groups, n_sets, t.p);
+  return n < 0 ? 0 : pr::grad_norm_scratch(t.p, n);
+}
+
+extern "C" int pr_adam_step_clipped(const pr_adam_group *groups, const pr_clip_rule *clips, int n_groups, int n_sets,
+                                    void *scratch, size_t scratch_bytes, float *norms, void *stream) {
+  if (n_groups < 0) return PR_EINVAL;
+  if (n_groups == 0) return PR_OK;
+  if (!groups || !clips || !scratch || ((uintptr_t)scratch & 7) || !norms) return PR_EINVAL;
+  pr::Tensors t(n_groups);
+  if (!t.p) return PR_ESCRATCH;
+  const int n = pr::clipped_tensors(groups, clips, n_groups, n_sets, t.p);
+  if (n < 0) return PR_EINVAL;
+  if (scratch_bytes < pr::grad_norm_scratch(t.p, n)) return PR_ESCRATCH;
+  hipStream_t st = (hipStream_t)stream;
+  pr::NormSets sets;
+  int rc = pr::check_groups(groups, n_groups);
+  if (rc != PR_OK) return rc;
+  rc = pr::write_empty_norms(t.p, n, n_sets, scratch, scratch_bytes, norms, stream);
+  if (rc != PR_OK) return rc;
+  rc = pr::launch_grad_norms(t.p, n, n_sets, PR_NORM_2, scratch, scratch_bytes, &sets, st);
+  for (int i = 0; rc == PR_OK && i < n_groups; i += pr::MAX_GROUPS)
+    rc = pr::adam_launch(groups + i, clips + i, &sets, norms, n_groups - i < pr::MAX_GROUPS ? n_groups - i : pr::MAX_GROUPS, st);
+  return rc;
 }

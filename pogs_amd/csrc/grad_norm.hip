@@ -1,4 +1,4 @@
-// Norm of the gradients of many tensors and their scaling to at most a given norm (pr_grad_norm / pr_grad_scale).
+// Norm of the gradients of many tensors and their scaling to at most a given norm (pr_grad_norm / pr_grad_clip).
 //
 // Stands in for torch.nn.utils.clip_grad_norm_, which nerfstudio's Optimizers.optimizer_scaler_step_some calls for every
 // parameter group with a max_norm (nerfstudio/engine/optimizers.py:159-172).
@@ -18,13 +18,12 @@
 
 #include <algorithm>
 
-#include "common.h"
+#include "grad_norm.h"
 
 namespace pr {
 namespace {
 
 constexpr int MAX_TENSORS = 128;  // per launch: the table travels in the kernel argument (at most 4 KB)
-constexpr int MAX_SETS = 32;
 constexpr int BLOCK = 256;
 constexpr int64_t CHUNK = 4096;  // elements a workgroup takes at a time: 16 each, in 16-byte accesses
 constexpr int MAX_BLOCKS = 2048;  // per launch, besides one for each tensor: eight workgroups for each CU
@@ -37,12 +36,8 @@ struct Table {
   int n;
 };
 
-struct SetRanges {  // partials of set s: [first[s], first[s + 1])
-  unsigned first[MAX_SETS + 1];
-};
-
 struct MaxNorms {
-  float of[MAX_SETS];
+  float of[NORM_SETS];
 };
 
 __device__ __forceinline__ float from_bits16(unsigned short b, int dtype) {
@@ -55,27 +50,9 @@ __device__ __forceinline__ unsigned short to_bits16(float v, int dtype) {
 }
 
 template <int KIND>
-__device__ __forceinline__ double combine(double a, double b) {
-  if (KIND != PR_NORM_INF) return a + b;
-  return (a > b || a != a) ? a : b;  // max that keeps NaN
-}
-template <int KIND>
 __device__ __forceinline__ void take(double &acc, float g) {
   if (KIND == PR_NORM_2) acc = fma((double)g, (double)g, acc);
-  else acc = combine<KIND>(acc, (double)fabsf(g));
-}
-
-template <int KIND>
-__device__ __forceinline__ double block_combine(double v) {
-  __shared__ double part[BLOCK / 64];
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = combine<KIND>(v, __shfl_xor(v, d));
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = part[0];
-#pragma unroll
-  for (int i = 1; i < BLOCK / 64; ++i) v = combine<KIND>(v, part[i]);
-  return v;
+  else acc = norm_combine<KIND>(acc, (double)fabsf(g));
 }
 
 // The tensor that a workgroup belongs to.
@@ -139,18 +116,24 @@ __global__ void __launch_bounds__(BLOCK) grad_norm_kernel(const Table t, double 
   double acc[4] = {0., 0., 0., 0.};
   for (int64_t lo = (int64_t)(blockIdx.x - first) * CHUNK; lo < n; lo += (int64_t)blocks * CHUNK)
     each_of_chunk(t.grad[k], t.dtype[k], lo, n - lo, [&](float g, int at) { take<KIND>(acc[at], g); });
-  const double all = block_combine<KIND>(combine<KIND>(combine<KIND>(acc[0], acc[1]), combine<KIND>(acc[2], acc[3])));
+  const double all = norm_block_combine<KIND>(norm_combine<KIND>(norm_combine<KIND>(acc[0], acc[1]), norm_combine<KIND>(acc[2], acc[3])));
   if (threadIdx.x == 0) partials[blockIdx.x] = all;
 }
 
+// A workgroup a set: its total, and (totals NULL) its norm.
 template <int KIND>
-__global__ void __launch_bounds__(BLOCK) grad_norm_finish_kernel(const SetRanges sets, const double *__restrict__ partials,
+__global__ void __launch_bounds__(BLOCK) grad_norm_finish_kernel(const NormSets sets, double *__restrict__ totals,
                                                                  float *__restrict__ norms) {
   const int s = blockIdx.x;
-  double acc = 0.;
-  for (unsigned i = sets.first[s] + threadIdx.x; i < sets.first[s + 1]; i += BLOCK) acc = combine<KIND>(acc, partials[i]);
-  acc = block_combine<KIND>(acc);
-  if (threadIdx.x == 0) norms[s] = (float)(KIND == PR_NORM_2 ? sqrt(acc) : acc);
+  if (totals) {
+    double v = 0.;
+    for (unsigned i = sets.first[s] + threadIdx.x; i < sets.first[s + 1]; i += BLOCK) v = norm_combine<KIND>(v, sets.partials[i]);
+    v = norm_block_combine<KIND>(v);
+    if (threadIdx.x == 0) totals[s] = v;
+  } else {
+    const float norm = norm_of_set<KIND>(sets, s);
+    if (threadIdx.x == 0) norms[s] = norm;
+  }
 }
 
 __device__ __forceinline__ void scale_chunk(void *grad, int dtype, int64_t lo, int64_t left, float c) {
@@ -194,14 +177,16 @@ __device__ __forceinline__ void scale_chunk(void *grad, int dtype, int64_t lo, i
   }
 }
 
-__global__ void __launch_bounds__(BLOCK) grad_scale_kernel(const Table t, const float *__restrict__ norms,
-                                                           const MaxNorms max_norms) {
+template <int KIND>
+__global__ void __launch_bounds__(BLOCK) grad_scale_kernel(const Table t, const NormSets sets, const MaxNorms max_norms,
+                                                           float *__restrict__ norms) {
   const unsigned block = gridDim.x - 1 - blockIdx.x;
-  const int k = find_tensor(t, block);
-  const float c = clip_coefficient(norms[t.set[k]], max_norms.of[t.set[k]]);
+  const int k = find_tensor(t, block), set = t.set[k];
+  const float norm = norm_of_set<KIND>(sets, set), c = clip_coefficient(norm, max_norms.of[set]);
+  const unsigned first = t.first_block[k], blocks = t.first_block[k + 1] - first;
+  if (block == first && threadIdx.x == 0) norms[set] = norm;   // (every tensor of the set writes the same)
   // a norm within bounds leaves every value as it is: nothing to read or write (NaN is no such norm)
   if (c == 1.f) return;
-  const unsigned first = t.first_block[k], blocks = t.first_block[k + 1] - first;
   const int64_t n = t.numel[k], chunks = (n + CHUNK - 1) / CHUNK;
   // this workgroup's chunks, the last one first
   int64_t i = block - first;
@@ -214,12 +199,12 @@ struct Launches {
   int n, at = 0;
   Table t;
   unsigned blocks = 0;
-  unsigned set_blocks[MAX_SETS];  // workgroups of each set in this launch
+  unsigned set_blocks[NORM_SETS];  // workgroups of each set in this launch
   Launches(const pr_grad_tensor *tensors_, int n_) : tensors(tensors_), n(n_) {}
   int next() {
     t.n = 0;
     blocks = 0;
-    std::fill(set_blocks, set_blocks + MAX_SETS, 0u);
+    std::fill(set_blocks, set_blocks + NORM_SETS, 0u);
     int64_t chunks = 0;
     for (; at < n && t.n < MAX_TENSORS; ++at) {
       const pr_grad_tensor &g = tensors[at];
@@ -245,17 +230,6 @@ struct Launches {
   }
 };
 
-int check_tensors(const pr_grad_tensor *tensors, int n, int n_sets) {
-  if (n < 0 || n_sets < 1 || n_sets > MAX_SETS || (n > 0 && !tensors)) return PR_EINVAL;
-  for (int i = 0; i < n; ++i) {
-    const pr_grad_tensor &g = tensors[i];
-    if (g.numel < 0 || g.numel > (1ll << 38) || (g.numel > 0 && !g.grad) || g.dtype < PR_F32 || g.dtype > PR_BF16) return PR_EINVAL;
-    if (((uintptr_t)g.grad & (g.dtype == PR_F32 ? 3 : 1)) != 0) return PR_EINVAL;
-    if (g.set < 0 || g.set >= n_sets || (i > 0 && g.set < tensors[i - 1].set)) return PR_EINVAL;
-  }
-  return PR_OK;
-}
-
 // Whether no two tensors share memory (scaling them in one launch would race).
 int check_apart(const pr_grad_tensor *tensors, int n) {
   struct Span {
@@ -273,65 +247,132 @@ int check_apart(const pr_grad_tensor *tensors, int n) {
   for (int i = 1; i < m; ++i) apart &= s[i - 1].hi <= s[i].lo;
   free(s);
   if (apart) return PR_OK;
-  set_error_text("pr_grad_scale: two gradients share memory");
+  set_error_text("pr_grad_clip: two gradients share memory");
   return PR_EUNSUPPORTED;
 }
 
+template <int KIND>
+int launch_kind(const pr_grad_tensor *tensors, int n, int n_sets, double *partials, size_t room, NormSets *sets,
+                hipStream_t st) {
+  unsigned of_set[NORM_SETS] = {};
+  size_t used = 0;
+  for (Launches l(tensors, n);;) {
+    l.next();
+    if (l.t.n == 0) break;
+    if (used + l.blocks > room) return PR_ESCRATCH;
+    hipLaunchKernelGGL(grad_norm_kernel<KIND>, dim3(l.blocks), dim3(BLOCK), 0, st, l.t, partials + used);
+    const int rc = check_launch("pr_grad_norm");
+    if (rc != PR_OK) return rc;
+    used += l.blocks;
+    for (int s = 0; s < n_sets; ++s) of_set[s] += l.set_blocks[s];
+  }
+  // tensors are ordered by set: a set's partials are consecutive, over launches too
+  sets->partials = partials;
+  sets->first[0] = 0;
+  unsigned most = 0;
+  for (int s = 0; s < n_sets; ++s) {
+    sets->first[s + 1] = sets->first[s] + of_set[s];
+    most = std::max(most, of_set[s]);
+  }
+  if (most <= JOIN_PARTIALS) return PR_OK;
+  if (used + n_sets > room) return PR_ESCRATCH;
+  hipLaunchKernelGGL(grad_norm_finish_kernel<KIND>, dim3(n_sets), dim3(BLOCK), 0, st, *sets, partials + used, (float *)nullptr);
+  sets->partials = partials + used;
+  for (int s = 0; s <= n_sets; ++s) sets->first[s] = s;
+  return check_launch("pr_grad_norm");
+}
+
+}  // namespace
+
+int check_grad_tensors(const pr_grad_tensor *tensors, int n, int n_sets) {
+  if (n < 0 || n_sets < 1 || n_sets > NORM_SETS || (n > 0 && !tensors)) return PR_EINVAL;
+  for (int i = 0; i < n; ++i) {
+    const pr_grad_tensor &g = tensors[i];
+    if (g.numel < 0 || g.numel > (1ll << 38) || (g.numel > 0 && !g.grad) || g.dtype < PR_F32 || g.dtype > PR_BF16) return PR_EINVAL;
+    if (((uintptr_t)g.grad & (g.dtype == PR_F32 ? 3 : 1)) != 0) return PR_EINVAL;
+    if (g.set < 0 || g.set >= n_sets || (i > 0 && g.set < tensors[i - 1].set)) return PR_EINVAL;
+  }
+  return PR_OK;
+}
+
+size_t grad_norm_scratch(const pr_grad_tensor *tensors, int n) {
+  Launches l(tensors, n);
+  size_t blocks = NORM_SETS;
+  do {
+    l.next();
+    blocks += l.blocks;
+  } while (l.t.n > 0);
+  return blocks * sizeof(double);
+}
+
+int write_empty_norms(const pr_grad_tensor *tensors, int n, int n_sets, void *scratch, size_t scratch_bytes, float *norms,
+                      void *stream) {
+  for (int s = 0; s < n_sets; ++s) {
+    int64_t elements = 0;
+    for (int i = 0; i < n; ++i) elements += tensors[i].set == s ? tensors[i].numel : 0;
+    if (elements == 0) return pr_grad_norm(tensors, n, n_sets, PR_NORM_2, scratch, scratch_bytes, norms, stream);
+  }
+  return PR_OK;
+}
+
+int launch_grad_norms(const pr_grad_tensor *tensors, int n, int n_sets, int kind, void *scratch, size_t scratch_bytes,
+                      NormSets *sets, hipStream_t st) {
+  double *partials = (double *)scratch;
+  const size_t room = scratch_bytes / sizeof(double);
+  if (kind == PR_NORM_1) return launch_kind<PR_NORM_1>(tensors, n, n_sets, partials, room, sets, st);
+  if (kind == PR_NORM_2) return launch_kind<PR_NORM_2>(tensors, n, n_sets, partials, room, sets, st);
+  return launch_kind<PR_NORM_INF>(tensors, n, n_sets, partials, room, sets, st);
+}
+
+namespace {
+template <int KIND>
+int scale_by_norms(const pr_grad_tensor *tensors, int n, const NormSets &sets, const MaxNorms &m, float *norms, hipStream_t st) {
+  for (Launches l(tensors, n);;) {
+    l.next();
+    if (l.t.n == 0) return PR_OK;
+    hipLaunchKernelGGL(grad_scale_kernel<KIND>, dim3(l.blocks), dim3(BLOCK), 0, st, l.t, sets, m, norms);
+    const int rc = check_launch("pr_grad_clip");
+    if (rc != PR_OK) return rc;
+  }
+}
+
+int check_norm_call(const pr_grad_tensor *tensors, int n, int n_sets, int kind, const void *scratch, size_t scratch_bytes,
+                    const float *norms) {
+  const int rc = check_grad_tensors(tensors, n, n_sets);
+  if (rc != PR_OK) return rc;
+  if (kind < PR_NORM_1 || kind > PR_NORM_INF || !norms || !scratch || ((uintptr_t)scratch & 7)) return PR_EINVAL;
+  return scratch_bytes < grad_norm_scratch(tensors, n) ? PR_ESCRATCH : PR_OK;
+}
 }  // namespace
 }  // namespace pr
 
-extern "C" int pr_grad_norm_max_sets(void) { return pr::MAX_SETS; }
+extern "C" int pr_grad_norm_max_sets(void) { return pr::NORM_SETS; }
 
 extern "C" size_t pr_grad_norm_scratch_bytes(const pr_grad_tensor *tensors, int n, int n_sets) {
-  if (pr::check_tensors(tensors, n, n_sets) != PR_OK) return 0;
-  pr::Launches l(tensors, n);
-  size_t blocks = 0;
-  do {
-    if (l.next() != PR_OK) return 0;
-    blocks += l.blocks;
-  } while (l.t.n > 0);
-  return std::max<size_t>(blocks, 1) * sizeof(double);
+  return pr::check_grad_tensors(tensors, n, n_sets) == PR_OK ? pr::grad_norm_scratch(tensors, n) : 0;
 }
 
 extern "C" int pr_grad_norm(const pr_grad_tensor *tensors, int n, int n_sets, int kind, void *scratch,
                             size_t scratch_bytes, float *norms, void *stream) {
-  int rc = pr::check_tensors(tensors, n, n_sets);
+  int rc = pr::check_norm_call(tensors, n, n_sets, kind, scratch, scratch_bytes, norms);
   if (rc != PR_OK) return rc;
-  if (kind < PR_NORM_1 || kind > PR_NORM_INF || !norms || !scratch || ((uintptr_t)scratch & 7)) return PR_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  double *partials = (double *)scratch;
-  size_t used = 0;
-  pr::SetRanges sets;
-  unsigned set_partials[pr::MAX_SETS] = {};
-  for (pr::Launches l(tensors, n);;) {
-    rc = l.next();
-    if (rc != PR_OK) return rc;
-    if (l.t.n == 0) break;
-    if ((used + l.blocks) * sizeof(double) > scratch_bytes) return PR_ESCRATCH;
-    const dim3 grid(l.blocks), block(pr::BLOCK);
-    if (kind == PR_NORM_2) hipLaunchKernelGGL(pr::grad_norm_kernel<PR_NORM_2>, grid, block, 0, st, l.t, partials + used);
-    else if (kind == PR_NORM_1) hipLaunchKernelGGL(pr::grad_norm_kernel<PR_NORM_1>, grid, block, 0, st, l.t, partials + used);
-    else hipLaunchKernelGGL(pr::grad_norm_kernel<PR_NORM_INF>, grid, block, 0, st, l.t, partials + used);
-    rc = pr::check_launch("pr_grad_norm");
-    if (rc != PR_OK) return rc;
-    used += l.blocks;
-    for (int s = 0; s < n_sets; ++s) set_partials[s] += l.set_blocks[s];
-  }
-  // tensors are ordered by set: a set's partials are consecutive, over launches too
-  sets.first[0] = 0;
-  for (int s = 0; s < n_sets; ++s) sets.first[s + 1] = sets.first[s] + set_partials[s];
+  pr::NormSets sets;
+  rc = pr::launch_grad_norms(tensors, n, n_sets, kind, scratch, scratch_bytes, &sets, st);
+  if (rc != PR_OK) return rc;
   const dim3 grid(n_sets), block(pr::BLOCK);
-  if (kind == PR_NORM_2) hipLaunchKernelGGL(pr::grad_norm_finish_kernel<PR_NORM_2>, grid, block, 0, st, sets, partials, norms);
-  else if (kind == PR_NORM_1) hipLaunchKernelGGL(pr::grad_norm_finish_kernel<PR_NORM_1>, grid, block, 0, st, sets, partials, norms);
-  else hipLaunchKernelGGL(pr::grad_norm_finish_kernel<PR_NORM_INF>, grid, block, 0, st, sets, partials, norms);
+  double *const none = nullptr;
+  if (kind == PR_NORM_2) hipLaunchKernelGGL(pr::grad_norm_finish_kernel<PR_NORM_2>, grid, block, 0, st, sets, none, norms);
+  else if (kind == PR_NORM_1) hipLaunchKernelGGL(pr::grad_norm_finish_kernel<PR_NORM_1>, grid, block, 0, st, sets, none, norms);
+  else hipLaunchKernelGGL(pr::grad_norm_finish_kernel<PR_NORM_INF>, grid, block, 0, st, sets, none, norms);
   return pr::check_launch("pr_grad_norm");
 }
 
-extern "C" int pr_grad_scale(const pr_grad_tensor *tensors, int n, int n_sets, const float *norms, const double *max_norms,
-                             void *stream) {
-  int rc = pr::check_tensors(tensors, n, n_sets);
+extern "C" int pr_grad_clip(const pr_grad_tensor *tensors, int n, int n_sets, int kind, const double *max_norms,
+                            void *scratch, size_t scratch_bytes, float *norms, void *stream) {
+  int rc = pr::check_norm_call(tensors, n, n_sets, kind, scratch, scratch_bytes, norms);
   if (rc != PR_OK) return rc;
-  if (!norms || !max_norms) return PR_EINVAL;
+  if (!max_norms) return PR_EINVAL;
   rc = pr::check_apart(tensors, n);
   if (rc != PR_OK) return rc;
   pr::MaxNorms m{};
@@ -339,12 +380,13 @@ extern "C" int pr_grad_scale(const pr_grad_tensor *tensors, int n, int n_sets, c
     if (!(max_norms[s] >= 0.0)) return PR_EINVAL;
     m.of[s] = (float)max_norms[s];
   }
-  for (pr::Launches l(tensors, n);;) {
-    rc = l.next();
-    if (rc != PR_OK) return rc;
-    if (l.t.n == 0) return PR_OK;
-    hipLaunchKernelGGL(pr::grad_scale_kernel, dim3(l.blocks), dim3(pr::BLOCK), 0, (hipStream_t)stream, l.t, norms, m);
-    rc = pr::check_launch("pr_grad_scale");
-    if (rc != PR_OK) return rc;
-  }
+  rc = pr::write_empty_norms(tensors, n, n_sets, scratch, scratch_bytes, norms, stream);
+  if (rc != PR_OK) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  pr::NormSets sets;
+  rc = pr::launch_grad_norms(tensors, n, n_sets, kind, scratch, scratch_bytes, &sets, st);
+  if (rc != PR_OK) return rc;
+  if (kind == PR_NORM_1) return pr::scale_by_norms<PR_NORM_1>(tensors, n, sets, m, norms, st);
+  if (kind == PR_NORM_2) return pr::scale_by_norms<PR_NORM_2>(tensors, n, sets, m, norms, st);
+  return pr::scale_by_norms<PR_NORM_INF>(tensors, n, sets, m, norms, st);
 }

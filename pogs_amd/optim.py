@@ -30,7 +30,7 @@ from .rendering import _call, _on, _stream
 
 
 _ADAM_GROUP = struct.Struct("=4Q2q4d")     # pr_adam_group
-_GRAD_CLIP = struct.Struct("=Qd")           # pr_grad_clip
+_CLIP_RULE = struct.Struct("=2id")          # pr_clip_rule
 _GRAD_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}        # PR_F32, PR_F16, PR_BF16
 _NORM_KINDS = {1.0: 1, 2.0: 2, math.inf: 3}                                   # PR_NORM_1, PR_NORM_2, PR_NORM_INF
 
@@ -45,11 +45,12 @@ def _one_block(t: Tensor) -> bool:
     return True
 
 
-def _grad_table(grads: Sequence[Tensor], sets: Optional[Sequence[int]] = None) -> array:
-    """The grads as an array of ``pr_grad_tensor``: pointer, elements, type and set (the upper half word)."""
-    words = array("q")
-    for i, g in enumerate(grads):
-        words.extend((g.data_ptr(), g.numel(), _GRAD_TYPES[g.dtype] | (sets[i] << 32 if sets else 0)))
+def _grad_table(grads: Sequence[Tensor]) -> array:
+    """The grads as an array of ``pr_grad_tensor``: pointer, elements, type and (in the upper half word) set 0."""
+    words = array("q", bytes(24 * len(grads)))
+    words[0::3] = array("q", [g.data_ptr() for g in grads])
+    words[1::3] = array("q", [g.numel() for g in grads])
+    words[2::3] = array("q", [_GRAD_TYPES[g.dtype] for g in grads])
     return words
 
 
@@ -57,27 +58,28 @@ def _address(a: array) -> ctypes.c_void_p:
     return ctypes.c_void_p(a.buffer_info()[0])
 
 
-def _set_norms(table: array, shape: tuple, kind: int, device, stream: int) -> Tensor:
-    """The norms (float32, on the device) of the sets of a table of gradients ordered by set: ``()`` or ``(sets,)``."""
-    lib = _lib.load()
-    at, n, n_sets = _address(table), len(table) // 3, shape[0] if shape else 1
-    nbytes = lib.pr_grad_norm_scratch_bytes(at, n, n_sets)
-    scratch = torch.empty(max(nbytes // 8, 1), dtype=torch.float64, device=device)
-    norms = torch.empty(shape, dtype=torch.float32, device=device)
-    _call("pr_grad_norm", at, n, n_sets, kind, scratch.data_ptr(), nbytes, norms.data_ptr(), stream)
-    return norms
+def _norm_buffers(nbytes: int, shape: tuple, device) -> Tuple[Tensor, Tensor]:
+    return (torch.empty(max(nbytes // 8, 1), dtype=torch.float64, device=device),
+            torch.empty(shape, dtype=torch.float32, device=device))
 
 
 def _check_grads(grads: Sequence[Tensor]) -> torch.device:
-    dev = grads[0].device
-    for g in grads:
-        if g.is_sparse or not g.is_cuda:
-            raise RuntimeError("pogs_amd.optim needs dense gradients on a HIP device (no CPU fallback)")
-        if g.dtype not in _GRAD_TYPES:
-            raise TypeError(f"gradients must be float32, float16 or bfloat16, got {g.dtype}")
-        if g.device != dev:
-            raise RuntimeError(f"gradients are on different devices: {dev} and {g.device}")
-    return dev
+    if {g.layout for g in grads} != {torch.strided} or not all([g.is_cuda for g in grads]):
+        raise RuntimeError("pogs_amd.optim needs dense gradients on a HIP device (no CPU fallback)")
+    for t in {g.dtype for g in grads}:
+        if t not in _GRAD_TYPES:
+            raise TypeError(f"gradients must be float32, float16 or bfloat16, got {t}")
+    devices = {g.device for g in grads}
+    if len(devices) > 1:
+        raise RuntimeError(f"gradients are on different devices: {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def _flat(grads: List[Tensor]) -> List[Tensor]:
+    """The gradients as blocks of memory: themselves, or a copy of one whose elements are scattered."""
+    if all([g.is_contiguous() for g in grads]):
+        return grads
+    return [g if g.is_contiguous() or _one_block(g) else g.detach().contiguous() for g in grads]
 
 
 def _norm_kind(norm_type: float) -> int:
@@ -104,9 +106,15 @@ def grad_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) 
     if not grads:
         return torch.tensor(0.0)
     dev = _check_grads(grads)
+    lib = _lib.load()
     with _on(dev):
-        flat = [g if g.is_contiguous() or _one_block(g) else g.detach().contiguous() for g in grads]
-        return _set_norms(_grad_table(flat), (), kind, dev, _stream())
+        flat = _flat(grads)
+        table = _grad_table(flat)
+        at, n = _address(table), len(flat)
+        nbytes = lib.pr_grad_norm_scratch_bytes(at, n, 1)
+        scratch, norm = _norm_buffers(nbytes, (), dev)
+        _call("pr_grad_norm", at, n, 1, kind, scratch.data_ptr(), nbytes, norm.data_ptr(), _stream())
+    return norm
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -121,25 +129,27 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     only then does the host wait for the device."""
     kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
     params = [parameters] if isinstance(parameters, Tensor) else list(parameters)
-    grads = [p.grad for p in params if p.grad is not None]
+    grads = [g for p in params if (g := p.grad) is not None]
     if not grads:
         return torch.tensor(0.0)
-    dev = _check_grads(grads)
+    if error_if_nonfinite and not math.isfinite(grad_norm(grads, norm_type).item()):
+        raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is non-finite, so it "
+                           "cannot be clipped. To disable this error and scale the gradients by the non-finite norm "
+                           "anyway, set `error_if_nonfinite=False`")
+    dev, lib = _check_grads(grads), _lib.load()
     with _on(dev):
-        flat = [g if g.is_contiguous() or _one_block(g) else g.detach().contiguous() for g in grads]
-        table, stream = _grad_table(flat), _stream()
-        norms = _set_norms(table, (), kind, dev, stream)
-        if error_if_nonfinite and not math.isfinite(norms.item()):
-            raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is "
-                               "non-finite, so it cannot be clipped. To disable this error and scale the gradients by "
-                               "the non-finite norm anyway, set `error_if_nonfinite=False`")
-        limit = ctypes.c_double(max_norm)
-        _call("pr_grad_scale", _address(table), len(flat), 1, norms.data_ptr(), ctypes.addressof(limit), stream)
-        for g, f in zip(grads, flat):
-            if f is not g:
-                with torch.no_grad():
-                    g.copy_(f)
-        return norms
+        flat = _flat(grads)
+        table, limit = _grad_table(flat), ctypes.c_double(max_norm)
+        at, n = _address(table), len(flat)
+        nbytes = lib.pr_grad_norm_scratch_bytes(at, n, 1)
+        scratch, norm = _norm_buffers(nbytes, (), dev)
+        _call("pr_grad_clip", at, n, 1, kind, ctypes.addressof(limit), scratch.data_ptr(), nbytes, norm.data_ptr(), _stream())
+        if flat is not grads:
+            with torch.no_grad():
+                for g, f in zip(grads, flat):
+                    if f is not g:
+                        g.copy_(f)
+    return norm
 
 
 class ExponentialDecay:
@@ -175,7 +185,8 @@ class Optimizers:
         self.config, self.parameters = config, {}
         self._state: Dict[str, List[dict]] = {}
         self._sched_steps: Dict[str, int] = {}
-        self._norms: List[Tuple[Tensor, Dict[str, int]]] = []
+        self._norms: List[Tuple[Tensor, Dict[str, int]]] = []      # of the last step: norms, place of each group
+        self._norm_of: Optional[Dict[str, Tensor]] = None          # made from them when asked for
         for name, params in param_groups.items():
             if name not in config:
                 raise RuntimeError(f"Optimizer config for '{name}' not found in config file. Provided configs "
@@ -230,7 +241,7 @@ class Optimizers:
             max_norm = _max_norm(max_norm)
             if any(m is not None for m in limits):
                 raise ValueError("a max_norm over all groups and a max_norm of a group's own exclude each other")
-        entries, keep, clipped = [], [], []      # clipped: (group or None for all, limit, entry's index)
+        entries, rules, keep = [], [], []        # rules: (group or None for all together, its limit or None)
         for name, limit in zip(param_groups, limits):
             cfg = self.config[name]
             b1, b2 = cfg.get("betas", (0.9, 0.999))
@@ -246,54 +257,52 @@ class Optimizers:
                     st["exp_avg"] = torch.zeros_like(p)
                     st["exp_avg_sq"] = torch.zeros_like(p)
                 st["step"] += 1
-                if max_norm is not None:
-                    clipped.append((None, max_norm, len(entries)))
-                elif limit is not None:
-                    clipped.append((name, _max_norm(limit), len(entries)))
+                rules.append((None, max_norm) if max_norm is not None else (name, limit))
                 keep.append(g)
                 entries.append(_ADAM_GROUP.pack(p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(),
                                                 st["exp_avg_sq"].data_ptr(), p.numel(), st["step"], lr, b1, b2, eps))
-        self._norms = []
+        self._norms, self._norm_of = [], None
         if not entries:
             return
-        lib = _lib.load()
-        chunk = lib.pr_adam_max_groups()
-        with _on(keep[0].device):
-            stream = _stream()
-            clips = self._clips(clipped, keep, param_groups, len(entries), stream) if clipped else None
-            for i in range(0, len(entries), chunk):
-                part = entries[i:i + chunk]
-                if clips is None:
-                    _call("pr_adam_step", b"".join(part), len(part), stream)
-                else:
-                    _call("pr_adam_step_clipped", b"".join(part), b"".join(clips[i:i + chunk]), len(part), stream)
+        dev = keep[0].device
+        with _on(dev):
+            if all(limit is None for _, limit in rules):
+                chunk = _lib.load().pr_adam_max_groups()
+                for i in range(0, len(entries), chunk):
+                    part = entries[i:i + chunk]
+                    _call("pr_adam_step", b"".join(part), len(part), _stream())
+            else:
+                self._step_clipped(entries, rules, param_groups, dev, _stream())
         del keep
 
-    def _clips(self, clipped, grads: List[Tensor], param_groups: List[str], n: int, stream: int) -> List[bytes]:
-        """``pr_grad_clip`` of every entry of a step, the norms on their way on the given stream."""
-        clips = [_GRAD_CLIP.pack(0, 0.0)] * n
-        names = list(dict.fromkeys(name for name, _, _ in clipped))
-        most = _lib.load().pr_grad_norm_max_sets()
-        for lo in range(0, len(names), most):
-            of = {name: i for i, name in enumerate(names[lo:lo + most])}
-            mine = [c for c in clipped if c[0] in of]
-            table = _grad_table([grads[k] for _, _, k in mine], [of[name] for name, _, _ in mine])
-            norms = _set_norms(table, (len(of),), 2, grads[0].device, stream)
-            at = norms.data_ptr()
-            for name, limit, k in mine:
-                clips[k] = _GRAD_CLIP.pack(at + 4 * of[name], limit)
-            # (this holds the storage that the step's kernel reads)
+    def _step_clipped(self, entries: List[bytes], rules: list, param_groups: List[str], device, stream: int) -> None:
+        """The step where a group at least has a limit, for as many norms at once as a call takes."""
+        lib = _lib.load()
+        most, i = lib.pr_grad_norm_max_sets(), 0
+        while i < len(entries):
+            of, clips, lo = {}, [], i
+            for name, limit in rules[i:]:
+                if limit is not None and name not in of:
+                    if len(of) == most:
+                        break
+                    of[name] = len(of)
+                clips.append(_CLIP_RULE.pack(-1, 0, 0.0) if limit is None else _CLIP_RULE.pack(of[name], 0, _max_norm(limit)))
+            i = lo + len(clips)
+            groups, by, n, sets = b"".join(entries[lo:i]), b"".join(clips), len(clips), max(len(of), 1)
+            nbytes = lib.pr_adam_clip_scratch_bytes(groups, by, n, sets)
+            scratch, norms = _norm_buffers(nbytes, (sets,), device)
+            _call("pr_adam_step_clipped", groups, by, n, sets, scratch.data_ptr(), nbytes, norms.data_ptr(), stream)
             self._norms.append((norms, {g: 0 for g in param_groups} if None in of else of))
-        return clips
 
     @property
     def grad_norms(self) -> Dict[str, Tensor]:
         """The norms that the last step clipped by, one 0-d tensor on the device for each group."""
-        out = {}
-        for norms, of in self._norms:
-            each = norms.unbind()
-            out.update((name, each[i]) for name, i in of.items())
-        return out
+        if self._norm_of is None:
+            self._norm_of = {}
+            for norms, of in self._norms:
+                each = norms.unbind()
+                self._norm_of.update((name, each[i]) for name, i in of.items())
+        return self._norm_of
 
     def state(self, name: str, index: int = 0) -> dict:
         """The Adam state of one parameter of a group (``step``, ``exp_avg``, ``exp_avg_sq``; empty before its first

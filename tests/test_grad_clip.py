@@ -1,4 +1,4 @@
-"""Gradient norm and clipping (pr_grad_norm, pr_grad_scale, pr_adam_step_clipped; pogs_amd.optim) against the formulas
+"""Gradient norm and clipping (pr_grad_norm, pr_grad_clip, pr_adam_step_clipped; pogs_amd.optim) against the formulas
 in float64.
 
 Tolerances.  u = 2^-24 is half a float32 step.  Norms are summed in float64 and rounded once: u, and 2^-40 for the sums.
@@ -46,41 +46,57 @@ def test_entry_points_validate_without_a_gpu():
     lib = _lib.load()
     assert lib.pr_grad_norm_max_sets() >= 16
     one, at = _table([(1024, 100, 0, 0)])
-    assert lib.pr_grad_norm_scratch_bytes(at, 1, 1) == 8
+    need = lib.pr_grad_norm_scratch_bytes(at, 1, 1)
+    assert need >= 8
     big, big_at = _table([(1024, 1 << 40, 0, 0)])
-    assert lib.pr_grad_norm_scratch_bytes(big_at, 1, 1) == 0        # more than a launch's index space
+    assert lib.pr_grad_norm_scratch_bytes(big_at, 1, 1) == 0        # more than an address space of gradients
     two, two_at = _table([(1024, 100, 0, 0), (1 << 20, 100, 2, 3)])
-    assert lib.pr_grad_norm_scratch_bytes(two_at, 2, 4) == 16       # one partial a set at least
-    scratch = ctypes.create_string_buffer(64)
+    assert lib.pr_grad_norm_scratch_bytes(two_at, 2, 4) == need + 8  # one partial a tensor at least
+    scratch = ctypes.create_string_buffer(4096)
     sc = ctypes.c_void_p((ctypes.addressof(scratch) + 7) & ~7)
+    odd = ctypes.c_void_p(sc.value + 1)
+    m = (ctypes.c_double * 40)(*[1.0] * 40)
     bad = [([(1024, 100, 3, 0)], 1, 1), ([(1024, -1, 0, 0)], 1, 1), ([(0, 4, 0, 0)], 1, 1), ([(1025, 4, 0, 0)], 1, 1),
            ([(1025, 4, 2, 0)], 1, 1), ([(1024, 4, 0, 1)], 1, 1), ([(1024, 4, 0, 1), (4096, 4, 0, 0)], 2, 2),
            ([(1024, 4, 0, 0)], 1, 0), ([(1024, 4, 0, 0)], 1, 1000), ([(1024, 4, 0, 0)], -1, 1)]
     for rows, n, n_sets in bad:
         keep, p = _table(rows)
-        assert lib.pr_grad_norm(p, n, n_sets, 2, sc, 64, sc, None) == -1, rows
-        assert lib.pr_grad_scale(p, n, n_sets, sc, sc, None) == -1, rows
+        assert lib.pr_grad_norm(p, n, n_sets, 2, sc, 4000, sc, None) == -1, rows
+        assert lib.pr_grad_clip(p, n, n_sets, 2, m, sc, 4000, sc, None) == -1, rows
         assert lib.pr_grad_norm_scratch_bytes(p, n, n_sets) == 0
-    assert lib.pr_grad_norm(None, 1, 1, 2, sc, 64, sc, None) == -1
+    assert lib.pr_grad_norm(None, 1, 1, 2, sc, 4000, sc, None) == -1
     for kind in (0, 4):
-        assert lib.pr_grad_norm(at, 1, 1, kind, sc, 64, sc, None) == -1
-    assert lib.pr_grad_norm(at, 1, 1, 2, sc, 64, None, None) == -1
-    assert lib.pr_grad_norm(at, 1, 1, 2, sc, 4, sc, None) == -3
+        assert lib.pr_grad_norm(at, 1, 1, kind, sc, 4000, sc, None) == -1
+        assert lib.pr_grad_clip(at, 1, 1, kind, m, sc, 4000, sc, None) == -1
+    for buffers in ((sc, 4000, None), (None, 4000, sc), (odd, 4000, sc)):
+        assert lib.pr_grad_norm(at, 1, 1, 2, *buffers, None) == -1
+        assert lib.pr_grad_clip(at, 1, 1, 2, m, *buffers, None) == -1
+    assert lib.pr_grad_norm(at, 1, 1, 2, sc, need - 1, sc, None) == -3
+    assert lib.pr_grad_clip(at, 1, 1, 2, m, sc, need - 1, sc, None) == -3
+    assert lib.pr_grad_clip(at, 1, 1, 2, None, sc, 4000, sc, None) == -1
     for limit in (-1.0, math.nan):
-        m = ctypes.c_double(limit)
-        assert lib.pr_grad_scale(at, 1, 1, sc, ctypes.addressof(m), None) == -1
-    m = (ctypes.c_double * 1)(1.0)
+        assert lib.pr_grad_clip(at, 1, 1, 2, (ctypes.c_double * 1)(limit), sc, 4000, sc, None) == -1
     for rows in ([(1024, 100, 0, 0), (1024, 100, 0, 0)], [(1024, 100, 0, 0), (1422, 9, 2, 0)],
                  [(5000, 1, 2, 0), (1024, 100, 0, 0), (1420, 1, 0, 0)]):
         keep, p = _table(rows)
-        assert lib.pr_grad_scale(p, len(rows), 1, sc, m, None) == -2
+        assert lib.pr_grad_clip(p, len(rows), 1, 2, m, sc, 4000, sc, None) == -2
         assert b"share memory" in lib.pr_last_hip_error()
-    assert lib.pr_adam_step_clipped(None, None, 0, None) == 0
-    g = (_lib.AdamGroup * 1)(_lib.AdamGroup(16, 16, 16, 16, 8, 1, 1e-3, 0.9, 0.999, 1e-15))
-    gp = ctypes.cast(g, ctypes.c_void_p)
-    assert lib.pr_adam_step_clipped(gp, None, 1, None) == -1
-    c = (_lib.GradClip * 1)(_lib.GradClip(16, -1.0))
-    assert lib.pr_adam_step_clipped(gp, ctypes.cast(c, ctypes.c_void_p), 1, None) == -1
+    # the clipped step
+    good = _lib.AdamGroup(1024, 1024, 1024, 1024, 8, 1, 1e-3, 0.9, 0.999, 1e-15)
+
+    def step(group=good, rule=(0, 1.0), n=1, sets=1, scratch=sc, nbytes=4000, norms=sc):
+        g, c = (_lib.AdamGroup * 1)(group), (_lib.ClipRule * 1)(_lib.ClipRule(rule[0], 0, rule[1]))
+        return lib.pr_adam_step_clipped(g, c, n, sets, scratch, nbytes, norms, None)
+
+    assert lib.pr_adam_step_clipped(None, None, 0, 1, None, 0, None, None) == 0
+    assert lib.pr_adam_step_clipped(None, None, 1, 1, sc, 4000, sc, None) == -1
+    for kw in (dict(n=-1), dict(rule=(0, -1.0)), dict(rule=(0, math.nan)), dict(rule=(1, 1.0)), dict(sets=0), dict(sets=1000),
+               dict(scratch=None), dict(scratch=odd), dict(norms=None),
+               dict(group=_lib.AdamGroup(1024, 1024, 1024, 1024, 8, 0, 1e-3, 0.9, 0.999, 1e-15)),
+               dict(group=_lib.AdamGroup(1024, 1028, 1024, 1024, 8, 1, 1e-3, 0.9, 0.999, 1e-15)),
+               dict(group=_lib.AdamGroup(1024, 0, 1024, 1024, 8, 1, 1e-3, 0.9, 0.999, 1e-15))):
+        assert step(**kw) == -1, kw
+    assert step(nbytes=8) == -3
 
 
 def test_refusals():
@@ -190,6 +206,23 @@ def test_views_of_one_buffer_layouts_and_strides():
     # an expanded gradient has a norm, over all its elements, but cannot be scaled in place
     e = torch.full((1, 3), 2.0, device="cuda").expand(4, 3)
     assert grad_norm([e]).item() == pytest.approx(math.sqrt(48), rel=2 * U)
+
+
+@pytest.mark.gpu
+def test_gradients_without_elements():
+    from pogs_amd.optim import Optimizers, clip_grad_norm_, grad_norm
+
+    for dtype in (torch.float32, torch.bfloat16):
+        p = _params([torch.zeros(0, 3, device="cuda", dtype=dtype), torch.zeros(0, device="cuda", dtype=dtype)])
+        torch.full((4096,), 7.0, device="cuda")                # what the norm's memory may have held before
+        assert clip_grad_norm_(p, 1.0).item() == 0.0
+        assert grad_norm([q.grad for q in p]).item() == 0.0
+    q = {"a": [torch.zeros(0, device="cuda", requires_grad=True)], "b": [torch.ones(5, device="cuda", requires_grad=True)]}
+    q["a"][0].grad, q["b"][0].grad = torch.zeros(0, device="cuda"), torch.full((5,), 2.0, device="cuda")
+    opt = Optimizers({k: {"lr": 0.5, "max_norm": 1.0} for k in q}, q)
+    opt.optimizer_step_all()
+    assert opt.grad_norms["a"].item() == 0.0 and opt.grad_norms["b"].item() == pytest.approx(math.sqrt(20), rel=2 * U)
+    assert ((q["b"][0] - 0.5).abs() <= 8 * U).all()            # a first step moves by the rate
 
 
 @pytest.mark.gpu
