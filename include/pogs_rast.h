@@ -485,8 +485,8 @@ int pr_densify_split_children(int64_t n_out, const int32_t *map_src, const int32
  * The reference has no such loss; this is torch.nn.functional.cross_entropy(scale * x @ w.T, labels) and its gradients.
  * A row whose label is ignore_index has row_loss 0, lse 0 and no gradient, whatever its features hold; any other label
  * outside 0..V-1 makes the row's loss NaN and, through it, its gradients.
- * pr_vocab_ce_fwd: P >= 1.  row_loss[P]; lse[P] and loss[1] may be NULL (a backward pass with mean != 0
- * needs the loss); loss = sum of row_loss, or (mean != 0) their mean
+ * pr_vocab_ce_fwd: P >= 1.  row_loss[P] (may be NULL where loss is not), lse[P] (may be NULL) and loss[1] (may be NULL,
+ * but a backward pass with mean != 0 needs it); loss = sum of row_loss, or (mean != 0) their mean
  * over the rows not ignored (NaN if there are none).  kept: what pr_vocab_ce_bwd reads (packed operands, row statistics);
  * NULL, for at most pr_vocab_ce_score_rows() rows and no backward pass: the vocabulary is read once and not packed.
  * pr_vocab_ce_bwd: dx[P,D] and dw[V,D] (contiguous, 16-byte aligned, the inputs' type, either may be NULL) from the

@@ -22,7 +22,8 @@
 //          lane's eight accumulators are eight consecutive slots of the contraction of dX = G W as they stand, if W's
 //          packed copy uses the same slot order; for dW = G^T X the tile is transposed by two products with the
 //          identity, which are exact
-//   DX     dX partials in float32, one plane per split of the contraction over words, added to over the pieces
+//   DX     partials of a gradient in float32, one plane per split of its contraction; dX's are added to over the pieces.
+//          Two such products may share a launch: dX's and, where dW has too few tiles for the chip, dW's
 //   DW     dW rows of the piece, contraction over all rows, written in the output type
 // G of one piece is all that is ever held of the P x V logits.
 #include <math.h>
@@ -391,7 +392,7 @@ __device__ __forceinline__ void store4(T *dst, float a, float b, float c, float 
 // the other multiplies.  One workgroup a CU, which takes tile after tile and starts the next one's loads before it turns
 // to the epilogue.
 template <int NP, int MT, int MODE, typename T>
-__global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g) {
+__global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, const GemmArgs g2) {
   extern __shared__ u4v lds[];
   constexpr int WM = 2, WN = 4, NT = 2, WAVES = WM * WN, KB = NP == 1 ? 2 : 1;
   constexpr int A_TILES = WM * MT, B_TILES = WN * NT;
@@ -402,20 +403,30 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g) {
 
   // Workgroups go to the eight XCDs in turn: each XCD takes a run of consecutive tiles, ordered as bands of eight
   // M tiles walked along N, so that its L2 holds the operands of the tiles it works on together.
-  const unsigned tiles = (unsigned)g.m_tiles * g.n_tiles * g.splits, per_xcd = (tiles + 7) / 8;
+  const unsigned tiles1 = (unsigned)g.m_tiles * g.n_tiles * g.splits;
+  const unsigned tiles = tiles1 + (MODE == DX ? (unsigned)g2.m_tiles * g2.n_tiles * g2.splits : 0u), per_xcd = (tiles + 7) / 8;
   const unsigned lo = (blockIdx.x & 7) * per_xcd, hi = min(lo + per_xcd, tiles);
   unsigned tile = lo + (blockIdx.x >> 3);
   if (tile >= hi) return;
 
   int m_tile, n_tile, split, stages;
+  bool other;             // DX: the tile is of the second product
   const u4v *src[LOADS];  // this wavefront's blocks of a stage, ordered [half: k block or plane][tile] for A, then for B
   auto place = [&](unsigned t) {
-    split = (int)(t / ((unsigned)g.m_tiles * g.n_tiles));
-    t -= split * (unsigned)g.m_tiles * g.n_tiles;
-    const unsigned band = t / (8u * g.n_tiles), in_band = t - band * 8u * g.n_tiles;
-    const unsigned band_m = min(8u, (unsigned)g.m_tiles - band * 8u);
+    other = MODE == DX && t >= tiles1;
+    if (other) t -= tiles1;
+    const unsigned m_tiles = other ? g2.m_tiles : g.m_tiles, n_tiles = other ? g2.n_tiles : g.n_tiles;
+    const int k_split = other ? g2.k_split : g.k_split, kblocks = other ? g2.kblocks : g.kblocks;
+    const int a_tiles = other ? g2.a_tiles : g.a_tiles, b_tiles = other ? g2.b_tiles : g.b_tiles;
+    const u4v *A = other ? g2.A : g.A, *B = other ? g2.B : g.B;
+    const int64_t plane_a = other ? g2.plane_a : g.plane_a, plane_b = other ? g2.plane_b : g.plane_b;
+    const int64_t ld_a = other ? g2.ld_a : g.ld_a, ld_b = other ? g2.ld_b : g.ld_b;
+    split = (int)(t / (m_tiles * n_tiles));
+    t -= split * m_tiles * n_tiles;
+    const unsigned band = t / (8u * n_tiles), in_band = t - band * 8u * n_tiles;
+    const unsigned band_m = min(8u, m_tiles - band * 8u);
     m_tile = (int)(band * 8u + in_band % band_m), n_tile = (int)(in_band / band_m);
-    stages = min(g.k_split, g.kblocks - split * g.k_split) / KB;
+    stages = min(k_split, kblocks - split * k_split) / KB;
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) {
       const int j = min(wave * LOADS + l, STAGE - 1);  // (a share past the end repeats the last block, into its own place)
@@ -423,9 +434,9 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g) {
       const int q = is_a ? j : j - 2 * A_TILES, per = is_a ? A_TILES : B_TILES;
       const int at = q % per, half = q / per;
       const int kb = NP == 1 ? half : 0, plane = NP == 1 ? 0 : half;
-      const int64_t row = is_a ? min(m_tile * A_TILES + at, g.a_tiles - 1) : min(n_tile * B_TILES + at, g.b_tiles - 1);
-      const u4v *base = is_a ? g.A + plane * g.plane_a + row * g.ld_a * 64 : g.B + plane * g.plane_b + row * g.ld_b * 64;
-      src[l] = base + ((int64_t)split * g.k_split + kb) * 64;
+      const int64_t row = is_a ? min(m_tile * A_TILES + at, a_tiles - 1) : min(n_tile * B_TILES + at, b_tiles - 1);
+      const u4v *base = is_a ? A + plane * plane_a + row * ld_a * 64 : B + plane * plane_b + row * ld_b * 64;
+      src[l] = base + ((int64_t)split * k_split + kb) * 64;
     }
   };
   auto fill = [&](int buf) {
@@ -476,6 +487,7 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g) {
     const int m0 = (m_tile * WM + wm) * 32 * MT;                                   // first row of A of this wavefront
     const int64_t n0 = ((int64_t)n_tile * WN + wn) * 32 * NT + (lane & 31);        // this lane's row of B, tile 0
     const int of_split = split, of_m = m_tile, of_n = n_tile;
+    const bool of_other = other;
     // what the epilogue needs of its rows, ahead of the loads that it would wait for otherwise
     int place_of[NT];             // the label's place among this wavefront's words, or something out of their range
     float lse2[NT], coef_a[NT], coef_b[NT];
@@ -634,17 +646,20 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g) {
         }
       }
     } else if constexpr (MODE == DX) {
+      const int64_t rows = of_other ? g2.Pp : g.Pp, ld = of_other ? g2.ld_acc : g.ld_acc;
+      float *const to = (of_other ? g2.acc : g.acc) + ((int64_t)of_split * rows + n0) * ld;
+      const bool add = of_other ? g2.add : g.add;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int d = m0 + 32 * i + 8 * q + 4 * h;
-            if (d >= g.ld_acc) continue;
-            float4 *dst = reinterpret_cast<float4 *>(g.acc + ((int64_t)of_split * g.Pp + n0 + 32 * n) * g.ld_acc + d);
+            if (d >= ld) continue;
+            float4 *dst = reinterpret_cast<float4 *>(to + 32 * n * ld + d);
             float4 v = make_float4(acc[i][n][4 * q], acc[i][n][4 * q + 1], acc[i][n][4 * q + 2], acc[i][n][4 * q + 3]);
-            if (g.add) {
+            if (add) {
               const float4 o = *dst;
               v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
             }
@@ -797,21 +812,23 @@ __global__ void __launch_bounds__(256, 2) vce_score_kernel(Matrix w, Matrix x, c
   }
   const int64_t tiles = (w.rows + 31) / 32;
   const int groups = (int)((w.cols + 63) / 64);
+  auto words = [&](int64_t t, int g, Eight<T> (&a)[4]) {
+    const int64_t v = min(t * 32 + (lane & 31), w.rows - 1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) a[q] = fetch8<T, WIDE>(w, v, (int64_t)g * 64 + 16 * q + 8 * h);
+  };
+  Eight<T> a[4], next[4];
+  if (wave < groups) words(blockIdx.x, wave, a);
   for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int64_t v = t * 32 + (lane & 31);
     f16v acc[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
-    auto words = [&](int g, Eight<T> (&a)[4]) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) a[q] = fetch8<T, WIDE>(w, min(v, w.rows - 1), (int64_t)g * 64 + 16 * q + 8 * h);
-    };
-    Eight<T> a[4], next[4];
-    if (wave < groups) words(wave, a);
     for (int g = wave; g < groups; g += 4) {
-      if (g + 4 < groups) words(g + 4, next);
+      // what comes next, of these words or of the next tile's, is on its way while this is multiplied and joined
+      if (g + 4 < groups) words(t, g + 4, next);
+      else if (t + gridDim.x < tiles) words(t + gridDim.x, wave, next);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const Operand<T> oa = operand(a[q]);
@@ -949,37 +966,46 @@ __global__ void __launch_bounds__(1024) vce_reduce_kernel(int64_t P, const float
   }
   sum = block_sum(sum);
   n = block_sum(n);
-  if (threadIdx.x == 0) {
-    if (s) s->n_valid = (float)n;
-    *loss = (float)(mean ? sum / n : sum);
-  }
+  if (threadIdx.x != 0) return;
+  if (s) s->n_valid = (float)n;
+  *loss = (float)(mean ? sum / n : sum);
 }
 
-// Rows of a gradient = sum of the splits, scaled, in the output type: a row per wavefront, four features per lane.
+struct FinishJob {
+  int64_t rows, D, plane, ld;  // rows of the result; rows of a split and their stride in `acc`
+  int splits;
+  float scale;
+  const float *acc;
+  const int *exp_other, *exp_g;
+  void *out;
+};
+
+// Rows of a gradient = sum of the splits, scaled, in the output type: a row per wavefront, four features per lane.  Up to
+// two gradients a launch.
 template <typename T>
-__global__ void __launch_bounds__(256) vce_finish_kernel(int64_t P, int64_t D, int64_t Pp, int64_t ld, int splits, float scale,
-                                                     const float *__restrict__ acc,
-                                                         const int *__restrict__ exp_other, const int *__restrict__ exp_g,
-                                                         T *__restrict__ out) {
-  const int64_t p = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (p >= P) return;
-  const int e = -(*exp_g + *exp_other);
-  for (int64_t d = (threadIdx.x & 63) * 4; d < D; d += 256) {
-    const float *src = acc + p * ld + d;
+__global__ void __launch_bounds__(256) vce_finish_kernel(const FinishJob a, const FinishJob b) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const bool first = row < a.rows;
+  const FinishJob &j = first ? a : b;
+  const int64_t p = first ? row : row - a.rows;
+  if (p >= j.rows) return;
+  const int e = -(*j.exp_g + *j.exp_other);
+  for (int64_t d = (threadIdx.x & 63) * 4; d < j.D; d += 256) {
+    const float *src = j.acc + p * j.ld + d;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
-      const float4 a = *reinterpret_cast<const float4 *>(src + k * Pp * ld);
-      v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+    for (int k = 0; k < j.splits; ++k) {
+      const float4 q = *reinterpret_cast<const float4 *>(src + k * j.plane * j.ld);
+      v.x += q.x, v.y += q.y, v.z += q.z, v.w += q.w;
     }
-    const float x[4] = {ldexpf(v.x * scale, e), ldexpf(v.y * scale, e), ldexpf(v.z * scale, e), ldexpf(v.w * scale, e)};
-    T *dst = out + p * D + d;
-    if ((D & 3) == 0) {
+    const float x[4] = {ldexpf(v.x * j.scale, e), ldexpf(v.y * j.scale, e), ldexpf(v.z * j.scale, e), ldexpf(v.w * j.scale, e)};
+    T *dst = (T *)j.out + p * j.D + d;
+    if ((j.D & 3) == 0) {
       store4<T>(dst, x[0], x[1], x[2], x[3]);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (d + k < D) dst[k] = (T)x[k];
+        if (d + k < j.D) dst[k] = (T)x[k];
     }
   }
 }
@@ -1025,36 +1051,33 @@ struct Kept {  // what the forward pass leaves for the backward pass
   }
 };
 
-int word_units(int64_t words, int64_t rows);
+int word_units(int np, int64_t words, int64_t rows);
 
 struct FwdScratch {
-  float *amax, *target;
+  float *amax, *target, *row_loss;
   float2 *partial;
   int pairs;
   FwdScratch(Carve &c, const Shape &s) {
-    const int64_t words = 64 * word_units(s.Vp, s.Pp);
+    const int64_t words = 64 * word_units(s.np, s.Vp, s.Pp);
     pairs = (int)((s.Vp + words - 1) / words * 2);   // a wavefront's words each
     amax = c.take<float>(2 * AMAX_BLOCKS);
     target = c.take<float>(s.Pp);
+    row_loss = c.take<float>(s.Pp);
     partial = c.take<float2>((int64_t)pairs * s.Pp);
   }
 };
 
 constexpr int64_t PIECE_BYTES = 512ll << 20;  // G of one piece of the vocabulary, all copies and planes
 
-// Splits of a contraction of `k` blocks: the number up to 16 that leaves the fewest of the CUs without work (fewer if
-// that is within 2 %: each split writes and reads its own partial result), at least four blocks each.
+// Splits of a contraction of `k` blocks, where its tiles alone are fewer than the CUs: as many, up to 16, as give each CU
+// a tile at most, of at least four blocks each.  Every split writes and reads a partial result of its own, which costs
+// more than CUs without work where there is a round of tiles already (50021 words x 768 dims: 1441 against 745 us).
 struct Splits {
   int n, blocks;  // blocks of each but the last
 };
 Splits choose_splits(int64_t Dk, int64_t n_rows, int64_t k) {
   const int64_t tiles = round_up(Dk, 256) / 256 * ((n_rows + 255) / 256);
-  int want = 1;
-  double best = 0.;
-  for (int n = 1; n <= 16 && k / n >= 4; ++n) {
-    const double used = (double)(tiles * n) / (double)round_up(tiles * n, CUS);
-    if (used > best + 0.02) best = used, want = n;
-  }
+  const int64_t want = std::max<int64_t>(1, std::min({CUS / tiles, k / 4, (int64_t)16}));
   const int blocks = (int)round_up((k + want - 1) / want, 2);
   return Splits{(int)((k + blocks - 1) / blocks), blocks};
 }
@@ -1084,12 +1107,22 @@ struct BwdScratch {
   }
 };
 
+struct Product {
+  GemmArgs g;
+  int64_t m_rows, n_rows;  // multiples of 32 and of 256
+};
+
 template <int NP, int MT, int MODE, typename T>
-int launch_tiles(GemmArgs g, int64_t m_rows, int64_t n_rows, hipStream_t st) {
+int launch_tiles(const Product &a, const Product *b, hipStream_t st) {
   const size_t bytes = (size_t)3 * (2 * MT + 8) * 2 * 1024;
-  g.m_tiles = (int)((m_rows + 64 * MT - 1) / (64 * MT)), g.n_tiles = (int)((n_rows + 255) / 256);
-  g.a_tiles = (int)(m_rows / 32), g.b_tiles = (int)(n_rows / 32);
-  const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles * g.splits;
+  auto cut = [](const Product &p) {
+    GemmArgs g = p.g;
+    g.m_tiles = (int)((p.m_rows + 64 * MT - 1) / (64 * MT)), g.n_tiles = (int)((p.n_rows + 255) / 256);
+    g.a_tiles = (int)(p.m_rows / 32), g.b_tiles = (int)(p.n_rows / 32);
+    return g;
+  };
+  const GemmArgs g = cut(a), g2 = b ? cut(*b) : GemmArgs{};
+  const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles * g.splits + (int64_t)g2.m_tiles * g2.n_tiles * g2.splits;
   if (tiles > (1ll << 30)) {
     set_error_text("pr_vocab_ce: too many tiles for one launch");
     return PR_EUNSUPPORTED;
@@ -1103,46 +1136,51 @@ int launch_tiles(GemmArgs g, int64_t m_rows, int64_t n_rows, hipStream_t st) {
     PR_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     known.fetch_or(bit, std::memory_order_release);
   }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(CUS, (tiles + 7) / 8 * 8)), dim3(512), bytes, st, g);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(CUS, (tiles + 7) / 8 * 8)), dim3(512), bytes, st, g, g2);
   return check_launch("pr_vocab_ce");
 }
 
-// Words per workgroup of STATS and GRAD, in units of 64: the number whose rounds over the CUs take the least time, a
-// tile taking its share of products plus what does not shrink with it.
-int word_units(int64_t words, int64_t rows) {
+// Time of so many tiles of 64 mt by 256, in arbitrary units.  A tile costs its products and the operand rows that it does
+// not share: 1.5 with one plane (256 features by 256 words against 128 by 256: 178 and 219 us for the same product), less
+// with two, which make 1.5 times the products of what they load (320 words by 256 rows against 256 by 256: 233 and 222 us).
+// The chip is bound by its power, so a last round that leaves CUs without work runs at a higher clock: three quarters of a
+// full one.
+double tile_time(int np, int64_t tiles, int mt) {
+  return ((double)(tiles / CUS) + (tiles % CUS ? 0.75 : 0.)) * (mt + (np == 1 ? 1.5 : 0.6));
+}
+
+// Words per workgroup of STATS and GRAD, in units of 64.
+int word_units(int np, int64_t words, int64_t rows) {
   int best = 1;
-  double least = 1e300;
-  for (int mt = 1; mt <= 5; ++mt) {
-    const int64_t tiles = (words + 64 * mt - 1) / (64 * mt) * ((rows + 255) / 256);
-    const double time = (double)((tiles + CUS - 1) / CUS) * (mt + 0.6);
-    if (time < least) least = time, best = mt;
+  for (int mt = 2; mt <= 5; ++mt) {
+    auto time = [&](int m) { return tile_time(np, (words + 64 * m - 1) / (64 * m) * ((rows + 255) / 256), m); };
+    if (time(mt) < time(best)) best = mt;
   }
   return best;
 }
 template <int NP, int MODE>
 int launch_words(const GemmArgs &g, int64_t words, int64_t rows, hipStream_t st) {
-  switch (word_units(words, rows)) {
-    case 1: return launch_tiles<NP, 1, MODE, float>(g, words, rows, st);
-    case 2: return launch_tiles<NP, 2, MODE, float>(g, words, rows, st);
-    case 3: return launch_tiles<NP, 3, MODE, float>(g, words, rows, st);
-    case 4: return launch_tiles<NP, 4, MODE, float>(g, words, rows, st);
-    default: return launch_tiles<NP, 5, MODE, float>(g, words, rows, st);
+  const Product p{g, words, rows};
+  switch (word_units(NP, words, rows)) {
+    case 1: return launch_tiles<NP, 1, MODE, float>(p, nullptr, st);
+    case 2: return launch_tiles<NP, 2, MODE, float>(p, nullptr, st);
+    case 3: return launch_tiles<NP, 3, MODE, float>(p, nullptr, st);
+    case 4: return launch_tiles<NP, 4, MODE, float>(p, nullptr, st);
+    default: return launch_tiles<NP, 5, MODE, float>(p, nullptr, st);
   }
 }
 
-// The same for the products whose M rows are features, `n_rows` by `splits` of them.
+// The same for the products whose M rows are features.
 template <int NP, int MODE, typename T>
-int launch_features(const GemmArgs &g, int64_t Dk, int64_t n_rows, hipStream_t st) {
-  int best = 4;
-  double least = 1e300;
-  for (int mt = 4; mt >= 1; mt /= 2) {
-    const int64_t tiles = (Dk + 64 * mt - 1) / (64 * mt) * ((n_rows + 255) / 256) * g.splits;
-    const double time = (double)((tiles + CUS - 1) / CUS) * (mt + 0.6);
-    if (time < least) least = time, best = mt;
-  }
-  if (best == 4) return launch_tiles<NP, 4, MODE, T>(g, Dk, n_rows, st);
-  if (best == 2) return launch_tiles<NP, 2, MODE, T>(g, Dk, n_rows, st);
-  return launch_tiles<NP, 1, MODE, T>(g, Dk, n_rows, st);
+int launch_features(const Product &a, const Product *b, hipStream_t st) {
+  auto time = [&](int mt) {
+    auto tiles = [mt](const Product &p) { return (p.m_rows + 64 * mt - 1) / (64 * mt) * ((p.n_rows + 255) / 256) * p.g.splits; };
+    return tile_time(NP, tiles(a) + (b ? tiles(*b) : 0), mt);
+  };
+  const int best = time(4) <= time(2) && time(4) <= time(1) ? 4 : time(2) <= time(1) ? 2 : 1;
+  if (best == 4) return launch_tiles<NP, 4, MODE, T>(a, b, st);
+  if (best == 2) return launch_tiles<NP, 2, MODE, T>(a, b, st);
+  return launch_tiles<NP, 1, MODE, T>(a, b, st);
 }
 
 struct Call {
@@ -1194,12 +1232,13 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
 }
 
 struct ScoreScratch {  // of the forward pass for few rows
-  float *target;
+  float *target, *row_loss;
   float2 *partial;
   int blocks;
   ScoreScratch(Carve &c, const Shape &s) {
     blocks = (int)std::min<int64_t>(SCORE_BLOCKS, (s.V + 31) / 32);
     target = c.take<float>(SCORE_ROWS);
+    row_loss = c.take<float>(SCORE_ROWS);
     partial = c.take<float2>((int64_t)blocks * SCORE_ROWS);
   }
 };
@@ -1247,36 +1286,31 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
     g.gx = dx ? b.gx : nullptr, g.gw = dw ? b.gw : nullptr;
     g.plane_gx = g.plane_gw = s.Pp * b.piece / 8, g.ld_gx = b.piece / 16, g.ld_gw = kp;
     PR_TRY((launch_words<NP, GRAD>(g, words, s.Pp, st)));
-    if (dx) {
-      GemmArgs x{};
-      x.A = b.wt + v0 / 16 * 64, x.B = b.gx, x.plane_a = s.plane(s.Vp), x.plane_b = g.plane_gx, x.ld_a = kv, x.ld_b = g.ld_gx;
-      x.scal = k.scal, x.acc = b.acc, x.Pp = s.Pp, x.ld_acc = s.Dk, x.add = v0 > 0;
-      // the splits of a full piece; a shorter last piece leaves the rest of them as they are
-      x.kblocks = (int)(words / 16), x.k_split = b.split_words.blocks;
-      x.splits = (x.kblocks + x.k_split - 1) / x.k_split;
-      PR_TRY((launch_features<NP, DX, float>(x, s.Dk, s.Pp, st)));
+    const bool last = v0 + words >= s.Vp, split_dw = dw && b.split_rows.n > 1;
+    Product px{{}, s.Dk, s.Pp}, pw{{}, s.Dk, words};
+    GemmArgs &x = px.g, &w = pw.g;
+    x.A = b.wt + v0 / 16 * 64, x.B = b.gx, x.plane_a = s.plane(s.Vp), x.plane_b = g.plane_gx, x.ld_a = kv, x.ld_b = g.ld_gx;
+    x.scal = k.scal, x.acc = b.acc, x.Pp = s.Pp, x.ld_acc = s.Dk, x.add = v0 > 0;
+    // the splits of a full piece; a shorter last piece leaves the rest of them as they are
+    x.kblocks = (int)(words / 16), x.k_split = b.split_words.blocks, x.splits = (x.kblocks + x.k_split - 1) / x.k_split;
+    w.A = b.xt, w.B = b.gw, w.plane_a = s.plane(s.Pp), w.plane_b = g.plane_gw, w.ld_a = w.ld_b = kp;
+    w.kblocks = kp, w.k_split = b.split_rows.blocks, w.splits = b.split_rows.n;
+    w.scal = k.scal, w.exp_g = b.exp_g, w.scale = c.scale, w.V = c.V, w.v0 = v0, w.out = dw, w.D = c.D;
+    w.acc = b.acc_w, w.Pp = words, w.ld_acc = s.Dk;
+    if (dx || split_dw)
+      PR_TRY((launch_features<NP, DX, float>(dx ? px : pw, dx && split_dw ? &pw : nullptr, st)));
+    if (dw && !split_dw) PR_TRY((launch_features<NP, DW, T>(pw, nullptr, st)));
+    FinishJob jobs[2] = {};
+    int n = 0;
+    if (dx && last) jobs[n++] = FinishJob{c.P, c.D, s.Pp, s.Dk, b.split_words.n, c.scale, b.acc, &k.scal->exp_w, b.exp_g, dx};
+    if (split_dw)
+      jobs[n++] = FinishJob{std::min(words, c.V - v0), c.D, words, s.Dk, w.splits, fabsf(c.scale), b.acc_w, &k.scal->exp_x,
+                            b.exp_g, dw + v0 * c.D};
+    if (n) {
+      hipLaunchKernelGGL((vce_finish_kernel<T>), dim3((unsigned)((jobs[0].rows + jobs[1].rows + 3) / 4)), dim3(256), 0, st,
+                         jobs[0], jobs[1]);
+      PR_TRY(check_launch("pr_vocab_ce"));
     }
-    if (dw) {
-      GemmArgs w{};
-      w.A = b.xt, w.B = b.gw, w.plane_a = s.plane(s.Pp), w.plane_b = g.plane_gw, w.ld_a = w.ld_b = kp;
-      w.kblocks = kp, w.k_split = b.split_rows.blocks, w.splits = b.split_rows.n;
-      w.scal = k.scal, w.exp_g = b.exp_g, w.scale = c.scale, w.V = c.V, w.v0 = v0, w.out = dw, w.D = c.D;
-      if (w.splits == 1) {
-        PR_TRY((launch_features<NP, DW, T>(w, s.Dk, words, st)));
-      } else {
-        w.acc = b.acc_w, w.Pp = words, w.ld_acc = s.Dk;
-        PR_TRY((launch_features<NP, DX, float>(w, s.Dk, words, st)));
-        const int64_t rows = std::min(words, c.V - v0);
-        hipLaunchKernelGGL((vce_finish_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, rows, c.D, words, s.Dk,
-                           w.splits, fabsf(c.scale), b.acc_w, &k.scal->exp_x, b.exp_g, dw + v0 * c.D);
-        PR_TRY(check_launch("pr_vocab_ce"));
-      }
-    }
-  }
-  if (dx && c.P > 0) {
-    hipLaunchKernelGGL((vce_finish_kernel<T>), dim3((unsigned)((c.P + 3) / 4)), dim3(256), 0, st, c.P, c.D, s.Pp, s.Dk,
-                       b.split_words.n, c.scale, b.acc, &k.scal->exp_w, b.exp_g, dx);
-    PR_TRY(check_launch("pr_vocab_ce"));
   }
   return PR_OK;
 }
@@ -1324,7 +1358,7 @@ extern "C" int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const
                                float *row_loss, float *lse, float *loss, void *stream) {
   const pr::Call c{dtype, P, V, D, {x, P, D, ldx_row, ldx_col}, {w, V, D, ldw_row, ldw_col}, labels, ignore_index, scale};
   PR_TRY(pr::check_call(c));
-  if ((!kept && P > pr::SCORE_ROWS) || !scratch || !row_loss || ((uintptr_t)kept & 15) || ((uintptr_t)scratch & 15))
+  if ((!kept && P > pr::SCORE_ROWS) || !scratch || (!row_loss && !loss) || ((uintptr_t)kept & 15) || ((uintptr_t)scratch & 15))
     return PR_EINVAL;
   if ((kept && kept_bytes < pr_vocab_ce_kept_bytes(dtype, P, V, D)) ||
       scratch_bytes < pr_vocab_ce_fwd_scratch_bytes(dtype, P, V, D))
@@ -1334,12 +1368,14 @@ extern "C" int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const
   pr::Carve ck(kept), cs(scratch);
   if (!kept) {
     pr::ScoreScratch f(cs, s);
+    if (!row_loss) row_loss = f.row_loss;
     if (dtype == PR_F32) return pr::score<float>(c, mean, f, row_loss, lse, loss, st);
     if (dtype == PR_F16) return pr::score<_Float16>(c, mean, f, row_loss, lse, loss, st);
     return pr::score<__bf16>(c, mean, f, row_loss, lse, loss, st);
   }
   pr::Kept k(ck, s);
   pr::FwdScratch f(cs, s);
+  if (!row_loss) row_loss = f.row_loss;
   if (dtype == PR_F32) return pr::forward<float, 2>(c, mean, k, f, row_loss, lse, loss, st);
   if (dtype == PR_F16) return pr::forward<_Float16, 1>(c, mean, k, f, row_loss, lse, loss, st);
   return pr::forward<__bf16, 1>(c, mean, k, f, row_loss, lse, loss, st);

@@ -16,7 +16,6 @@ from typing import Tuple, Union
 import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
-from torch.autograd.graph import get_gradient_edge
 
 from . import _lib
 from .rendering import _call, _on, _ptr, _stream
@@ -29,33 +28,34 @@ def _scratch(nbytes: int, device) -> Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
-def _forward(x, w, labels, scale, ignore_index, reduction, want_lse, with_grad):
+def _forward(x, w, labels, scale, ignore_index, reduction, want_lse, with_grad, stream):
     """``x [P, D]``, ``w [V, D]``, ``labels [P]`` int64 -> loss (``[P]`` or 0-d), lse ``[P]`` or None, what backward keeps."""
     (P, D), V, dev = x.shape, w.shape[0], x.device
-    row_loss = torch.empty(P, dtype=torch.float32, device=dev)
     lse = torch.empty(P, dtype=torch.float32, device=dev) if want_lse else None
+    loss = torch.empty(P if reduction == "none" else (), dtype=torch.float32, device=dev)
     if P == 0:
-        total = {"none": row_loss, "sum": row_loss.new_zeros(()), "mean": row_loss.new_full((), math.nan)}
-        return total[reduction], lse, None
-    loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
+        if reduction != "none":
+            loss.fill_(math.nan if reduction == "mean" else 0.0)
+        return loss, lse, None
     lib, t = _lib.load(), _TYPES[x.dtype]
     # few rows and no gradient to come: nothing is packed and nothing kept
     plain = not with_grad and P <= lib.pr_vocab_ce_score_rows()
     kept = None if plain else _scratch(lib.pr_vocab_ce_kept_bytes(t, P, V, D), dev)
     scratch = _scratch(lib.pr_vocab_ce_fwd_scratch_bytes(t, P, V, D), dev)
+    per_row, scalar = (loss, None) if reduction == "none" else (None, loss)
     with _on(dev):
         _call("pr_vocab_ce_fwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index, scale,
               int(reduction == "mean"), _ptr(kept), 0 if plain else kept.numel(), _ptr(scratch), scratch.numel(),
-              _ptr(row_loss), _ptr(lse), _ptr(loss), _stream())
-    return (row_loss if loss is None else loss), lse, kept
+              _ptr(per_row), _ptr(lse), _ptr(scalar), stream)
+    return loss, lse, kept
 
 
 class _VocabularyCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, labels, scale, ignore_index, reduction, want_lse):
+    def forward(ctx, x, w, labels, scale, ignore_index, reduction, want_lse, stream):
         ctx.set_materialize_grads(False)
         ctx.args = scale, ignore_index, reduction
-        loss, lse, kept = _forward(x, w, labels, scale, ignore_index, reduction, want_lse, True)
+        loss, lse, kept = _forward(x, w, labels, scale, ignore_index, reduction, want_lse, True, stream)
         ctx.save_for_backward(x, w, labels, kept)
         return loss, lse
 
@@ -67,7 +67,7 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
         (P, D), V, dev = x.shape, w.shape[0], x.device
         want_x, want_w = ctx.needs_input_grad[:2]
         if P == 0 or (g_loss is None and g_lse is None):
-            return (torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None) + (None,) * 5
+            return (torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None) + (None,) * 6
         g_loss = None if g_loss is None else g_loss.float().contiguous()
         g_lse = None if g_lse is None else g_lse.float().contiguous()
         dx = torch.empty(P, D, dtype=x.dtype, device=dev) if want_x else None
@@ -78,26 +78,21 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
             _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index,
                   scale, int(reduction == "mean"), int(reduction == "none"), _ptr(kept), kept.numel(), _ptr(g_loss),
                   _ptr(g_lse), _ptr(scratch), scratch.numel(), _ptr(dx), _ptr(dw), _stream())
-        return (dx, dw) + (None,) * 5
+        return (dx, dw) + (None,) * 6
 
 
 _STREAM_KEY = "pogs_amd.stream"
 
 
-def _leaf_nodes(*tensors: Tensor) -> list:
-    """The gradient nodes of the leaves among ``tensors``, marked with the stream they came up on.  A leaf's node lives as
-    long as any graph of it does and keeps its first stream; a backward pass captured on another stream would make that
-    one part of the capture, which ends the process.  So the call that would lead there is refused."""
-    nodes = []
-    for t in tensors:
-        if t.is_leaf and t.requires_grad:
-            node = get_gradient_edge(t).node
-            stream = torch.cuda.current_stream(t.device).cuda_stream
+def _mark_leaves(output: Tensor, stream: int) -> None:
+    """Marks the gradient nodes of the leaves among features and vocabulary with the stream that they came up on.  A leaf's
+    node lives as long as any graph of it does and keeps its first stream; a backward pass captured on another stream would
+    make that one part of the capture, which ends the process.  So the call that would lead there is refused."""
+    for node, _ in output.grad_fn.next_functions[:2]:
+        if node is not None and hasattr(node, "variable"):     # a leaf's
             if node.metadata.setdefault(_STREAM_KEY, stream) != stream and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a graph of the same features or vocabulary, made outside the capture, is still alive: "
                                    "its backward pass cannot be captured; drop that graph's outputs first")
-            nodes.append(node)
-    return nodes
 
 
 def _check(features: Tensor, vocabulary: Tensor, labels: Tensor, scale: float, reduction: str) -> float:
@@ -118,7 +113,7 @@ def _check(features: Tensor, vocabulary: Tensor, labels: Tensor, scale: float, r
         raise ValueError(f"scale must be finite, got {scale}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
-    if not (features.is_cuda and vocabulary.is_cuda and labels.is_cuda):
+    if not features.is_cuda:
         raise RuntimeError("pogs_amd.vocabulary runs on a HIP device only (no CPU fallback)")
     if not features.device == vocabulary.device == labels.device:
         raise RuntimeError("features, vocabulary and labels are on different devices")
@@ -145,12 +140,13 @@ def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tenso
     flat = labels if labels.dim() == 1 else labels.reshape(-1)
     if flat.dtype != torch.int64 or not flat.is_contiguous():
         flat = flat.to(torch.int64).contiguous()
-    if torch.is_grad_enabled() and (features.requires_grad or vocabulary.requires_grad):
-        nodes = _leaf_nodes(features, vocabulary)    # held until the new graph holds them
-        loss, lse = _VocabularyCrossEntropy.apply(x, vocabulary, flat, scale, int(ignore_index), reduction, return_lse)
-        del nodes
+    stream = torch.cuda.current_stream(x.device).cuda_stream
+    args = x, vocabulary, flat, scale, int(ignore_index), reduction, return_lse
+    if torch.is_grad_enabled() and (x.requires_grad or vocabulary.requires_grad):
+        loss, lse = _VocabularyCrossEntropy.apply(*args, stream)
+        _mark_leaves(loss, stream)
     else:
-        loss, lse, _ = _forward(x, vocabulary, flat, scale, int(ignore_index), reduction, return_lse, False)
+        loss, lse, _ = _forward(*args, False, stream)
     if reduction == "none" and labels.dim() != 1:
         loss = loss.reshape(labels.shape)
     return (loss, lse.reshape(labels.shape)) if return_lse else loss

@@ -139,7 +139,7 @@ def test_entry_points_validate_without_a_gpu():
     def fwd(dtype=0, P=4, V=8, D=16, x=ok, ld=(16, 1), w=ok, labels=ok, scale=1.0, kept=ok, kb=1 << 30, scratch=ok, sb=1 << 30,
             row=ok):
         return lib.pr_vocab_ce_fwd(dtype, P, V, D, x, *ld, w, *ld, labels, -100, scale, 0, kept, kb, scratch, sb, row, None,
-                                   None, None)
+                                   None, None)      # row None: neither the rows' losses nor their sum are wanted
 
     for kw in (dict(dtype=3), dict(P=0), dict(V=0), dict(D=0), dict(x=None), dict(w=None), dict(labels=None), dict(x=odd),
                dict(labels=odd), dict(ld=(-1, 1)), dict(scale=math.nan), dict(scale=math.inf), dict(kept=None, P=0),
