@@ -501,10 +501,9 @@ int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const void *x, i
                     const void *w, int64_t ldw_row, int64_t ldw_col, const int64_t *labels, int64_t ignore_index,
                     float scale, int mean, void *kept, size_t kept_bytes, void *scratch, size_t scratch_bytes,
                     float *row_loss, float *lse, float *loss, void *stream);
-int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const void *x, int64_t ldx_row, int64_t ldx_col,
-                    const void *w, int64_t ldw_row, int64_t ldw_col, const int64_t *labels, int64_t ignore_index,
-                    float scale, int mean, int per_row, const void *kept, size_t kept_bytes, const float *g_loss,
-                    const float *g_lse, void *scratch, size_t scratch_bytes, void *dx, void *dw, void *stream);
+int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const int64_t *labels, int64_t ignore_index, float scale,
+                    int mean, int per_row, const void *kept, size_t kept_bytes, const float *g_loss, const float *g_lse,
+                    void *scratch, size_t scratch_bytes, void *dx, void *dw, void *stream);
 
 #ifdef __cplusplus
 }

@@ -69,8 +69,8 @@ SIGNATURES = {
     "pr_vocab_ce_bwd_scratch_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int, c_int]),
     "pr_vocab_ce_fwd": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64,
                                 c_float, c_int, _P, c_size_t, _P, c_size_t, _P, _P, _P, _P]),
-    "pr_vocab_ce_bwd": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64,
-                                c_float, c_int, c_int, _P, c_size_t, _P, _P, _P, c_size_t, _P, _P, _P]),
+    "pr_vocab_ce_bwd": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, c_float, c_int, c_int, _P, c_size_t, _P, _P,
+                                _P, c_size_t, _P, _P, _P]),
     "pr_densify_accumulate": (c_int, [c_int, c_int, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P]),
     "pr_densify_plan_scratch_bytes": (c_size_t, [c_int]),
     "pr_densify_plan": (c_int, [c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),

@@ -54,30 +54,31 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, labels, scale, ignore_index, reduction, want_lse, stream):
         ctx.set_materialize_grads(False)
-        ctx.args = scale, ignore_index, reduction
+        ctx.args = x.shape, w.shape[0], x.dtype, scale, ignore_index, reduction
         loss, lse, kept = _forward(x, w, labels, scale, ignore_index, reduction, want_lse, True, stream)
-        ctx.save_for_backward(x, w, labels, kept)
+        ctx.save_for_backward(labels, kept)      # kept has its own copy of features and vocabulary
         return loss, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_loss, g_lse):
-        x, w, labels, kept = ctx.saved_tensors
-        scale, ignore_index, reduction = ctx.args
-        (P, D), V, dev = x.shape, w.shape[0], x.device
+        labels, kept = ctx.saved_tensors
+        (P, D), V, dtype, scale, ignore_index, reduction = ctx.args
         want_x, want_w = ctx.needs_input_grad[:2]
-        if P == 0 or (g_loss is None and g_lse is None):
-            return (torch.zeros_like(x) if want_x else None, torch.zeros_like(w) if want_w else None) + (None,) * 6
-        g_loss = None if g_loss is None else g_loss.float().contiguous()
-        g_lse = None if g_lse is None else g_lse.float().contiguous()
-        dx = torch.empty(P, D, dtype=x.dtype, device=dev) if want_x else None
-        dw = torch.empty(V, D, dtype=w.dtype, device=dev) if want_w else None
-        lib, t = _lib.load(), _TYPES[x.dtype]
-        scratch = _scratch(lib.pr_vocab_ce_bwd_scratch_bytes(t, P, V, D, int(want_x), int(want_w)), dev)
-        with _on(dev):
-            _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(x), *x.stride(), _ptr(w), *w.stride(), _ptr(labels), ignore_index,
-                  scale, int(reduction == "mean"), int(reduction == "none"), _ptr(kept), kept.numel(), _ptr(g_loss),
-                  _ptr(g_lse), _ptr(scratch), scratch.numel(), _ptr(dx), _ptr(dw), _stream())
+        dev = labels.device
+        empty = P == 0 or (g_loss is None and g_lse is None)
+        make = torch.zeros if empty else torch.empty
+        dx = make(P, D, dtype=dtype, device=dev) if want_x else None
+        dw = make(V, D, dtype=dtype, device=dev) if want_w else None
+        if not empty:
+            g_loss = None if g_loss is None else g_loss.float().contiguous()
+            g_lse = None if g_lse is None else g_lse.float().contiguous()
+            lib, t = _lib.load(), _TYPES[dtype]
+            scratch = _scratch(lib.pr_vocab_ce_bwd_scratch_bytes(t, P, V, D, int(want_x), int(want_w)), dev)
+            with _on(dev):
+                _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(labels), ignore_index, scale, int(reduction == "mean"),
+                      int(reduction == "none"), _ptr(kept), kept.numel(), _ptr(g_loss), _ptr(g_lse), _ptr(scratch),
+                      scratch.numel(), _ptr(dx), _ptr(dw), _stream())
         return (dx, dw) + (None,) * 6
 
 

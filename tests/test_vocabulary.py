@@ -150,8 +150,7 @@ def test_entry_points_validate_without_a_gpu():
     assert fwd(kb=16) == -3 and fwd(sb=16) == -3
 
     def bwd(dx=ok, dw=ok, kept=ok, kb=1 << 30, scratch=ok, sb=1 << 30, P=4):
-        return lib.pr_vocab_ce_bwd(0, P, 8, 16, ok, 16, 1, ok, 16, 1, ok, -100, 1.0, 0, 0, kept, kb, ok, None, scratch, sb, dx,
-                                   dw, None)
+        return lib.pr_vocab_ce_bwd(0, P, 8, 16, ok, -100, 1.0, 0, 0, kept, kb, ok, None, scratch, sb, dx, dw, None)
 
     assert bwd(dx=None, dw=None) == 0
     for kw in (dict(dx=odd), dict(dw=odd), dict(kept=None), dict(scratch=None), dict(scratch=odd), dict(P=0)):
@@ -321,19 +320,41 @@ def test_values_that_are_not_finite_stay_with_their_rows():
 @pytest.mark.gpu
 @pytest.mark.parametrize("exp_x,exp_w", [(90, -90), (-90, 90), (-60, 0), (0, 60), (-100, -100)])
 def test_magnitudes(exp_x, exp_w):
-    """Powers of two in features and vocabulary: the same bits where their product with the scale is the same."""
+    """Powers of two in features and vocabulary: the same bits where their product with the scale is the same, with and
+    without gradients to come."""
     from pogs_amd.vocabulary import vocabulary_cross_entropy
 
     x, w, y = inputs(40, 300, 64, torch.float32, seed=8)
-    base = vocabulary_cross_entropy(x, w, y, reduction="none", return_lse=True)
-    xs, ws = x * 2.0 ** exp_x, w * 2.0 ** exp_w
     total = exp_x + exp_w
-    if total == -200:          # logits vanish: the loss is the logarithm of the number of words
-        loss, lse = vocabulary_cross_entropy(xs, ws, y, reduction="none", return_lse=True)
-        assert ((loss - math.log(300)).abs() <= 16 * U * math.log(300)).all()
-        return
-    loss, lse = vocabulary_cross_entropy(xs, ws, y, scale=2.0 ** -total, reduction="none", return_lse=True)
-    assert torch.equal(loss, base[0]) and torch.equal(lse, base[1])
+    for grads in (False, True):
+        a, b = x.clone().requires_grad_(grads), w.clone().requires_grad_(grads)
+        xs, ws = (x * 2.0 ** exp_x).requires_grad_(grads), (w * 2.0 ** exp_w).requires_grad_(grads)
+        base = vocabulary_cross_entropy(a, b, y, reduction="none", return_lse=True)
+        if total == -200:      # logits vanish: the loss is the logarithm of the number of words
+            loss, _ = vocabulary_cross_entropy(xs, ws, y, reduction="none", return_lse=True)
+            assert ((loss - math.log(300)).abs() <= 16 * U * math.log(300)).all()
+            continue
+        loss, lse = vocabulary_cross_entropy(xs, ws, y, scale=2.0 ** -total, reduction="none", return_lse=True)
+        assert torch.equal(loss, base[0]) and torch.equal(lse, base[1])
+        if grads:
+            for got, want, e in zip(torch.autograd.grad(loss.sum(), (xs, ws)), torch.autograd.grad(base[0].sum(), (a, b)),
+                                    (exp_x, exp_w)):
+                assert torch.equal(got * 2.0 ** e, want)
+
+
+@pytest.mark.gpu
+def test_half_precision_below_its_normal_range():
+    """float16 features of a few steps of 2^-24: the matrix cores take them as they are.  (The features' gradient, 2^20
+    times a mean of the vocabulary, is beyond float16.)"""
+    g = torch.Generator().manual_seed(12)
+    w = torch.randn(200, 64, generator=g).half().cuda()
+    x = (torch.randint(-40, 41, (70, 64), generator=g).double() * 2.0 ** -24).half().cuda()
+    y = torch.randint(0, 200, (70,), generator=g).cuda()
+    check(x, w, y, scale=2.0 ** 20, reduction="none", want=("w",))
+    z = torch.zeros(64, device="cuda", dtype=torch.float64)
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+    close(vocabulary_cross_entropy(x[:64], w, y[:64], 2.0 ** 20, reduction="none"),
+          reference(x[:64], w, y[:64], 2.0 ** 20, z, z)["loss"], "few rows")
 
 
 @pytest.mark.gpu
@@ -430,6 +451,56 @@ def test_features_beyond_32_bit_offsets():
     ref = reference(x.detach()[rows], w, y[rows], 1.0, ones, 0 * ones)
     close(loss[rows], ref["loss"], "loss")
     close(gx[rows], ref["dx"], "dx")
+
+
+@pytest.mark.gpu
+def test_vocabulary_beyond_32_bit_offsets():
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    P, V, D = 5, (1 << 21) + 77, 1030
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.empty(V, D, dtype=torch.bfloat16, device="cuda")
+    assert w.numel() > 1 << 31
+    w.normal_(generator=g).mul_(0.125)
+    x = torch.randn(P, D, generator=g, device="cuda").to(torch.bfloat16) * 0.25
+    y = torch.tensor([0, V - 1, V - 78, 1 << 20, IGN], device="cuda")
+    z = torch.cat([x.double() @ w[lo:lo + (1 << 18)].double().t() for lo in range(0, V, 1 << 18)], 1)
+    lse = torch.logsumexp(z, 1)
+    want = lse[:4] - z[torch.arange(4), y[:4]]
+    wr = w.requires_grad_(True)
+    loss = vocabulary_cross_entropy(x, wr, y, reduction="none")
+    # |x| |w| of a row is about 0.25 * 0.125 * 1030 * 0.64: the logits' error is below 1e-4 by the bound above
+    assert ((loss[:4].double() - want).abs() <= 1e-3).all() and loss[4].item() == 0.0
+    with torch.no_grad():
+        few = vocabulary_cross_entropy(x, w, y, reduction="none")
+    assert ((few[:4].double() - want).abs() <= 1e-3).all()
+    dw = torch.autograd.grad(loss.sum(), wr)[0]
+    for v in (0, 1, V // 2, V - 78, V - 1):
+        p = (z[:4, v] - lse[:4]).exp() - (y[:4] == v).double()
+        ref = p @ x[:4].double()
+        mag = p.abs() @ x[:4].double().abs()
+        # logits 1e-3, G 2^-11, bf16 2^-8
+        assert ((dw[v].double() - ref).abs() <= mag * (2e-3 + 2.0 ** -11) + ref.abs() * 2.0 ** -8 + 2.0 ** -40).all(), v
+
+
+@pytest.mark.gpu
+def test_inputs_changed_after_the_forward_pass():
+    """The backward pass has its own copy of features and vocabulary; changed labels are noticed."""
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    x, w, y = inputs(50, 120, 32, torch.float32, seed=9)
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    want = torch.autograd.grad(vocabulary_cross_entropy(a, b, y), (a, b))
+    a2, b2 = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = vocabulary_cross_entropy(a2, b2, y)
+    with torch.no_grad():
+        a2.zero_(), b2.mul_(3.0)
+    got = torch.autograd.grad(loss, (a2, b2))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    loss = vocabulary_cross_entropy(a, b, y)
+    y.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, (a, b))
 
 
 @pytest.mark.gpu
