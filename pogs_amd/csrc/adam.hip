@@ -41,7 +41,7 @@ struct AdamTable {
 struct ClipTable {  // per group: the set whose norm its gradient is clipped by (-1: not clipped) and what it may be
   NormSets sets;
   int set[MAX_GROUPS];
-  float max_norm[MAX_GROUPS];
+  double max_norm[MAX_GROUPS];
   float *norms;
 };
 struct NoClip {};
@@ -52,8 +52,8 @@ __device__ __forceinline__ float gradient_factor(const NoClip &, int, bool) { re
 __device__ __forceinline__ float gradient_factor(const ClipTable &c, int gi, bool first) {
   const int s = c.set[gi];
   if (s < 0) return 1.f;
-  const float norm = norm_of_set<PR_NORM_2>(c.sets, s);
-  if (first && threadIdx.x == 0) c.norms[s] = norm;   // (every group of the set writes the same)
+  const double norm = norm_of_set<PR_NORM_2>(c.sets, s);
+  if (first && threadIdx.x == 0) c.norms[s] = (float)norm;   // (every group of the set writes the same)
   return clip_coefficient(norm, c.max_norm[gi]);
 }
 
@@ -142,7 +142,7 @@ int adam_launch(const pr_adam_group *groups, const pr_clip_rule *clips, const No
     if (g.numel == 0) continue;
     const int k = t.n++;
     c.set[k] = clips ? clips[i].set : -1;
-    c.max_norm[k] = clips ? (float)clips[i].max_norm : 0.f;
+    c.max_norm[k] = clips ? clips[i].max_norm : 0.;
     t.param[k] = g.param;
     t.grad[k] = g.grad;
     t.exp_avg[k] = g.exp_avg;
@@ -226,7 +226,7 @@ extern "C" int pr_adam_step_clipped(const pr_adam_group *groups, const pr_clip_r
   if (rc != PR_OK) return rc;
   rc = pr::write_empty_norms(t.p, n, n_sets, scratch, scratch_bytes, norms, stream);
   if (rc != PR_OK) return rc;
-  rc = pr::launch_grad_norms(t.p, n, n_sets, PR_NORM_2, scratch, scratch_bytes, &sets, st);
+  rc = pr::launch_grad_norms(t.p, n, n_sets, PR_NORM_2, pr::ADAM_JOINS, scratch, scratch_bytes, &sets, st);
   for (int i = 0; rc == PR_OK && i < n_groups; i += pr::MAX_GROUPS)
     rc = pr::adam_launch(groups + i, clips + i, &sets, norms, n_groups - i < pr::MAX_GROUPS ? n_groups - i : pr::MAX_GROUPS, st);
   return rc;

@@ -188,13 +188,6 @@ __device__ __forceinline__ bool touches_region_log2(float gx, float gy, float o,
   return o * __builtin_amdgcn_exp2f(1e-3f - smin) >= ALPHA_MIN;
 }
 
-// Factor that brings gradients of this norm to at most max_norm, as torch.nn.utils.clip_grad_norm_ forms it: a norm
-// within bounds gives exactly 1, a NaN norm NaN.
-__device__ __forceinline__ float clip_coefficient(float norm, float max_norm) {
-  const float c = max_norm / (norm + 1e-6f);
-  return c >= 1.f ? 1.f : c;
-}
-
 __device__ __forceinline__ float wave_sum_all(float v) {
   v = wave_sum_to_lane63(v);
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));

@@ -37,7 +37,7 @@ struct Table {
 };
 
 struct MaxNorms {
-  float of[NORM_SETS];
+  double of[NORM_SETS];
 };
 
 __device__ __forceinline__ float from_bits16(unsigned short b, int dtype) {
@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(BLOCK) grad_norm_finish_kernel(const NormSets 
     v = norm_block_combine<KIND>(v);
     if (threadIdx.x == 0) totals[s] = v;
   } else {
-    const float norm = norm_of_set<KIND>(sets, s);
-    if (threadIdx.x == 0) norms[s] = norm;
+    const double norm = norm_of_set<KIND>(sets, s);
+    if (threadIdx.x == 0) norms[s] = (float)norm;
   }
 }
 
@@ -182,9 +182,10 @@ __global__ void __launch_bounds__(BLOCK) grad_scale_kernel(const Table t, const 
                                                            float *__restrict__ norms) {
   const unsigned block = gridDim.x - 1 - blockIdx.x;
   const int k = find_tensor(t, block), set = t.set[k];
-  const float norm = norm_of_set<KIND>(sets, set), c = clip_coefficient(norm, max_norms.of[set]);
+  const double norm = norm_of_set<KIND>(sets, set);
+  const float c = clip_coefficient(norm, max_norms.of[set]);
   const unsigned first = t.first_block[k], blocks = t.first_block[k + 1] - first;
-  if (block == first && threadIdx.x == 0) norms[set] = norm;   // (every tensor of the set writes the same)
+  if (block == first && threadIdx.x == 0) norms[set] = (float)norm;   // (every tensor of the set writes the same)
   // a norm within bounds leaves every value as it is: nothing to read or write (NaN is no such norm)
   if (c == 1.f) return;
   const int64_t n = t.numel[k], chunks = (n + CHUNK - 1) / CHUNK;
@@ -252,8 +253,8 @@ int check_apart(const pr_grad_tensor *tensors, int n) {
 }
 
 template <int KIND>
-int launch_kind(const pr_grad_tensor *tensors, int n, int n_sets, double *partials, size_t room, NormSets *sets,
-                hipStream_t st) {
+int launch_kind(const pr_grad_tensor *tensors, int n, int n_sets, unsigned joins, double *partials, size_t room,
+                NormSets *sets, hipStream_t st) {
   unsigned of_set[NORM_SETS] = {};
   size_t used = 0;
   for (Launches l(tensors, n);;) {
@@ -274,7 +275,7 @@ int launch_kind(const pr_grad_tensor *tensors, int n, int n_sets, double *partia
     sets->first[s + 1] = sets->first[s] + of_set[s];
     most = std::max(most, of_set[s]);
   }
-  if (most <= JOIN_PARTIALS) return PR_OK;
+  if (most <= joins) return PR_OK;
   if (used + n_sets > room) return PR_ESCRATCH;
   hipLaunchKernelGGL(grad_norm_finish_kernel<KIND>, dim3(n_sets), dim3(BLOCK), 0, st, *sets, partials + used, (float *)nullptr);
   sets->partials = partials + used;
@@ -315,13 +316,13 @@ int write_empty_norms(const pr_grad_tensor *tensors, int n, int n_sets, void *sc
   return PR_OK;
 }
 
-int launch_grad_norms(const pr_grad_tensor *tensors, int n, int n_sets, int kind, void *scratch, size_t scratch_bytes,
-                      NormSets *sets, hipStream_t st) {
+int launch_grad_norms(const pr_grad_tensor *tensors, int n, int n_sets, int kind, unsigned joins, void *scratch,
+                      size_t scratch_bytes, NormSets *sets, hipStream_t st) {
   double *partials = (double *)scratch;
   const size_t room = scratch_bytes / sizeof(double);
-  if (kind == PR_NORM_1) return launch_kind<PR_NORM_1>(tensors, n, n_sets, partials, room, sets, st);
-  if (kind == PR_NORM_2) return launch_kind<PR_NORM_2>(tensors, n, n_sets, partials, room, sets, st);
-  return launch_kind<PR_NORM_INF>(tensors, n, n_sets, partials, room, sets, st);
+  if (kind == PR_NORM_1) return launch_kind<PR_NORM_1>(tensors, n, n_sets, joins, partials, room, sets, st);
+  if (kind == PR_NORM_2) return launch_kind<PR_NORM_2>(tensors, n, n_sets, joins, partials, room, sets, st);
+  return launch_kind<PR_NORM_INF>(tensors, n, n_sets, joins, partials, room, sets, st);
 }
 
 namespace {
@@ -358,7 +359,7 @@ extern "C" int pr_grad_norm(const pr_grad_tensor *tensors, int n, int n_sets, in
   if (rc != PR_OK) return rc;
   hipStream_t st = (hipStream_t)stream;
   pr::NormSets sets;
-  rc = pr::launch_grad_norms(tensors, n, n_sets, kind, scratch, scratch_bytes, &sets, st);
+  rc = pr::launch_grad_norms(tensors, n, n_sets, kind, pr::SCALE_JOINS, scratch, scratch_bytes, &sets, st);
   if (rc != PR_OK) return rc;
   const dim3 grid(n_sets), block(pr::BLOCK);
   double *const none = nullptr;
@@ -378,13 +379,13 @@ extern "C" int pr_grad_clip(const pr_grad_tensor *tensors, int n, int n_sets, in
   pr::MaxNorms m{};
   for (int s = 0; s < n_sets; ++s) {
     if (!(max_norms[s] >= 0.0)) return PR_EINVAL;
-    m.of[s] = (float)max_norms[s];
+    m.of[s] = max_norms[s];
   }
   rc = pr::write_empty_norms(tensors, n, n_sets, scratch, scratch_bytes, norms, stream);
   if (rc != PR_OK) return rc;
   hipStream_t st = (hipStream_t)stream;
   pr::NormSets sets;
-  rc = pr::launch_grad_norms(tensors, n, n_sets, kind, scratch, scratch_bytes, &sets, st);
+  rc = pr::launch_grad_norms(tensors, n, n_sets, kind, pr::SCALE_JOINS, scratch, scratch_bytes, &sets, st);
   if (rc != PR_OK) return rc;
   if (kind == PR_NORM_1) return pr::scale_by_norms<PR_NORM_1>(tensors, n, sets, m, norms, st);
   if (kind == PR_NORM_2) return pr::scale_by_norms<PR_NORM_2>(tensors, n, sets, m, norms, st);
