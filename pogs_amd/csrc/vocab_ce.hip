@@ -455,6 +455,7 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
       __builtin_amdgcn_global_load_lds((global_ptr)(src[l] + lane), (lds_ptr)(lds + (buf * STAGE + j) * 64), 16, 0, 0);
       src[l] += KB * 64;
     }
+    asm volatile("" ::: "memory");   // fills stay in order: the waits below count on it
   };
   struct Half {  // one k block, or one plane, of a stage
     h8v a[MT], b[NT];
@@ -537,6 +538,7 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
       buf = buf == 2 ? 0 : buf + 1;
     }
     if (!late) __builtin_amdgcn_s_barrier();   // in step again: every wavefront has read the last stage
+    asm volatile("" ::: "memory");
 
     tile += gridDim.x >> 3;
     const bool again = tile < hi;

@@ -484,6 +484,42 @@ def test_vocabulary_beyond_32_bit_offsets():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("P,V,D", [(1, 1, 1), (3, 257, 31), (65, 700, 33), (257, 1300, 130), (600, 90, 96), (513, 5000, 520)])
+def test_nothing_is_written_outside_the_buffers(P, V, D, dtype):
+    """Every buffer of the C entry points at its exact size between guard bytes."""
+    lib, t = _lib.load(), {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    x, w, y = inputs(P, V, D, dtype, seed=3)
+    guarded = []
+
+    def buffer(nbytes):
+        b = torch.full((nbytes + 8192,), 0x5A, dtype=torch.uint8, device="cuda")
+        guarded.append((b, nbytes))
+        return ctypes.c_void_p(b.data_ptr() + 4096)
+
+    e = x.element_size()
+    nk, nf = lib.pr_vocab_ce_kept_bytes(t, P, V, D), lib.pr_vocab_ce_fwd_scratch_bytes(t, P, V, D)
+    st = torch.cuda.current_stream().cuda_stream
+
+    def fwd(kept):
+        return lib.pr_vocab_ce_fwd(t, P, V, D, x.data_ptr(), D, 1, w.data_ptr(), D, 1, y.data_ptr(), -100, 2.0, 1, kept, nk,
+                                   buffer(nf), nf, buffer(4 * P), buffer(4 * P), buffer(4), st)
+
+    kept = buffer(nk)
+    assert fwd(kept) == 0
+    if P <= lib.pr_vocab_ce_score_rows():
+        assert fwd(None) == 0
+    g = torch.ones(1, device="cuda")
+    for dx, dw in ((1, 1), (1, 0), (0, 1)):
+        nb = lib.pr_vocab_ce_bwd_scratch_bytes(t, P, V, D, dx, dw)
+        assert lib.pr_vocab_ce_bwd(t, P, V, D, y.data_ptr(), -100, 2.0, 1, 0, kept, nk, g.data_ptr(), None, buffer(nb), nb,
+                                   buffer(e * P * D) if dx else None, buffer(e * V * D) if dw else None, st) == 0
+    torch.cuda.synchronize()
+    for b, n in guarded:
+        assert (b[:4096] == 0x5A).all() and (b[4096 + n:] == 0x5A).all()
+
+
+@pytest.mark.gpu
 def test_inputs_changed_after_the_forward_pass():
     """The backward pass has its own copy of features and vocabulary; changed labels are noticed."""
     from pogs_amd.vocabulary import vocabulary_cross_entropy
