@@ -144,6 +144,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
         nbytes = lib.pr_grad_norm_scratch_bytes(at, n, 1)
         scratch, norm = _norm_buffers(nbytes, (), dev)
         _call("pr_grad_clip", at, n, 1, kind, ctypes.addressof(limit), scratch.data_ptr(), nbytes, norm.data_ptr(), _stream())
+        torch.autograd.graph.increment_version(flat)     # written in place, as far as autograd is concerned too
         if flat is not grads:
             with torch.no_grad():
                 for g, f in zip(grads, flat):

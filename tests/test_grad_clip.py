@@ -209,6 +209,19 @@ def test_views_of_one_buffer_layouts_and_strides():
 
 
 @pytest.mark.gpu
+def test_autograd_notices_that_gradients_were_scaled():
+    from pogs_amd.optim import clip_grad_norm_
+
+    p = torch.ones(100, device="cuda", requires_grad=True)
+    p.grad = torch.full((100,), 3.0, device="cuda")
+    q = torch.ones(100, device="cuda", requires_grad=True)
+    loss = (q * p.grad).sum()
+    clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.gpu
 def test_gradients_without_elements():
     from pogs_amd.optim import Optimizers, clip_grad_norm_, grad_norm
 
