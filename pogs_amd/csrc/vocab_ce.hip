@@ -1329,7 +1329,8 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
 }
 
 int check_call(const Call &c) {
-  if (!valid_shape(c.dtype, c.P, c.V, c.D) || c.P < 1 || !(fabsf(c.scale) < INFINITY)) return PR_EINVAL;
+  if (!valid_shape(c.dtype, c.P, c.V, c.D) || c.P < 1) return PR_EINVAL;
+  if (!(fabsf(c.scale) <= 1e38f)) return PR_EINVAL;   // its product with log2(e) is finite
   return !c.labels || ((uintptr_t)c.labels & 7) ? PR_EINVAL : PR_OK;
 }
 

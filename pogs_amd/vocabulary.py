@@ -110,8 +110,8 @@ def _check(features: Tensor, vocabulary: Tensor, labels: Tensor, scale: float, r
                         f"{features.dtype} and {vocabulary.dtype}")
     if isinstance(scale, Tensor):
         raise TypeError("scale is a plain number; multiply the features by a learned one")
-    if not math.isfinite(scale) or abs(scale) > 3e38:
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= 1e38:
+        raise ValueError(f"scale must be finite (within 1e38), got {scale}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
     if not features.is_cuda:

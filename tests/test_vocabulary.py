@@ -178,6 +178,21 @@ def test_refusals():
             f(x, w, y, **kw)
 
 
+def test_scale_whose_logits_cannot_be_formed_is_refused():
+    from pogs_amd.vocabulary import vocabulary_cross_entropy as f
+
+    x, w, y = torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(3, dtype=torch.int64)
+    at, n = ctypes.c_void_p(1 << 20), 1 << 30
+    lib = _lib.load()
+    for scale in (1.1e38, -3e38):      # times log2(e), 3e38 is infinite
+        with pytest.raises(ValueError, match="finite"):
+            f(x, w, y, scale=scale)
+        assert lib.pr_vocab_ce_fwd(0, 3, 5, 4, at, 4, 1, at, 4, 1, at, -100, scale, 0, at, n, at, n, at, None, None, None) == -1
+        assert lib.pr_vocab_ce_bwd(0, 3, 5, 4, at, -100, scale, 0, 1, at, n, at, None, at, n, at, at, None) == -1
+    with pytest.raises(RuntimeError, match="HIP device"):
+        f(x, w, y, scale=1e38)
+
+
 # ---- on the GPU -------------------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (1, 2, 3), (5, 7, 9), (2, 300, 33), (33, 256, 32), (128, 257, 64), (129, 511, 65), (300, 1000, 128),
           (64, 5001, 96), (257, 513, 520), (1000, 77, 100), (31, 2048, 200)]
