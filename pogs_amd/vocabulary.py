@@ -85,11 +85,15 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
 _STREAM_KEY = "pogs_amd.stream"
 
 
-def _mark_leaves(output: Tensor, stream: int) -> None:
+def _mark_leaves(output: Tensor, stream: int, reshaped: bool) -> None:
     """Marks the gradient nodes of the leaves among features and vocabulary with the stream that they came up on.  A leaf's
     node lives as long as any graph of it does and keeps its first stream; a backward pass captured on another stream would
-    make that one part of the capture, which ends the process.  So the call that would lead there is refused."""
+    make that one part of the capture, which ends the process.  So the call that would lead there is refused.
+    ``reshaped``: the features are a leaf, and the call has made rows of them itself."""
     for node, _ in output.grad_fn.next_functions[:2]:
+        while reshaped and node is not None and not hasattr(node, "variable"):
+            node = node.next_functions[0][0]
+        reshaped = False
         if node is not None and hasattr(node, "variable"):     # a leaf's
             if node.metadata.setdefault(_STREAM_KEY, stream) != stream and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a graph of the same features or vocabulary, made outside the capture, is still alive: "
@@ -145,7 +149,7 @@ def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tenso
     args = x, vocabulary, flat, scale, int(ignore_index), reduction, return_lse
     if torch.is_grad_enabled() and (x.requires_grad or vocabulary.requires_grad):
         loss, lse = _VocabularyCrossEntropy.apply(*args, stream)
-        _mark_leaves(loss, stream)
+        _mark_leaves(loss, stream, x is not features and features.is_leaf)
     else:
         loss, lse, _ = _forward(*args, False, stream)
     if reduction == "none" and labels.dim() != 1:

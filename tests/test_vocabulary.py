@@ -626,6 +626,31 @@ def test_graphs_and_streams():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["rows", "batch", "one row", "transposed"])
+def test_capture_is_refused_while_a_graph_of_the_leaves_lives(layout):
+    """Features that the call makes rows of itself are leaves all the same; nothing is captured past the refusal."""
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    x, w, y = inputs(12, 50, 16, torch.float32, seed=44)
+    x, y = {"rows": lambda: (x, y), "batch": lambda: (x.view(3, 4, 16), y.view(3, 4)), "one row": lambda: (x[0], y[0]),
+            "transposed": lambda: (x.view(3, 4, 16).transpose(0, 1), y.view(3, 4).t())}[layout]()
+    x = x.detach().requires_grad_(True)
+    loss = vocabulary_cross_entropy(x, w, y)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            vocabulary_cross_entropy(x, w, y)
+    eager, = torch.autograd.grad(loss, x)
+    del loss
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured, = torch.autograd.grad(vocabulary_cross_entropy(x, w, y), x)
+    for _ in range(3):
+        captured.zero_()
+        g.replay()
+        assert torch.equal(captured, eager)
+
+
+@pytest.mark.gpu
 def test_training_step_of_heads_loss_clipping_and_adam():
     """The operators as they are used together: clip head -> vocabulary loss -> gradients -> step clipped to the head's
     own norm.  The head's products are split-bf16 (2^-16 each), four layers deep: 1e-4 of the loss.  A gradient through a
