@@ -242,6 +242,8 @@ class Optimizers:
             max_norm = _max_norm(max_norm)
             if any(m is not None for m in limits):
                 raise ValueError("a max_norm over all groups and a max_norm of a group's own exclude each other")
+        if max_norm is not None or any(m is not None for m in limits):
+            limits = self._check_clipped(param_groups, limits)       # before any state is touched
         entries, rules, keep = [], [], []        # rules: (group or None for all together, its limit or None)
         for name, limit in zip(param_groups, limits):
             cfg = self.config[name]
@@ -276,6 +278,16 @@ class Optimizers:
                 self._step_clipped(entries, rules, param_groups, dev, _stream())
         del keep
 
+    def _check_clipped(self, param_groups: List[str], limits: list) -> List[Optional[float]]:
+        """The groups' limits.  A parameter that is there twice would count twice in the norm and be stepped by two
+        workgroups at once; a norm is taken on one device."""
+        params = [p for name in param_groups for p in self.parameters[name]]
+        if len(set(map(id, params))) < len(params):
+            raise ValueError("a clipped step takes every parameter once: a group or a parameter is listed twice")
+        if len({p.get_device() for p in params}) > 1 and len({p.get_device() for p in params if p.grad is not None}) > 1:
+            raise RuntimeError("a clipped step takes parameters of one device: step the groups of each device on their own")
+        return [None if m is None else _max_norm(m) for m in limits]
+
     def _step_clipped(self, entries: List[bytes], rules: list, param_groups: List[str], device, stream: int) -> None:
         """The step where a group at least has a limit, for as many norms at once as a call takes."""
         lib = _lib.load()
@@ -287,7 +299,7 @@ class Optimizers:
                     if len(of) == most:
                         break
                     of[name] = len(of)
-                clips.append(_CLIP_RULE.pack(-1, 0, 0.0) if limit is None else _CLIP_RULE.pack(of[name], 0, _max_norm(limit)))
+                clips.append(_CLIP_RULE.pack(-1, 0, 0.0) if limit is None else _CLIP_RULE.pack(of[name], 0, limit))
             i = lo + len(clips)
             groups, by, n, sets = b"".join(entries[lo:i]), b"".join(clips), len(clips), max(len(of), 1)
             nbytes = lib.pr_adam_clip_scratch_bytes(groups, by, n, sets)

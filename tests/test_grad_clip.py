@@ -124,6 +124,44 @@ def test_refusals():
     ShardAdam({"a": {"lr": 1e-3, "max_norm": None}})
 
 
+class _OnADevice:
+    """As much of a parameter with a gradient as the optimiser looks at before it touches anything."""
+
+    is_cuda, dtype, grad = True, torch.float32, torch.ones(4)
+
+    def __init__(self, device):
+        self.device = device
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return self.device
+
+
+def test_clipped_steps_are_refused_before_they_begin():
+    from pogs_amd.optim import Optimizers
+
+    p, q, r = _OnADevice(0), _OnADevice(0), _OnADevice(1)
+    clip = {"lr": 1e-3, "max_norm": 1.0}
+
+    def refused(opt, error, match, names, **kw):
+        with pytest.raises(error, match=match):
+            opt.optimizer_step_some(names, **kw)
+        assert all(opt.state(name, i) == {} for name in opt.parameters for i in range(len(opt.parameters[name])))
+
+    opt = Optimizers({"a": dict(clip), "b": dict(clip), "c": {"lr": 1e-3}}, {"a": [p], "b": [p, q], "c": [r]})
+    refused(opt, ValueError, "twice", ["a", "a"])
+    refused(opt, ValueError, "twice", ["a", "b"])
+    refused(opt, RuntimeError, "one device", ["a", "c"])
+    free = Optimizers({"a": {"lr": 1e-3}, "b": {"lr": 1e-3}}, {"a": [p, p], "b": [q, r]})
+    refused(free, ValueError, "twice", ["a"], max_norm=1.0)
+    refused(free, RuntimeError, "one device", ["b"], max_norm=1.0)
+    for bad in (-1.0, math.nan):                # set after the optimiser was made
+        opt.config["a"]["max_norm"] = bad
+        refused(opt, ValueError, "max_norm", ["a"])
+
+
 def test_one_block_recognises_dense_layouts():
     from pogs_amd.optim import _one_block
 
