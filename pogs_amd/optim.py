@@ -122,9 +122,9 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     """``torch.nn.utils.clip_grad_norm_``: multiplies the ``.grad`` of every parameter that has one by
     ``min(1, max_norm / (norm + 1e-6))``, in place, and returns the norm over all of them before that (0-d float32).
 
-    Gradients may be float32, float16 or bfloat16, of any layout, all on one device and in memory of their own: two
-    gradients that share memory (a parameter listed twice) are refused, as scaling them at once is a race.  Each value is
-    rounded once, to its own type.  Where the norm is within bounds no gradient is written.  A norm that is not finite
+    Gradients may be float32, float16 or bfloat16, of any layout, all on one device and in memory of their own: two that
+    begin at the same place (a parameter listed twice) or whose blocks overlap are refused, as scaling them at once is a
+    race.  Each value is rounded once, to its own type.  Where the norm is within bounds no gradient is written.  A norm that is not finite
     gives what torch gives: factor 0 for an infinite norm, NaN for a NaN one; ``error_if_nonfinite`` raises instead, and
     only then does the host wait for the device."""
     kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
@@ -139,6 +139,10 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     dev, lib = _check_grads(grads), _lib.load()
     with _on(dev):
         flat = _flat(grads)
+        if flat is not grads:      # a copy shares nothing, so the blocks' own check would miss it
+            starts = [g.data_ptr() for g in grads if g.numel()]
+            if len(set(starts)) < len(starts):
+                raise RuntimeError("clip_grad_norm_: two gradients share memory")
         table, limit = _grad_table(flat), ctypes.c_double(max_norm)
         at, n = _address(table), len(flat)
         nbytes = lib.pr_grad_norm_scratch_bytes(at, n, 1)

@@ -247,6 +247,18 @@ def test_views_of_one_buffer_layouts_and_strides():
 
 
 @pytest.mark.gpu
+def test_a_scattered_gradient_listed_twice_is_refused():
+    from pogs_amd.optim import clip_grad_norm_
+
+    p = torch.zeros(6, 4, device="cuda", requires_grad=True)
+    p.grad = torch.ones(6, 8, device="cuda")[:, ::2]
+    with pytest.raises(RuntimeError, match="share memory"):
+        clip_grad_norm_([p, p], 1.0)
+    assert float(p.grad.min()) == 1.0
+    assert clip_grad_norm_([p], 1.0).item() == pytest.approx(math.sqrt(24), rel=2 * U)
+
+
+@pytest.mark.gpu
 def test_autograd_notices_that_gradients_were_scaled():
     from pogs_amd.optim import clip_grad_norm_
 
