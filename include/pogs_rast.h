@@ -488,12 +488,16 @@ int pr_densify_split_children(int64_t n_out, const int32_t *map_src, const int32
  * pr_vocab_ce_fwd: P >= 1.  row_loss[P] (may be NULL where loss is not), lse[P] (may be NULL) and loss[1] (may be NULL,
  * but a backward pass with mean != 0 needs it); loss = sum of row_loss, or (mean != 0) their mean
  * over the rows not ignored (NaN if there are none).  kept: what pr_vocab_ce_bwd reads (packed operands, row statistics);
- * NULL, for at most pr_vocab_ce_score_rows() rows and no backward pass: the vocabulary is read once and not packed.
+ * NULL where no backward pass follows, for at most pr_vocab_ce_score_rows() rows and wherever
+ * pr_vocab_ce_keeps_vocabulary is 0: the vocabulary is read once and not packed.
  * pr_vocab_ce_bwd: dx[P,D] and dw[V,D] (contiguous, 16-byte aligned, the inputs' type, either may be NULL) from the
  * gradient g_loss of row_loss (per_row != 0: [P]) or of loss (one value) and g_lse[P] of lse; a NULL one is 0.  kept is
- * read only: several calls may share it.  Products take float16 operands (float32 input: two planes, 2^-22) and add in
+ * read only: several calls may share it.  Where pr_vocab_ce_keeps_vocabulary is 0 (few rows, a large vocabulary) kept holds
+ * the logits and no copy of w: the backward pass reads the same w again for dx, which must not have changed; elsewhere its w
+ * is not looked at.  Products take float16 operands (float32 input: two planes, 2^-22) and add in
  * float32; sums run in a fixed order, so equal inputs give equal bits. */
 int pr_vocab_ce_score_rows(void);
+int pr_vocab_ce_keeps_vocabulary(int64_t P, int64_t V, int64_t D);
 size_t pr_vocab_ce_kept_bytes(int dtype, int64_t P, int64_t V, int64_t D);
 size_t pr_vocab_ce_fwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D);
 size_t pr_vocab_ce_bwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D, int want_dx, int want_dw);
@@ -501,9 +505,10 @@ int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const void *x, i
                     const void *w, int64_t ldw_row, int64_t ldw_col, const int64_t *labels, int64_t ignore_index,
                     float scale, int mean, void *kept, size_t kept_bytes, void *scratch, size_t scratch_bytes,
                     float *row_loss, float *lse, float *loss, void *stream);
-int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const int64_t *labels, int64_t ignore_index, float scale,
-                    int mean, int per_row, const void *kept, size_t kept_bytes, const float *g_loss, const float *g_lse,
-                    void *scratch, size_t scratch_bytes, void *dx, void *dw, void *stream);
+int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const void *w, int64_t ldw_row, int64_t ldw_col,
+                    const int64_t *labels, int64_t ignore_index, float scale, int mean, int per_row, const void *kept,
+                    size_t kept_bytes, const float *g_loss, const float *g_lse, void *scratch, size_t scratch_bytes, void *dx,
+                    void *dw, void *stream);
 
 #ifdef __cplusplus
 }

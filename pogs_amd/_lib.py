@@ -64,13 +64,14 @@ SIGNATURES = {
     "pr_l2norm_fwd": (c_int, [c_int64, c_int, _P, c_float, _P, _P, _P]),
     "pr_l2norm_bwd": (c_int, [c_int64, c_int, _P, _P, c_float, _P, _P, _P]),
     "pr_vocab_ce_score_rows": (c_int, []),
+    "pr_vocab_ce_keeps_vocabulary": (c_int, [c_int64, c_int64, c_int64]),
     "pr_vocab_ce_kept_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
     "pr_vocab_ce_fwd_scratch_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
     "pr_vocab_ce_bwd_scratch_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int, c_int]),
     "pr_vocab_ce_fwd": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64,
                                 c_float, c_int, _P, c_size_t, _P, c_size_t, _P, _P, _P, _P]),
-    "pr_vocab_ce_bwd": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, c_float, c_int, c_int, _P, c_size_t, _P, _P,
-                                _P, c_size_t, _P, _P, _P]),
+    "pr_vocab_ce_bwd": (c_int, [c_int, c_int64, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_float, c_int, c_int, _P,
+                                c_size_t, _P, _P, _P, c_size_t, _P, _P, _P]),
     "pr_densify_accumulate": (c_int, [c_int, c_int, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P]),
     "pr_densify_plan_scratch_bytes": (c_size_t, [c_int]),
     "pr_densify_plan": (c_int, [c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),

@@ -52,11 +52,11 @@ constexpr int CUS = 256;
 constexpr int TOP_EXP = 13;  // packed magnitudes are below 2^(TOP_EXP + 1)
 constexpr float MAX_FLOOR = -3.0e38f;  // a maximum over nothing: exp2 of anything minus it is 0, not NaN
 constexpr float LN2F = 0.69314718055994531f;
-// Rows that the forward pass without packing takes at most.  It reads the vocabulary once where packing reads it three
-// times and writes it once, but multiplies 32 rows at a time whatever there are (131072 words x 1024 dims, bfloat16: 1 row
-// 51 against 234 us, 64 rows 102 against 237; float32: 137 against 428 and 265 against 433, nearing each other).
-constexpr int SCORE_ROWS = 64;
-constexpr int SCORE_BLOCKS = 1024;  // its workgroups: four per CU
+// Rows that the kernels for few rows take at most: without gradients, and with a large vocabulary.
+constexpr int SCORE_ROWS = 64, FEW_ROWS = 128;
+constexpr int SCORE_BLOCKS = 1024;  // workgroups of the score kernel: four per CU
+constexpr int FEW_BLOCKS = 512;     // of the gradients' kernels, where there is work for so many
+constexpr int64_t FEW_VOCABULARY = 1 << 19;
 constexpr int AMAX_BLOCKS = 1024;  // partial maxima per tensor at most
 
 struct Matrix {  // rows x cols with any strides (elements)
@@ -71,13 +71,15 @@ struct Scalars {  // per call, on the device
 
 // ---- packing --------------------------------------------------------------------------------------------------------
 template <typename T>
-struct Eight;  // eight consecutive elements as one or two 16-byte accesses
+struct Eight;  // eight consecutive elements as one or two 16-byte accesses, at any element's address
 template <>
 struct Eight<float> {
-  float4 a, b;
+  typedef float f4v __attribute__((ext_vector_type(4)));
+  typedef f4v f4_at __attribute__((aligned(4)));
+  f4v a, b;
   __device__ __forceinline__ void load(const float *p) {
-    a = reinterpret_cast<const float4 *>(p)[0];
-    b = reinterpret_cast<const float4 *>(p)[1];
+    a = reinterpret_cast<const f4_at *>(p)[0];
+    b = reinterpret_cast<const f4_at *>(p)[1];
   }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
@@ -85,8 +87,9 @@ struct Eight<float> {
 };
 template <typename T>
 struct Eight {
+  typedef u4v u4_at __attribute__((aligned(2)));
   u4v a;
-  __device__ __forceinline__ void load(const T *p) { a = *reinterpret_cast<const u4v *>(p); }
+  __device__ __forceinline__ void load(const T *p) { a = *reinterpret_cast<const u4_at *>(p); }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     typedef T t8 __attribute__((ext_vector_type(8)));
     const t8 t = __builtin_bit_cast(t8, a);
@@ -95,16 +98,10 @@ struct Eight {
   }
 };
 
-// Whether eight consecutive elements of a row can be read by 16-byte accesses: unit column stride, aligned rows.
 template <typename T>
-__device__ __forceinline__ bool wide_rows(const Matrix &m) {
-  return m.ld_col == 1 && (((uintptr_t)m.data | (uintptr_t)(m.ld_row * (int64_t)sizeof(T))) & 15) == 0;
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const Matrix &m, bool wide, int64_t row, int64_t k, float (&v)[8]) {
+__device__ __forceinline__ void load8(const Matrix &m, int64_t row, int64_t k, float (&v)[8]) {
   const T *src = (const T *)m.data + row * m.ld_row;
-  if (wide && k + 8 <= m.cols) {
+  if (m.ld_col == 1 && k + 8 <= m.cols) {
     Eight<T> e;
     e.load(src + k);
     e.get(v);
@@ -136,14 +133,13 @@ template <typename T>
 __global__ void __launch_bounds__(256) vce_amax_kernel(AmaxJob w, AmaxJob x, float *__restrict__ partial) {
   const bool first = (int)blockIdx.x < w.blocks;
   const AmaxJob &j = first ? w : x;
-  const bool wide = wide_rows<T>(j.m);
   const int block = (int)blockIdx.x - (first ? 0 : w.blocks);
   float top = 0.f;
   auto take = [&](const float (&v)[8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) top = fabsf(v[k]) < INFINITY ? fmaxf(top, fabsf(v[k])) : top;
   };
-  if (!j.labels && wide && j.m.ld_row == j.m.cols && (j.m.cols & 7) == 0) {
+  if (!j.labels && j.m.ld_col == 1 && j.m.ld_row == j.m.cols && (j.m.cols & 7) == 0) {
     const T *src = (const T *)j.m.data;
     const int64_t units = j.m.rows * (j.m.cols / 8), step = (int64_t)j.blocks * 256;
     int64_t u = (int64_t)block * 256 + threadIdx.x;
@@ -174,7 +170,7 @@ __global__ void __launch_bounds__(256) vce_amax_kernel(AmaxJob w, AmaxJob x, flo
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[q][i] = 0.f;
           const int64_t row = r0 + q;
-          if (row < j.m.rows && !(j.labels && j.labels[row] == j.ignore)) load8<T>(j.m, wide, row, k, v[q]);
+          if (row < j.m.rows && !(j.labels && j.labels[row] == j.ignore)) load8<T>(j.m, row, k, v[q]);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) take(v[q]);
@@ -211,7 +207,6 @@ __global__ void __launch_bounds__(256) vce_pack_kernel(PackJob w, PackJob x, con
                                                        Scalars *__restrict__ s) {
   const int ew = top_exponent(partial, w.partials), ex = top_exponent(partial + w.partials, x.partials);
   if (blockIdx.x == 0 && threadIdx.x == 0) s->exp_w = ew, s->exp_x = ex;
-  const bool wide_w = wide_rows<T>(w.m), wide_x = wide_rows<T>(x.m);
   const int lane = threadIdx.x & 63, piece = lane & 7;
   for (int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); u < w.units + x.units; u += (int64_t)gridDim.x * 4) {
     const bool first = u < w.units;
@@ -228,7 +223,7 @@ __global__ void __launch_bounds__(256) vce_pack_kernel(PackJob w, PackJob x, con
       const bool live = row < j.m.rows && k < j.m.cols && !(j.labels && j.labels[row] == j.ignore);
 #pragma unroll
       for (int i = 0; i < 8; ++i) val[q][i] = 0.f;
-      if (live) load8<T>(j.m, first ? wide_w : wide_x, row, k, val[q]);
+      if (live) load8<T>(j.m, row, k, val[q]);
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -707,18 +702,24 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
-// Forward alone for at most 32 NB rows: the vocabulary is read once, as it is, and nothing is packed.  16-bit operands go
-// to the matrix cores in their own type; a float32 value is cut into three bfloat16 pieces that hold all its 24 bits (by
-// truncation, so the largest values do not overflow), six products of which leave out less than 2^-21 of a product.
-// A workgroup takes 32 words at a time; its four wavefronts take the 64-wide pieces of the contraction in turn, add
-// their tiles through LDS, and each keeps the running maximum and sum over a quarter of the words.
+// At most 32 NB rows: the vocabulary is read as it is, and nothing of its size is packed.  16-bit operands go to the matrix
+// cores in their own type; a float32 value is cut into three bfloat16 pieces that hold all its 24 bits (by truncation, so
+// the largest values do not overflow), six products of which leave out less than 2^-21 of a product.
+// SCORE  A workgroup takes 32 words at a time; its four wavefronts take the 64-wide pieces of the contraction in turn, add
+//        their tiles through LDS, and each keeps the running maximum and sum over a quarter of the words.  For a backward
+//        pass the logits stay, 4 bytes for each word and row: P / D of a float32 vocabulary.
+// DW     32 words a wavefront: G of all rows is made from the logits in registers and multiplies the features, a 64-wide
+//        piece at a time.  Writes dW once.
+// DX     32 words a step, 64 features a wavefront and 256 a workgroup, whose wavefronts make G of the step in LDS together;
+//        reads the vocabulary once.  Partials per run of words, added by FINISH.
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 
 template <typename T>
 struct Operand;  // the pieces of eight consecutive values, ready for the matrix cores
 template <>
 struct Operand<float> {
-  u4v piece[3];
+  static constexpr int N = 3;
+  u4v piece[N];
   __device__ __forceinline__ void set(const float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -746,7 +747,14 @@ struct Operand<float> {
 };
 template <>
 struct Operand<_Float16> {
-  u4v piece[1];
+  static constexpr int N = 1;
+  u4v piece[N];
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    h8v z;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = (_Float16)v[i];
+    piece[0] = __builtin_bit_cast(u4v, z);
+  }
   static __device__ __forceinline__ f16v product(const Operand &a, const Operand &b, f16v acc) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a.piece[0]), __builtin_bit_cast(h8v, b.piece[0]),
                                                   acc, 0, 0, 0);
@@ -754,15 +762,25 @@ struct Operand<_Float16> {
 };
 template <>
 struct Operand<__bf16> {
-  u4v piece[1];
+  static constexpr int N = 1;
+  u4v piece[N];
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    b8v z;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = (__bf16)v[i];
+    piece[0] = __builtin_bit_cast(u4v, z);
+  }
   static __device__ __forceinline__ f16v product(const Operand &a, const Operand &b, f16v acc) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a.piece[0]), __builtin_bit_cast(b8v, b.piece[0]),
                                                    acc, 0, 0, 0);
   }
 };
 
-// Elements k..k+7 of a row as they are (16 or 32 bytes).  WIDE: 16-byte accesses (wide_rows, and the row's length is a
-// multiple of eight).  Past the end of the row its last elements are read again: the other factor is zero there.
+
+// Elements k..k+7 of a row as they are.  WIDE (unit column stride, eight columns at least): by 16-byte accesses.  Where
+// they cross the end of the row the last eight columns are read in their place: few_column says which column a place holds,
+// and the other factor is zero where that is one of an earlier place or none.
+__device__ __forceinline__ int64_t few_column(int64_t k, int64_t cols) { return cols < 8 ? k : min(k, cols - 8); }
 template <typename T, bool WIDE>
 __device__ __forceinline__ Eight<T> fetch8(const Matrix &m, int64_t row, int64_t k) {
   const T *src = (const T *)m.data + row * m.ld_row;
@@ -773,17 +791,10 @@ __device__ __forceinline__ Eight<T> fetch8(const Matrix &m, int64_t row, int64_t
   }
   typedef T t8 __attribute__((ext_vector_type(8)));
   t8 z;
+  const int64_t c = few_column(k, m.cols);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] = src[min(k + i, m.cols - 1) * m.ld_col];
+  for (int i = 0; i < 8; ++i) z[i] = src[min(c + i, m.cols - 1) * m.ld_col];
   return __builtin_bit_cast(Eight<T>, z);
-}
-template <typename T>
-__device__ __forceinline__ void zero_past(Eight<T> &e, int64_t left) {  // keeps the first `left` elements
-  typedef T t8 __attribute__((ext_vector_type(8)));
-  t8 z = __builtin_bit_cast(t8, e);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] = i < left ? z[i] : (T)0.f;
-  e = __builtin_bit_cast(Eight<T>, z);
 }
 __device__ __forceinline__ Operand<float> operand(const Eight<float> &e) {
   float v[8];
@@ -796,6 +807,58 @@ template <typename T>
 __device__ __forceinline__ Operand<T> operand(const Eight<T> &e) {
   return Operand<T>{{e.a}};
 }
+template <typename O>
+__device__ __forceinline__ O packed_operand(const u4v *src) {  // pieces 1 KB apart
+  O o;
+#pragma unroll
+  for (int k = 0; k < O::N; ++k) o.piece[k] = src[k * 64];
+  return o;
+}
+template <typename O>
+__device__ __forceinline__ void store_operand(const O &o, u4v *dst) {
+#pragma unroll
+  for (int k = 0; k < O::N; ++k) dst[k * 64] = o.piece[k];
+}
+
+// Column of a 32-wide tile's lane, in the products whose columns are features: float32 tiles are 32 consecutive ones; two
+// 16-bit tiles share 64, the even ones and the odd ones, so that a lane reads and writes both at once.
+template <typename T>
+__device__ __forceinline__ int64_t tile_column(int64_t tile, int lane) {
+  return sizeof(T) == 4 ? tile * 32 + (lane & 31) : (tile >> 1) * 64 + 2 * (lane & 31) + (tile & 1);
+}
+
+struct FewPack {
+  Matrix x;
+  const int64_t *labels;  // rows with the ignored label are zeros
+  int64_t ignore;
+  int kblocks, row_blocks;  // 16 wide, of features and of rows
+  u4v *xf, *xt;             // [32 rows][k block], [32 features][row block], pieces of 1 KB; either may be NULL
+};
+
+// A block of a packed copy of the features per wavefront.
+template <typename T>
+__global__ void __launch_bounds__(256) vce_few_pack_kernel(const FewPack j) {
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), nf = j.xf ? (int64_t)j.row_blocks / 2 * j.kblocks : 0;
+  auto at = [&](int64_t row, int64_t col) {
+    return row < j.x.rows && j.labels[row] != j.ignore ? (float)((const T *)j.x.data)[row * j.x.ld_row + col * j.x.ld_col] : 0.f;
+  };
+  float v[8];
+  Operand<T> o;
+  if (u < nf) {
+    const int64_t n = u / j.kblocks, k = (u - n * j.kblocks) * 16 + 8 * h, c = few_column(k, j.x.cols);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i >= k && c + i < j.x.cols ? at(32 * n + (lane & 31), c + i) : 0.f;
+    o.set(v);
+    store_operand(o, j.xf + u * (Operand<T>::N * 64) + lane);
+  } else if (j.xt && u - nf < (int64_t)j.kblocks / 2 * j.row_blocks) {
+    const int64_t tile = (u - nf) / j.row_blocks, b = u - nf - tile * j.row_blocks, d = tile_column<T>(tile, lane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = d < j.x.cols ? at(16 * b + 8 * h + i, d) : 0.f;
+    o.set(v);
+    store_operand(o, j.xt + (u - nf) * (Operand<T>::N * 64) + lane);
+  }
+}
 
 __device__ __forceinline__ void merge(float &m, float &s, float m2, float s2) {
   const float top = fmaxf(m, m2);
@@ -803,24 +866,28 @@ __device__ __forceinline__ void merge(float &m, float &s, float m2, float s2) {
   m = top;
 }
 
-template <typename T, int NB, bool WIDE>
-__global__ void __launch_bounds__(256, 2) vce_score_kernel(Matrix w, Matrix x, const int64_t *__restrict__ labels,
-                                                        int64_t ignore, float scale, float2 *__restrict__ partial,
-                                                        float *__restrict__ target) {
-  __shared__ float sum[4][NB][16][64];
+// XP: the features are packed (xf); otherwise they are read as they are, eight aligned columns at a time (D % 8 == 0), which
+// saves a launch where it counts, with the fewest rows.
+template <typename T, int NB, bool WIDE, bool XP>
+__global__ void __launch_bounds__(256, 2) vce_score_kernel(Matrix w, Matrix x, const u4v *__restrict__ xf,
+                                                           const int64_t *__restrict__ labels, int64_t ignore, float scale,
+                                                           float2 *__restrict__ partial, float *__restrict__ target,
+                                                           float *__restrict__ logits) {
+  constexpr int NJ = NB < 2 ? NB : 2;   // 32-row tiles that are added at once
+  __shared__ float sum[4][NJ][16][64];
   __shared__ float2 join[4][NB][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const float c = scale * LOG2E;
-  int64_t label[NB], xrow[NB], xlen[NB];   // a row that does not count has length 0
+  int64_t label[NB];
   float top[NB], tot[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const int64_t p = 32 * n + (lane & 31);
-    label[n] = p < x.rows ? labels[p] : ignore;
-    xrow[n] = min(p, x.rows - 1);
-    xlen[n] = label[n] != ignore ? x.cols : 0;
+    label[n] = p < x.rows ? labels[p] : -1;
     top[n] = MAX_FLOOR, tot[n] = 0.f;
   }
+  const int64_t row = min((int64_t)(lane & 31), x.rows - 1);             // !XP
+  const bool counts = label[0] != ignore && (lane & 31) < x.rows;
   const int64_t tiles = (w.rows + 31) / 32;
   const int groups = (int)((w.cols + 63) / 64);
   auto words = [&](int64_t t, int g, Eight<T> (&a)[4]) {
@@ -845,36 +912,48 @@ __global__ void __launch_bounds__(256, 2) vce_score_kernel(Matrix w, Matrix x, c
         const Operand<T> oa = operand(a[q]);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const int64_t k = (int64_t)g * 64 + 16 * q + 8 * h;
-          Eight<T> b = fetch8<T, WIDE>(x, xrow[n], k);
-          zero_past(b, WIDE ? (k < xlen[n] ? 8 : 0) : xlen[n] - k);
-          acc[n] = Operand<T>::product(oa, operand(b), acc[n]);
+          Operand<T> ob;
+          if (XP) {
+            ob = packed_operand<Operand<T>>(xf + (((int64_t)n * groups + g) * 4 + q) * (Operand<T>::N * 64) + lane);
+          } else {
+            const int64_t k = (int64_t)g * 64 + 16 * q + 8 * h;
+            ob = operand(fetch8<T, true>(x, row, k));
+            const unsigned keep = counts && k < x.cols ? ~0u : 0u;
+#pragma unroll
+            for (int pc = 0; pc < Operand<T>::N; ++pc) ob.piece[pc] &= keep;
+          }
+          acc[n] = Operand<T>::product(oa, ob, acc[n]);
         }
         a[q] = next[q];
       }
     }
-    __syncthreads();  // the tile before has been read
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sum[wave][n][r][lane] = acc[n][r];
-    __syncthreads();
     // this wavefront's registers 4 wave..4 wave + 3: words 8 wave + 4 h + 0..3 of the tile
     const int64_t v0 = t * 32 + 8 * wave + 4 * h;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      float z[4], most = MAX_FLOOR;
+    for (int n0 = 0; n0 < NB; n0 += NJ) {
+      __syncthreads();  // what was added before has been read
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = 4 * wave + k;
-        z[k] = ((sum[0][n][r][lane] + sum[1][n][r][lane]) + (sum[2][n][r][lane] + sum[3][n][r][lane])) * c;
-        if (label[n] == v0 + k) target[32 * n + (lane & 31)] = z[k];
-        if (v0 + k < w.rows) most = fmaxf(most, z[k]);
+      for (int n = 0; n < NJ; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[wave][n][r][lane] = acc[n0 + n][r];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int n = n0 + j;
+        float z[4], most = MAX_FLOOR;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 4 * wave + k;
+          z[k] = ((sum[0][j][r][lane] + sum[1][j][r][lane]) + (sum[2][j][r][lane] + sum[3][j][r][lane])) * c;
+          if (label[n] == v0 + k) target[32 * n + (lane & 31)] = z[k];
+          if (v0 + k < w.rows) most = fmaxf(most, z[k]);
+        }
+        if (logits) store4<float>(logits + (t * 32 * NB + 32 * n + (lane & 31)) * 32 + 8 * wave + 4 * h, z[0], z[1], z[2], z[3]);
+        float add = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) add += v0 + k < w.rows ? __builtin_amdgcn_exp2f(z[k] - most) : 0.f;
+        merge(top[n], tot[n], most, add);
       }
-      float add = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) add += v0 + k < w.rows ? __builtin_amdgcn_exp2f(z[k] - most) : 0.f;
-      merge(top[n], tot[n], most, add);
     }
   }
 #pragma unroll
@@ -892,6 +971,268 @@ __global__ void __launch_bounds__(256, 2) vce_score_kernel(Matrix w, Matrix x, c
     }
     if (i < x.rows) partial[(int64_t)i * gridDim.x + blockIdx.x] = q;
   }
+}
+
+// G as an operand that meets one of type T.  bfloat16 takes two pieces of it (2^-14 of an entry), float16 its own type, with
+// the row factors scaled by exp_g; the others have float32's range and need no scaling.
+template <typename T>
+struct GradOperand : Operand<T> {
+  static __device__ __forceinline__ f16v times(const GradOperand &a, const Operand<T> &b, f16v acc) {
+    return Operand<T>::product(a, b, acc);
+  }
+};
+template <>
+struct GradOperand<__bf16> {
+  static constexpr int N = 2;
+  u4v piece[N];
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    Operand<float> o;
+    o.set(v);
+    piece[0] = o.piece[0], piece[1] = o.piece[1];
+  }
+  static __device__ __forceinline__ f16v times(const GradOperand &a, const Operand<__bf16> &b, f16v acc) {
+#pragma unroll
+    for (int k = 1; k >= 0; --k)
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a.piece[k]), __builtin_bit_cast(b8v, b.piece[0]),
+                                                    acc, 0, 0, 0);
+    return acc;
+  }
+};
+template <typename T>
+constexpr bool FEW_SCALED = false;
+template <>
+constexpr bool FEW_SCALED<_Float16> = true;
+
+struct FewGrad {  // what G is made of
+  int64_t P, V, D, Dk;
+  const int64_t *labels;
+  const float *lse2, *coef_a, *coef_b, *logits;
+  const int *exp_g;
+  // row p as {lse2, a, b, label's bits}
+  template <typename T>
+  __device__ __forceinline__ void rows(float4 *to, int n) const {
+    const int e = FEW_SCALED<T> ? 0 : -*exp_g;
+    for (int p = threadIdx.x; p < n; p += blockDim.x) {
+      const int64_t label = p < P ? labels[p] : -1;
+      to[p] = make_float4(p < P ? lse2[p] : 0.f, ldexpf(coef_a[p], e), ldexpf(coef_b[p], e),
+                          __builtin_bit_cast(float, label >= 0 && label < V ? (int)label : -1));
+    }
+  }
+  static __device__ __forceinline__ float entry(float z, const float4 &row, int word) {
+    const float g = row.y * __builtin_amdgcn_exp2f(z - row.x);
+    return __builtin_bit_cast(int, row.w) == word ? g - row.z : g;
+  }
+};
+
+template <typename T, int NB>
+__global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, const u4v *__restrict__ xt, float scale,
+                                                            T *__restrict__ out) {
+  constexpr int KB = 2 * NB;
+  __shared__ float4 rows[32 * NB];
+  f.rows<T>(rows, 32 * NB);
+  __syncthreads();
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t * 32 >= f.V) return;
+  GradOperand<T> ga[KB];
+  const float *z = f.logits + t * (1024 * NB) + (lane & 31);
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int p = 16 * b + 8 * h + i;
+      v[i] = FewGrad::entry(z[p * 32], rows[p], (int)(t * 32) + (lane & 31));
+    }
+    ga[b].set(v);
+  }
+  const int e = FEW_SCALED<T> ? -*f.exp_g : 0;
+  for (int64_t c = blockIdx.y; c * 64 < f.D; c += gridDim.y) {
+    f16v acc[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+        acc[j] = GradOperand<T>::times(
+            ga[b], packed_operand<Operand<T>>(xt + ((2 * c + j) * KB + b) * (Operand<T>::N * 64) + lane), acc[j]);
+    }
+    const int64_t d0 = tile_column<T>(2 * c, lane), d1 = tile_column<T>(2 * c + 1, lane);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int64_t v = t * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
+      if (v >= f.V) continue;
+      const T g0 = (T)ldexpf(acc[0][r] * scale, e), g1 = (T)ldexpf(acc[1][r] * scale, e);
+      T *dst = out + v * f.D;
+      if (sizeof(T) == 2 && (f.D & 1) == 0) {
+        typedef T t2 __attribute__((ext_vector_type(2)));
+        if (d0 < f.D) *reinterpret_cast<t2 *>(dst + d0) = t2{g0, g1};
+      } else {
+        if (d0 < f.D) dst[d0] = g0;
+        if (d1 < f.D) dst[d1] = g1;
+      }
+    }
+  }
+}
+
+// WIDE (unit column stride, two columns at least): a lane's two 16-bit columns by one access.
+template <typename T, int NB, bool WIDE>
+__global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Matrix w, int64_t steps, float *__restrict__ acc_out) {
+  typedef GradOperand<T> G;
+  constexpr int R = 32 * NB, TASKS = (2 * NB + 3) / 4;     // (16 words, 32 rows) tiles of G for each wavefront
+  constexpr bool PAIRS = sizeof(T) == 2;
+  __shared__ float4 rows[R];
+  __shared__ u4v g[2][2 * NB][G::N][64];
+  f.rows<T>(rows, R);
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int64_t lo = blockIdx.y * steps, hi = min(lo + steps, (f.V + 31) / 32);
+  const int64_t c0 = (int64_t)blockIdx.x * 256 + 64 * wave;
+  const bool active = c0 < f.D;
+  // this lane's two columns; the last ones again past the end
+  const int64_t d0 = tile_column<T>(c0 / 32, lane), d1 = tile_column<T>(c0 / 32 + 1, lane);
+  const int64_t at0 = WIDE && PAIRS ? min(d0, f.D - 2) : min(d0, f.D - 1), at1 = min(d1, f.D - 1);
+  const unsigned shift = d0 == f.D - 1 ? 16 : 0;           // WIDE pairs: the last column of an odd number
+  typedef unsigned u1_at __attribute__((aligned(2)));
+  struct Raw {
+    unsigned a[8], b[PAIRS && WIDE ? 1 : 8];
+  };
+  auto load = [&](int64_t step, int kb, Raw &raw) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T *src = (const T *)w.data + min(step * 32 + 16 * kb + 8 * h + i, f.V - 1) * w.ld_row;
+      if constexpr (!PAIRS) {
+        raw.a[i] = __builtin_bit_cast(unsigned, src[at0 * w.ld_col]), raw.b[i] = __builtin_bit_cast(unsigned, src[at1 * w.ld_col]);
+      } else if constexpr (WIDE) {
+        raw.a[i] = *reinterpret_cast<const u1_at *>(src + at0) >> shift;
+      } else {
+        raw.a[i] = __builtin_bit_cast(unsigned short, src[at0 * w.ld_col]), raw.b[i] = __builtin_bit_cast(unsigned short, src[at1 * w.ld_col]);
+      }
+    }
+  };
+  auto operands = [&](const Raw &raw, Operand<T> (&o)[2]) {
+    if constexpr (!PAIRS) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, raw.a[i]);
+      o[0].set(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, raw.b[i]);
+      o[1].set(v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[0].piece[0][i] = __builtin_amdgcn_perm(raw.a[2 * i + 1], raw.a[2 * i], 0x05040100);
+        o[1].piece[0][i] = WIDE ? __builtin_amdgcn_perm(raw.a[2 * i + 1], raw.a[2 * i], 0x07060302)
+                                : __builtin_amdgcn_perm(raw.b[PAIRS && WIDE ? 0 : 2 * i + 1], raw.b[PAIRS && WIDE ? 0 : 2 * i], 0x05040100);
+      }
+    }
+  };
+  struct Logits {
+    float4 a[TASKS], b[TASKS];
+  };
+  auto logits = [&](int64_t step, Logits &z) {
+#pragma unroll
+    for (int k = 0; k < TASKS; ++k) {
+      const int task = wave + 4 * k;
+      if (task < 2 * NB) {
+        const float *src = f.logits + (step * R + 32 * (task >> 1) + (lane & 31)) * 32 + 16 * (task & 1) + 8 * h;
+        z.a[k] = reinterpret_cast<const float4 *>(src)[0], z.b[k] = reinterpret_cast<const float4 *>(src)[1];
+      }
+    }
+  };
+  auto make = [&](int64_t step, const Logits &z, int buf) {
+#pragma unroll
+    for (int k = 0; k < TASKS; ++k) {
+      const int task = wave + 4 * k;
+      if (task < 2 * NB) {
+        const float4 row = rows[32 * (task >> 1) + (lane & 31)];
+        const float v[8] = {z.a[k].x, z.a[k].y, z.a[k].z, z.a[k].w, z.b[k].x, z.b[k].y, z.b[k].z, z.b[k].w};
+        const int word = (int)step * 32 + 16 * (task & 1) + 8 * h;
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = word + i < f.V ? FewGrad::entry(v[i], row, word + i) : 0.f;
+        G o;
+        o.set(e);
+        store_operand(o, &g[buf][task][0][lane]);
+      }
+    }
+  };
+  f16v acc[NB][2];
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[n][j][r] = 0.f;
+  Logits z;
+  Raw raw[2];
+  logits(lo, z);
+  if (active) load(lo, 0, raw[0]);
+  make(lo, z, 0);
+  __syncthreads();
+  int buf = 0;
+  for (int64_t s = lo; s < hi; ++s) {
+    const bool more = s + 1 < hi;
+    if (more) logits(s + 1, z);
+    if (active) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        if (kb == 0) load(s, 1, raw[1]);
+        else if (more) load(s + 1, 0, raw[0]);
+        Operand<T> o[2];
+        operands(raw[kb], o);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const G ga = packed_operand<G>(&g[buf][2 * n + kb][0][lane]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[n][j] = G::times(ga, o[j], acc[n][j]);
+        }
+      }
+    }
+    if (more) make(s + 1, z, buf ^ 1);
+    __syncthreads();
+    buf ^= 1;
+  }
+  if (!active) return;
+  float *dst = acc_out + (int64_t)blockIdx.y * R * f.Dk;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float *to = dst + (int64_t)(32 * n + (r & 3) + 8 * (r >> 2) + 4 * h) * f.Dk;
+      if (PAIRS) *reinterpret_cast<float2 *>(to + d0) = make_float2(acc[n][0][r], acc[n][1][r]);
+      else to[d0] = acc[n][0][r], to[d1] = acc[n][1][r];
+    }
+}
+
+// dX = scale times the sum of the runs' partials, added in a fixed order: a row's 256 features per workgroup.
+template <typename T>
+__global__ void __launch_bounds__(1024) vce_few_finish_kernel(const FewGrad f, int64_t plane, int splits, float scale,
+                                                              const float *__restrict__ acc, T *__restrict__ dx) {
+  __shared__ float4 part[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t p = blockIdx.y, d = (int64_t)blockIdx.x * 256 + 4 * lane;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (d < f.Dk)
+#pragma unroll 8
+    for (int k = wave; k < splits; k += 16) {
+      const float4 q = *reinterpret_cast<const float4 *>(acc + k * plane + p * f.Dk + d);
+      v.x += q.x, v.y += q.y, v.z += q.z, v.w += q.w;
+    }
+  part[wave][lane] = v;
+  __syncthreads();
+  if (wave != 0) return;
+  for (int k = 1; k < 16; ++k) {
+    const float4 q = part[k][lane];
+    v.x += q.x, v.y += q.y, v.z += q.z, v.w += q.w;
+  }
+  const int e = FEW_SCALED<T> ? -*f.exp_g : 0;
+  const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (d + k < f.D) dx[p * f.D + d + k] = (T)ldexpf(x[k] * scale, e);
 }
 
 // ---- rows -----------------------------------------------------------------------------------------------------------
@@ -1037,6 +1378,9 @@ bool valid_shape(int dtype, int64_t P, int64_t V, int64_t D) {
   return dtype >= PR_F32 && dtype <= PR_BF16 && P >= 0 && V >= 1 && D >= 1 && P < (1ll << 30) && V < (1ll << 30) &&
          D < (1ll << 20) && P * D < (1ll << 38) && V * D < (1ll << 38);
 }
+
+// Whether a call goes to the kernels for few rows, with a backward pass to come or without.
+bool few(int64_t P, int64_t V, int64_t D) { return P <= FEW_ROWS && V * D >= FEW_VOCABULARY; }
 
 struct Carve {  // consecutive 256-byte-aligned pieces of a buffer
   char *at;
@@ -1244,38 +1588,132 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
   return check_launch("pr_vocab_ce");
 }
 
-struct ScoreScratch {  // of the forward pass for few rows
-  float *target, *row_loss;
-  float2 *partial;
-  int blocks;
-  ScoreScratch(Carve &c, const Shape &s) {
-    blocks = (int)std::min<int64_t>(SCORE_BLOCKS, (s.V + 31) / 32);
-    target = c.take<float>(SCORE_ROWS);
-    row_loss = c.take<float>(SCORE_ROWS);
-    partial = c.take<float2>((int64_t)blocks * SCORE_ROWS);
+// 32-row tiles of the kernels for few rows, and the padded rows and features that go with them.
+struct FewShape {
+  int64_t P, V, D, R, Dk, tiles;
+  int nb, pieces;
+  FewShape(int dtype, int64_t P_, int64_t V_, int64_t D_)
+      : P(P_), V(V_), D(D_), Dk(round_up(D_, 64)), tiles((V_ + 31) / 32), nb(P_ <= 32 ? 1 : P_ <= 64 ? 2 : 4),
+        pieces(dtype == PR_F32 ? 3 : 1) {
+    R = 32 * nb;
+  }
+  int64_t packed() const { return R * Dk / 8 * pieces; }   // 16-byte units of a copy of the features
+};
+
+struct FewKept {
+  Scalars *scal;
+  float *lse2, *logits;   // logits in the log2 domain: [32 words][R][32]
+  u4v *xt;
+  FewKept(Carve &c, const FewShape &s) {
+    scal = c.take<Scalars>(1);
+    lse2 = c.take<float>(s.R);
+    xt = c.take<u4v>(s.packed());
+    logits = c.take<float>(s.tiles * s.R * 32);
   }
 };
 
-template <typename T>
-int score(const Call &c, int mean, ScoreScratch &f, float *row_loss, float *lse, float *loss, hipStream_t st) {
-  const dim3 grid(f.blocks), block(256);
-  auto aligned = [](const Matrix &m) {
-    return m.ld_col == 1 && ((uintptr_t)m.data & 15) == 0 && (m.ld_row * (int64_t)sizeof(T)) % 16 == 0 && m.cols % 8 == 0;
-  };
-  const bool wide = aligned(c.w) && aligned(c.x);
+struct ScoreScratch {  // of the forward pass for few rows
+  float *target, *row_loss;
+  float2 *partial;
+  u4v *xf;
+  int blocks;
+  ScoreScratch(Carve &c, const FewShape &s) {
+    blocks = (int)std::min<int64_t>(SCORE_BLOCKS, s.tiles);
+    target = c.take<float>(s.R);
+    row_loss = c.take<float>(s.R);
+    partial = c.take<float2>(blocks * s.R);
+    xf = c.take<u4v>(s.packed());
+  }
+};
+
+template <typename T, int NB>
+int launch_score(const Call &c, const FewShape &s, ScoreScratch &f, FewKept *k, hipStream_t st) {
+  const bool wide = c.D >= 8 && c.w.ld_col == 1, packed = NB > 1 || !wide || c.x.ld_col != 1 || c.D % 8;
+  if (packed || k) {
+    const FewPack job{c.x, c.labels, c.ignore, (int)(s.Dk / 16), 2 * NB, packed ? f.xf : nullptr, k ? k->xt : nullptr};
+    const int64_t units = s.Dk / 16 * NB * ((packed ? 1 : 0) + (k ? 1 : 0));
+    hipLaunchKernelGGL((vce_few_pack_kernel<T>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, job);
+    PR_TRY(check_launch("pr_vocab_ce"));
+  }
   auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, block, 0, st, c.w, c.x, c.labels, c.ignore, c.scale, f.partial, f.target);
+    hipLaunchKernelGGL(kernel, dim3(f.blocks), dim3(256), 0, st, c.w, c.x, f.xf, c.labels, c.ignore, c.scale, f.partial,
+                       f.target, k ? k->logits : nullptr);
+    return check_launch("pr_vocab_ce");
   };
-  if (c.P <= 32) wide ? launch(vce_score_kernel<T, 1, true>) : launch(vce_score_kernel<T, 1, false>);
-  else wide ? launch(vce_score_kernel<T, 2, true>) : launch(vce_score_kernel<T, 2, false>);
-  PR_TRY(check_launch("pr_vocab_ce"));
-  const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, nullptr, lse, row_loss};
-  hipLaunchKernelGGL(vce_join_row_kernel, dim3((unsigned)c.P), block, 0, st, rows, f.blocks, f.partial);
+  if constexpr (NB == 1)
+    if (!packed) return launch(vce_score_kernel<T, NB, true, false>);
+  return wide ? launch(vce_score_kernel<T, NB, true, true>) : launch(vce_score_kernel<T, NB, false, true>);
+}
+
+// k: for a backward pass, or NULL.
+template <typename T>
+int score(const Call &c, int mean, ScoreScratch &f, FewKept *k, float *row_loss, float *lse, float *loss, hipStream_t st) {
+  const FewShape s(c.dtype, c.P, c.V, c.D);
+  if (s.nb == 1) PR_TRY((launch_score<T, 1>(c, s, f, k, st)));
+  else if (s.nb == 2) PR_TRY((launch_score<T, 2>(c, s, f, k, st)));
+  else PR_TRY((launch_score<T, 4>(c, s, f, k, st)));
+  const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k ? k->lse2 : nullptr, lse, row_loss};
+  hipLaunchKernelGGL(vce_join_row_kernel, dim3((unsigned)c.P), dim3(256), 0, st, rows, f.blocks, f.partial);
   PR_TRY(check_launch("pr_vocab_ce"));
   if (!loss) return PR_OK;
   hipLaunchKernelGGL(vce_reduce_kernel, dim3(1), dim3(1024), 0, st, c.P, row_loss, c.labels, c.ignore, mean, loss,
-                     (Scalars *)nullptr);
+                     k ? k->scal : nullptr);
   return check_launch("pr_vocab_ce");
+}
+
+struct FewBwdScratch {
+  int *exp_g;
+  float *coef_a, *coef_b, *acc;
+  int64_t steps;   // of 32 words, in a run of DX
+  int splits;
+  FewBwdScratch(Carve &c, const FewShape &s, bool dx) {
+    const int64_t chunks = (s.Dk + 255) / 256, want = std::max<int64_t>(1, std::min<int64_t>(FEW_BLOCKS / chunks, s.tiles));
+    steps = (s.tiles + want - 1) / want;
+    splits = (int)((s.tiles + steps - 1) / steps);
+    exp_g = c.take<int>(1);
+    coef_a = c.take<float>(s.R);
+    coef_b = c.take<float>(s.R);
+    acc = c.take<float>(dx ? splits * s.R * s.Dk : 0);
+  }
+};
+
+template <typename T, int NB>
+int few_gradients(const Call &c, const FewShape &s, const FewKept &k, const FewBwdScratch &b, const FewGrad &f, T *dx, T *dw,
+                  hipStream_t st) {
+  if (dx) {
+    const dim3 grid((unsigned)((s.Dk + 255) / 256), b.splits);
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, f, c.w, b.steps, b.acc);
+      return check_launch("pr_vocab_ce");
+    };
+    if constexpr (sizeof(T) == 2)
+      PR_TRY(c.w.ld_col == 1 && c.D >= 2 ? launch(vce_few_dx_kernel<T, NB, true>) : launch(vce_few_dx_kernel<T, NB, false>));
+    else
+      PR_TRY(launch(vce_few_dx_kernel<T, NB, false>));
+    hipLaunchKernelGGL((vce_few_finish_kernel<T>), dim3(grid.x, (unsigned)c.P), dim3(1024), 0, st, f, s.R * s.Dk, b.splits,
+                       c.scale, b.acc, dx);
+    PR_TRY(check_launch("pr_vocab_ce"));
+  }
+  if (dw) {
+    const unsigned blocks = (unsigned)((s.tiles + 3) / 4);
+    const unsigned parts = (unsigned)std::max<int64_t>(1, std::min<int64_t>(FEW_BLOCKS / blocks, s.Dk / 64));
+    hipLaunchKernelGGL((vce_few_dw_kernel<T, NB>), dim3(blocks, parts), dim3(256), 0, st, f, k.xt, c.scale, dw);
+    PR_TRY(check_launch("pr_vocab_ce"));
+  }
+  return PR_OK;
+}
+
+template <typename T>
+int few_backward(const Call &c, int per_row, int mean, const FewKept &k, const FewBwdScratch &b, const float *g_loss,
+                 const float *g_lse, T *dx, T *dw, hipStream_t st) {
+  const FewShape s(c.dtype, c.P, c.V, c.D);
+  const CoefJob coef{c.P, s.R, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, b.exp_g, b.coef_a, b.coef_b};
+  hipLaunchKernelGGL(vce_prepare_kernel, dim3(1), dim3(1024), 0, st, coef, TransposeJob{}, TransposeJob{}, 0);
+  PR_TRY(check_launch("pr_vocab_ce"));
+  const FewGrad f{c.P, c.V, c.D, s.Dk, c.labels, k.lse2, b.coef_a, b.coef_b, k.logits, b.exp_g};
+  if (s.nb == 1) return few_gradients<T, 1>(c, s, k, b, f, dx, dw, st);
+  if (s.nb == 2) return few_gradients<T, 2>(c, s, k, b, f, dx, dw, st);
+  return few_gradients<T, 4>(c, s, k, b, f, dx, dw, st);
 }
 
 template <typename T, int NP>
@@ -1334,20 +1772,21 @@ int check_call(const Call &c) {
   return !c.labels || ((uintptr_t)c.labels & 7) ? PR_EINVAL : PR_OK;
 }
 
-int check_inputs(const Call &c) {
-  const uintptr_t mask = c.dtype == PR_F32 ? 3 : 1;
-  for (const Matrix *m : {&c.x, &c.w})
-    if (!m->data || ((uintptr_t)m->data & mask) || m->ld_row < 0 || m->ld_col < 0) return PR_EINVAL;
-  return PR_OK;
+int check_matrix(int dtype, const Matrix &m) {
+  const uintptr_t mask = dtype == PR_F32 ? 3 : 1;
+  return !m.data || ((uintptr_t)m.data & mask) || m.ld_row < 0 || m.ld_col < 0 ? PR_EINVAL : PR_OK;
 }
 
 }  // namespace
 }  // namespace pr
 
+extern "C" int pr_vocab_ce_keeps_vocabulary(int64_t P, int64_t V, int64_t D) { return !pr::few(P, V, D); }
+
 extern "C" size_t pr_vocab_ce_kept_bytes(int dtype, int64_t P, int64_t V, int64_t D) {
   if (!pr::valid_shape(dtype, P, V, D)) return 0;
   pr::Carve c(nullptr);
-  pr::Kept k(c, pr::Shape(dtype, P, V, D));
+  if (pr::few(P, V, D)) pr::FewKept k(c, pr::FewShape(dtype, P, V, D));
+  else pr::Kept k(c, pr::Shape(dtype, P, V, D));
   return c.used;
 }
 
@@ -1355,17 +1794,17 @@ extern "C" int pr_vocab_ce_score_rows(void) { return pr::SCORE_ROWS; }
 
 extern "C" size_t pr_vocab_ce_fwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D) {
   if (!pr::valid_shape(dtype, P, V, D)) return 0;
-  const pr::Shape s(dtype, P, V, D);
   pr::Carve packed(nullptr), plain(nullptr);
-  pr::FwdScratch f(packed, s);
-  pr::ScoreScratch g(plain, s);
-  return P <= pr::SCORE_ROWS ? std::max(packed.used, plain.used) : packed.used;
+  if (!pr::few(P, V, D)) pr::FwdScratch f(packed, pr::Shape(dtype, P, V, D));
+  if (P <= pr::SCORE_ROWS || pr::few(P, V, D)) pr::ScoreScratch g(plain, pr::FewShape(dtype, P, V, D));
+  return std::max(packed.used, plain.used);
 }
 
 extern "C" size_t pr_vocab_ce_bwd_scratch_bytes(int dtype, int64_t P, int64_t V, int64_t D, int want_dx, int want_dw) {
   if (!pr::valid_shape(dtype, P, V, D) || P < 1 || (!want_dx && !want_dw)) return 0;
   pr::Carve c(nullptr);
-  pr::BwdScratch b(c, pr::Shape(dtype, P, V, D), want_dx, want_dw);
+  if (pr::few(P, V, D)) pr::FewBwdScratch b(c, pr::FewShape(dtype, P, V, D), want_dx);
+  else pr::BwdScratch b(c, pr::Shape(dtype, P, V, D), want_dx, want_dw);
   return c.used;
 }
 
@@ -1375,22 +1814,25 @@ extern "C" int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const
                                float *row_loss, float *lse, float *loss, void *stream) {
   const pr::Call c{dtype, P, V, D, {x, P, D, ldx_row, ldx_col}, {w, V, D, ldw_row, ldw_col}, labels, ignore_index, scale};
   PR_TRY(pr::check_call(c));
-  PR_TRY(pr::check_inputs(c));
-  if ((!kept && P > pr::SCORE_ROWS) || !scratch || (!row_loss && !loss) || ((uintptr_t)kept & 15) || ((uintptr_t)scratch & 15))
+  PR_TRY(pr::check_matrix(dtype, c.x));
+  PR_TRY(pr::check_matrix(dtype, c.w));
+  if ((!kept && P > pr::SCORE_ROWS && !pr::few(P, V, D)) || !scratch || (!row_loss && !loss) || ((uintptr_t)kept & 15) || ((uintptr_t)scratch & 15))
     return PR_EINVAL;
   if ((kept && kept_bytes < pr_vocab_ce_kept_bytes(dtype, P, V, D)) ||
       scratch_bytes < pr_vocab_ce_fwd_scratch_bytes(dtype, P, V, D))
     return PR_ESCRATCH;
-  const pr::Shape s(dtype, P, V, D);
   hipStream_t st = (hipStream_t)stream;
   pr::Carve ck(kept), cs(scratch);
-  if (!kept) {
+  if (!kept || pr::few(P, V, D)) {
+    const pr::FewShape s(dtype, P, V, D);
     pr::ScoreScratch f(cs, s);
+    pr::FewKept few(ck, s), *k = kept ? &few : nullptr;
     if (!row_loss) row_loss = f.row_loss;
-    if (dtype == PR_F32) return pr::score<float>(c, mean, f, row_loss, lse, loss, st);
-    if (dtype == PR_F16) return pr::score<_Float16>(c, mean, f, row_loss, lse, loss, st);
-    return pr::score<__bf16>(c, mean, f, row_loss, lse, loss, st);
+    if (dtype == PR_F32) return pr::score<float>(c, mean, f, k, row_loss, lse, loss, st);
+    if (dtype == PR_F16) return pr::score<_Float16>(c, mean, f, k, row_loss, lse, loss, st);
+    return pr::score<__bf16>(c, mean, f, k, row_loss, lse, loss, st);
   }
+  const pr::Shape s(dtype, P, V, D);
   pr::Kept k(ck, s);
   pr::FwdScratch f(cs, s);
   if (!row_loss) row_loss = f.row_loss;
@@ -1399,22 +1841,34 @@ extern "C" int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const
   return pr::forward<__bf16, 1>(c, mean, k, f, row_loss, lse, loss, st);
 }
 
-extern "C" int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const int64_t *labels, int64_t ignore_index,
-                               float scale, int mean, int per_row, const void *kept, size_t kept_bytes, const float *g_loss,
-                               const float *g_lse, void *scratch, size_t scratch_bytes, void *dx, void *dw, void *stream) {
-  const pr::Call c{dtype, P, V, D, {}, {}, labels, ignore_index, scale};
+extern "C" int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const void *w, int64_t ldw_row, int64_t ldw_col,
+                               const int64_t *labels, int64_t ignore_index, float scale, int mean, int per_row,
+                               const void *kept, size_t kept_bytes, const float *g_loss, const float *g_lse, void *scratch,
+                               size_t scratch_bytes, void *dx, void *dw, void *stream) {
+  const pr::Call c{dtype, P, V, D, {}, {w, V, D, ldw_row, ldw_col}, labels, ignore_index, scale};
   PR_TRY(pr::check_call(c));
   if (!dx && !dw) return PR_OK;
+  const bool few = pr::few(P, V, D);
+  if (few && dx) PR_TRY(pr::check_matrix(dtype, c.w));
   if (!kept || !scratch || ((uintptr_t)kept & 15) || ((uintptr_t)scratch & 15)) return PR_EINVAL;
   if (((uintptr_t)dx & 15) || ((uintptr_t)dw & 15)) return PR_EINVAL;
   if (kept_bytes < pr_vocab_ce_kept_bytes(dtype, P, V, D) ||
       scratch_bytes < pr_vocab_ce_bwd_scratch_bytes(dtype, P, V, D, dx != nullptr, dw != nullptr))
     return PR_ESCRATCH;
-  const pr::Shape s(dtype, P, V, D);
   pr::Carve ck(const_cast<void *>(kept)), cs(scratch);
+  hipStream_t st = (hipStream_t)stream;
+  if (few) {
+    const pr::FewShape s(dtype, P, V, D);
+    const pr::FewKept k(ck, s);
+    const pr::FewBwdScratch b(cs, s, dx != nullptr);
+    if (dtype == PR_F32) return pr::few_backward<float>(c, per_row, mean, k, b, g_loss, g_lse, (float *)dx, (float *)dw, st);
+    if (dtype == PR_F16)
+      return pr::few_backward<_Float16>(c, per_row, mean, k, b, g_loss, g_lse, (_Float16 *)dx, (_Float16 *)dw, st);
+    return pr::few_backward<__bf16>(c, per_row, mean, k, b, g_loss, g_lse, (__bf16 *)dx, (__bf16 *)dw, st);
+  }
+  const pr::Shape s(dtype, P, V, D);
   const pr::Kept k(ck, s);
   pr::BwdScratch b(cs, s, dx != nullptr, dw != nullptr);
-  hipStream_t st = (hipStream_t)stream;
   if (dtype == PR_F32) return pr::backward<float, 2>(c, per_row, mean, k, b, g_loss, g_lse, (float *)dx, (float *)dw, st);
   if (dtype == PR_F16)
     return pr::backward<_Float16, 1>(c, per_row, mean, k, b, g_loss, g_lse, (_Float16 *)dx, (_Float16 *)dw, st);

@@ -39,7 +39,7 @@ def _forward(x, w, labels, scale, ignore_index, reduction, want_lse, with_grad, 
         return loss, lse, None
     lib, t = _lib.load(), _TYPES[x.dtype]
     # few rows and no gradient to come: nothing is packed and nothing kept
-    plain = not with_grad and P <= lib.pr_vocab_ce_score_rows()
+    plain = not with_grad and (P <= lib.pr_vocab_ce_score_rows() or not lib.pr_vocab_ce_keeps_vocabulary(P, V, D))
     kept = None if plain else _scratch(lib.pr_vocab_ce_kept_bytes(t, P, V, D), dev)
     scratch = _scratch(lib.pr_vocab_ce_fwd_scratch_bytes(t, P, V, D), dev)
     per_row, scalar = (loss, None) if reduction == "none" else (None, loss)
@@ -56,13 +56,15 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.args = x.shape, w.shape[0], x.dtype, scale, ignore_index, reduction
         loss, lse, kept = _forward(x, w, labels, scale, ignore_index, reduction, want_lse, True, stream)
-        ctx.save_for_backward(labels, kept)      # kept has its own copy of features and vocabulary
+        # kept has its own copy of the features and, but for few rows, of the vocabulary
+        reads = x.shape[0] > 0 and ctx.needs_input_grad[0] and not _lib.load().pr_vocab_ce_keeps_vocabulary(*x.shape[:1], *w.shape)
+        ctx.save_for_backward(labels, kept, w if reads else None)
         return loss, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_loss, g_lse):
-        labels, kept = ctx.saved_tensors
+        labels, kept, w = ctx.saved_tensors
         (P, D), V, dtype, scale, ignore_index, reduction = ctx.args
         want_x, want_w = ctx.needs_input_grad[:2]
         dev = labels.device
@@ -76,7 +78,7 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
             lib, t = _lib.load(), _TYPES[dtype]
             scratch = _scratch(lib.pr_vocab_ce_bwd_scratch_bytes(t, P, V, D, int(want_x), int(want_w)), dev)
             with _on(dev):
-                _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(labels), ignore_index, scale, int(reduction == "mean"),
+                _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(w), *(w.stride() if w is not None else (0, 0)), _ptr(labels), ignore_index, scale, int(reduction == "mean"),
                       int(reduction == "none"), _ptr(kept), kept.numel(), _ptr(g_loss), _ptr(g_lse), _ptr(scratch),
                       scratch.numel(), _ptr(dx), _ptr(dw), _stream())
         return (dx, dw) + (None,) * 6

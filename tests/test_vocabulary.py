@@ -84,7 +84,7 @@ def inputs(P, V, D, dtype, seed, scale=1.0, ignored=0.0):
     return x.to(dtype).cuda(), w.to(dtype).cuda(), labels.cuda()
 
 
-def check(x, w, labels, scale=1.0, reduction="mean", lse_weight=0.0, ignore=IGN, want=("x", "w"), dtype=None):
+def check(x, w, labels, scale=1.0, reduction="mean", lse_weight=0.0, ignore=IGN, want=("x", "w"), dtype=None, n3=None):
     """One call with its gradients, every output against the reference.  A random row gradient for "none"."""
     from pogs_amd.vocabulary import vocabulary_cross_entropy
 
@@ -95,7 +95,7 @@ def check(x, w, labels, scale=1.0, reduction="mean", lse_weight=0.0, ignore=IGN,
     n = max(1, int((labels != ignore).sum()))
     up = {"none": per_row.double(), "sum": torch.full((P,), 0.7, dtype=torch.float64, device="cuda"),
           "mean": torch.full((P,), 0.7 / n, dtype=torch.float64, device="cuda")}[reduction]
-    ref = reference(x.detach(), w.detach(), labels.long(), scale, up, per_lse.double(), ignore, dtype)
+    ref = reference(x.detach(), w.detach(), labels.long(), scale, up, per_lse.double(), ignore, dtype, n3)
     xr, wr = x.detach().requires_grad_("x" in want), w.detach().requires_grad_("w" in want)
     loss, lse = vocabulary_cross_entropy(xr, wr, labels, scale, ignore, reduction, return_lse=True)
     assert loss.dtype == lse.dtype == torch.float32
@@ -150,7 +150,7 @@ def test_entry_points_validate_without_a_gpu():
     assert fwd(kb=16) == -3 and fwd(sb=16) == -3
 
     def bwd(dx=ok, dw=ok, kept=ok, kb=1 << 30, scratch=ok, sb=1 << 30, P=4):
-        return lib.pr_vocab_ce_bwd(0, P, 8, 16, ok, -100, 1.0, 0, 0, kept, kb, ok, None, scratch, sb, dx, dw, None)
+        return lib.pr_vocab_ce_bwd(0, P, 8, 16, None, 0, 0, ok, -100, 1.0, 0, 0, kept, kb, ok, None, scratch, sb, dx, dw, None)
 
     assert bwd(dx=None, dw=None) == 0
     for kw in (dict(dx=odd), dict(dw=odd), dict(kept=None), dict(scratch=None), dict(scratch=odd), dict(P=0)):
@@ -188,7 +188,7 @@ def test_scale_whose_logits_cannot_be_formed_is_refused():
         with pytest.raises(ValueError, match="finite"):
             f(x, w, y, scale=scale)
         assert lib.pr_vocab_ce_fwd(0, 3, 5, 4, at, 4, 1, at, 4, 1, at, -100, scale, 0, at, n, at, n, at, None, None, None) == -1
-        assert lib.pr_vocab_ce_bwd(0, 3, 5, 4, at, -100, scale, 0, 1, at, n, at, None, at, n, at, at, None) == -1
+        assert lib.pr_vocab_ce_bwd(0, 3, 5, 4, at, 4, 1, at, -100, scale, 0, 1, at, n, at, None, at, n, at, at, None) == -1
     with pytest.raises(RuntimeError, match="HIP device"):
         f(x, w, y, scale=1e38)
 
@@ -412,6 +412,113 @@ def test_scoring_without_gradients(P, V, D, dtype):
         assert torch.equal(again, loss)
 
 
+FEW_SHAPES = [(1, 40_000, 64), (5, 33_001, 65), (32, 16_384, 128), (33, 2049, 1030), (64, 9000, 520), (65, 4200, 500),
+              (100, 131_073, 16), (127, 300_001, 7), (128, 21_001, 100), (17, 3, 700_001), (2, 3, 1_040_000)]
+FEW_PASSES = {torch.float32: 6, torch.float16: 1, torch.bfloat16: 2}     # products added for one of operands
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("P,V,D", FEW_SHAPES)
+def test_few_rows_and_a_large_vocabulary(P, V, D, dtype):
+    """The vocabulary is not packed: float32 products as in scoring (left out: less than rho), a bfloat16 vocabulary meets
+    G in two pieces (2^-14 of an entry, inside its rounding to float16)."""
+    assert not _lib.load().pr_vocab_ce_keeps_vocabulary(P, V, D)
+    x, w, y = inputs(P, V, D, dtype, seed=P + V + D, ignored=0.2 if P > 4 else 0.0)
+    n3 = FEW_PASSES[dtype]
+    check(x, w, y, scale=3.0, reduction="none", lse_weight=1.0, n3=n3)
+    check(x, w, y, scale=-2.5, n3=n3)
+    check(x, w, y, reduction="sum", want=("x",), n3=n3)
+    check(x, w, y, want=("w",), n3=n3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+def test_few_rows_layouts(dtype):
+    P, V, D = 40, 30_000, 75
+    x, w, y = inputs(P, V, D, dtype, seed=3, ignored=0.2)
+    want = check(x, w, y, scale=2.0, n3=FEW_PASSES[dtype])
+    wide = torch.full((V, D + 24), float("nan"), dtype=dtype, device="cuda")
+    for xs, ws in ((x, wide[:, 3:D + 3].copy_(w)), (x.t().contiguous().t(), w), (x, w.t().contiguous().t()),
+                   (torch.cat([x, x])[::2].copy_(x), torch.cat([w, w], 1).view(V, 2, D)[:, 0])):
+        got = check(xs, ws, y, scale=2.0, n3=FEW_PASSES[dtype])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert all(torch.equal(got[2][k], want[2][k]) for k in "xw")
+    one = w[:1].expand(V, D)                    # every word the same: probabilities 1 / V, a broadcast vocabulary's gradient
+    check(x, one, y, scale=2.0, n3=FEW_PASSES[dtype])
+    check(x[:1].expand(P, D), w, y, scale=2.0, n3=FEW_PASSES[dtype])
+
+
+@pytest.mark.gpu
+def test_few_rows_what_is_masked_or_not_finite():
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    P, V, D = 70, 30_000, 72
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        x, w, y = inputs(P, V, D, dtype, seed=5)
+
+        def step(x, y, ignore=IGN):
+            a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+            loss, lse = vocabulary_cross_entropy(a, b, y, 2.0, ignore, "none", return_lse=True)
+            return (loss.detach(), lse.detach()) + torch.autograd.grad(loss.sum() + lse[10:].sum(), (a, b))
+
+        good = step(x, torch.where(torch.arange(P, device="cuda") < 9, IGN, y))
+        x2, y2 = x.clone(), y.clone()
+        x2[:3], x2[3:6], x2[6:9] = math.nan, math.inf, torch.finfo(dtype).min
+        y2[:9] = 12                             # ignored rows hold anything; the ignored label may be a word's
+        y2[9:][y2[9:] == 12] = 13
+        got = step(x2, y2, 12)
+        want = step(x, torch.where(torch.arange(P, device="cuda") < 9, IGN, y2))
+        assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(got, want))
+        assert (got[0][:9] == 0).all() and (got[1][:9] == 0).all() and (got[2][:9] == 0).all()
+        # nothing left; a label that no word has; a row that is not finite
+        none = step(x, torch.full_like(y, IGN))
+        assert all((t == 0).all() for t in none)
+        for bad in (V, -1, 1 << 40):
+            y3 = y.clone()
+            y3[20] = bad
+            got = step(x, y3)
+            rest = torch.arange(P, device="cuda") != 20
+            assert torch.isnan(got[0][20]) and torch.isfinite(got[0][rest]).all() and torch.isfinite(got[1]).all()
+            assert torch.isnan(got[2][20]).all() and torch.isfinite(got[2][rest]).all() and torch.isnan(got[3]).all()
+        x4 = x.clone()
+        x4[33, 1] = math.nan
+        got, want = step(x4, y), step(x, y)
+        rest = torch.arange(P, device="cuda") != 33
+        assert torch.isnan(got[0][33]) and torch.equal(got[0][rest], want[0][rest]) and torch.equal(got[2][rest], want[2][rest])
+
+
+@pytest.mark.gpu
+def test_few_rows_in_a_graph_and_a_vocabulary_that_changes():
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    x, w, y = inputs(48, 40_000, 60, torch.float32, seed=15, ignored=0.1)
+    x.requires_grad_(True), w.requires_grad_(True)
+
+    def step():
+        loss = vocabulary_cross_entropy(x, w, y, 3.0)
+        return (loss.detach(),) + torch.autograd.grad(loss, (x, w))
+
+    eager = step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = step()
+    for k in range(4):
+        with torch.no_grad():
+            x.mul_(0.5)
+        want = step()
+        for t in res:
+            t.zero_()
+        g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(res, want))
+    assert not torch.equal(want[0], eager[0])
+    loss = vocabulary_cross_entropy(x, w, y, 3.0)
+    with torch.no_grad():
+        w.mul_(2.0)                             # the backward pass would read it: refused
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, (x, w))
+
+
 @pytest.mark.gpu
 def test_gradients_against_differences():
     """Central differences of the float64 loss, at steps small enough for 1e-5 of the gradient's scale."""
@@ -500,7 +607,8 @@ def test_vocabulary_beyond_32_bit_offsets():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
-@pytest.mark.parametrize("P,V,D", [(1, 1, 1), (3, 257, 31), (65, 700, 33), (257, 1300, 130), (600, 90, 96), (513, 5000, 520)])
+@pytest.mark.parametrize("P,V,D", [(1, 1, 1), (3, 257, 31), (65, 700, 33), (257, 1300, 130), (600, 90, 96), (513, 5000, 520),
+                                   (1, 40_000, 64), (33, 2049, 1030), (100, 33_001, 65)])
 def test_nothing_is_written_outside_the_buffers(P, V, D, dtype):
     """Every buffer of the C entry points at its exact size between guard bytes."""
     lib, t = _lib.load(), {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
@@ -527,7 +635,7 @@ def test_nothing_is_written_outside_the_buffers(P, V, D, dtype):
     g = torch.ones(1, device="cuda")
     for dx, dw in ((1, 1), (1, 0), (0, 1)):
         nb = lib.pr_vocab_ce_bwd_scratch_bytes(t, P, V, D, dx, dw)
-        assert lib.pr_vocab_ce_bwd(t, P, V, D, y.data_ptr(), -100, 2.0, 1, 0, kept, nk, g.data_ptr(), None, buffer(nb), nb,
+        assert lib.pr_vocab_ce_bwd(t, P, V, D, w.data_ptr(), D, 1, y.data_ptr(), -100, 2.0, 1, 0, kept, nk, g.data_ptr(), None, buffer(nb), nb,
                                    buffer(e * P * D) if dx else None, buffer(e * V * D) if dw else None, st) == 0
     torch.cuda.synchronize()
     for b, n in guarded:
