@@ -973,6 +973,122 @@ __global__ void __launch_bounds__(256, 2) vce_score_kernel(Matrix w, Matrix x, c
   }
 }
 
+template <typename T>
+constexpr int few_blocks = sizeof(T) == 4 ? 2 : 4;     // 16-wide blocks in 128 bytes of a row
+constexpr size_t score_lds(int nb, int blocks, int pieces) { return (size_t)2 * nb * blocks * pieces * 1024; }
+
+// The same where there are enough words for the chip at 128 a workgroup: a wavefront has 32 words and the whole
+// contraction, 128 bytes of each word's row at a time, and the four share the features' operands through LDS, where each of
+// the kernel above reads all of them from L2 for every 32 words.
+template <typename T, int NB, bool WIDE>
+__global__ void __launch_bounds__(256, 2) vce_score_shared_kernel(Matrix w, int64_t rows, const u4v *__restrict__ xf,
+                                                                  const int64_t *__restrict__ labels, float scale,
+                                                                  float2 *__restrict__ partial, float *__restrict__ target,
+                                                                  float *__restrict__ logits) {
+  typedef Operand<T> O;
+  constexpr int Q = few_blocks<T>, STAGE = NB * Q * O::N, LOADS = STAGE / 4;
+  extern __shared__ u4v lds[];    // two stages
+  __shared__ float2 join[4][NB][32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const float c = scale * LOG2E;
+  int label[NB];
+  float top[NB], tot[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int64_t p = 32 * n + (lane & 31), y = p < rows ? labels[p] : -1;
+    label[n] = y >= 0 && y < w.rows ? (int)y : -1;
+    top[n] = MAX_FLOOR, tot[n] = 0.f;
+  }
+  const int64_t tiles = (w.rows + 127) / 128;
+  const int chunks = (int)((w.cols + 63) / 64) * (4 / Q);
+  auto fill = [&](int k, int buf) {
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) {
+      const int j = wave + 4 * l, n = j / (Q * O::N), at = j % (Q * O::N);
+      __builtin_amdgcn_global_load_lds((global_ptr)(xf + ((int64_t)(n * chunks + k) * (Q * O::N) + at) * 64 + lane),
+                                       (lds_ptr)(lds + (buf * STAGE + j) * 64), 16, 0, 0);
+    }
+    asm volatile("" ::: "memory");
+  };
+  auto words = [&](int64_t t, int k, Eight<T> (&a)[Q]) {
+    const int64_t v = min(t * 128 + 32 * wave + (lane & 31), w.rows - 1);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) a[q] = fetch8<T, WIDE>(w, v, (int64_t)k * (16 * Q) + 16 * q + 8 * h);
+  };
+  Eight<T> a[Q], next[Q];
+  fill(0, 0);
+  words(blockIdx.x, 0, a);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int buf = 0;
+  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+    f16v acc[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
+    for (int k = 0; k < chunks; ++k) {
+      // the next chunk, of these words or of the next tile's, into the stage that was read before the last barrier
+      const bool last = k + 1 == chunks;
+      if (!last || t + gridDim.x < tiles) {
+        fill(last ? 0 : k + 1, buf ^ 1);
+        words(last ? t + gridDim.x : t, last ? 0 : k + 1, next);
+      }
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const O oa = operand(a[q]);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+          acc[n] = O::product(oa, packed_operand<O>(lds + (buf * STAGE + (n * Q + q) * O::N) * 64 + lane), acc[n]);
+      }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __syncthreads();
+      buf ^= 1;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) a[q] = next[q];
+    }
+    const int64_t v0 = t * 128 + 32 * wave;
+    const int left = (int)min(w.rows - v0, (int64_t)32) - 4 * h;     // words that exist, from this lane's first one on
+    if (v0 >= w.rows) continue;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int at = label[n] - (int)v0 - 4 * h;
+      float most = MAX_FLOOR;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        acc[n][r] *= c;
+        if (at == (r & 3) + 8 * (r >> 2)) target[32 * n + (lane & 31)] = acc[n][r];
+        most = (r & 3) + 8 * (r >> 2) < left ? fmaxf(most, acc[n][r]) : most;
+      }
+      if (logits)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          store4<float>(logits + (v0 * NB + 32 * n + (lane & 31)) * 32 + 8 * q + 4 * h, acc[n][4 * q], acc[n][4 * q + 1],
+                        acc[n][4 * q + 2], acc[n][4 * q + 3]);
+      float add = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        add += (r & 3) + 8 * (r >> 2) < left ? __builtin_amdgcn_exp2f(acc[n][r] - most) : 0.f;
+      merge(top[n], tot[n], most, add);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    merge(top[n], tot[n], __shfl_xor(top[n], 32), __shfl_xor(tot[n], 32));
+    if (h == 0) join[wave][n][lane] = make_float2(top[n], tot[n]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * NB; i += 256) {
+    float2 q = join[0][i / 32][i & 31];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+      const float2 o = join[k][i / 32][i & 31];
+      merge(q.x, q.y, o.x, o.y);
+    }
+    if (i < rows) partial[(int64_t)i * gridDim.x + blockIdx.x] = q;
+  }
+}
+
 // G as an operand that meets one of type T.  bfloat16 takes two pieces of it (2^-14 of an entry), float16 its own type, with
 // the row factors scaled by exp_g; the others have float32's range and need no scaling.
 template <typename T>
@@ -1024,53 +1140,96 @@ struct FewGrad {  // what G is made of
   }
 };
 
+// A chunk of features of DW: a tile of 32, or a 16-bit pair of tiles.
+template <typename T>
+constexpr int few_tiles = sizeof(T) == 4 ? 1 : 2;
+constexpr size_t dw_lds(int nb, int tiles, int pieces) { return (size_t)3 * 2 * nb * tiles * pieces * 1024; }
+
 template <typename T, int NB>
 __global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, const u4v *__restrict__ xt, float scale,
                                                             T *__restrict__ out) {
-  constexpr int KB = 2 * NB;
+  constexpr int KB = 2 * NB, NT = few_tiles<T>, STAGE = NT * KB * Operand<T>::N, LOADS = (STAGE + 3) / 4;
   __shared__ float4 rows[32 * NB];
+  extern __shared__ u4v lds[];    // three stages, of a chunk of the features' operands each
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int64_t chunks = (f.D + 32 * NT - 1) / (32 * NT);
+  auto fill = [&](int64_t c, int buf) {
+    const u4v *src = xt + c * (STAGE * 64) + lane;
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) {
+      const int j = min(wave + 4 * l, STAGE - 1);   // (past the end: the last block again, into its own place)
+      __builtin_amdgcn_global_load_lds((global_ptr)(src + j * 64), (lds_ptr)(lds + (buf * STAGE + j) * 64), 16, 0, 0);
+    }
+    asm volatile("" ::: "memory");
+  };
+  fill(blockIdx.y, 0);
+  if (blockIdx.y + gridDim.y < chunks) fill(blockIdx.y + gridDim.y, 1);
   f.rows<T>(rows, 32 * NB);
   __syncthreads();
-  const int lane = threadIdx.x & 63, h = lane >> 5;
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t * 32 >= f.V) return;
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave, at = min(t, (f.V - 1) / 32);   // (past the end: not stored)
   GradOperand<T> ga[KB];
-  const float *z = f.logits + t * (1024 * NB) + (lane & 31);
+  const float *z = f.logits + at * (1024 * NB) + 256 * h + (lane & 31);
+  float v[KB][8];
+#pragma unroll
+  for (int b = 0; b < KB; ++b)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[b][i] = z[(16 * b + i) * 32];
 #pragma unroll
   for (int b = 0; b < KB; ++b) {
-    float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int p = 16 * b + 8 * h + i;
-      v[i] = FewGrad::entry(z[p * 32], rows[p], (int)(t * 32) + (lane & 31));
-    }
-    ga[b].set(v);
+    for (int i = 0; i < 8; ++i) v[b][i] = FewGrad::entry(v[b][i], rows[16 * b + 8 * h + i], (int)(at * 32) + (lane & 31));
+    ga[b].set(v[b]);
+    // a block at a time: the row factors of all of them would not fit in registers
+#pragma unroll
+    for (int k = 0; k < GradOperand<T>::N; ++k) asm volatile("" : "+v"(ga[b].piece[k])::"memory");
+    __builtin_amdgcn_sched_barrier(0);
   }
   const int e = FEW_SCALED<T> ? -*f.exp_g : 0;
-  for (int64_t c = blockIdx.y; c * 64 < f.D; c += gridDim.y) {
-    f16v acc[2];
+  const bool whole = t * 32 + 32 <= f.V;
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+  int buf = 0;
+  for (int64_t c = blockIdx.y; c < chunks; c += gridDim.y) {
+    // two chunks ahead, into the stage that was read before the last barrier
+    const bool more = c + 2 * (int64_t)gridDim.y < chunks;
+    if (more) fill(c + 2 * (int64_t)gridDim.y, buf == 0 ? 2 : buf - 1);
+    f16v acc[2];     // of two tiles, or of the even and the odd blocks of one
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
+    Operand<T> x[2];
+    x[0] = packed_operand<Operand<T>>(lds + buf * STAGE * 64 + lane);
 #pragma unroll
-      for (int b = 0; b < KB; ++b)
-        acc[j] = GradOperand<T>::times(
-            ga[b], packed_operand<Operand<T>>(xt + ((2 * c + j) * KB + b) * (Operand<T>::N * 64) + lane), acc[j]);
+    for (int i = 0; i < NT * KB; ++i) {
+      if (i + 1 < NT * KB) x[(i + 1) & 1] = packed_operand<Operand<T>>(lds + (buf * STAGE + (i + 1) * Operand<T>::N) * 64 + lane);
+      const int j = NT == 1 ? i & 1 : i / KB;
+      acc[j] = GradOperand<T>::times(ga[i % KB], x[i & 1], acc[j]);
     }
-    const int64_t d0 = tile_column<T>(2 * c, lane), d1 = tile_column<T>(2 * c + 1, lane);
+    // all but the youngest fill have come, and what was written a chunk ago; this chunk's stores have until the next wait
+    if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    buf = buf == 2 ? 0 : buf + 1;
+    const int64_t d = tile_column<T>(NT * c, lane);
+    if (d >= f.D) continue;
+    T *dst = out + (t * 32 + 4 * h) * f.D + d;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int64_t v = t * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
-      if (v >= f.V) continue;
-      const T g0 = (T)ldexpf(acc[0][r] * scale, e), g1 = (T)ldexpf(acc[1][r] * scale, e);
-      T *dst = out + v * f.D;
-      if (sizeof(T) == 2 && (f.D & 1) == 0) {
-        typedef T t2 __attribute__((ext_vector_type(2)));
-        if (d0 < f.D) *reinterpret_cast<t2 *>(dst + d0) = t2{g0, g1};
+      const int v = (r & 3) + 8 * (r >> 2);
+      if (!whole && t * 32 + 4 * h + v >= f.V) continue;
+      if constexpr (NT == 1) {
+        dst[v * f.D] = (acc[0][r] + acc[1][r]) * scale;
       } else {
-        if (d0 < f.D) dst[d0] = g0;
-        if (d1 < f.D) dst[d1] = g1;
+        typedef T t2 __attribute__((ext_vector_type(2)));
+        const t2 g = {(T)ldexpf(acc[0][r] * scale, e), (T)ldexpf(acc[1][r] * scale, e)};
+        if ((f.D & 1) == 0) {
+          *reinterpret_cast<t2 *>(dst + v * f.D) = g;
+        } else {
+          dst[v * f.D] = g.x;
+          if (d + 1 < f.D) dst[v * f.D + 1] = g.y;
+        }
       }
     }
   }
@@ -1464,6 +1623,21 @@ struct BwdScratch {
   }
 };
 
+// Launches a kernel whose dynamic LDS may be above the 64 KB that need no leave.
+template <auto KERNEL, typename... Args>
+int launch_lds(dim3 grid, dim3 block, size_t bytes, hipStream_t st, const Args &...args) {
+  static std::atomic<uint64_t> known{0};   // devices that know the kernel's LDS size
+  int device = 0;
+  PR_HIP(hipGetDevice(&device));
+  const uint64_t bit = 1ull << (device & 63);
+  if (device > 63 || !(known.load(std::memory_order_acquire) & bit)) {
+    PR_HIP(hipFuncSetAttribute((const void *)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    known.fetch_or(bit, std::memory_order_release);
+  }
+  hipLaunchKernelGGL(KERNEL, grid, block, bytes, st, args...);
+  return check_launch("pr_vocab_ce");
+}
+
 struct Product {
   GemmArgs g;
   int64_t m_rows, n_rows;  // multiples of 32 and of 256
@@ -1484,17 +1658,8 @@ int launch_tiles(const Product &a, const Product *b, hipStream_t st) {
     set_error_text("pr_vocab_ce: too many tiles for one launch");
     return PR_EUNSUPPORTED;
   }
-  const auto kernel = vce_gemm_kernel<NP, MT, MODE, T>;
-  static std::atomic<uint64_t> known{0};   // devices that know the kernel's LDS size
-  int device = 0;
-  PR_HIP(hipGetDevice(&device));
-  const uint64_t bit = 1ull << (device & 63);
-  if (device > 63 || !(known.load(std::memory_order_acquire) & bit)) {
-    PR_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    known.fetch_or(bit, std::memory_order_release);
-  }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(CUS, (tiles + 7) / 8 * 8)), dim3(512), bytes, st, g, g2);
-  return check_launch("pr_vocab_ce");
+  return launch_lds<vce_gemm_kernel<NP, MT, MODE, T>>(dim3((unsigned)std::min<int64_t>(CUS, (tiles + 7) / 8 * 8)), dim3(512),
+                                                      bytes, st, g, g2);
 }
 
 // Time of so many tiles of 64 mt by 256, in arbitrary units.  A tile costs its products and the operand rows that it does
@@ -1592,10 +1757,12 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
 struct FewShape {
   int64_t P, V, D, R, Dk, tiles;
   int nb, pieces;
+  bool shared;   // the score kernel that shares the features' operands
   FewShape(int dtype, int64_t P_, int64_t V_, int64_t D_)
       : P(P_), V(V_), D(D_), Dk(round_up(D_, 64)), tiles((V_ + 31) / 32), nb(P_ <= 32 ? 1 : P_ <= 64 ? 2 : 4),
         pieces(dtype == PR_F32 ? 3 : 1) {
     R = 32 * nb;
+    shared = nb > 1 && V >= 128 * CUS;
   }
   int64_t packed() const { return R * Dk / 8 * pieces; }   // 16-byte units of a copy of the features
 };
@@ -1618,7 +1785,7 @@ struct ScoreScratch {  // of the forward pass for few rows
   u4v *xf;
   int blocks;
   ScoreScratch(Carve &c, const FewShape &s) {
-    blocks = (int)std::min<int64_t>(SCORE_BLOCKS, s.tiles);
+    blocks = (int)(s.shared ? std::min<int64_t>(FEW_BLOCKS, (s.V + 127) / 128) : std::min<int64_t>(SCORE_BLOCKS, s.tiles));
     target = c.take<float>(s.R);
     row_loss = c.take<float>(s.R);
     partial = c.take<float2>(blocks * s.R);
@@ -1635,9 +1802,18 @@ int launch_score(const Call &c, const FewShape &s, ScoreScratch &f, FewKept *k, 
     hipLaunchKernelGGL((vce_few_pack_kernel<T>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, job);
     PR_TRY(check_launch("pr_vocab_ce"));
   }
+  float *const logits = k ? k->logits : nullptr;
+  if constexpr (NB > 1)
+    if (s.shared) {
+      const size_t bytes = score_lds(NB, few_blocks<T>, s.pieces);
+      return wide ? launch_lds<vce_score_shared_kernel<T, NB, true>>(dim3(f.blocks), dim3(256), bytes, st, c.w, c.P, f.xf, c.labels,
+                                                                     c.scale, f.partial, f.target, logits)
+                  : launch_lds<vce_score_shared_kernel<T, NB, false>>(dim3(f.blocks), dim3(256), bytes, st, c.w, c.P, f.xf,
+                                                                      c.labels, c.scale, f.partial, f.target, logits);
+    }
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(f.blocks), dim3(256), 0, st, c.w, c.x, f.xf, c.labels, c.ignore, c.scale, f.partial,
-                       f.target, k ? k->logits : nullptr);
+                       f.target, logits);
     return check_launch("pr_vocab_ce");
   };
   if constexpr (NB == 1)
@@ -1696,9 +1872,10 @@ int few_gradients(const Call &c, const FewShape &s, const FewKept &k, const FewB
   }
   if (dw) {
     const unsigned blocks = (unsigned)((s.tiles + 3) / 4);
-    const unsigned parts = (unsigned)std::max<int64_t>(1, std::min<int64_t>(FEW_BLOCKS / blocks, s.Dk / 64));
-    hipLaunchKernelGGL((vce_few_dw_kernel<T, NB>), dim3(blocks, parts), dim3(256), 0, st, f, k.xt, c.scale, dw);
-    PR_TRY(check_launch("pr_vocab_ce"));
+    // (a part has a chunk at least: of 32 float32 features, of 64 others)
+    const unsigned parts = (unsigned)std::max<int64_t>(1, std::min<int64_t>(FEW_BLOCKS / blocks, c.D / 64));
+    PR_TRY((launch_lds<vce_few_dw_kernel<T, NB>>(dim3(blocks, parts), dim3(256), dw_lds(NB, few_tiles<T>, s.pieces), st, f,
+                                                 (const u4v *)k.xt, c.scale, dw)));
   }
   return PR_OK;
 }
