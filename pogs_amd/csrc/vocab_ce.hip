@@ -986,7 +986,7 @@ __global__ void __launch_bounds__(256, 2) vce_score_shared_kernel(Matrix w, int6
                                                                   float2 *__restrict__ partial, float *__restrict__ target,
                                                                   float *__restrict__ logits) {
   typedef Operand<T> O;
-  constexpr int Q = few_blocks<T>, STAGE = NB * Q * O::N, LOADS = STAGE / 4;
+  constexpr int Q = few_blocks<T>, STAGE = NB * Q * O::N, LOADS = (STAGE + 3) / 4;
   extern __shared__ u4v lds[];    // two stages
   __shared__ float2 join[4][NB][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
@@ -1004,7 +1004,7 @@ __global__ void __launch_bounds__(256, 2) vce_score_shared_kernel(Matrix w, int6
   auto fill = [&](int k, int buf) {
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) {
-      const int j = wave + 4 * l, n = j / (Q * O::N), at = j % (Q * O::N);
+      const int j = min(wave + 4 * l, STAGE - 1), n = j / (Q * O::N), at = j % (Q * O::N);   // (past the end: as in DW)
       __builtin_amdgcn_global_load_lds((global_ptr)(xf + ((int64_t)(n * chunks + k) * (Q * O::N) + at) * 64 + lane),
                                        (lds_ptr)(lds + (buf * STAGE + j) * 64), 16, 0, 0);
     }
@@ -1762,7 +1762,7 @@ struct FewShape {
       : P(P_), V(V_), D(D_), Dk(round_up(D_, 64)), tiles((V_ + 31) / 32), nb(P_ <= 32 ? 1 : P_ <= 64 ? 2 : 4),
         pieces(dtype == PR_F32 ? 3 : 1) {
     R = 32 * nb;
-    shared = nb > 1 && V >= 128 * CUS;
+    shared = V >= 128 * CUS;
   }
   int64_t packed() const { return R * Dk / 8 * pieces; }   // 16-byte units of a copy of the features
 };
@@ -1795,7 +1795,7 @@ struct ScoreScratch {  // of the forward pass for few rows
 
 template <typename T, int NB>
 int launch_score(const Call &c, const FewShape &s, ScoreScratch &f, FewKept *k, hipStream_t st) {
-  const bool wide = c.D >= 8 && c.w.ld_col == 1, packed = NB > 1 || !wide || c.x.ld_col != 1 || c.D % 8;
+  const bool wide = c.D >= 8 && c.w.ld_col == 1, packed = NB > 1 || s.shared || !wide || c.x.ld_col != 1 || c.D % 8;
   if (packed || k) {
     const FewPack job{c.x, c.labels, c.ignore, (int)(s.Dk / 16), 2 * NB, packed ? f.xf : nullptr, k ? k->xt : nullptr};
     const int64_t units = s.Dk / 16 * NB * ((packed ? 1 : 0) + (k ? 1 : 0));
@@ -1803,14 +1803,15 @@ int launch_score(const Call &c, const FewShape &s, ScoreScratch &f, FewKept *k, 
     PR_TRY(check_launch("pr_vocab_ce"));
   }
   float *const logits = k ? k->logits : nullptr;
-  if constexpr (NB > 1)
-    if (s.shared) {
-      const size_t bytes = score_lds(NB, few_blocks<T>, s.pieces);
-      return wide ? launch_lds<vce_score_shared_kernel<T, NB, true>>(dim3(f.blocks), dim3(256), bytes, st, c.w, c.P, f.xf, c.labels,
-                                                                     c.scale, f.partial, f.target, logits)
-                  : launch_lds<vce_score_shared_kernel<T, NB, false>>(dim3(f.blocks), dim3(256), bytes, st, c.w, c.P, f.xf,
-                                                                      c.labels, c.scale, f.partial, f.target, logits);
-    }
+  if (s.shared) {
+    const size_t bytes = score_lds(NB, few_blocks<T>, s.pieces);
+    return wide ? launch_lds<vce_score_shared_kernel<T, NB, true>>(dim3(f.blocks), dim3(256), bytes, st, c.w, c.P,
+                                                                   (const u4v *)f.xf, c.labels, c.scale, f.partial, f.target,
+                                                                   logits)
+                : launch_lds<vce_score_shared_kernel<T, NB, false>>(dim3(f.blocks), dim3(256), bytes, st, c.w, c.P,
+                                                                    (const u4v *)f.xf, c.labels, c.scale, f.partial, f.target,
+                                                                    logits);
+  }
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(f.blocks), dim3(256), 0, st, c.w, c.x, f.xf, c.labels, c.ignore, c.scale, f.partial,
                        f.target, logits);
