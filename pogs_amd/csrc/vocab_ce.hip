@@ -52,11 +52,20 @@ constexpr int CUS = 256;
 constexpr int TOP_EXP = 13;  // packed magnitudes are below 2^(TOP_EXP + 1)
 constexpr float MAX_FLOOR = -3.0e38f;  // a maximum over nothing: exp2 of anything minus it is 0, not NaN
 constexpr float LN2F = 0.69314718055994531f;
-// Rows that the kernels for few rows take at most: without gradients, and with a large vocabulary.
-constexpr int SCORE_ROWS = 64, FEW_ROWS = 128;
-constexpr int SCORE_BLOCKS = 1024;  // workgroups of the score kernel: four per CU
-constexpr int FEW_BLOCKS = 512;     // of the gradients' kernels, where there is work for so many
+// The kernels for few rows read the vocabulary once for the scores and once for dX, where the packed path reads it three
+// times and writes it twice before its products; they multiply 32, 64 or 128 rows, whatever there are.  131072 words x 1024
+// dims, loss and both gradients: 1 row 455 against 1355 us (bfloat16 221 against 720), 128 rows 654 against 1398 (324
+// against 739); loss alone, 128 rows: 203 against 466 (71 against 252).  256 rows would be two such passes, which is what
+// the packed path takes for them (1419 and 728 us with gradients).
+constexpr int FEW_ROWS = 128;
+// Below so many elements of the vocabulary there is little to gain (2000 words x 256 dims: 42 against 64 us on the GPU,
+// less than the host takes), and the packed path's backward pass has its own copy of the vocabulary.
 constexpr int64_t FEW_VOCABULARY = 1 << 19;
+constexpr int SCORE_ROWS = 64;      // rows that they take from any vocabulary where no backward pass follows
+constexpr int SCORE_BLOCKS = 1024;  // workgroups of the score kernel: four per CU
+// Workgroups of the others, where there is work for so many: two per CU.  (One row to 128 of 131072 words x 1024 dims,
+// bfloat16, loss and gradients: 221 to 324 us; 256 workgroups 267 to 386, 1024 workgroups 223 to 359.)
+constexpr int FEW_BLOCKS = 512;
 constexpr int AMAX_BLOCKS = 1024;  // partial maxima per tensor at most
 
 struct Matrix {  // rows x cols with any strides (elements)
@@ -705,13 +714,16 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
 // At most 32 NB rows: the vocabulary is read as it is, and nothing of its size is packed.  16-bit operands go to the matrix
 // cores in their own type; a float32 value is cut into three bfloat16 pieces that hold all its 24 bits (by truncation, so
 // the largest values do not overflow), six products of which leave out less than 2^-21 of a product.
-// SCORE  A workgroup takes 32 words at a time; its four wavefronts take the 64-wide pieces of the contraction in turn, add
-//        their tiles through LDS, and each keeps the running maximum and sum over a quarter of the words.  For a backward
-//        pass the logits stay, 4 bytes for each word and row: P / D of a float32 vocabulary.
-// DW     32 words a wavefront: G of all rows is made from the logits in registers and multiplies the features, a 64-wide
-//        piece at a time.  Writes dW once.
-// DX     32 words a step, 64 features a wavefront and 256 a workgroup, whose wavefronts make G of the step in LDS together;
-//        reads the vocabulary once.  Partials per run of words, added by FINISH.
+//   SCORE   logits, maxima and sums of 32 words a wavefront.  For a backward pass the logits stay, 4 bytes for each word and
+//           row: at 32 rows a 32nd of a float32 vocabulary of 1024 dims.
+//   DX      32 words a step, 64 features a wavefront and 256 a workgroup, whose wavefronts make G of the step in LDS
+//           together; reads the vocabulary once.  Partials per run of words, added by FINISH.
+//   DW      32 words a wavefront: G of all rows is made from the logits in registers and multiplies the features, a 32- or
+//           64-wide chunk at a time, which the workgroup shares through LDS, three stages deep.  Writes dW once.
+// Bound: HBM for the fewest rows (131072 words x 1024 dims, one row: float32 SCORE 140 us, DX 111, DW 119 for 537 MB each,
+// 3.8 to 4.8 TB/s; bfloat16 53, 65 and 53 for 268 MB), the matrix cores and the conversions more and more from 64 rows on
+// (128 rows: float32 205, 262 and 258 us; bfloat16 70, 129 and 109).  After a DW its lines are still on their way out of
+// the cache, which a SCORE waits for (float32 213 us instead of 140).
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 
 template <typename T>
@@ -866,6 +878,8 @@ __device__ __forceinline__ void merge(float &m, float &s, float m2, float s2) {
   m = top;
 }
 
+// SCORE for a small vocabulary: a workgroup takes 32 words at a time; its four wavefronts take the 64-wide pieces of the
+// contraction in turn, add their tiles through LDS, and each keeps the running maximum and sum over a quarter of the words.
 // XP: the features are packed (xf); otherwise they are read as they are, eight aligned columns at a time (D % 8 == 0), which
 // saves a launch where it counts, with the fewest rows.
 template <typename T, int NB, bool WIDE, bool XP>
@@ -977,9 +991,9 @@ template <typename T>
 constexpr int few_blocks = sizeof(T) == 4 ? 2 : 4;     // 16-wide blocks in 128 bytes of a row
 constexpr size_t score_lds(int nb, int blocks, int pieces) { return (size_t)2 * nb * blocks * pieces * 1024; }
 
-// The same where there are enough words for the chip at 128 a workgroup: a wavefront has 32 words and the whole
-// contraction, 128 bytes of each word's row at a time, and the four share the features' operands through LDS, where each of
-// the kernel above reads all of them from L2 for every 32 words.
+// SCORE where there are enough words for the chip at 128 a workgroup: a wavefront has 32 words and the whole contraction,
+// 128 bytes of each word's row at a time, and the four share the features' operands through LDS, where each wavefront of the
+// kernel above reads all of them from L2 for every 32 words.
 template <typename T, int NB, bool WIDE>
 __global__ void __launch_bounds__(256, 2) vce_score_shared_kernel(Matrix w, int64_t rows, const u4v *__restrict__ xf,
                                                                   const int64_t *__restrict__ labels, float scale,
@@ -1757,11 +1771,13 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
 struct FewShape {
   int64_t P, V, D, R, Dk, tiles;
   int nb, pieces;
-  bool shared;   // the score kernel that shares the features' operands
+  bool shared;   // which score kernel
   FewShape(int dtype, int64_t P_, int64_t V_, int64_t D_)
       : P(P_), V(V_), D(D_), Dk(round_up(D_, 64)), tiles((V_ + 31) / 32), nb(P_ <= 32 ? 1 : P_ <= 64 ? 2 : 4),
         pieces(dtype == PR_F32 ? 3 : 1) {
     R = 32 * nb;
+    // Below, CUs would be without work (20011 words x 1024 dims: 64 rows 53 against 47 us, 24 bfloat16 rows 32 against 27;
+    // 60000 x 512: 41 against 58, 25 against 28)
     shared = V >= 128 * CUS;
   }
   int64_t packed() const { return R * Dk / 8 * pieces; }   // 16-byte units of a copy of the features

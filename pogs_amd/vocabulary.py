@@ -4,8 +4,8 @@ What the clip head's unit features (``FieldHeads.get_clip_outputs_from_feature``
 are trained and scored on when every pixel has a label in a table of phrase embeddings.  The value and the gradients of
 ``torch.nn.functional.cross_entropy(scale * features @ vocabulary.T, labels)``, without the ``[rows, words]`` logits: the
 forward pass keeps one maximum and sum a row, the backward pass makes the products again for one piece of the vocabulary
-at a time.  Products take float16 operands scaled by powers of two and add in float32; float32 inputs are split into two
-float16 planes (2^-22 a product), so float32 stays float32 in accuracy.  Results do not depend on the order in which
+at a time.  (Up to 128 rows of a large vocabulary do keep them for it, 4 bytes each, and read the vocabulary as it is.)  Products take 16-bit operands and add in float32; float32 inputs are split into two
+float16 planes or three bfloat16 pieces (2^-21 of a product at most is left out), so float32 stays float32 in accuracy.  Results do not depend on the order in which
 workgroups run.  HIP kernels only (``pr_vocab_ce_fwd``, ``pr_vocab_ce_bwd``); there is no CPU path.
 """
 from __future__ import annotations
@@ -139,7 +139,8 @@ def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tenso
     features and vocabulary, through the loss and the log-sum (gradients in the inputs' type, from the formula; not
     twice).  Ignored rows contribute nothing, even if their features are not finite.  A label that is neither in
     ``0..V-1`` nor ``ignore_index`` makes its row's loss NaN and the gradients with it: nothing is read out of range,
-    and the host does not wait to look.  Safe in a captured graph, gradients included, as long as no graph of the same
+    and the host does not wait to look.  Features may be changed in place before the backward pass, labels may not, and
+    neither may the vocabulary where it is large and the rows are at most 128 (autograd refuses).  Safe in a captured graph, gradients included, as long as no graph of the same
     leaves made outside the capture is alive (refused where one of this function is)."""
     scale = _check(features, vocabulary, labels, scale, reduction)
     D = features.shape[-1]

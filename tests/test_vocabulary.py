@@ -156,6 +156,12 @@ def test_entry_points_validate_without_a_gpu():
     for kw in (dict(dx=odd), dict(dw=odd), dict(kept=None), dict(scratch=None), dict(scratch=odd), dict(P=0)):
         assert bwd(**kw) == -1, kw
     assert bwd(kb=16) == -3 and bwd(sb=16) == -3
+    # few rows and a large vocabulary: the features' gradient reads the vocabulary again
+    assert lib.pr_vocab_ce_keeps_vocabulary(4, 8, 16) == 1 and lib.pr_vocab_ce_keeps_vocabulary(4, 1 << 17, 16) == 0
+    for w, ld in ((None, (16, 1)), (odd, (16, 1)), (ok, (-1, 1))):
+        assert lib.pr_vocab_ce_bwd(0, 4, 1 << 17, 16, w, *ld, ok, -100, 1.0, 0, 0, ok, 1 << 30, ok, None, ok, 1 << 30, ok, ok,
+                                   None) == -1
+    assert lib.pr_vocab_ce_bwd(0, 4, 1 << 17, 16, ok, 16, 1, ok, -100, 1.0, 0, 0, ok, 16, ok, None, ok, 1 << 30, ok, ok, None) == -3
 
 
 def test_refusals():
@@ -413,7 +419,7 @@ def test_scoring_without_gradients(P, V, D, dtype):
 
 
 FEW_SHAPES = [(1, 40_000, 64), (5, 33_001, 65), (32, 16_384, 128), (33, 2049, 1030), (64, 9000, 520), (65, 4200, 500),
-              (100, 131_073, 16), (127, 300_001, 7), (128, 21_001, 100), (17, 3, 700_001), (2, 3, 1_040_000)]
+              (100, 131_073, 16), (127, 300_001, 7), (128, 21_001, 100), (40, 33_000, 130), (64, 40_001, 33), (96, 32_768, 200), (17, 3, 700_001), (2, 3, 1_040_000)]
 FEW_PASSES = {torch.float32: 6, torch.float16: 1, torch.bfloat16: 2}     # products added for one of operands
 
 
@@ -450,42 +456,41 @@ def test_few_rows_layouts(dtype):
 
 
 @pytest.mark.gpu
-def test_few_rows_what_is_masked_or_not_finite():
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("P,V", [(20, 30_000), (20, 40_000), (50, 30_000), (50, 40_000), (70, 30_000), (128, 40_000)])
+def test_few_rows_what_is_masked_or_not_finite(P, V, dtype):
     from pogs_amd.vocabulary import vocabulary_cross_entropy
 
-    P, V, D = 70, 30_000, 72
-    for dtype in (torch.float32, torch.float16, torch.bfloat16):
-        x, w, y = inputs(P, V, D, dtype, seed=5)
+    x, w, y = inputs(P, V, 72, dtype, seed=5)
+    row = torch.arange(P, device="cuda")
 
-        def step(x, y, ignore=IGN):
-            a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
-            loss, lse = vocabulary_cross_entropy(a, b, y, 2.0, ignore, "none", return_lse=True)
-            return (loss.detach(), lse.detach()) + torch.autograd.grad(loss.sum() + lse[10:].sum(), (a, b))
+    def step(x, y, ignore=IGN):
+        a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss, lse = vocabulary_cross_entropy(a, b, y, 2.0, ignore, "none", return_lse=True)
+        with torch.no_grad():
+            again = vocabulary_cross_entropy(a, b, y, 2.0, ignore, "none")
+        assert ((again == loss) | torch.isnan(loss)).all()
+        return (loss.detach(), lse.detach()) + torch.autograd.grad(loss.sum() + lse[10:].sum(), (a, b))
 
-        good = step(x, torch.where(torch.arange(P, device="cuda") < 9, IGN, y))
-        x2, y2 = x.clone(), y.clone()
-        x2[:3], x2[3:6], x2[6:9] = math.nan, math.inf, torch.finfo(dtype).min
-        y2[:9] = 12                             # ignored rows hold anything; the ignored label may be a word's
-        y2[9:][y2[9:] == 12] = 13
-        got = step(x2, y2, 12)
-        want = step(x, torch.where(torch.arange(P, device="cuda") < 9, IGN, y2))
-        assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(got, want))
-        assert (got[0][:9] == 0).all() and (got[1][:9] == 0).all() and (got[2][:9] == 0).all()
-        # nothing left; a label that no word has; a row that is not finite
-        none = step(x, torch.full_like(y, IGN))
-        assert all((t == 0).all() for t in none)
-        for bad in (V, -1, 1 << 40):
-            y3 = y.clone()
-            y3[20] = bad
-            got = step(x, y3)
-            rest = torch.arange(P, device="cuda") != 20
-            assert torch.isnan(got[0][20]) and torch.isfinite(got[0][rest]).all() and torch.isfinite(got[1]).all()
-            assert torch.isnan(got[2][20]).all() and torch.isfinite(got[2][rest]).all() and torch.isnan(got[3]).all()
-        x4 = x.clone()
-        x4[33, 1] = math.nan
-        got, want = step(x4, y), step(x, y)
-        rest = torch.arange(P, device="cuda") != 33
-        assert torch.isnan(got[0][33]) and torch.equal(got[0][rest], want[0][rest]) and torch.equal(got[2][rest], want[2][rest])
+    x2, y2 = x.clone(), y.clone()
+    x2[:3], x2[3:6], x2[6:9] = math.nan, math.inf, torch.finfo(dtype).min
+    y2[:9] = 12                                 # ignored rows hold anything; the ignored label may be a word's
+    y2[9:][y2[9:] == 12] = 13
+    got, want = step(x2, y2, 12), step(x, torch.where(row < 9, IGN, y2))
+    assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(got, want))
+    assert (got[0][:9] == 0).all() and (got[1][:9] == 0).all() and (got[2][:9] == 0).all()
+    none = step(x, torch.full_like(y, IGN))     # nothing left
+    assert all((t == 0).all() for t in none)
+    for bad in (V, -1, 1 << 40):                # a label that no word has
+        y3 = y.clone()
+        y3[11] = bad
+        got = step(x, y3)
+        assert torch.isnan(got[0][11]) and torch.isfinite(got[0][row != 11]).all() and torch.isfinite(got[1]).all()
+        assert torch.isnan(got[2][11]).all() and torch.isfinite(got[2][row != 11]).all() and torch.isnan(got[3]).all()
+    x4 = x.clone()
+    x4[P - 3, 1] = math.nan                     # a row that is not finite
+    got, want, rest = step(x4, y), step(x, y), row != P - 3
+    assert torch.isnan(got[0][P - 3]) and torch.equal(got[0][rest], want[0][rest]) and torch.equal(got[2][rest], want[2][rest])
 
 
 @pytest.mark.gpu
