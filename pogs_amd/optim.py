@@ -26,7 +26,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .rendering import _call, _on, _stream
+from .rendering import _call, _on, _raw_stream
 
 
 _ADAM_GROUP = struct.Struct("=4Q2q4d")     # pr_adam_group
@@ -113,7 +113,7 @@ def grad_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) 
         at, n = _address(table), len(flat)
         nbytes = lib.pr_grad_norm_scratch_bytes(at, n, 1)
         scratch, norm = _norm_buffers(nbytes, (), dev)
-        _call("pr_grad_norm", at, n, 1, kind, scratch.data_ptr(), nbytes, norm.data_ptr(), _stream())
+        _call("pr_grad_norm", at, n, 1, kind, scratch.data_ptr(), nbytes, norm.data_ptr(), _raw_stream(dev.index))
     return norm
 
 
@@ -147,7 +147,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
         at, n = _address(table), len(flat)
         nbytes = lib.pr_grad_norm_scratch_bytes(at, n, 1)
         scratch, norm = _norm_buffers(nbytes, (), dev)
-        _call("pr_grad_clip", at, n, 1, kind, ctypes.addressof(limit), scratch.data_ptr(), nbytes, norm.data_ptr(), _stream())
+        _call("pr_grad_clip", at, n, 1, kind, ctypes.addressof(limit), scratch.data_ptr(), nbytes, norm.data_ptr(), _raw_stream(dev.index))
         torch.autograd.graph.increment_version(flat)     # written in place, as far as autograd is concerned too
         if flat is not grads:
             with torch.no_grad():
@@ -277,9 +277,9 @@ class Optimizers:
                 chunk = _lib.load().pr_adam_max_groups()
                 for i in range(0, len(entries), chunk):
                     part = entries[i:i + chunk]
-                    _call("pr_adam_step", b"".join(part), len(part), _stream())
+                    _call("pr_adam_step", b"".join(part), len(part), _raw_stream(dev.index))
             else:
-                self._step_clipped(entries, rules, param_groups, dev, _stream())
+                self._step_clipped(entries, rules, param_groups, dev, _raw_stream(dev.index))
         del keep
 
     def _check_clipped(self, param_groups: List[str], limits: list) -> List[Optional[float]]:

@@ -36,11 +36,15 @@ def _stream():
 
 
 _HERE = contextlib.nullcontext()
+# The same without torch.cuda's Python around it, which takes 10 us and more on an autograd thread; there is a device by
+# the time they are called, and torch.cuda itself if a build lacks them.
+_raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _on(device: torch.device):
     """Context in which ``device`` is the current one: nothing to do where it already is (the change costs 3 us)."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if _raw_device() == device.index else torch.cuda.device(device)
 
 
 class StageTimer:

@@ -18,7 +18,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .rendering import _call, _on, _ptr, _stream
+from .rendering import _call, _on, _ptr, _raw_stream
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # PR_F32, PR_F16, PR_BF16
 _REDUCTIONS = ("none", "sum", "mean")
@@ -80,7 +80,7 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
             with _on(dev):
                 _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(w), *(w.stride() if w is not None else (0, 0)), _ptr(labels), ignore_index, scale, int(reduction == "mean"),
                       int(reduction == "none"), _ptr(kept), kept.numel(), _ptr(g_loss), _ptr(g_lse), _ptr(scratch),
-                      scratch.numel(), _ptr(dx), _ptr(dw), _stream())
+                      scratch.numel(), _ptr(dx), _ptr(dw), _raw_stream(dev.index))
         return (dx, dw) + (None,) * 6
 
 
@@ -148,7 +148,7 @@ def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tenso
     flat = labels if labels.dim() == 1 else labels.reshape(-1)
     if flat.dtype != torch.int64 or not flat.is_contiguous():
         flat = flat.to(torch.int64).contiguous()
-    stream = torch.cuda.current_stream(x.device).cuda_stream
+    stream = _raw_stream(x.device.index)
     args = x, vocabulary, flat, scale, int(ignore_index), reduction, return_lse
     if torch.is_grad_enabled() and (x.requires_grad or vocabulary.requires_grad):
         loss, lse = _VocabularyCrossEntropy.apply(*args, stream)
