@@ -310,23 +310,30 @@ struct CoefJob {
     ra = rb + (g_lse ? g_lse[p] : 0.f);
     if (g_loss && (labels[p] < 0 || labels[p] >= V)) ra = NAN;   // no such word: the row's loss is NaN
   }
+  // the loss's gradient of every row, where it is one for all
+  __device__ __forceinline__ float one() const {
+    return g_loss && !per_row ? *g_loss * (mean ? 1.f / s->n_valid : 1.f) : 0.f;
+  }
+  __device__ __forceinline__ void largest(int64_t p, float one, float &top) const {
+    float ra, rb;
+    row(p, one, ra, rb);
+    ra = fabsf(ra), rb = fabsf(rb);
+    if (ra < INFINITY) top = fmaxf(top, ra);
+    if (rb < INFINITY) top = fmaxf(top, rb);
+  }
 };
+// Brings the largest factor to 2^12..2^13 (|G| <= |a| + |b|).
+__device__ __forceinline__ int coef_exponent(float top) { return top > 0.f ? TOP_EXP - 1 - ilogbf(top) : 0; }
 
 constexpr int COEF_ROWS = 4096;  // rows whose factors one workgroup writes
 
-// Row factors of G, scaled by the power of two that brings the largest to 2^12..2^13 (|G| <= |a| + |b|).  Every
-// workgroup looks for the largest itself; with one gradient for all rows there is nothing to look for.
+// Row factors of G, scaled by coef_exponent.  Every workgroup looks for the largest itself; with one gradient for all rows
+// there is nothing to look for.
 __device__ __forceinline__ void row_factors(const CoefJob &c, int block) {
-  const float one = c.g_loss && !c.per_row ? *c.g_loss * (c.mean ? 1.f / c.s->n_valid : 1.f) : 0.f;
+  const float one = c.one();
   float top = fabsf(one) < INFINITY ? fabsf(one) : 0.f;
   if (c.per_row || c.g_lse) {
-    for (int64_t p = threadIdx.x; p < c.P; p += 1024) {
-      float a, b;
-      c.row(p, one, a, b);
-      a = fabsf(a), b = fabsf(b);
-      if (a < INFINITY) top = fmaxf(top, a);
-      if (b < INFINITY) top = fmaxf(top, b);
-    }
+    for (int64_t p = threadIdx.x; p < c.P; p += 1024) c.largest(p, one, top);
     __shared__ float part[16];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -335,7 +342,7 @@ __device__ __forceinline__ void row_factors(const CoefJob &c, int block) {
     top = part[0];
     for (int i = 1; i < 16; ++i) top = fmaxf(top, part[i]);
   }
-  const int e = top > 0.f ? TOP_EXP - 1 - ilogbf(top) : 0;
+  const int e = coef_exponent(top);
   if (block == 0 && threadIdx.x == 0) *c.exp_g = e;
   const int64_t end = min((int64_t)(block + 1) * COEF_ROWS, c.Pp);
   for (int64_t p = (int64_t)block * COEF_ROWS + threadIdx.x; p < end; p += 1024) {
@@ -1134,19 +1141,29 @@ template <>
 constexpr bool FEW_SCALED<_Float16> = true;
 
 struct FewGrad {  // what G is made of
-  int64_t P, V, D, Dk;
-  const int64_t *labels;
-  const float *lse2, *coef_a, *coef_b, *logits;
-  const int *exp_g;
-  // row p as {lse2, a, b, label's bits}
+  CoefJob c;      // P, V, labels, upstream gradients; exp_g: where DX leaves it for FINISH
+  int64_t D, Dk;
+  const float *lse2, *logits;
+  // Row p as {lse2, a, b, label's bits}, made by every workgroup for itself (256 threads; a launch would cost more).  Returns
+  // the power of two that a and b are scaled by.
   template <typename T>
-  __device__ __forceinline__ void rows(float4 *to, int n) const {
-    const int e = FEW_SCALED<T> ? 0 : -*exp_g;
-    for (int p = threadIdx.x; p < n; p += blockDim.x) {
-      const int64_t label = p < P ? labels[p] : -1;
-      to[p] = make_float4(p < P ? lse2[p] : 0.f, ldexpf(coef_a[p], e), ldexpf(coef_b[p], e),
-                          __builtin_bit_cast(float, label >= 0 && label < V ? (int)label : -1));
+  __device__ __forceinline__ int rows(float4 *to, int n) const {
+    const float one = c.one();
+    int e = 0;
+    if (FEW_SCALED<T>) {
+      float top = 0.f;
+      for (int p = threadIdx.x; p < c.P; p += 256) c.largest(p, one, top);
+      top = block_max(top);
+      e = coef_exponent(top);
     }
+    for (int p = threadIdx.x; p < n; p += 256) {
+      float a, b;
+      c.row(p, one, a, b);
+      const int64_t label = p < c.P ? c.labels[p] : -1;
+      to[p] = make_float4(p < c.P ? lse2[p] : 0.f, ldexpf(a, e), ldexpf(b, e),
+                          __builtin_bit_cast(float, label >= 0 && label < c.V ? (int)label : -1));
+    }
+    return e;
   }
   static __device__ __forceinline__ float entry(float z, const float4 &row, int word) {
     const float g = row.y * __builtin_amdgcn_exp2f(z - row.x);
@@ -1178,9 +1195,9 @@ __global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, con
   };
   fill(blockIdx.y, 0);
   if (blockIdx.y + gridDim.y < chunks) fill(blockIdx.y + gridDim.y, 1);
-  f.rows<T>(rows, 32 * NB);
+  const int e = -f.rows<T>(rows, 32 * NB);
   __syncthreads();
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave, at = min(t, (f.V - 1) / 32);   // (past the end: not stored)
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave, at = min(t, (f.c.V - 1) / 32);   // (past the end: not stored)
   GradOperand<T> ga[KB];
   const float *z = f.logits + at * (1024 * NB) + 256 * h + (lane & 31);
   float v[KB][8];
@@ -1198,8 +1215,7 @@ __global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, con
     for (int k = 0; k < GradOperand<T>::N; ++k) asm volatile("" : "+v"(ga[b].piece[k])::"memory");
     __builtin_amdgcn_sched_barrier(0);
   }
-  const int e = FEW_SCALED<T> ? -*f.exp_g : 0;
-  const bool whole = t * 32 + 32 <= f.V;
+  const bool whole = t * 32 + 32 <= f.c.V;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
   int buf = 0;
@@ -1232,7 +1248,7 @@ __global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, con
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int v = (r & 3) + 8 * (r >> 2);
-      if (!whole && t * 32 + 4 * h + v >= f.V) continue;
+      if (!whole && t * 32 + 4 * h + v >= f.c.V) continue;
       if constexpr (NT == 1) {
         dst[v * f.D] = (acc[0][r] + acc[1][r]) * scale;
       } else {
@@ -1257,10 +1273,11 @@ __global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Mat
   constexpr bool PAIRS = sizeof(T) == 2;
   __shared__ float4 rows[R];
   __shared__ u4v g[2][2 * NB][G::N][64];
-  f.rows<T>(rows, R);
+  const int e = f.rows<T>(rows, R);
+  if (FEW_SCALED<T> && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *f.c.exp_g = e;
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int64_t lo = blockIdx.y * steps, hi = min(lo + steps, (f.V + 31) / 32);
+  const int64_t lo = blockIdx.y * steps, hi = min(lo + steps, (f.c.V + 31) / 32);
   const int64_t c0 = (int64_t)blockIdx.x * 256 + 64 * wave;
   const bool active = c0 < f.D;
   // this lane's two columns; the last ones again past the end
@@ -1274,7 +1291,7 @@ __global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Mat
   auto load = [&](int64_t step, int kb, Raw &raw) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const T *src = (const T *)w.data + min(step * 32 + 16 * kb + 8 * h + i, f.V - 1) * w.ld_row;
+      const T *src = (const T *)w.data + min(step * 32 + 16 * kb + 8 * h + i, f.c.V - 1) * w.ld_row;
       if constexpr (!PAIRS) {
         raw.a[i] = __builtin_bit_cast(unsigned, src[at0 * w.ld_col]), raw.b[i] = __builtin_bit_cast(unsigned, src[at1 * w.ld_col]);
       } else if constexpr (WIDE) {
@@ -1323,11 +1340,11 @@ __global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Mat
         const float4 row = rows[32 * (task >> 1) + (lane & 31)];
         const float v[8] = {z.a[k].x, z.a[k].y, z.a[k].z, z.a[k].w, z.b[k].x, z.b[k].y, z.b[k].z, z.b[k].w};
         const int word = (int)step * 32 + 16 * (task & 1) + 8 * h;
-        float e[8];
+        float entry[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = word + i < f.V ? FewGrad::entry(v[i], row, word + i) : 0.f;
+        for (int i = 0; i < 8; ++i) entry[i] = word + i < f.c.V ? FewGrad::entry(v[i], row, word + i) : 0.f;
         G o;
-        o.set(e);
+        o.set(entry);
         store_operand(o, &g[buf][task][0][lane]);
       }
     }
@@ -1401,7 +1418,7 @@ __global__ void __launch_bounds__(1024) vce_few_finish_kernel(const FewGrad f, i
     const float4 q = part[k][lane];
     v.x += q.x, v.y += q.y, v.z += q.z, v.w += q.w;
   }
-  const int e = FEW_SCALED<T> ? -*f.exp_g : 0;
+  const int e = FEW_SCALED<T> ? -*f.c.exp_g : 0;
   const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -1493,6 +1510,32 @@ __global__ void __launch_bounds__(1024) vce_reduce_kernel(int64_t P, const float
   n = block_sum(n);
   if (threadIdx.x != 0) return;
   if (s) s->n_valid = (float)n;
+  *loss = (float)(mean ? sum / n : sum);
+}
+
+// Both for few rows, [row][pair]: a wavefront takes a row at a time, one workgroup all of them.
+__global__ void __launch_bounds__(1024) vce_join_reduce_kernel(RowsOut o, int pairs, const float2 *__restrict__ partial,
+                                                               int mean, float *__restrict__ loss, Scalars *sc) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t p = threadIdx.x >> 6; p < o.P; p += 16) {
+    const float2 *src = partial + p * pairs;
+    float m = MAX_FLOOR, s = 0.f;
+#pragma unroll 8
+    for (int j = lane; j < pairs; j += 64) merge(m, s, src[j].x, src[j].y);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) merge(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
+    if (lane == 0) finish_row(o, p, m, s);
+  }
+  __syncthreads();
+  double sum = 0., n = 0.;
+  for (int64_t p = threadIdx.x; p < o.P; p += 1024) {
+    sum += (double)o.row_loss[p];
+    n += o.labels[p] != o.ignore ? 1. : 0.;
+  }
+  sum = block_sum(sum);
+  n = block_sum(n);
+  if (threadIdx.x != 0) return;
+  if (sc) sc->n_valid = (float)n;
   *loss = (float)(mean ? sum / n : sum);
 }
 
@@ -1846,6 +1889,12 @@ int score(const Call &c, int mean, ScoreScratch &f, FewKept *k, float *row_loss,
   else if (s.nb == 2) PR_TRY((launch_score<T, 2>(c, s, f, k, st)));
   else PR_TRY((launch_score<T, 4>(c, s, f, k, st)));
   const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k ? k->lse2 : nullptr, lse, row_loss};
+  // (one workgroup for all rows: up to 32 no slower than two launches; 128 rows of 8000 words 15 us slower)
+  if (loss && s.nb == 1) {
+    hipLaunchKernelGGL(vce_join_reduce_kernel, dim3(1), dim3(1024), 0, st, rows, f.blocks, f.partial, mean, loss,
+                       k ? k->scal : nullptr);
+    return check_launch("pr_vocab_ce");
+  }
   hipLaunchKernelGGL(vce_join_row_kernel, dim3((unsigned)c.P), dim3(256), 0, st, rows, f.blocks, f.partial);
   PR_TRY(check_launch("pr_vocab_ce"));
   if (!loss) return PR_OK;
@@ -1856,7 +1905,7 @@ int score(const Call &c, int mean, ScoreScratch &f, FewKept *k, float *row_loss,
 
 struct FewBwdScratch {
   int *exp_g;
-  float *coef_a, *coef_b, *acc;
+  float *acc;
   int64_t steps;   // of 32 words, in a run of DX
   int splits;
   FewBwdScratch(Carve &c, const FewShape &s, bool dx) {
@@ -1864,8 +1913,6 @@ struct FewBwdScratch {
     steps = (s.tiles + want - 1) / want;
     splits = (int)((s.tiles + steps - 1) / steps);
     exp_g = c.take<int>(1);
-    coef_a = c.take<float>(s.R);
-    coef_b = c.take<float>(s.R);
     acc = c.take<float>(dx ? splits * s.R * s.Dk : 0);
   }
 };
@@ -1901,10 +1948,8 @@ template <typename T>
 int few_backward(const Call &c, int per_row, int mean, const FewKept &k, const FewBwdScratch &b, const float *g_loss,
                  const float *g_lse, T *dx, T *dw, hipStream_t st) {
   const FewShape s(c.dtype, c.P, c.V, c.D);
-  const CoefJob coef{c.P, s.R, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, b.exp_g, b.coef_a, b.coef_b};
-  hipLaunchKernelGGL(vce_prepare_kernel, dim3(1), dim3(1024), 0, st, coef, TransposeJob{}, TransposeJob{}, 0);
-  PR_TRY(check_launch("pr_vocab_ce"));
-  const FewGrad f{c.P, c.V, c.D, s.Dk, c.labels, k.lse2, b.coef_a, b.coef_b, k.logits, b.exp_g};
+  const FewGrad f{{c.P, s.R, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, b.exp_g, nullptr, nullptr},
+                  c.D, s.Dk, k.lse2, k.logits};
   if (s.nb == 1) return few_gradients<T, 1>(c, s, k, b, f, dx, dw, st);
   if (s.nb == 2) return few_gradients<T, 2>(c, s, k, b, f, dx, dw, st);
   return few_gradients<T, 4>(c, s, k, b, f, dx, dw, st);
