@@ -481,7 +481,7 @@ int pr_densify_split_children(int64_t n_out, const int32_t *map_src, const int32
 /* ---- softmax cross entropy over a large vocabulary of embeddings ------------------------------------------------
  * For feature rows x[P,D] (the clip head's outputs, pogs/fields/gaussian_field.py:194-204) and embeddings w[V,D] of the
  * same type (PR_F32, PR_F16, PR_BF16; any strides, in elements): z = scale <x_p, w_v>, lse_p = log sum_v exp z_pv,
- * row_loss_p = lse_p - z_p,label; logits and gradients of logits are never held for more than a piece of the vocabulary.
+ * row_loss_p = lse_p - z_p,label; but for few rows, logits and their gradients are never held for more than a piece of it.
  * The reference has no such loss; this is torch.nn.functional.cross_entropy(scale * x @ w.T, labels) and its gradients.
  * A row whose label is ignore_index has row_loss 0, lse 0 and no gradient, whatever its features hold; any other label
  * outside 0..V-1 makes the row's loss NaN and, through it, its gradients.
@@ -494,8 +494,8 @@ int pr_densify_split_children(int64_t n_out, const int32_t *map_src, const int32
  * gradient g_loss of row_loss (per_row != 0: [P]) or of loss (one value) and g_lse[P] of lse; a NULL one is 0.  kept is
  * read only: several calls may share it.  Where pr_vocab_ce_keeps_vocabulary is 0 (few rows, a large vocabulary) kept holds
  * the logits and no copy of w: the backward pass reads the same w again for dx, which must not have changed; elsewhere its w
- * is not looked at.  Products take float16 operands (float32 input: two planes, 2^-22) and add in
- * float32; sums run in a fixed order, so equal inputs give equal bits. */
+ * is not looked at.  Products take 16-bit operands (float32 input: two float16 planes or three bfloat16 pieces, 2^-21) and
+ * add in float32; sums run in a fixed order, so equal inputs give equal bits. */
 int pr_vocab_ce_score_rows(void);
 int pr_vocab_ce_keeps_vocabulary(int64_t P, int64_t V, int64_t D);
 size_t pr_vocab_ce_kept_bytes(int dtype, int64_t P, int64_t V, int64_t D);

@@ -1,4 +1,4 @@
-// Softmax cross entropy of feature rows over a large vocabulary of embeddings, without keeping the logits
+// Softmax cross entropy of feature rows over a large vocabulary of embeddings, without keeping the logits but for few rows
 // (pr_vocab_ce_fwd / pr_vocab_ce_bwd).
 //
 //   z_pv  = scale <x_p, w_v>          p < P rows, v < V words, contraction over D features
@@ -6,7 +6,7 @@
 //   with upstream gradients u_p of loss_p and l_p of lse_p, a_p = u_p + l_p, b_p = u_p:
 //   G_pv  = a_p exp(z_pv - lse_p) - b_p [v = label(p)],   dX = scale G W,   dW = scale G^T X
 //
-// All products run on the matrix cores as v_mfma_f32_32x32x16_f16 with float32 accumulators.  Operands are packed once
+// Few rows have kernels of their own (below).  All other products run on the matrix cores as v_mfma_f32_32x32x16_f16 with float32 accumulators.  Operands are packed once
 // per call into fragment order, 1 KB blocks [32 rows][16 of the contraction] with lane l's eight values consecutive, so
 // that a block moves memory -> LDS by one direct 16-byte-a-lane load and LDS -> registers by one conflict-free
 // ds_read_b128.  Packing scales each tensor by one power of two that brings its largest magnitude to 2^13..2^14: a

@@ -4,9 +4,10 @@ What the clip head's unit features (``FieldHeads.get_clip_outputs_from_feature``
 are trained and scored on when every pixel has a label in a table of phrase embeddings.  The value and the gradients of
 ``torch.nn.functional.cross_entropy(scale * features @ vocabulary.T, labels)``, without the ``[rows, words]`` logits: the
 forward pass keeps one maximum and sum a row, the backward pass makes the products again for one piece of the vocabulary
-at a time.  (Up to 128 rows of a large vocabulary do keep them for it, 4 bytes each, and read the vocabulary as it is.)  Products take 16-bit operands and add in float32; float32 inputs are split into two
-float16 planes or three bfloat16 pieces (2^-21 of a product at most is left out), so float32 stays float32 in accuracy.  Results do not depend on the order in which
-workgroups run.  HIP kernels only (``pr_vocab_ce_fwd``, ``pr_vocab_ce_bwd``); there is no CPU path.
+at a time.  (Up to 128 rows of a large vocabulary do keep them for it, 4 bytes each, and read the vocabulary as it is.)
+Products take 16-bit operands and add in float32; float32 inputs are split into two float16 planes or three bfloat16 pieces
+(2^-21 of a product at most is left out), so float32 stays float32 in accuracy.  Results do not depend on the order in
+which workgroups run.  HIP kernels only (``pr_vocab_ce_fwd``, ``pr_vocab_ce_bwd``); there is no CPU path.
 """
 from __future__ import annotations
 
