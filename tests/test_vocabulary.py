@@ -494,6 +494,24 @@ def test_few_rows_what_is_masked_or_not_finite(P, V, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("P,V", [(40, 20_000), (20, 40_000), (100, 40_000)])
+@pytest.mark.parametrize("exp_x,exp_w", [(90, -90), (-90, 90), (-60, 0), (0, 60), (-50, -50)])
+def test_few_rows_magnitudes(exp_x, exp_w, P, V):
+    """Nothing is scaled, and a power of two changes no bit of a piece or a product: the same bits as at 1."""
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    x, w, y = inputs(P, V, 32, torch.float32, seed=8)
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    xs, ws = (x * 2.0 ** exp_x).requires_grad_(True), (w * 2.0 ** exp_w).requires_grad_(True)
+    base = vocabulary_cross_entropy(a, b, y, reduction="none", return_lse=True)
+    loss = vocabulary_cross_entropy(xs, ws, y, scale=2.0 ** -(exp_x + exp_w), reduction="none", return_lse=True)
+    assert torch.equal(loss[0], base[0]) and torch.equal(loss[1], base[1])
+    want = torch.autograd.grad(base[0].sum(), (a, b))
+    for got, ref, e in zip(torch.autograd.grad(loss[0].sum(), (xs, ws)), want, (exp_x, exp_w)):
+        assert torch.equal(got * 2.0 ** e, ref)
+
+
+@pytest.mark.gpu
 def test_few_rows_in_a_graph_and_a_vocabulary_that_changes():
     from pogs_amd.vocabulary import vocabulary_cross_entropy
 
