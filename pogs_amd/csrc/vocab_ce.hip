@@ -54,7 +54,7 @@ constexpr float MAX_FLOOR = -3.0e38f;  // a maximum over nothing: exp2 of anythi
 constexpr float LN2F = 0.69314718055994531f;
 // The kernels for few rows read the vocabulary once for the scores and once for dX, where the packed path reads it three
 // times and writes it twice before its products; they multiply 32, 64 or 128 rows, whatever there are.  131072 words x 1024
-// dims, loss and both gradients: 1 row 455 against 1355 us (bfloat16 221 against 720), 128 rows 654 against 1398 (324
+// dims, loss and both gradients: 1 row 465 against 1355 us (bfloat16 223 against 720), 128 rows 660 against 1398 (322
 // against 739); loss alone, 128 rows: 203 against 466 (71 against 252).  256 rows would be two such passes, which is what
 // the packed path takes for them (1419 and 728 us with gradients).
 constexpr int FEW_ROWS = 128;
@@ -64,7 +64,7 @@ constexpr int64_t FEW_VOCABULARY = 1 << 19;
 constexpr int SCORE_ROWS = 64;      // rows that they take from any vocabulary where no backward pass follows
 constexpr int SCORE_BLOCKS = 1024;  // workgroups of the score kernel: four per CU
 // Workgroups of the others, where there is work for so many: two per CU.  (One row to 128 of 131072 words x 1024 dims,
-// bfloat16, loss and gradients: 221 to 324 us; 256 workgroups 267 to 386, 1024 workgroups 223 to 359.)
+// bfloat16, loss and gradients: 223 to 322 us; 256 workgroups 267 to 386, 1024 workgroups 223 to 359.)
 constexpr int FEW_BLOCKS = 512;
 constexpr int AMAX_BLOCKS = 1024;  // partial maxima per tensor at most
 
