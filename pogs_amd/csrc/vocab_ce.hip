@@ -6,10 +6,10 @@
 //   with upstream gradients u_p of loss_p and l_p of lse_p, a_p = u_p + l_p, b_p = u_p:
 //   G_pv  = a_p exp(z_pv - lse_p) - b_p [v = label(p)],   dX = scale G W,   dW = scale G^T X
 //
-// Few rows have kernels of their own (below).  All other products run on the matrix cores as v_mfma_f32_32x32x16_f16 with float32 accumulators.  Operands are packed once
-// per call into fragment order, 1 KB blocks [32 rows][16 of the contraction] with lane l's eight values consecutive, so
-// that a block moves memory -> LDS by one direct 16-byte-a-lane load and LDS -> registers by one conflict-free
-// ds_read_b128.  Packing scales each tensor by one power of two that brings its largest magnitude to 2^13..2^14: a
+// Few rows have kernels of their own (below).  All other products run on the matrix cores as v_mfma_f32_32x32x16_f16 with
+// float32 accumulators.  Operands are packed once per call into fragment order, 1 KB blocks [32 rows][16 of the
+// contraction] with lane l's eight values consecutive, so that a block moves memory -> LDS by one direct 16-byte-a-lane load
+// and LDS -> registers by one conflict-free ds_read_b128.  Packing scales each tensor by one power of two that brings its largest magnitude to 2^13..2^14: a
 // bfloat16 value keeps all its bits down to 2^-31 of the largest, and a float32 value becomes two float16 planes (head
 // and residual, 22 bits down to 2^-15 of the largest) whose products head*head + head*residual + residual*head lose 2^-22.
 // float16 input is packed as it is.  X takes the scale's sign.  Values that are not finite stay so; rows with the ignored
@@ -1267,7 +1267,8 @@ __global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, con
 
 // WIDE (unit column stride, two columns at least): a lane's two 16-bit columns by one access.
 template <typename T, int NB, bool WIDE>
-__global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Matrix w, int64_t steps, float *__restrict__ acc_out) {
+__global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Matrix w, int64_t steps,
+                                                            float *__restrict__ acc_out) {
   typedef GradOperand<T> G;
   constexpr int R = 32 * NB, TASKS = (2 * NB + 3) / 4;     // (16 words, 32 rows) tiles of G for each wavefront
   constexpr bool PAIRS = sizeof(T) == 2;
@@ -1293,11 +1294,13 @@ __global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Mat
     for (int i = 0; i < 8; ++i) {
       const T *src = (const T *)w.data + min(step * 32 + 16 * kb + 8 * h + i, f.c.V - 1) * w.ld_row;
       if constexpr (!PAIRS) {
-        raw.a[i] = __builtin_bit_cast(unsigned, src[at0 * w.ld_col]), raw.b[i] = __builtin_bit_cast(unsigned, src[at1 * w.ld_col]);
+        raw.a[i] = __builtin_bit_cast(unsigned, src[at0 * w.ld_col]);
+        raw.b[i] = __builtin_bit_cast(unsigned, src[at1 * w.ld_col]);
       } else if constexpr (WIDE) {
         raw.a[i] = *reinterpret_cast<const u1_at *>(src + at0) >> shift;
       } else {
-        raw.a[i] = __builtin_bit_cast(unsigned short, src[at0 * w.ld_col]), raw.b[i] = __builtin_bit_cast(unsigned short, src[at1 * w.ld_col]);
+        raw.a[i] = __builtin_bit_cast(unsigned short, src[at0 * w.ld_col]);
+        raw.b[i] = __builtin_bit_cast(unsigned short, src[at1 * w.ld_col]);
       }
     }
   };

@@ -113,7 +113,8 @@ def grad_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) 
         at, n = _address(table), len(flat)
         nbytes = lib.pr_grad_norm_scratch_bytes(at, n, 1)
         scratch, norm = _norm_buffers(nbytes, (), dev)
-        _call("pr_grad_norm", at, n, 1, kind, scratch.data_ptr(), nbytes, norm.data_ptr(), _raw_stream(dev.index))
+        _call("pr_grad_norm", at, n, 1, kind, scratch.data_ptr(), nbytes, norm.data_ptr(),
+              _raw_stream(dev.index))
     return norm
 
 
@@ -147,7 +148,8 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
         at, n = _address(table), len(flat)
         nbytes = lib.pr_grad_norm_scratch_bytes(at, n, 1)
         scratch, norm = _norm_buffers(nbytes, (), dev)
-        _call("pr_grad_clip", at, n, 1, kind, ctypes.addressof(limit), scratch.data_ptr(), nbytes, norm.data_ptr(), _raw_stream(dev.index))
+        _call("pr_grad_clip", at, n, 1, kind, ctypes.addressof(limit), scratch.data_ptr(), nbytes, norm.data_ptr(),
+              _raw_stream(dev.index))
         torch.autograd.graph.increment_version(flat)     # written in place, as far as autograd is concerned too
         if flat is not grads:
             with torch.no_grad():

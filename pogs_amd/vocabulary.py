@@ -58,8 +58,8 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
         ctx.args = x.shape, w.shape[0], x.dtype, scale, ignore_index, reduction
         loss, lse, kept = _forward(x, w, labels, scale, ignore_index, reduction, want_lse, True, stream)
         # kept has its own copy of the features and, but for few rows, of the vocabulary
-        reads = x.shape[0] > 0 and ctx.needs_input_grad[0] and not _lib.load().pr_vocab_ce_keeps_vocabulary(*x.shape[:1], *w.shape)
-        ctx.save_for_backward(labels, kept, w if reads else None)
+        again = kept is not None and ctx.needs_input_grad[0] and not _lib.load().pr_vocab_ce_keeps_vocabulary(len(x), *w.shape)
+        ctx.save_for_backward(labels, kept, w if again else None)
         return loss, lse
 
     @staticmethod
@@ -79,9 +79,9 @@ class _VocabularyCrossEntropy(torch.autograd.Function):
             lib, t = _lib.load(), _TYPES[dtype]
             scratch = _scratch(lib.pr_vocab_ce_bwd_scratch_bytes(t, P, V, D, int(want_x), int(want_w)), dev)
             with _on(dev):
-                _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(w), *(w.stride() if w is not None else (0, 0)), _ptr(labels), ignore_index, scale, int(reduction == "mean"),
-                      int(reduction == "none"), _ptr(kept), kept.numel(), _ptr(g_loss), _ptr(g_lse), _ptr(scratch),
-                      scratch.numel(), _ptr(dx), _ptr(dw), _raw_stream(dev.index))
+                _call("pr_vocab_ce_bwd", t, P, V, D, _ptr(w), *(w.stride() if w is not None else (0, 0)), _ptr(labels),
+                      ignore_index, scale, int(reduction == "mean"), int(reduction == "none"), _ptr(kept), kept.numel(),
+                      _ptr(g_loss), _ptr(g_lse), _ptr(scratch), scratch.numel(), _ptr(dx), _ptr(dw), _raw_stream(dev.index))
         return (dx, dw) + (None,) * 6
 
 
@@ -131,7 +131,7 @@ def _check(features: Tensor, vocabulary: Tensor, labels: Tensor, scale: float, r
 def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tensor, scale: float = 1.0,
                              ignore_index: int = -100, reduction: str = "mean",
                              return_lse: bool = False) -> Union[Tensor, Tuple[Tensor, Tensor]]:
-    """Cross entropy of ``scale * features @ vocabulary.T`` against ``labels``, logits never stored.
+    """Cross entropy of ``scale * features @ vocabulary.T`` against ``labels``, without the logits.
 
     ``features``: ``[..., D]`` and ``vocabulary``: ``[V, D]``, both float32, float16 or bfloat16, any strides;
     ``labels``: ``[...]`` int64 or int32.  Returns float32: the mean over the rows whose label is not ``ignore_index``
@@ -141,8 +141,9 @@ def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tenso
     twice).  Ignored rows contribute nothing, even if their features are not finite.  A label that is neither in
     ``0..V-1`` nor ``ignore_index`` makes its row's loss NaN and the gradients with it: nothing is read out of range,
     and the host does not wait to look.  Features may be changed in place before the backward pass, labels may not, and
-    neither may the vocabulary where it is large and the rows are at most 128 (autograd refuses).  Safe in a captured graph, gradients included, as long as no graph of the same
-    leaves made outside the capture is alive (refused where one of this function is)."""
+    neither may the vocabulary where it is large and the rows are at most 128 (autograd refuses).  Safe in a captured
+    graph, gradients included, as long as no graph of the same leaves made outside the capture is alive (refused where one
+    of this function is)."""
     scale = _check(features, vocabulary, labels, scale, reduction)
     D = features.shape[-1]
     x = features if features.dim() == 2 else features.reshape(-1, D)
