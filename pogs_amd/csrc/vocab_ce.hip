@@ -6,32 +6,39 @@
 //   with upstream gradients u_p of loss_p and l_p of lse_p, a_p = u_p + l_p, b_p = u_p:
 //   G_pv  = a_p exp(z_pv - lse_p) - b_p [v = label(p)],   dX = scale G W,   dW = scale G^T X
 //
-// Few rows have kernels of their own (below).  All other products run on the matrix cores as v_mfma_f32_32x32x16_f16 with
+// Few rows have kernels of their own (below).  All other products run on the matrix cores as v_mfma_f32_32x32x16 with
 // float32 accumulators.  Operands are packed once per call into fragment order, 1 KB blocks [32 rows][16 of the
 // contraction] with lane l's eight values consecutive, so that a block moves memory -> LDS by one direct 16-byte-a-lane load
-// and LDS -> registers by one conflict-free ds_read_b128.  Packing scales each tensor by one power of two that brings its largest magnitude to 2^13..2^14: a
+// and LDS -> registers by one conflict-free ds_read_b128.
+//
+// The logits' operands are float16.  Packing scales each tensor by one power of two that brings its largest magnitude to 2^13..2^14: a
 // bfloat16 value keeps all its bits down to 2^-31 of the largest, and a float32 value becomes two float16 planes (head
 // and residual, 22 bits down to 2^-15 of the largest) whose products head*head + head*residual + residual*head lose 2^-22.
 // float16 input is packed as it is.  X takes the scale's sign.  Values that are not finite stay so; rows with the ignored
 // label are packed as zeros, whatever they hold.
 //
+// The gradients' operands are bfloat16 pieces, which have float32's range: the entries of G go from the probability of a
+// word that nobody means to the largest row's weight, so a row's or a word's gradient would be lost under a common scale in
+// float16.  G is kept in two pieces (three for float32 input), to 2^-16 (2^-24) of each entry, below half a step of the
+// output's type, as one piece of 8 or 11 bits would not be: the label's entry carries most of a word's gradient, and its
+// rounding would show.  W and X are one piece (bfloat16), two (float16) or three (float32), which hold every bit of the packed
+// value, and two, three and six products of pieces are made.
+//
 // One product kernel with four epilogues:
 //   STATS  64 to 320 words x 256 rows: the row of X is on the lane, so the maximum and sum over the words are taken in
 //          registers; one (max, sum) pair per row and wavefront leaves, in the log2 domain
-//   GRAD   the same product again for a piece of the vocabulary, turned into G and rounded to float16 (two planes for
-//          float32), scaled by a power of two: 2^-11 of each entry, below the 2^-8 of a bfloat16 gradient and equal to that
-//          of a float16 one, and half a step of bfloat16 would be 2^-8 once more.  A lane's eight accumulators are eight
-//          consecutive slots of the contraction of dX = G W as they stand, if W's packed copy uses the same slot order; for
-//          dW = G^T X the tile is transposed by two products with the identity, which are exact
+//   GRAD   the same product again for a piece of the vocabulary, turned into the pieces of G.  A lane's eight accumulators
+//          are eight consecutive slots of the contraction of dX = G W as they stand, if W's packed copy uses the same slot
+//          order; for dW = G^T X the tile is transposed by two products with the identity, which are exact
 //   DX     partials of a gradient in float32, one plane per split of its contraction; dX's are added to over the pieces.
 //          Two such products may share a launch: dX's and, where dW has too few tiles for the chip, dW's
 //   DW     dW rows of the piece, contraction over all rows, written in the output type
-// G of one piece is all that is ever held of the P x V logits.
+// G of one piece of the vocabulary is all that is ever held of the P x V logits.
 //
 // Bound: the matrix cores, at the clock that the chip's power allows (1.75 to 1.8 GHz under these kernels, of 2.4).
-// 8192 rows x 131072 words x 1024 dims, bfloat16, loss and both gradients, 7.8 ms: STATS 1.83 ms (1200 TFLOP/s), and for
-// each of eight pieces GRAD 0.295 (930), DX 0.245 (1120), DW 0.221 (1245); largest magnitude 0.07, packing 0.11,
-// transposing 0.09.  A library product of 8192^3 float16 runs at 1415 on the same card.
+// 8192 rows x 131072 words x 1024 dims, bfloat16, loss and both gradients, 11.0 ms: STATS 1.76 ms (1250 TFLOP/s), and for
+// each of eight pieces GRAD 0.39 (700, with 1 GB of G to write), DX 0.40 and DW 0.38 (1380 and 1460, two products each);
+// largest magnitude 0.07, packing 0.11, transposing 0.09.  A library product of 8192^3 bfloat16 runs at 1290 on the same card.
 #include <math.h>
 
 #include <algorithm>
@@ -44,6 +51,7 @@ namespace {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 typedef unsigned u4v __attribute__((ext_vector_type(4)));
 
 constexpr int TILE_V = 256;  // words of the packed copies are padded to it
@@ -72,6 +80,57 @@ struct Matrix {  // rows x cols with any strides (elements)
   const void *data;
   int64_t rows, cols, ld_row, ld_col;
 };
+
+// Operands of a product A B^T as sums of NA and NB planes (or pieces) of type E.  Of the planes' products those are made
+// whose numbers add up to less than the larger count.
+template <typename E_, int NA_, int NB_>
+struct Form {
+  typedef E_ E;
+  typedef E_ E8 __attribute__((ext_vector_type(8)));
+  static constexpr int NA = NA_, NB = NB_, MOST = NA > NB ? NA : NB;
+  static constexpr int KB = MOST == 1 ? 2 : 1;   // 16-wide blocks of the contraction in a stage
+  static constexpr int PRODUCTS = NA == 1 || NB == 1 ? MOST : MOST * (MOST + 1) / 2;
+};
+template <typename T>
+struct Types {  // bfloat16
+  typedef Form<_Float16, 1, 1> Logits;
+  typedef Form<__bf16, 1, 2> Grads;
+};
+template <>
+struct Types<_Float16> {
+  typedef Form<_Float16, 1, 1> Logits;
+  typedef Form<__bf16, 2, 2> Grads;
+};
+template <>
+struct Types<float> {
+  typedef Form<_Float16, 2, 2> Logits;
+  typedef Form<__bf16, 3, 3> Grads;
+};
+
+__device__ __forceinline__ f16v mfma(h8v a, h8v b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f16v mfma(b8v a, b8v b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// v as N bfloat16 pieces, 8 bits of it each: all but the last by truncation, so that the largest values do not overflow, the
+// last one rounded.  Three hold all of a float32 value, two all of a float16 one and any other to 2^-16.
+template <int N>
+__device__ __forceinline__ void bf16_pieces(const float (&v)[8], b8v (&out)[N]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = v[i];
+#pragma unroll
+  for (int n = 0; n + 1 < N; ++n) {
+    u4v w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned a = __builtin_bit_cast(unsigned, r[2 * i]), b = __builtin_bit_cast(unsigned, r[2 * i + 1]);
+      w[i] = __builtin_amdgcn_perm(b, a, 0x07060302);   // the upper halves
+      r[2 * i] -= __builtin_bit_cast(float, a & 0xffff0000u), r[2 * i + 1] -= __builtin_bit_cast(float, b & 0xffff0000u);
+    }
+    out[n] = __builtin_bit_cast(b8v, w);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) out[N - 1][i] = (__bf16)r[i];
+}
 
 struct Scalars {  // per call, on the device
   int exp_x, exp_w;  // packed = value * 2^exp
@@ -260,10 +319,11 @@ struct TransposeJob {
   int64_t row_tiles, col_tiles;
 };
 
-// The packed copies for the contraction over rows, from those over columns: one 32x32 tile and plane per wavefront, as
-// two products with the identity.  Each value passes the matrix core as itself times one: exact.
-__device__ __forceinline__ void transpose_tiles(const TransposeJob &w, const TransposeJob &x, int planes, int64_t u,
-                                                int64_t step) {
+// The packed copies for the contraction over rows, from those over columns: one 32x32 tile per wavefront, every plane as two
+// products with the identity.  Each value passes the matrix core as itself times one and its planes add up to it: exact.
+template <typename T>
+__device__ __forceinline__ void transpose_tiles(const TransposeJob &w, const TransposeJob &x, int64_t u, int64_t step) {
+  constexpr int FROM = Types<T>::Logits::NA, TO = Types<T>::Grads::NA;
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const int64_t nw = w.row_tiles * w.col_tiles, nx = x.row_tiles * x.col_tiles;
   h8v ident[2];
@@ -271,26 +331,29 @@ __device__ __forceinline__ void transpose_tiles(const TransposeJob &w, const Tra
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int i = 0; i < 8; ++i) ident[s][i] = 16 * s + 8 * h + i == (lane & 31) ? (_Float16)1.f : (_Float16)0.f;
-  for (; u < (nw + nx) * planes; u += step) {
-    const int64_t pl = u >= nw + nx, v = pl ? u - (nw + nx) : u;
-    const bool first = v < nw;
+  for (; u < nw + nx; u += step) {
+    const bool first = u < nw;
     const TransposeJob &j = first ? w : x;
-    const unsigned q = (unsigned)(first ? v : v - nw), by = q / (unsigned)j.col_tiles;                 // tiles < 2^31
+    const unsigned q = (unsigned)(first ? u : u - nw), by = q / (unsigned)j.col_tiles;                 // tiles < 2^31
     const int64_t rt = by, ct = q - by * (unsigned)j.col_tiles;
-    const u4v *src = j.src + pl * j.plane + (rt * j.col_tiles + ct) * 128 + lane;
+    const u4v *src = j.src + (rt * j.col_tiles + ct) * 128 + lane;
     f16v tr;
 #pragma unroll
     for (int r = 0; r < 16; ++r) tr[r] = 0.f;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-      tr = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, src[s * 64]), ident[s], tr, 0, 0, 0);
-    u4v *dst = j.dst + pl * j.plane + (ct * j.row_tiles + rt) * 128 + lane;
+    for (int pl = 0; pl < FROM; ++pl)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) tr = mfma(__builtin_bit_cast(h8v, src[pl * j.plane + s * 64]), ident[s], tr);
+    u4v *dst = j.dst + (ct * j.row_tiles + rt) * 128 + lane;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      h8v o;
+      float v[8];
+      b8v o[TO];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = (_Float16)tr[8 * s + k];
-      dst[s * 64] = __builtin_bit_cast(u4v, o);
+      for (int k = 0; k < 8; ++k) v[k] = tr[8 * s + k];
+      bf16_pieces<TO>(v, o);
+#pragma unroll
+      for (int pl = 0; pl < TO; ++pl) dst[pl * j.plane + s * 64] = __builtin_bit_cast(u4v, o[pl]);
     }
   }
 }
@@ -355,19 +418,18 @@ __device__ __forceinline__ void row_factors(const CoefJob &c, int block) {
 
 // What the gradients' products need besides the packed operands, in one launch: the first workgroups write the row
 // factors, the others the transposed copies.
-__global__ void __launch_bounds__(1024) vce_prepare_kernel(CoefJob c, TransposeJob w, TransposeJob x, int planes) {
+template <typename T>
+__global__ void __launch_bounds__(1024) vce_prepare_kernel(CoefJob c, TransposeJob w, TransposeJob x) {
   const int coef_blocks = (int)((c.Pp + COEF_ROWS - 1) / COEF_ROWS);
   if ((int)blockIdx.x < coef_blocks) {
     row_factors(c, blockIdx.x);
     return;
   }
-  transpose_tiles(w, x, planes, (int64_t)(blockIdx.x - coef_blocks) * 16 + (threadIdx.x >> 6),
-                  (int64_t)(gridDim.x - coef_blocks) * 16);
+  transpose_tiles<T>(w, x, (int64_t)(blockIdx.x - coef_blocks) * 16 + (threadIdx.x >> 6),
+                     (int64_t)(gridDim.x - coef_blocks) * 16);
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------
-enum { STATS, GRAD, DX, DW };
-
 struct GemmArgs {
   const u4v *A, *B;            // operand blocks, already at the first block of the contraction
   int64_t plane_a, plane_b;    // 16-byte units between planes
@@ -406,17 +468,35 @@ __device__ __forceinline__ void store4(T *dst, float a, float b, float c, float 
   *reinterpret_cast<t4 *>(dst) = t4{(T)a, (T)b, (T)c, (T)d};
 }
 
+enum { STATS, GRAD, DX, DW };
+template <typename T, int MODE>
+struct FormOf {
+  typedef typename Types<T>::Grads F;
+};
+template <typename T>
+struct FormOf<T, STATS> {
+  typedef typename Types<T>::Logits F;
+};
+template <typename T>
+struct FormOf<T, GRAD> {
+  typedef typename Types<T>::Logits F;
+};
+template <typename F, int MT>
+constexpr int STAGE_BLOCKS = F::KB * (F::NA * 2 * MT + F::NB * 8);   // of 1 KB
+
 // Eight wavefronts, 2 x 4, of MT x 2 accumulator tiles each: 64 MT rows of A by 256 rows of B.  LDS holds three stages of
-// 16 (two planes) or 32 (one plane) of the contraction, filled by direct loads two stages ahead.  The wavefronts form two
+// 16 or (one plane each) 32 of the contraction, filled by direct loads two stages ahead.  The wavefronts form two
 // groups, one wavefront of each on every SIMD, that take turns between barriers: one reads its next stage from LDS while
 // the other multiplies.  One workgroup a CU, which takes tile after tile and starts the next one's loads before it turns
 // to the epilogue.
-template <int NP, int MT, int MODE, typename T>
+template <typename T, int MT, int MODE>
 __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, const GemmArgs g2) {
   extern __shared__ u4v lds[];
-  constexpr int WM = 2, WN = 4, NT = 2, WAVES = WM * WN, KB = NP == 1 ? 2 : 1;
-  constexpr int A_TILES = WM * MT, B_TILES = WN * NT;
-  constexpr int STAGE = (A_TILES + B_TILES) * 2, LOADS = (STAGE + WAVES - 1) / WAVES;
+  typedef typename FormOf<T, MODE>::F F;
+  typedef typename F::E8 E8;
+  constexpr int WM = 2, WN = 4, NT = 2, WAVES = WM * WN, KB = F::KB, NA = F::NA, NB = F::NB;
+  constexpr int A_TILES = WM * MT, B_TILES = WN * NT, A_BLOCKS = KB * NA * A_TILES;
+  constexpr int STAGE = STAGE_BLOCKS<F, MT>, LOADS = (STAGE + WAVES - 1) / WAVES;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
   const bool late = wave >= WAVES / 2;
@@ -431,7 +511,7 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
 
   int m_tile, n_tile, split, stages;
   bool other;             // DX: the tile is of the second product
-  const u4v *src[LOADS];  // this wavefront's blocks of a stage, ordered [half: k block or plane][tile] for A, then for B
+  const u4v *src[LOADS];  // this wavefront's blocks of a stage, ordered [k block][plane][tile] for A, then for B
   auto place = [&](unsigned t) {
     other = MODE == DX && t >= tiles1;
     if (other) t -= tiles1;
@@ -450,10 +530,9 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) {
       const int j = min(wave * LOADS + l, STAGE - 1);  // (a share past the end repeats the last block, into its own place)
-      const bool is_a = j < 2 * A_TILES;
-      const int q = is_a ? j : j - 2 * A_TILES, per = is_a ? A_TILES : B_TILES;
-      const int at = q % per, half = q / per;
-      const int kb = NP == 1 ? half : 0, plane = NP == 1 ? 0 : half;
+      const bool is_a = j < A_BLOCKS;
+      const int q = is_a ? j : j - A_BLOCKS, per = is_a ? A_TILES : B_TILES, planes = is_a ? NA : NB;
+      const int at = q % per, kb = q / per / planes, plane = q / per % planes;
       const int64_t row = is_a ? min(m_tile * A_TILES + at, a_tiles - 1) : min(n_tile * B_TILES + at, b_tiles - 1);
       const u4v *base = is_a ? A + plane * plane_a + row * ld_a * 64 : B + plane * plane_b + row * ld_b * 64;
       src[l] = base + ((int64_t)split * k_split + kb) * 64;
@@ -468,23 +547,33 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
     }
     asm volatile("" ::: "memory");   // fills stay in order: the waits below count on it
   };
-  struct Half {  // one k block, or one plane, of a stage
-    h8v a[MT], b[NT];
+  struct Block {  // of the contraction
+    E8 a[NA][MT], b[NB][NT];
   };
-  auto read = [&](int buf, int half, Half &f) {
-    const u4v *sa = lds + (buf * STAGE + half * A_TILES + wm * MT) * 64 + lane;
-    const u4v *sb = lds + (buf * STAGE + 2 * A_TILES + half * B_TILES + wn * NT) * 64 + lane;
+  auto read = [&](int buf, int kb, Block &f) {
+    const u4v *sa = lds + (buf * STAGE + kb * NA * A_TILES + wm * MT) * 64 + lane;
+    const u4v *sb = lds + (buf * STAGE + A_BLOCKS + kb * NB * B_TILES + wn * NT) * 64 + lane;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) f.b[n] = __builtin_bit_cast(h8v, sb[n * 64]);
+    for (int j = 0; j < NB; ++j)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) f.a[i] = __builtin_bit_cast(h8v, sa[i * 64]);
+      for (int n = 0; n < NT; ++n) f.b[j][n] = __builtin_bit_cast(E8, sb[(j * B_TILES + n) * 64]);
+#pragma unroll
+    for (int j = 0; j < NA; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) f.a[j][i] = __builtin_bit_cast(E8, sa[(j * A_TILES + i) * 64]);
   };
   f16v acc[MT][NT];
-  auto multiply = [&](const Half &fa, const Half &fb) {
+  auto multiply = [&](const Block &f) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int sum = 0; sum < F::MOST; ++sum)     // the sum of the planes' numbers; more would be left out
 #pragma unroll
-      for (int n = 0; n < NT; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa.a[i], fb.b[n], acc[i][n], 0, 0, 0);
+      for (int j = 0; j < NA && j <= sum; ++j)
+        if (sum - j < NB) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[i][n] = mfma(f.a[j][i], f.b[sum - j][n], acc[i][n]);
+        }
   };
   // Waits for all but the youngest fill of this wavefront (`more`: there is one) and for its own LDS reads; after the
   // barrier both hold for all wavefronts that have come to it.
@@ -524,9 +613,9 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
     if (late) __builtin_amdgcn_s_barrier();    // the second group is one barrier behind
     int buf = 0;
     for (int st = 0; st < stages; ++st) {
-      Half first, second;
-      read(buf, 0, first);
-      read(buf, 1, second);
+      Block f[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) read(buf, kb, f[kb]);
       // into the stage before this one: this group has read it two barriers ago, the other one barrier ago
       if (st + 2 < stages) fill(buf == 0 ? 2 : buf - 1);
       __builtin_amdgcn_sched_barrier(0);
@@ -535,13 +624,8 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
       arrive(st + 2 < stages);
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
-      multiply(first, first);
-      if (NP == 1) {
-        multiply(second, second);
-      } else {  // head by residual and residual by head; residual by residual is left out
-        multiply(second, first);
-        multiply(first, second);
-      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) multiply(f[kb]);
       __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_barrier();
@@ -612,54 +696,50 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
           if (h == 0) g.partial[(int64_t)(of_m * WM + wm) * g.Pp + p] = make_float2(top, sum);
         } else {
           const float l2 = lse2[n], ca = coef_a[n], cb = coef_b[n];
-          h8v ident[2];
+          constexpr int NG = Types<T>::Grads::NB;
+          b8v ident[2];
 #pragma unroll
           for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ident[s][i] = slot_place(s, h, i) == (lane & 31) ? (_Float16)1.f : (_Float16)0.f;
+            for (int i = 0; i < 8; ++i) ident[s][i] = slot_place(s, h, i) == (lane & 31) ? (__bf16)1.f : (__bf16)0.f;
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
-            float v[16];
+            float v[2][8];     // register r: slot r & 7 of step r >> 3
 #pragma unroll
-            for (int r = 0; r < 16; ++r) v[r] = ca * __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -l2));
+            for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = ca * __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -l2));
             if (here) {
 #pragma unroll
-              for (int r = 0; r < 16; ++r) v[r] -= at == 32 * i + (r & 3) + 8 * (r >> 2) ? cb : 0.f;
+              for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] -= at == 32 * i + (r & 3) + 8 * (r >> 2) ? cb : 0.f;
             }
             if (!whole) {
 #pragma unroll
               for (int r = 0; r < 16; ++r)
-                if (32 * i + (r & 3) + 8 * (r >> 2) >= left) v[r] = 0.f;
+                if (32 * i + (r & 3) + 8 * (r >> 2) >= left) v[r >> 3][r & 7] = 0.f;
             }
-            h8v f[NP][2];
+            b8v f[2][NG];
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                f[0][s][k] = (_Float16)v[8 * s + k];
-                if (NP == 2) f[NP - 1][s][k] = (_Float16)(v[8 * s + k] - (float)f[0][s][k]);
-              }
+            for (int s = 0; s < 2; ++s) bf16_pieces<NG>(v[s], f[s]);
             const int64_t pt = ((int64_t)of_n * WN + wn) * NT + n, vt = m0 / 32 + i;
             if (vt >= g.a_tiles) continue;     // past the piece
 #pragma unroll
-            for (int pl = 0; pl < NP; ++pl) {
+            for (int pl = 0; pl < NG; ++pl) {
               if (g.gx) {
                 u4v *dst = g.gx + pl * g.plane_gx + (pt * g.ld_gx + vt * 2) * 64 + lane;
 #pragma unroll
-                for (int s = 0; s < 2; ++s) dst[s * 64] = __builtin_bit_cast(u4v, f[pl][s]);
+                for (int s = 0; s < 2; ++s) dst[s * 64] = __builtin_bit_cast(u4v, f[s][pl]);
               }
               if (g.gw) {
                 f16v tr;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) tr[r] = 0.f;
 #pragma unroll
-                for (int s = 0; s < 2; ++s) tr = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[pl][s], ident[s], tr, 0, 0, 0);
+                for (int s = 0; s < 2; ++s) tr = mfma(f[s][pl], ident[s], tr);
                 u4v *dst = g.gw + pl * g.plane_gw + (vt * g.ld_gw + pt * 2) * 64 + lane;
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                  h8v o;
+                  b8v o;
 #pragma unroll
-                  for (int k = 0; k < 8; ++k) o[k] = (_Float16)tr[8 * s + k];
+                  for (int k = 0; k < 8; ++k) o[k] = (__bf16)tr[8 * s + k];
                   dst[s * 64] = __builtin_bit_cast(u4v, o);
                 }
               }
@@ -731,8 +811,6 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
 // 3.8 to 4.8 TB/s; bfloat16 53, 65 and 53 for 268 MB), the matrix cores and the conversions more and more from 64 rows on
 // (128 rows: float32 205, 262 and 258 us; bfloat16 70, 129 and 109).  After a DW its lines are still on their way out of
 // the cache, which a SCORE waits for (float32 213 us instead of 140).
-typedef __bf16 b8v __attribute__((ext_vector_type(8)));
-
 template <typename T>
 struct Operand;  // the pieces of eight consecutive values, ready for the matrix cores
 template <>
@@ -1586,10 +1664,17 @@ int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 struct Shape {
   int64_t P, V, D, Pp, Vp, Dk;
-  int np;
+  int np, na, ng;   // planes of the logits' operands; pieces of the gradients' operands and of G
   Shape(int dtype, int64_t P_, int64_t V_, int64_t D_)
-      : P(P_), V(V_), D(D_), Pp(round_up(P_, TILE_P)), Vp(round_up(V_, TILE_V)), Dk(round_up(D_, 32)),
-        np(dtype == PR_F32 ? 2 : 1) {}
+      : P(P_), V(V_), D(D_), Pp(round_up(P_, TILE_P)), Vp(round_up(V_, TILE_V)), Dk(round_up(D_, 32)) {
+    if (dtype == PR_F32) of<float>();
+    else if (dtype == PR_F16) of<_Float16>();
+    else of<__bf16>();
+  }
+  template <typename T>
+  void of() {
+    np = Types<T>::Logits::NA, na = Types<T>::Grads::NA, ng = Types<T>::Grads::NB;
+  }
   int64_t plane(int64_t rows) const { return rows * Dk / 8; }   // 16-byte units of one packed plane
 };
 
@@ -1625,7 +1710,7 @@ struct Kept {  // what the forward pass leaves for the backward pass
   }
 };
 
-int word_units(int np, int64_t words, int64_t rows);
+int word_units(int planes, int64_t words, int64_t rows);
 
 struct FwdScratch {
   float *amax, *target, *row_loss;
@@ -1641,9 +1726,9 @@ struct FwdScratch {
   }
 };
 
-// G of one piece of the vocabulary, all copies and planes (8192 rows x 16384 words x 1024 dims, both gradients: 770 us for
-// 512 MB, 960 for two halves, 825 as a half of 1 GB).
-constexpr int64_t PIECE_BYTES = 512ll << 20;
+// G of one piece of the vocabulary, all copies and pieces (bfloat16, 8192 rows x 131072 words x 1024 dims, loss and both
+// gradients: 11.0 ms with 1 GB, 11.9 with 512 MB).
+constexpr int64_t PIECE_BYTES = 1024ll << 20;
 
 // Splits of a contraction of `k` blocks, where its tiles alone are fewer than the CUs: as many, up to 16, as give each CU
 // a tile at most, of at least four blocks each.  Every split writes and reads a partial result of its own, which costs
@@ -1665,7 +1750,7 @@ struct BwdScratch {
   int64_t piece;  // words
   Splits split_words, split_rows;  // of the contractions of dX (a full piece's words) and of dW
   BwdScratch(Carve &c, const Shape &s, bool dx, bool dw) {
-    const int64_t per_word = s.Pp * 2 * s.np * (int(dx) + int(dw));
+    const int64_t per_word = s.Pp * 2 * s.ng * (int(dx) + int(dw));
     piece = std::min(s.Vp, std::max<int64_t>(PIECE_BYTES / per_word / TILE_V, 1) * TILE_V);
     const int64_t pieces = (s.Vp + piece - 1) / piece;
     piece = round_up((s.Vp + pieces - 1) / pieces, TILE_V);   // of equal size
@@ -1676,10 +1761,10 @@ struct BwdScratch {
     coef_b = c.take<float>(s.Pp);
     acc = c.take<float>(dx ? split_words.n * s.Pp * s.Dk : 0);
     acc_w = c.take<float>(dw && split_rows.n > 1 ? split_rows.n * piece * s.Dk : 0);
-    wt = c.take<u4v>(dx ? s.np * s.plane(s.Vp) : 0);
-    xt = c.take<u4v>(dw ? s.np * s.plane(s.Pp) : 0);
-    gx = c.take<u4v>(dx ? s.np * s.Pp * piece / 8 : 0);
-    gw = c.take<u4v>(dw ? s.np * s.Pp * piece / 8 : 0);
+    wt = c.take<u4v>(dx ? s.na * s.plane(s.Vp) : 0);
+    xt = c.take<u4v>(dw ? s.na * s.plane(s.Pp) : 0);
+    gx = c.take<u4v>(dx ? s.ng * s.Pp * piece / 8 : 0);
+    gw = c.take<u4v>(dw ? s.ng * s.Pp * piece / 8 : 0);
   }
 };
 
@@ -1703,9 +1788,9 @@ struct Product {
   int64_t m_rows, n_rows;  // multiples of 32 and of 256
 };
 
-template <int NP, int MT, int MODE, typename T>
+template <typename T, int MT, int MODE>
 int launch_tiles(const Product &a, const Product *b, hipStream_t st) {
-  const size_t bytes = (size_t)3 * (2 * MT + 8) * 2 * 1024;
+  const size_t bytes = (size_t)3 * STAGE_BLOCKS<typename FormOf<T, MODE>::F, MT> * 1024;
   auto cut = [](const Product &p) {
     GemmArgs g = p.g;
     g.m_tiles = (int)((p.m_rows + 64 * MT - 1) / (64 * MT)), g.n_tiles = (int)((p.n_rows + 255) / 256);
@@ -1718,51 +1803,52 @@ int launch_tiles(const Product &a, const Product *b, hipStream_t st) {
     set_error_text("pr_vocab_ce: too many tiles for one launch");
     return PR_EUNSUPPORTED;
   }
-  return launch_lds<vce_gemm_kernel<NP, MT, MODE, T>>(dim3((unsigned)std::min<int64_t>(CUS, (tiles + 7) / 8 * 8)), dim3(512),
+  return launch_lds<vce_gemm_kernel<T, MT, MODE>>(dim3((unsigned)std::min<int64_t>(CUS, (tiles + 7) / 8 * 8)), dim3(512),
                                                       bytes, st, g, g2);
 }
 
 // Time of so many tiles of 64 mt by 256, in arbitrary units.  A tile costs its products and the operand rows that it does
-// not share: 1.5 with one plane (256 features by 256 words against 128 by 256: 178 and 219 us for the same product), less
-// with two, which make 1.5 times the products of what they load (320 words by 256 rows against 256 by 256: 233 and 222 us).
+// not share: 1.5 of one plane's products (256 features by 256 words against 128 by 256: 178 and 219 us for the same product),
+// 1.8 where there are three (320 words by 256 rows against 256 by 256: 233 and 222 us).
 // The chip is bound by its power, so a last round that leaves CUs without work runs at a higher clock: three quarters of a
 // full one.
-double tile_time(int np, int64_t tiles, int mt) {
-  return ((double)(tiles / CUS) + (tiles % CUS ? 0.75 : 0.)) * (mt + (np == 1 ? 1.5 : 0.6));
+double tile_time(int products, int64_t tiles, int mt) {
+  return ((double)(tiles / CUS) + (tiles % CUS ? 0.75 : 0.)) * (mt * products + (products == 1 ? 1.5 : 1.8));
 }
 
 // Words per workgroup of STATS and GRAD, in units of 64.
-int word_units(int np, int64_t words, int64_t rows) {
+int word_units(int planes, int64_t words, int64_t rows) {
+  const int products = planes == 1 ? 1 : 3;
   int best = 1;
   for (int mt = 2; mt <= 5; ++mt) {
-    auto time = [&](int m) { return tile_time(np, (words + 64 * m - 1) / (64 * m) * ((rows + 255) / 256), m); };
+    auto time = [&](int m) { return tile_time(products, (words + 64 * m - 1) / (64 * m) * ((rows + 255) / 256), m); };
     if (time(mt) < time(best)) best = mt;
   }
   return best;
 }
-template <int NP, int MODE>
+template <typename T, int MODE>
 int launch_words(const GemmArgs &g, int64_t words, int64_t rows, hipStream_t st) {
   const Product p{g, words, rows};
-  switch (word_units(NP, words, rows)) {
-    case 1: return launch_tiles<NP, 1, MODE, float>(p, nullptr, st);
-    case 2: return launch_tiles<NP, 2, MODE, float>(p, nullptr, st);
-    case 3: return launch_tiles<NP, 3, MODE, float>(p, nullptr, st);
-    case 4: return launch_tiles<NP, 4, MODE, float>(p, nullptr, st);
-    default: return launch_tiles<NP, 5, MODE, float>(p, nullptr, st);
+  switch (word_units(Types<T>::Logits::NA, words, rows)) {
+    case 1: return launch_tiles<T, 1, MODE>(p, nullptr, st);
+    case 2: return launch_tiles<T, 2, MODE>(p, nullptr, st);
+    case 3: return launch_tiles<T, 3, MODE>(p, nullptr, st);
+    case 4: return launch_tiles<T, 4, MODE>(p, nullptr, st);
+    default: return launch_tiles<T, 5, MODE>(p, nullptr, st);
   }
 }
 
 // The same for the products whose M rows are features.
-template <int NP, int MODE, typename T>
+template <typename T, int MODE>
 int launch_features(const Product &a, const Product *b, hipStream_t st) {
   auto time = [&](int mt) {
     auto tiles = [mt](const Product &p) { return (p.m_rows + 64 * mt - 1) / (64 * mt) * ((p.n_rows + 255) / 256) * p.g.splits; };
-    return tile_time(NP, tiles(a) + (b ? tiles(*b) : 0), mt);
+    return tile_time(Types<T>::Grads::PRODUCTS, tiles(a) + (b ? tiles(*b) : 0), mt);
   };
   const int best = time(4) <= time(2) && time(4) <= time(1) ? 4 : time(2) <= time(1) ? 2 : 1;
-  if (best == 4) return launch_tiles<NP, 4, MODE, T>(a, b, st);
-  if (best == 2) return launch_tiles<NP, 2, MODE, T>(a, b, st);
-  return launch_tiles<NP, 1, MODE, T>(a, b, st);
+  if (best == 4) return launch_tiles<T, 4, MODE>(a, b, st);
+  if (best == 2) return launch_tiles<T, 2, MODE>(a, b, st);
+  return launch_tiles<T, 1, MODE>(a, b, st);
 }
 
 struct Call {
@@ -1780,7 +1866,7 @@ struct Call {
     if (_rc != PR_OK) return _rc;  \
   } while (0)
 
-template <typename T, int NP>
+template <typename T>
 int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, float *lse, float *loss, hipStream_t st) {
   const Shape s(c.dtype, c.P, c.V, c.D);
   const bool scaled = c.dtype != PR_F16;
@@ -1797,14 +1883,14 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
   const PackJob jx{c.x, c.labels, c.ignore, k.xf, s.plane(s.Pp), s.Pp / 32 * ((kb + 3) / 4), kb, ax.blocks,
                    c.scale < 0.f ? -1.f : 1.f};
   const int64_t pack_blocks = std::min<int64_t>(2048, (jw.units + jx.units + 3) / 4);
-  hipLaunchKernelGGL((vce_pack_kernel<T, NP>), dim3((unsigned)pack_blocks), dim3(256), 0, st, jw, jx, f.amax, k.scal);
+  hipLaunchKernelGGL((vce_pack_kernel<T, Types<T>::Logits::NA>), dim3((unsigned)pack_blocks), dim3(256), 0, st, jw, jx, f.amax, k.scal);
   PR_TRY(check_launch("pr_vocab_ce"));
   GemmArgs g{};
   g.A = k.wf, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
   g.kblocks = g.k_split = kb, g.splits = 1;
   g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.labels = c.labels;
   g.partial = f.partial, g.target = f.target, g.Pp = s.Pp;
-  PR_TRY((launch_words<NP, STATS>(g, s.Vp, s.Pp, st)));
+  PR_TRY((launch_words<T, STATS>(g, s.Vp, s.Pp, st)));
   const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k.lse2, lse, row_loss};
   hipLaunchKernelGGL(vce_join_kernel, dim3((unsigned)(s.Pp / 8)), dim3(256), 0, st, rows, s.Pp, f.pairs, f.partial);
   PR_TRY(check_launch("pr_vocab_ce"));
@@ -1958,7 +2044,7 @@ int few_backward(const Call &c, int per_row, int mean, const FewKept &k, const F
   return few_gradients<T, 4>(c, s, k, b, f, dx, dw, st);
 }
 
-template <typename T, int NP>
+template <typename T>
 int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b, const float *g_loss, const float *g_lse, T *dx,
              T *dw, hipStream_t st) {
   const Shape s(c.dtype, c.P, c.V, c.D);
@@ -1966,9 +2052,9 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
   const CoefJob coef{c.P, s.Pp, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, b.exp_g, b.coef_a, b.coef_b};
   const TransposeJob tw{k.wf, b.wt, s.plane(s.Vp), dx ? s.Vp / 32 : 0, s.Dk / 32};
   const TransposeJob tx{k.xf, b.xt, s.plane(s.Pp), dw ? s.Pp / 32 : 0, s.Dk / 32};
-  const int64_t turns = ((tw.row_tiles + tx.row_tiles) * (s.Dk / 32) * NP + 15) / 16;
-  hipLaunchKernelGGL(vce_prepare_kernel, dim3((unsigned)((s.Pp + COEF_ROWS - 1) / COEF_ROWS + std::min<int64_t>(1024, turns))),
-                     dim3(1024), 0, st, coef, tw, tx, NP);
+  const int64_t turns = ((tw.row_tiles + tx.row_tiles) * (s.Dk / 32) + 15) / 16;
+  hipLaunchKernelGGL(vce_prepare_kernel<T>, dim3((unsigned)((s.Pp + COEF_ROWS - 1) / COEF_ROWS + std::min<int64_t>(1024, turns))),
+                     dim3(1024), 0, st, coef, tw, tx);
   PR_TRY(check_launch("pr_vocab_ce"));
   for (int64_t v0 = 0; v0 < s.Vp; v0 += b.piece) {
     const int64_t words = std::min(b.piece, s.Vp - v0);
@@ -1978,7 +2064,7 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
     g.lse2 = k.lse2, g.coef_a = b.coef_a, g.coef_b = b.coef_b;
     g.gx = dx ? b.gx : nullptr, g.gw = dw ? b.gw : nullptr;
     g.plane_gx = g.plane_gw = s.Pp * b.piece / 8, g.ld_gx = b.piece / 16, g.ld_gw = kp;
-    PR_TRY((launch_words<NP, GRAD>(g, words, s.Pp, st)));
+    PR_TRY((launch_words<T, GRAD>(g, words, s.Pp, st)));
     const bool last = v0 + words >= s.Vp, split_dw = dw && b.split_rows.n > 1;
     Product px{{}, s.Dk, s.Pp}, pw{{}, s.Dk, words};
     GemmArgs &x = px.g, &w = pw.g;
@@ -1991,8 +2077,8 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
     w.scal = k.scal, w.exp_g = b.exp_g, w.scale = c.scale, w.V = c.V, w.v0 = v0, w.out = dw, w.D = c.D;
     w.acc = b.acc_w, w.Pp = words, w.ld_acc = s.Dk;
     if (dx || split_dw)
-      PR_TRY((launch_features<NP, DX, float>(dx ? px : pw, dx && split_dw ? &pw : nullptr, st)));
-    if (dw && !split_dw) PR_TRY((launch_features<NP, DW, T>(pw, nullptr, st)));
+      PR_TRY((launch_features<T, DX>(dx ? px : pw, dx && split_dw ? &pw : nullptr, st)));
+    if (dw && !split_dw) PR_TRY((launch_features<T, DW>(pw, nullptr, st)));
     FinishJob jobs[2] = {};
     int n = 0;
     if (dx && last) jobs[n++] = FinishJob{c.P, c.D, s.Pp, s.Dk, b.split_words.n, c.scale, b.acc, &k.scal->exp_w, b.exp_g, dx};
@@ -2078,9 +2164,9 @@ extern "C" int pr_vocab_ce_fwd(int dtype, int64_t P, int64_t V, int64_t D, const
   pr::Kept k(ck, s);
   pr::FwdScratch f(cs, s);
   if (!row_loss) row_loss = f.row_loss;
-  if (dtype == PR_F32) return pr::forward<float, 2>(c, mean, k, f, row_loss, lse, loss, st);
-  if (dtype == PR_F16) return pr::forward<_Float16, 1>(c, mean, k, f, row_loss, lse, loss, st);
-  return pr::forward<__bf16, 1>(c, mean, k, f, row_loss, lse, loss, st);
+  if (dtype == PR_F32) return pr::forward<float>(c, mean, k, f, row_loss, lse, loss, st);
+  if (dtype == PR_F16) return pr::forward<_Float16>(c, mean, k, f, row_loss, lse, loss, st);
+  return pr::forward<__bf16>(c, mean, k, f, row_loss, lse, loss, st);
 }
 
 extern "C" int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const void *w, int64_t ldw_row, int64_t ldw_col,
@@ -2111,8 +2197,8 @@ extern "C" int pr_vocab_ce_bwd(int dtype, int64_t P, int64_t V, int64_t D, const
   const pr::Shape s(dtype, P, V, D);
   const pr::Kept k(ck, s);
   pr::BwdScratch b(cs, s, dx != nullptr, dw != nullptr);
-  if (dtype == PR_F32) return pr::backward<float, 2>(c, per_row, mean, k, b, g_loss, g_lse, (float *)dx, (float *)dw, st);
+  if (dtype == PR_F32) return pr::backward<float>(c, per_row, mean, k, b, g_loss, g_lse, (float *)dx, (float *)dw, st);
   if (dtype == PR_F16)
-    return pr::backward<_Float16, 1>(c, per_row, mean, k, b, g_loss, g_lse, (_Float16 *)dx, (_Float16 *)dw, st);
-  return pr::backward<__bf16, 1>(c, per_row, mean, k, b, g_loss, g_lse, (__bf16 *)dx, (__bf16 *)dw, st);
+    return pr::backward<_Float16>(c, per_row, mean, k, b, g_loss, g_lse, (_Float16 *)dx, (_Float16 *)dw, st);
+  return pr::backward<__bf16>(c, per_row, mean, k, b, g_loss, g_lse, (__bf16 *)dx, (__bf16 *)dw, st);
 }

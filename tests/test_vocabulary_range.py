@@ -1,0 +1,132 @@
+"""Vocabulary cross entropy where rows, words or upstream gradients differ by many orders of magnitude: every output is held
+to a bound from its own row's or word's magnitudes, not from the tensor's largest.
+
+With u = 2^-24 (half a float32 step), for float32 input tau = 3 * 2^-22 (a value is kept in 22 bits, and so is the product of
+two) and for 16-bit input 0:
+  logits     dz = |scale| (tau + (n D / 16 + 16) u) sum_d |x_d w_d|: D products added 16 at a time in n passes (n at most 6),
+             and for float32 2^-36 of the row's largest times the word's largest a feature (what 22 bits of two planes leave
+             out of values far below their row's largest)
+  log-sum    the largest dz that counts, (104 + words / 4096) u and 8 u |lse|
+  G          a p times (dz + dlse + 8 u (|z| + |lse|) in the exponent) + 16 u a p + 8 u b at the label + the pieces it is kept in:
+             2^-15 |G| (16-bit input), 2^-21 |G| (float32)
+  gradients  scale sum |dG| |m| + scale (tau + (n K / 16 + 24) u) sum |G| |m| over the axis of K that is added up (float32: the
+             planes' 2^-36 of the largest of a row m as well) + half a step of the output's type
+  underflow  2^-120 of the largest coefficient, G and m.
+"""
+import math
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+HALF = {torch.float32: U, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+PASSES = 6
+IGN = -100
+
+
+def reference(x, w, labels, scale, up, ignore=IGN):
+    """Values and bounds in float64: loss, lse, dx and dw; up: the rows' upstream gradients of the loss."""
+    dtype, (P, D), V = x.dtype, x.shape, w.shape[0]
+    tau = 3 * 2.0 ** -22 if dtype == torch.float32 else 0.0
+    held = 2.0 ** -21 if dtype == torch.float32 else 2.0 ** -15
+    keep = labels != ignore
+    x = torch.where(keep[:, None], x.double(), torch.zeros((), dtype=torch.float64, device=x.device))
+    w, up = w.double(), up.double() * keep
+    at = torch.where(keep, labels, torch.zeros_like(labels))[:, None]
+    z = scale * torch.mm(x, w.t().contiguous())
+    planes = 2.0 ** -36 if dtype == torch.float32 else 0.0
+    xmax, wmax = x.abs().amax(1), w.abs().amax(1)
+    dz = abs(scale) * (torch.mm(x.abs(), w.abs().t().contiguous()) * (tau + (PASSES * D / 16 + 16) * U)
+                       + planes * D * xmax[:, None] * wmax)
+    lse = torch.logsumexp(z, 1)
+    p = (z - lse[:, None]).exp()
+    # a word's logit counts in the log-sum as far as it is probable
+    dlse = (p * dz).sum(1) * 1.01 + (104 + V / 4096) * U + 8 * U * lse.abs()
+    zt = z.gather(1, at)[:, 0]
+    out = {"lse": (lse * keep, dlse * keep),
+           "loss": ((lse - zt) * keep, (dlse + dz.gather(1, at)[:, 0] + 8 * U * (lse.abs() + zt.abs())) * keep)}
+    hot = torch.zeros_like(p).scatter_(1, at, 1.0)
+    a = up.abs()[:, None]
+    G = up[:, None] * (p - hot)
+    dG = (a * p * ((dz + dlse[:, None] + 8 * U * (z.abs() + lse.abs()[:, None])) * 1.01 + 16 * U) + 8 * U * a * hot + held * G.abs()
+          + 2.0 ** -120 * a.max())
+
+    def grad(G, dG, m):
+        v = scale * torch.mm(G, m)
+        e = abs(scale) * (torch.mm(dG, m.abs()) + torch.mm(G.abs(), m.abs()) * (tau + (PASSES * G.shape[1] / 16 + 24) * U)
+                          + planes * torch.mm(G.abs(), m.abs().amax(1, keepdim=True)) + 2.0 ** -120 * G.abs().max() * m.abs().max())
+        return v, e * 1.01 + HALF[dtype] * v.abs() * 1.01 + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -140)
+
+    out["dx"], out["dw"] = grad(G, dG, w), grad(G.t().contiguous(), dG.t().contiguous(), x)
+    return out
+
+
+def close(got, want, what, tight=0.5, rows=None):
+    """Every element within its bound, and the bound below a tenth of the value for a share `tight` of the elements, so that
+    it could not hold for any result."""
+    value, bound = want
+    assert got.shape == value.shape, what
+    # (a value beyond the type's range, as of a float16 gradient of 1e4 times a feature of 8, has no finite result)
+    rows = (value.abs() + bound <= torch.finfo(got.dtype).max) & (True if rows is None else rows)
+    got, value, bound = got.detach().double()[rows], value[rows], bound[rows]
+    assert torch.isfinite(got).all(), what
+    off = (got - value).abs() - bound
+    worst = off.argmax()
+    assert off.max() <= 0, (what, worst.item(), got.reshape(-1)[worst].item(), value.reshape(-1)[worst].item(),
+                            bound.reshape(-1)[worst].item())
+    share = (bound <= 0.1 * value.abs()).double().mean().item()
+    assert share >= tight, (what, "bound too wide", share)
+
+
+def run(x, w, labels, scale, up):
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss, lse = vocabulary_cross_entropy(x, w, labels, scale, reduction="none", return_lse=True)
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    return {"loss": loss, "lse": lse, "dx": dx, "dw": dw}
+
+
+def inputs(P, V, D, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(V, D, generator=g) / D ** 0.5
+    labels = torch.randint(0, V, (P,), generator=g)
+    x = torch.randn(P, D, generator=g) + w[labels]
+    return x.to(dtype).cuda(), w.to(dtype).cuda(), labels.cuda(), g
+
+
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("P,V,D", [(300, 1000, 64), (513, 700, 130)])
+def test_rows_of_very_different_weight(P, V, D, dtype):
+    """Rows weighted over eight decades: the gradient of a row with a small weight is as good as that of a large one."""
+    x, w, y, g = inputs(P, V, D, dtype, seed=P)
+    weight = torch.logspace(4, -4, P)[torch.randperm(P, generator=g)].cuda()
+    if dtype == torch.float32:
+        weight = weight * 1e-4
+    ref = reference(x, w, y, 2.0, weight)
+    got = run(x, w, y, 2.0, weight)
+    for k in ("loss", "lse", "dx", "dw"):
+        close(got[k], ref[k], k)
+
+
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("P,V,D", [(300, 1000, 512)])
+def test_words_that_are_nobodys_label(P, V, D, dtype):
+    """Sharp logits: the words without a label have probabilities down to 1e-38, and their gradients are small, not zero."""
+    x, w, y, g = inputs(P, V, D, torch.float32, seed=5)
+    y = y % 200
+    w = w / w.norm(dim=1, keepdim=True)
+    x = w[y] + 0.02 * torch.randn(P, D, generator=g).cuda()
+    x, w = (x / x.norm(dim=1, keepdim=True)).to(dtype), w.to(dtype)
+    for scale in (10.0, 30.0, 100.0):
+        up = torch.full((P,), 2.0 ** 9 if dtype == torch.float16 else 1.0 / P, device="cuda")
+        ref = reference(x, w, y, scale, up)
+        got = run(x, w, y, scale, up)
+        for k in ("lse", "dw"):
+            # (float16 holds gradients down to 2^-24; at 100 many of these are near the smallest of float32)
+            close(got[k], ref[k], k, tight=0.0 if scale > 50 or (dtype == torch.float16 and scale > 20) else 0.4)
+        # (a single element may be below the smallest float32)
+        assert dtype == torch.float16 or (got["dw"][200:] != 0).any(dim=1).all()
