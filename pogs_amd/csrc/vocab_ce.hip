@@ -798,9 +798,10 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
-// At most 32 NB rows: the vocabulary is read as it is, and nothing of its size is packed.  16-bit operands go to the matrix
-// cores in their own type; a float32 value is cut into three bfloat16 pieces that hold all its 24 bits (by truncation, so
-// the largest values do not overflow), six products of which leave out less than 2^-21 of a product.
+// At most 32 NB rows: the vocabulary is read as it is, and nothing of its size is packed.  For the scores 16-bit operands go
+// to the matrix cores in their own type; a float32 value is cut into three bfloat16 pieces that hold all its 24 bits (by
+// truncation, so the largest values do not overflow), six products of which leave out less than 2^-21 of a product.  The
+// gradients' operands are bfloat16 pieces as in the packed path: float16's range would lose rows of small weight.
 //   SCORE   logits, maxima and sums of 32 words a wavefront.  For a backward pass the logits stay, 4 bytes for each word and
 //           row: at 32 rows a 32nd of a float32 vocabulary of 1024 dims.
 //   DX      32 words a step, 64 features a wavefront and 256 a workgroup, whose wavefronts make G of the step in LDS
@@ -873,6 +874,32 @@ struct Operand<__bf16> {
   }
 };
 
+// Eight values of a gradient's operand in bfloat16 pieces, as in the packed path.
+template <int N_>
+struct Pieces {
+  static constexpr int N = N_;
+  u4v piece[N];
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    b8v o[N];
+    bf16_pieces<N>(v, o);
+#pragma unroll
+    for (int k = 0; k < N; ++k) piece[k] = __builtin_bit_cast(u4v, o[k]);
+  }
+};
+template <typename T>
+using Factor = Pieces<Types<T>::Grads::NA>;        // of W or X
+template <typename T>
+using GradOperand = Pieces<Types<T>::Grads::NB>;   // of G
+template <int NA, int NB>
+__device__ __forceinline__ f16v times(const Pieces<NB> &g, const Pieces<NA> &x, f16v acc) {
+#pragma unroll
+  for (int n = (NA > NB ? NA : NB) - 1; n >= 0; --n)     // smallest first
+#pragma unroll
+    for (int k = 0; k <= n; ++k)
+      if (k < NB && n - k < NA)
+        acc = mfma(__builtin_bit_cast(b8v, g.piece[k]), __builtin_bit_cast(b8v, x.piece[n - k]), acc);
+  return acc;
+}
 
 // Elements k..k+7 of a row as they are.  WIDE (unit column stride, eight columns at least): by 16-byte accesses.  Where
 // they cross the end of the row the last eight columns are read in their place: few_column says which column a place holds,
@@ -941,8 +968,8 @@ __global__ void __launch_bounds__(256) vce_few_pack_kernel(const FewPack j) {
     return row < j.x.rows && j.labels[row] != j.ignore ? (float)((const T *)j.x.data)[row * j.x.ld_row + col * j.x.ld_col] : 0.f;
   };
   float v[8];
-  Operand<T> o;
   if (u < nf) {
+    Operand<T> o;
     const int64_t n = u / j.kblocks, k = (u - n * j.kblocks) * 16 + 8 * h, c = few_column(k, j.x.cols);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i >= k && c + i < j.x.cols ? at(32 * n + (lane & 31), c + i) : 0.f;
@@ -952,8 +979,9 @@ __global__ void __launch_bounds__(256) vce_few_pack_kernel(const FewPack j) {
     const int64_t tile = (u - nf) / j.row_blocks, b = u - nf - tile * j.row_blocks, d = tile_column<T>(tile, lane);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = d < j.x.cols ? at(16 * b + 8 * h + i, d) : 0.f;
+    Factor<T> o;
     o.set(v);
-    store_operand(o, j.xt + (u - nf) * (Operand<T>::N * 64) + lane);
+    store_operand(o, j.xt + (u - nf) * (Factor<T>::N * 64) + lane);
   }
 }
 
@@ -1188,60 +1216,19 @@ __global__ void __launch_bounds__(256, 2) vce_score_shared_kernel(Matrix w, int6
   }
 }
 
-// G as an operand that meets one of type T.  bfloat16 takes two pieces of it (2^-14 of an entry), float16 its own type, with
-// the row factors scaled by exp_g; the others have float32's range and need no scaling.
-template <typename T>
-struct GradOperand : Operand<T> {
-  static __device__ __forceinline__ f16v times(const GradOperand &a, const Operand<T> &b, f16v acc) {
-    return Operand<T>::product(a, b, acc);
-  }
-};
-template <>
-struct GradOperand<__bf16> {
-  static constexpr int N = 2;
-  u4v piece[N];
-  __device__ __forceinline__ void set(const float (&v)[8]) {
-    Operand<float> o;
-    o.set(v);
-    piece[0] = o.piece[0], piece[1] = o.piece[1];
-  }
-  static __device__ __forceinline__ f16v times(const GradOperand &a, const Operand<__bf16> &b, f16v acc) {
-#pragma unroll
-    for (int k = 1; k >= 0; --k)
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a.piece[k]), __builtin_bit_cast(b8v, b.piece[0]),
-                                                    acc, 0, 0, 0);
-    return acc;
-  }
-};
-template <typename T>
-constexpr bool FEW_SCALED = false;
-template <>
-constexpr bool FEW_SCALED<_Float16> = true;
-
 struct FewGrad {  // what G is made of
-  CoefJob c;      // P, V, labels, upstream gradients; exp_g: where DX leaves it for FINISH
+  CoefJob c;      // P, V, labels, upstream gradients
   int64_t D, Dk;
   const float *lse2, *logits;
-  // Row p as {lse2, a, b, label's bits}, made by every workgroup for itself (256 threads; a launch would cost more).  Returns
-  // the power of two that a and b are scaled by.
-  template <typename T>
-  __device__ __forceinline__ int rows(float4 *to, int n) const {
+  // Row p as {lse2, a, b, label's bits}, made by every workgroup for itself (256 threads; a launch would cost more).
+  __device__ __forceinline__ void rows(float4 *to, int n) const {
     const float one = c.one();
-    int e = 0;
-    if (FEW_SCALED<T>) {
-      float top = 0.f;
-      for (int p = threadIdx.x; p < c.P; p += 256) c.largest(p, one, top);
-      top = block_max(top);
-      e = coef_exponent(top);
-    }
     for (int p = threadIdx.x; p < n; p += 256) {
       float a, b;
       c.row(p, one, a, b);
       const int64_t label = p < c.P ? c.labels[p] : -1;
-      to[p] = make_float4(p < c.P ? lse2[p] : 0.f, ldexpf(a, e), ldexpf(b, e),
-                          __builtin_bit_cast(float, label >= 0 && label < c.V ? (int)label : -1));
+      to[p] = make_float4(p < c.P ? lse2[p] : 0.f, a, b, __builtin_bit_cast(float, label >= 0 && label < c.V ? (int)label : -1));
     }
-    return e;
   }
   static __device__ __forceinline__ float entry(float z, const float4 &row, int word) {
     const float g = row.y * __builtin_amdgcn_exp2f(z - row.x);
@@ -1257,7 +1244,8 @@ constexpr size_t dw_lds(int nb, int tiles, int pieces) { return (size_t)3 * 2 * 
 template <typename T, int NB>
 __global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, const u4v *__restrict__ xt, float scale,
                                                             T *__restrict__ out) {
-  constexpr int KB = 2 * NB, NT = few_tiles<T>, STAGE = NT * KB * Operand<T>::N, LOADS = (STAGE + 3) / 4;
+  typedef Factor<T> X;
+  constexpr int KB = 2 * NB, NT = few_tiles<T>, STAGE = NT * KB * X::N, LOADS = (STAGE + 3) / 4;
   __shared__ float4 rows[32 * NB];
   extern __shared__ u4v lds[];    // three stages, of a chunk of the features' operands each
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
@@ -1273,7 +1261,7 @@ __global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, con
   };
   fill(blockIdx.y, 0);
   if (blockIdx.y + gridDim.y < chunks) fill(blockIdx.y + gridDim.y, 1);
-  const int e = -f.rows<T>(rows, 32 * NB);
+  f.rows(rows, 32 * NB);
   __syncthreads();
   const int64_t t = (int64_t)blockIdx.x * 4 + wave, at = min(t, (f.c.V - 1) / 32);   // (past the end: not stored)
   GradOperand<T> ga[KB];
@@ -1306,13 +1294,13 @@ __global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, con
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
-    Operand<T> x[2];
-    x[0] = packed_operand<Operand<T>>(lds + buf * STAGE * 64 + lane);
+    X x[2];
+    x[0] = packed_operand<X>(lds + buf * STAGE * 64 + lane);
 #pragma unroll
     for (int i = 0; i < NT * KB; ++i) {
-      if (i + 1 < NT * KB) x[(i + 1) & 1] = packed_operand<Operand<T>>(lds + (buf * STAGE + (i + 1) * Operand<T>::N) * 64 + lane);
+      if (i + 1 < NT * KB) x[(i + 1) & 1] = packed_operand<X>(lds + (buf * STAGE + (i + 1) * X::N) * 64 + lane);
       const int j = NT == 1 ? i & 1 : i / KB;
-      acc[j] = GradOperand<T>::times(ga[i % KB], x[i & 1], acc[j]);
+      acc[j] = times(ga[i % KB], x[i & 1], acc[j]);
     }
     // all but the youngest fill have come, and what was written a chunk ago; this chunk's stores have until the next wait
     if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
@@ -1331,7 +1319,7 @@ __global__ void __launch_bounds__(256, 2) vce_few_dw_kernel(const FewGrad f, con
         dst[v * f.D] = (acc[0][r] + acc[1][r]) * scale;
       } else {
         typedef T t2 __attribute__((ext_vector_type(2)));
-        const t2 g = {(T)ldexpf(acc[0][r] * scale, e), (T)ldexpf(acc[1][r] * scale, e)};
+        const t2 g = {(T)(acc[0][r] * scale), (T)(acc[1][r] * scale)};
         if ((f.D & 1) == 0) {
           *reinterpret_cast<t2 *>(dst + v * f.D) = g;
         } else {
@@ -1352,8 +1340,7 @@ __global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Mat
   constexpr bool PAIRS = sizeof(T) == 2;
   __shared__ float4 rows[R];
   __shared__ u4v g[2][2 * NB][G::N][64];
-  const int e = f.rows<T>(rows, R);
-  if (FEW_SCALED<T> && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *f.c.exp_g = e;
+  f.rows(rows, R);
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int64_t lo = blockIdx.y * steps, hi = min(lo + steps, (f.c.V + 31) / 32);
@@ -1382,8 +1369,16 @@ __global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Mat
       }
     }
   };
-  auto operands = [&](const Raw &raw, Operand<T> (&o)[2]) {
-    if constexpr (!PAIRS) {
+  auto operands = [&](const Raw &raw, Factor<T> (&o)[2]) {
+    if constexpr (Factor<T>::N == 2) {   // float16
+      float v[2][8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[0][i] = (float)__builtin_bit_cast(T, (unsigned short)raw.a[i]);
+        v[1][i] = (float)__builtin_bit_cast(T, (unsigned short)(WIDE ? raw.a[i] >> 16 : raw.b[PAIRS && WIDE ? 0 : i]));
+      }
+      o[0].set(v[0]), o[1].set(v[1]);
+    } else if constexpr (!PAIRS) {
       float v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, raw.a[i]);
@@ -1452,13 +1447,13 @@ __global__ void __launch_bounds__(256, 2) vce_few_dx_kernel(const FewGrad f, Mat
       for (int kb = 0; kb < 2; ++kb) {
         if (kb == 0) load(s, 1, raw[1]);
         else if (more) load(s + 1, 0, raw[0]);
-        Operand<T> o[2];
+        Factor<T> o[2];
         operands(raw[kb], o);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           const G ga = packed_operand<G>(&g[buf][2 * n + kb][0][lane]);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) acc[n][j] = G::times(ga, o[j], acc[n][j]);
+          for (int j = 0; j < 2; ++j) acc[n][j] = times(ga, o[j], acc[n][j]);
         }
       }
     }
@@ -1499,11 +1494,10 @@ __global__ void __launch_bounds__(1024) vce_few_finish_kernel(const FewGrad f, i
     const float4 q = part[k][lane];
     v.x += q.x, v.y += q.y, v.z += q.z, v.w += q.w;
   }
-  const int e = FEW_SCALED<T> ? -*f.c.exp_g : 0;
   const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (d + k < f.D) dx[p * f.D + d + k] = (T)ldexpf(x[k] * scale, e);
+    if (d + k < f.D) dx[p * f.D + d + k] = (T)(x[k] * scale);
 }
 
 // ---- rows -----------------------------------------------------------------------------------------------------------
@@ -1902,17 +1896,17 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
 // 32-row tiles of the kernels for few rows, and the padded rows and features that go with them.
 struct FewShape {
   int64_t P, V, D, R, Dk, tiles;
-  int nb, pieces;
+  int nb, pieces, factors;   // pieces of the features for the scores and for dW
   bool shared;   // which score kernel
   FewShape(int dtype, int64_t P_, int64_t V_, int64_t D_)
       : P(P_), V(V_), D(D_), Dk(round_up(D_, 64)), tiles((V_ + 31) / 32), nb(P_ <= 32 ? 1 : P_ <= 64 ? 2 : 4),
-        pieces(dtype == PR_F32 ? 3 : 1) {
+        pieces(dtype == PR_F32 ? 3 : 1), factors(Shape(dtype, P_, V_, D_).na) {
     R = 32 * nb;
     // Below, CUs would be without work (20011 words x 1024 dims: 64 rows 53 against 47 us, 24 bfloat16 rows 32 against 27;
     // 60000 x 512: 41 against 58, 25 against 28)
     shared = V >= 128 * CUS;
   }
-  int64_t packed() const { return R * Dk / 8 * pieces; }   // 16-byte units of a copy of the features
+  int64_t packed(int n) const { return R * Dk / 8 * n; }   // 16-byte units of a copy of the features in n pieces
 };
 
 struct FewKept {
@@ -1922,7 +1916,7 @@ struct FewKept {
   FewKept(Carve &c, const FewShape &s) {
     scal = c.take<Scalars>(1);
     lse2 = c.take<float>(s.R);
-    xt = c.take<u4v>(s.packed());
+    xt = c.take<u4v>(s.packed(s.factors));
     logits = c.take<float>(s.tiles * s.R * 32);
   }
 };
@@ -1937,7 +1931,7 @@ struct ScoreScratch {  // of the forward pass for few rows
     target = c.take<float>(s.R);
     row_loss = c.take<float>(s.R);
     partial = c.take<float2>(blocks * s.R);
-    xf = c.take<u4v>(s.packed());
+    xf = c.take<u4v>(s.packed(s.pieces));
   }
 };
 
@@ -1993,7 +1987,6 @@ int score(const Call &c, int mean, ScoreScratch &f, FewKept *k, float *row_loss,
 }
 
 struct FewBwdScratch {
-  int *exp_g;
   float *acc;
   int64_t steps;   // of 32 words, in a run of DX
   int splits;
@@ -2001,8 +1994,7 @@ struct FewBwdScratch {
     const int64_t chunks = (s.Dk + 255) / 256, want = std::max<int64_t>(1, std::min<int64_t>(FEW_BLOCKS / chunks, s.tiles));
     steps = (s.tiles + want - 1) / want;
     splits = (int)((s.tiles + steps - 1) / steps);
-    exp_g = c.take<int>(1);
-    acc = c.take<float>(dx ? splits * s.R * s.Dk : 0);
+    acc = c.take<float>(dx ? splits * s.R * s.Dk : 1);   // (no buffer of no bytes)
   }
 };
 
@@ -2027,7 +2019,7 @@ int few_gradients(const Call &c, const FewShape &s, const FewKept &k, const FewB
     const unsigned blocks = (unsigned)((s.tiles + 3) / 4);
     // (a part has a chunk at least: of 32 float32 features, of 64 others)
     const unsigned parts = (unsigned)std::max<int64_t>(1, std::min<int64_t>(FEW_BLOCKS / blocks, c.D / 64));
-    PR_TRY((launch_lds<vce_few_dw_kernel<T, NB>>(dim3(blocks, parts), dim3(256), dw_lds(NB, few_tiles<T>, s.pieces), st, f,
+    PR_TRY((launch_lds<vce_few_dw_kernel<T, NB>>(dim3(blocks, parts), dim3(256), dw_lds(NB, few_tiles<T>, s.factors), st, f,
                                                  (const u4v *)k.xt, c.scale, dw)));
   }
   return PR_OK;
@@ -2037,7 +2029,7 @@ template <typename T>
 int few_backward(const Call &c, int per_row, int mean, const FewKept &k, const FewBwdScratch &b, const float *g_loss,
                  const float *g_lse, T *dx, T *dw, hipStream_t st) {
   const FewShape s(c.dtype, c.P, c.V, c.D);
-  const FewGrad f{{c.P, s.R, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, b.exp_g, nullptr, nullptr},
+  const FewGrad f{{c.P, s.R, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, nullptr, nullptr, nullptr},
                   c.D, s.Dk, k.lse2, k.logits};
   if (s.nb == 1) return few_gradients<T, 1>(c, s, k, b, f, dx, dw, st);
   if (s.nb == 2) return few_gradients<T, 2>(c, s, k, b, f, dx, dw, st);

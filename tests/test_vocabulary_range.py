@@ -98,7 +98,7 @@ def inputs(P, V, D, dtype, seed):
 
 @pytest.mark.gpu
 @TYPES
-@pytest.mark.parametrize("P,V,D", [(300, 1000, 64), (513, 700, 130)])
+@pytest.mark.parametrize("P,V,D", [(300, 1000, 64), (513, 700, 130), (20, 6000, 130), (50, 6000, 96), (100, 6000, 128)])
 def test_rows_of_very_different_weight(P, V, D, dtype):
     """Rows weighted over eight decades: the gradient of a row with a small weight is as good as that of a large one."""
     x, w, y, g = inputs(P, V, D, dtype, seed=P)
@@ -113,7 +113,7 @@ def test_rows_of_very_different_weight(P, V, D, dtype):
 
 @pytest.mark.gpu
 @TYPES
-@pytest.mark.parametrize("P,V,D", [(300, 1000, 512)])
+@pytest.mark.parametrize("P,V,D", [(300, 1000, 512), (100, 2000, 512)])
 def test_words_that_are_nobodys_label(P, V, D, dtype):
     """Sharp logits: the words without a label have probabilities down to 1e-38, and their gradients are small, not zero."""
     x, w, y, g = inputs(P, V, D, torch.float32, seed=5)
