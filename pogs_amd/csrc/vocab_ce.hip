@@ -364,13 +364,15 @@ struct CoefJob {
   const float *g_loss, *g_lse;  // either may be NULL
   int per_row, mean;
   const Scalars *s;
+  const float2 *stat;
   int *exp_g;
   float *a, *b;
+  // G = ra exp2(logit - maximum) - rb at the label: the sum of the exponentials goes into ra
   __device__ __forceinline__ void row(int64_t p, float one, float &ra, float &rb) const {
     ra = rb = 0.f;
     if (p >= P || labels[p] == ignore) return;
     rb = !g_loss ? 0.f : per_row ? g_loss[p] : one;
-    ra = rb + (g_lse ? g_lse[p] : 0.f);
+    ra = (rb + (g_lse ? g_lse[p] : 0.f)) / stat[p].y;
     if (g_loss && (labels[p] < 0 || labels[p] >= V)) ra = NAN;   // no such word: the row's loss is NaN
   }
   // the loss's gradient of every row, where it is one for all
@@ -385,7 +387,7 @@ struct CoefJob {
     if (rb < INFINITY) top = fmaxf(top, rb);
   }
 };
-// Brings the largest factor to 2^12..2^13 (|G| <= |a| + |b|).
+// Brings the largest factor to 2^12..2^13 (|G| <= |ra| + |rb|).
 __device__ __forceinline__ int coef_exponent(float top) { return top > 0.f ? TOP_EXP - 1 - ilogbf(top) : 0; }
 
 constexpr int COEF_ROWS = 4096;  // rows whose factors one workgroup writes
@@ -446,7 +448,7 @@ struct GemmArgs {
   float2 *partial;             // STATS: [pair][Pp]
   float *target;               // STATS: [Pp], the label's logit in the log2 domain
   int64_t Pp;
-  const float *lse2;           // GRAD
+  const float2 *stat;          // GRAD: maximum and sum of every row
   const float *coef_a, *coef_b;
   u4v *gx, *gw;                // GRAD: G as the operand of DX and of DW (either may be NULL)
   int64_t plane_gx, plane_gw, ld_gx, ld_gw;
@@ -491,6 +493,7 @@ constexpr int STAGE_BLOCKS = F::KB * (F::NA * 2 * MT + F::NB * 8);   // of 1 KB
 // to the epilogue.
 template <typename T, int MT, int MODE>
 __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, const GemmArgs g2) {
+#pragma clang fp contract(off)   // products are rounded before they are subtracted (the logits, below)
   extern __shared__ u4v lds[];
   typedef typename FormOf<T, MODE>::F F;
   typedef typename F::E8 E8;
@@ -600,13 +603,13 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
     const bool of_other = other;
     // what the epilogue needs of its rows, ahead of the loads that it would wait for otherwise
     int place_of[NT];             // the label's place among this wavefront's words, or something out of their range
-    float lse2[NT], coef_a[NT], coef_b[NT];
+    float top2[NT], coef_a[NT], coef_b[NT];
     if constexpr (MODE == STATS || MODE == GRAD) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int64_t p = n0 + 32 * n, rel = (p < g.P ? g.labels[p] : -1) - (g.v0 + m0);
         place_of[n] = rel >= 0 && rel < 32 * MT ? (int)rel : -32;
-        if constexpr (MODE == GRAD) lse2[n] = g.lse2[p], coef_a[n] = g.coef_a[p], coef_b[n] = g.coef_b[p];
+        if constexpr (MODE == GRAD) top2[n] = g.stat[p].x, coef_a[n] = g.coef_a[p], coef_b[n] = g.coef_b[p];
       }
     }
     arrive(stages > 1);
@@ -655,13 +658,19 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
         const bool mine = place_of[n] >= 0;
         const int at = place_of[n] - 4 * h;    // from this lane's first word on; the other half's places match no constant
         const bool here = __any(mine);
+        // Logits, rounded: maximum, exponentials and G have to mean the same number, or the difference of logits of 2^24 and
+        // more is not that of equal ones.
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][n][r] *= c;
         if constexpr (MODE == STATS) {
           if (here) {
             float z = 0.f;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) z = at == 32 * i + (r & 3) + 8 * (r >> 2) ? acc[i][n][r] * c : z;
+              for (int r = 0; r < 16; ++r) z = at == 32 * i + (r & 3) + 8 * (r >> 2) ? acc[i][n][r] : z;
             if (mine && (at & 4) == 0) g.target[p] = z;
           }
           if (!whole) {
@@ -677,25 +686,16 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][n][r]);
           top = fmaxf(top, __shfl_xor(top, 32));
-          top = fmaxf(top * c, MAX_FLOOR);
+          top = fmaxf(top, MAX_FLOOR);
           float sum = 0.f;
-          if (whole) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+          for (int i = 0; i < MT; ++i)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -top));
-          } else {  // (the selection and not the infinity keeps the others out: c may have underflowed to 0)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-              for (int r = 0; r < 16; ++r)
-                sum += 32 * i + (r & 3) + 8 * (r >> 2) >= left
-                           ? 0.f : __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -top));
-          }
+            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(acc[i][n][r] - top);
           sum += __shfl_xor(sum, 32);
           if (h == 0) g.partial[(int64_t)(of_m * WM + wm) * g.Pp + p] = make_float2(top, sum);
         } else {
-          const float l2 = lse2[n], ca = coef_a[n], cb = coef_b[n];
+          const float m2 = top2[n], ca = coef_a[n], cb = coef_b[n];
           constexpr int NG = Types<T>::Grads::NB;
           b8v ident[2];
 #pragma unroll
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
           for (int i = 0; i < MT; ++i) {
             float v[2][8];     // register r: slot r & 7 of step r >> 3
 #pragma unroll
-            for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = ca * __builtin_amdgcn_exp2f(fmaf(acc[i][n][r], c, -l2));
+            for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = ca * __builtin_amdgcn_exp2f(acc[i][n][r] - m2);
             if (here) {
 #pragma unroll
               for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] -= at == 32 * i + (r & 3) + 8 * (r >> 2) ? cb : 0.f;
@@ -1000,6 +1000,7 @@ __global__ void __launch_bounds__(256, 2) vce_score_kernel(Matrix w, Matrix x, c
                                                            const int64_t *__restrict__ labels, int64_t ignore, float scale,
                                                            float2 *__restrict__ partial, float *__restrict__ target,
                                                            float *__restrict__ logits) {
+#pragma clang fp contract(off)   // as in the product kernel
   constexpr int NJ = NB < 2 ? NB : 2;   // 32-row tiles that are added at once
   __shared__ float sum[4][NJ][16][64];
   __shared__ float2 join[4][NB][32];
@@ -1112,6 +1113,7 @@ __global__ void __launch_bounds__(256, 2) vce_score_shared_kernel(Matrix w, int6
                                                                   const int64_t *__restrict__ labels, float scale,
                                                                   float2 *__restrict__ partial, float *__restrict__ target,
                                                                   float *__restrict__ logits) {
+#pragma clang fp contract(off)   // as in the product kernel
   typedef Operand<T> O;
   constexpr int Q = few_blocks<T>, STAGE = NB * Q * O::N, LOADS = (STAGE + 3) / 4;
   extern __shared__ u4v lds[];    // two stages
@@ -1219,15 +1221,15 @@ __global__ void __launch_bounds__(256, 2) vce_score_shared_kernel(Matrix w, int6
 struct FewGrad {  // what G is made of
   CoefJob c;      // P, V, labels, upstream gradients
   int64_t D, Dk;
-  const float *lse2, *logits;
-  // Row p as {lse2, a, b, label's bits}, made by every workgroup for itself (256 threads; a launch would cost more).
+  const float *logits;
+  // Row p as {maximum, ra, rb, label's bits}, made by every workgroup for itself (256 threads; a launch would cost more).
   __device__ __forceinline__ void rows(float4 *to, int n) const {
     const float one = c.one();
     for (int p = threadIdx.x; p < n; p += 256) {
       float a, b;
       c.row(p, one, a, b);
       const int64_t label = p < c.P ? c.labels[p] : -1;
-      to[p] = make_float4(p < c.P ? lse2[p] : 0.f, a, b, __builtin_bit_cast(float, label >= 0 && label < c.V ? (int)label : -1));
+      to[p] = make_float4(p < c.P ? c.stat[p].x : 0.f, a, b, __builtin_bit_cast(float, label >= 0 && label < c.V ? (int)label : -1));
     }
   }
   static __device__ __forceinline__ float entry(float z, const float4 &row, int word) {
@@ -1505,18 +1507,19 @@ struct RowsOut {
   int64_t P, V, ignore;
   const int64_t *labels;
   const float *target;
-  float *lse2, *lse, *row_loss;  // lse2 and lse may be NULL
+  float2 *stat;                  // maximum and sum of exp2(logit - maximum), log2 domain; may be NULL
+  float *lse, *row_loss;         // lse may be NULL
 };
 
 __device__ __forceinline__ void finish_row(const RowsOut &o, int64_t p, float m, float s) {
-  const float l2 = m + log2f(s);
-  if (o.lse2) o.lse2[p] = p < o.P ? l2 : 0.f;
+  if (o.stat) o.stat[p] = p < o.P ? make_float2(m, s) : make_float2(0.f, 1.f);
   if (p >= o.P) return;
   const int64_t label = o.labels[p];
   const bool in = label != o.ignore;
-  if (o.lse) o.lse[p] = in ? l2 * LN2F : 0.f;
+  const float l = log2f(s);
+  if (o.lse) o.lse[p] = in ? (m + l) * LN2F : 0.f;
   // a label outside the vocabulary has no logit: the row's loss is NaN
-  o.row_loss[p] = !in ? 0.f : label < 0 || label >= o.V ? NAN : (l2 - o.target[p]) * LN2F;
+  o.row_loss[p] = !in ? 0.f : label < 0 || label >= o.V ? NAN : (l + (m - o.target[p])) * LN2F;
 }
 
 // Joins the (max, sum) pairs of the rows, [pair][Pp]: 8 rows x 32 lanes per workgroup.
@@ -1694,11 +1697,11 @@ struct Carve {  // consecutive 256-byte-aligned pieces of a buffer
 
 struct Kept {  // what the forward pass leaves for the backward pass
   Scalars *scal;
-  float *lse2;
+  float2 *stat;
   u4v *xf, *wf;
   Kept(Carve &c, const Shape &s) {
     scal = c.take<Scalars>(1);
-    lse2 = c.take<float>(s.Pp);
+    stat = c.take<float2>(s.Pp);
     xf = c.take<u4v>(s.np * s.plane(s.Pp));
     wf = c.take<u4v>(s.np * s.plane(s.Vp));
   }
@@ -1885,7 +1888,7 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
   g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.labels = c.labels;
   g.partial = f.partial, g.target = f.target, g.Pp = s.Pp;
   PR_TRY((launch_words<T, STATS>(g, s.Vp, s.Pp, st)));
-  const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k.lse2, lse, row_loss};
+  const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k.stat, lse, row_loss};
   hipLaunchKernelGGL(vce_join_kernel, dim3((unsigned)(s.Pp / 8)), dim3(256), 0, st, rows, s.Pp, f.pairs, f.partial);
   PR_TRY(check_launch("pr_vocab_ce"));
   if (!loss) return PR_OK;
@@ -1911,11 +1914,12 @@ struct FewShape {
 
 struct FewKept {
   Scalars *scal;
-  float *lse2, *logits;   // logits in the log2 domain: [32 words][R][32]
+  float2 *stat;
+  float *logits;          // in the log2 domain: [32 words][R][32]
   u4v *xt;
   FewKept(Carve &c, const FewShape &s) {
     scal = c.take<Scalars>(1);
-    lse2 = c.take<float>(s.R);
+    stat = c.take<float2>(s.R);
     xt = c.take<u4v>(s.packed(s.factors));
     logits = c.take<float>(s.tiles * s.R * 32);
   }
@@ -1971,7 +1975,7 @@ int score(const Call &c, int mean, ScoreScratch &f, FewKept *k, float *row_loss,
   if (s.nb == 1) PR_TRY((launch_score<T, 1>(c, s, f, k, st)));
   else if (s.nb == 2) PR_TRY((launch_score<T, 2>(c, s, f, k, st)));
   else PR_TRY((launch_score<T, 4>(c, s, f, k, st)));
-  const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k ? k->lse2 : nullptr, lse, row_loss};
+  const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k ? k->stat : nullptr, lse, row_loss};
   // (one workgroup for all rows: up to 32 no slower than two launches; 128 rows of 8000 words 15 us slower)
   if (loss && s.nb == 1) {
     hipLaunchKernelGGL(vce_join_reduce_kernel, dim3(1), dim3(1024), 0, st, rows, f.blocks, f.partial, mean, loss,
@@ -2029,8 +2033,8 @@ template <typename T>
 int few_backward(const Call &c, int per_row, int mean, const FewKept &k, const FewBwdScratch &b, const float *g_loss,
                  const float *g_lse, T *dx, T *dw, hipStream_t st) {
   const FewShape s(c.dtype, c.P, c.V, c.D);
-  const FewGrad f{{c.P, s.R, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, nullptr, nullptr, nullptr},
-                  c.D, s.Dk, k.lse2, k.logits};
+  const FewGrad f{{c.P, s.R, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, k.stat, nullptr, nullptr, nullptr},
+                  c.D, s.Dk, k.logits};
   if (s.nb == 1) return few_gradients<T, 1>(c, s, k, b, f, dx, dw, st);
   if (s.nb == 2) return few_gradients<T, 2>(c, s, k, b, f, dx, dw, st);
   return few_gradients<T, 4>(c, s, k, b, f, dx, dw, st);
@@ -2041,7 +2045,7 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
              T *dw, hipStream_t st) {
   const Shape s(c.dtype, c.P, c.V, c.D);
   const int kb = (int)(s.Dk / 16), kv = (int)(s.Vp / 16), kp = (int)(s.Pp / 16);
-  const CoefJob coef{c.P, s.Pp, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, b.exp_g, b.coef_a, b.coef_b};
+  const CoefJob coef{c.P, s.Pp, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, k.stat, b.exp_g, b.coef_a, b.coef_b};
   const TransposeJob tw{k.wf, b.wt, s.plane(s.Vp), dx ? s.Vp / 32 : 0, s.Dk / 32};
   const TransposeJob tx{k.xf, b.xt, s.plane(s.Pp), dw ? s.Pp / 32 : 0, s.Dk / 32};
   const int64_t turns = ((tw.row_tiles + tx.row_tiles) * (s.Dk / 32) + 15) / 16;
@@ -2053,7 +2057,7 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
     GemmArgs g{};
     g.A = k.wf + v0 / 32 * kb * 64, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
     g.kblocks = g.k_split = kb, g.splits = 1, g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.v0 = v0, g.labels = c.labels, g.Pp = s.Pp;
-    g.lse2 = k.lse2, g.coef_a = b.coef_a, g.coef_b = b.coef_b;
+    g.stat = k.stat, g.coef_a = b.coef_a, g.coef_b = b.coef_b;
     g.gx = dx ? b.gx : nullptr, g.gw = dw ? b.gw : nullptr;
     g.plane_gx = g.plane_gw = s.Pp * b.piece / 8, g.ld_gx = b.piece / 16, g.ld_gw = kp;
     PR_TRY((launch_words<T, GRAD>(g, words, s.Pp, st)));

@@ -130,3 +130,39 @@ def test_words_that_are_nobodys_label(P, V, D, dtype):
             close(got[k], ref[k], k, tight=0.0 if scale > 50 or (dtype == torch.float16 and scale > 20) else 0.4)
         # (a single element may be below the smallest float32)
         assert dtype == torch.float16 or (got["dw"][200:] != 0).any(dim=1).all()
+
+
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("P,V,D", [(300, 700, 40), (129, 64, 16), (20, 9000, 64), (100, 9000, 64), (20, 40_000, 16),
+                                   (100, 40_000, 16)])
+@pytest.mark.parametrize("exponent", [6, 20, 30, 60])
+def test_logits_far_beyond_the_differences_that_float32_holds(P, V, D, exponent, dtype):
+    """Small whole numbers and a power of two as scale: logits are exact, and equal ones have to stay equal.  A probability is
+    1 / ties for the largest and (from 2^6 on, below 2^-92) nothing for the others."""
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    g = torch.Generator().manual_seed(exponent)
+    x = torch.randint(-3, 4, (P, D), generator=g).to(dtype).cuda()
+    w = torch.randint(-3, 4, (V, D), generator=g).to(dtype).cuda()
+    y = torch.randint(0, V, (P,), generator=g).cuda()
+    up = torch.randint(1, 5, (P,), generator=g).float().cuda() * 2.0 ** -exponent
+    scale = 2.0 ** exponent
+    z = torch.mm(x.double(), w.double().t().contiguous())
+    best = z == z.amax(1, keepdim=True)
+    p = best / best.sum(1, keepdim=True)
+    lse = scale * z.amax(1) + best.sum(1).double().log()
+    zt = scale * z.gather(1, y[:, None])[:, 0]
+    G = up.double()[:, None] * (p - torch.zeros_like(p).scatter_(1, y[:, None], 1.0))
+    held = 2.0 ** -20 if dtype == torch.float32 else 2.0 ** -14
+    with torch.no_grad():
+        plain, plain_lse = vocabulary_cross_entropy(x, w, y, scale, reduction="none", return_lse=True)
+    got = run(x, w, y, scale, up)
+    # a logarithm to base 2 and back: two roundings of the logit and one of the result
+    for loss, s in ((got["loss"], got["lse"]), (plain, plain_lse)):
+        close(s, (lse, 8 * U * lse.abs() + 16 * U), "lse")
+        close(loss, (lse - zt, 8 * U * (lse.abs() + zt.abs()) + 16 * U), "loss")
+    for k, gr, m in (("dx", G, w), ("dw", G.t().contiguous(), x)):
+        v = scale * torch.mm(gr, m.double())
+        bound = scale * torch.mm(gr.abs(), m.double().abs()) * held + HALF[dtype] * 1.01 * v.abs() + 2.0 ** -80
+        close(got[k], (v, bound), k, tight=0.0)
