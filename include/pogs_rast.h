@@ -494,8 +494,9 @@ int pr_densify_split_children(int64_t n_out, const int32_t *map_src, const int32
  * gradient g_loss of row_loss (per_row != 0: [P]) or of loss (one value) and g_lse[P] of lse; a NULL one is 0.  kept is
  * read only: several calls may share it.  Where pr_vocab_ce_keeps_vocabulary is 0 (few rows, a large vocabulary) kept holds
  * the logits and no copy of w: the backward pass reads the same w again for dx, which must not have changed; elsewhere its w
- * is not looked at.  Products take 16-bit operands (float32 input: two float16 planes or three bfloat16 pieces, 2^-21) and
- * add in float32; sums run in a fixed order, so equal inputs give equal bits. */
+ * is not looked at.  Products take 16-bit operands (float32 input: two float16 planes, a power of two for each row of x and w,
+ * or three bfloat16 pieces, 2^-21; the gradients' are bfloat16 pieces of 16 or 24 bits) and add in float32; sums run in a fixed
+ * order, so equal inputs give equal bits. */
 int pr_vocab_ce_score_rows(void);
 int pr_vocab_ce_keeps_vocabulary(int64_t P, int64_t V, int64_t D);
 size_t pr_vocab_ce_kept_bytes(int dtype, int64_t P, int64_t V, int64_t D);

@@ -11,11 +11,12 @@
 // contraction] with lane l's eight values consecutive, so that a block moves memory -> LDS by one direct 16-byte-a-lane load
 // and LDS -> registers by one conflict-free ds_read_b128.
 //
-// The logits' operands are float16.  Packing scales each tensor by one power of two that brings its largest magnitude to 2^13..2^14: a
-// bfloat16 value keeps all its bits down to 2^-31 of the largest, and a float32 value becomes two float16 planes (head
-// and residual, 22 bits down to 2^-15 of the largest) whose products head*head + head*residual + residual*head lose 2^-22.
-// float16 input is packed as it is.  X takes the scale's sign.  Values that are not finite stay so; rows with the ignored
-// label are packed as zeros, whatever they hold.
+// The logits' operands: 16-bit input is packed as it is.  A float32 value becomes two float16 planes, head and residual, after
+// its row has been scaled by the power of two that brings its largest magnitude to 2^13..2^14 (22 bits down to 2^-15 of the
+// row's largest, below that to 2^-38 of it); head*head + head*residual + residual*head lose 2^-22.  A logit is the product's
+// accumulator times both rows' powers of two: a row or a word that is far larger than the others takes nothing from them.
+// X takes the scale's sign.  Values that are not finite stay so; rows with the ignored label are packed as zeros, whatever they
+// hold.
 //
 // The gradients' operands are bfloat16 pieces, which have float32's range: the entries of G go from the probability of a
 // word that nobody means to the largest row's weight, so a row's or a word's gradient would be lost under a common scale in
@@ -93,7 +94,7 @@ struct Form {
 };
 template <typename T>
 struct Types {  // bfloat16
-  typedef Form<_Float16, 1, 1> Logits;
+  typedef Form<__bf16, 1, 1> Logits;
   typedef Form<__bf16, 1, 2> Grads;
 };
 template <>
@@ -133,7 +134,7 @@ __device__ __forceinline__ void bf16_pieces(const float (&v)[8], b8v (&out)[N]) 
 }
 
 struct Scalars {  // per call, on the device
-  int exp_x, exp_w;  // packed = value * 2^exp
+  int exp_x, exp_w;  // the transposed copies are value * 2^exp
   float n_valid;     // rows whose label is not the ignored one
 };
 
@@ -184,6 +185,8 @@ struct AmaxJob {
   const int64_t *labels;  // rows with the ignored label do not count (NULL: all do)
   int64_t ignore;
   int blocks;             // workgroups, one partial each
+  int64_t padded;         // rows of the packed copy
+  int *exps;              // their exponents
 };
 
 __device__ __forceinline__ float block_max(float top) {
@@ -196,56 +199,48 @@ __device__ __forceinline__ float block_max(float top) {
   return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
 }
 
-// Largest finite magnitude of W, then of X.  One run of memory is read as such; otherwise a wavefront takes four rows.
+constexpr int OF_ZEROS = 200;  // exponent of a row without a finite value but zeros: above all others
+
+// Largest finite magnitude of each row of W, then of X, as the exponent that the row is packed with, and of all rows of a
+// workgroup.  `lanes` lanes (a power of two) take a row, a wavefront four rows for each of their groups.
 template <typename T>
-__global__ void __launch_bounds__(256) vce_amax_kernel(AmaxJob w, AmaxJob x, float *__restrict__ partial) {
+__global__ void __launch_bounds__(256) vce_amax_kernel(AmaxJob w, AmaxJob x, int lanes, float *__restrict__ partial) {
   const bool first = (int)blockIdx.x < w.blocks;
   const AmaxJob &j = first ? w : x;
   const int block = (int)blockIdx.x - (first ? 0 : w.blocks);
-  float top = 0.f;
-  auto take = [&](const float (&v)[8]) {
+  const int groups = 64 / lanes, lane = threadIdx.x & (lanes - 1);
+  float all = 0.f;
+  for (int64_t r0 = ((int64_t)block * 4 + (threadIdx.x >> 6)) * 4 * groups + (threadIdx.x & 63) / lanes; r0 < j.padded;
+       r0 += (int64_t)j.blocks * 16 * groups) {
+    float top[4] = {0.f, 0.f, 0.f, 0.f};
+    bool live[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) top = fabsf(v[k]) < INFINITY ? fmaxf(top, fabsf(v[k])) : top;
-  };
-  if (!j.labels && j.m.ld_col == 1 && j.m.ld_row == j.m.cols && (j.m.cols & 7) == 0) {
-    const T *src = (const T *)j.m.data;
-    const int64_t units = j.m.rows * (j.m.cols / 8), step = (int64_t)j.blocks * 256;
-    int64_t u = (int64_t)block * 256 + threadIdx.x;
-    for (; u + 3 * step < units; u += 4 * step) {
-      Eight<T> e[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) e[q].load(src + (u + q * step) * 8);
+    for (int q = 0; q < 4; ++q) {
+      const int64_t row = r0 + q * groups;
+      live[q] = row < j.m.rows && !(j.labels && j.labels[row] == j.ignore);
+    }
+    for (int64_t k = lane * 8; k < j.m.cols; k += lanes * 8) {
+      float v[4][8];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        float v[8];
-        e[q].get(v);
-        take(v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[q][i] = 0.f;
+        if (live[q]) load8<T>(j.m, r0 + q * groups, k, v[q]);
       }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top[q] = fabsf(v[q][i]) < INFINITY ? fmaxf(top[q], fabsf(v[q][i])) : top[q];
     }
-    for (; u < units; u += step) {
-      Eight<T> e;
-      e.load(src + u * 8);
-      float v[8];
-      e.get(v);
-      take(v);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      for (int d = lanes / 2; d > 0; d >>= 1) top[q] = fmaxf(top[q], __shfl_xor(top[q], d));
+      if (lane == 0 && r0 + q * groups < j.padded) j.exps[r0 + q * groups] = top[q] > 0.f ? TOP_EXP - ilogbf(top[q]) : OF_ZEROS;
+      all = fmaxf(all, top[q]);
     }
-  } else {
-    for (int64_t r0 = ((int64_t)block * 4 + (threadIdx.x >> 6)) * 4; r0 < j.m.rows; r0 += (int64_t)j.blocks * 16)
-      for (int64_t k = (threadIdx.x & 63) * 8; k < j.m.cols; k += 512) {
-        float v[4][8];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[q][i] = 0.f;
-          const int64_t row = r0 + q;
-          if (row < j.m.rows && !(j.labels && j.labels[row] == j.ignore)) load8<T>(j.m, row, k, v[q]);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) take(v[q]);
-      }
   }
-  top = block_max(top);
-  if (threadIdx.x == 0) partial[blockIdx.x] = top;
+  all = block_max(all);
+  if (threadIdx.x == 0) partial[blockIdx.x] = all;
 }
 
 __device__ __forceinline__ int top_exponent(const float *partial, int n) {
@@ -264,30 +259,34 @@ struct PackJob {
   int64_t units;    // (32-row tile, 64 columns) pairs
   int kblocks;      // 16-wide blocks of the contraction per 32-row tile
   int partials;     // of the largest magnitude
+  const int *exps;  // of the rows (NULL: values are packed as they are)
   float sign;
 };
 
 // A wavefront takes 32 rows x 64 columns: eight lanes read 128 (float32: 256) consecutive bytes of a row and store them
 // to the four blocks' places, 128 consecutive bytes for eight rows.
 // Block (tile t, k step s), lane (m, h): row 32 t + m, columns 16 s + 8 h + 0..7.
-template <typename T, int NP>
+template <typename T>
 __global__ void __launch_bounds__(256) vce_pack_kernel(PackJob w, PackJob x, const float *__restrict__ partial,
                                                        Scalars *__restrict__ s) {
+  typedef typename Types<T>::Logits F;
+  typedef typename F::E8 E8;
   const int ew = top_exponent(partial, w.partials), ex = top_exponent(partial + w.partials, x.partials);
   if (blockIdx.x == 0 && threadIdx.x == 0) s->exp_w = ew, s->exp_x = ex;
   const int lane = threadIdx.x & 63, piece = lane & 7;
   for (int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); u < w.units + x.units; u += (int64_t)gridDim.x * 4) {
     const bool first = u < w.units;
     const PackJob &j = first ? w : x;
-    const int e = first ? ew : ex;
     const unsigned groups = (j.kblocks + 3) / 4, v = (unsigned)(first ? u : u - w.units), at = v / groups;  // units < 2^31
     const int64_t tile = at, kb = (v - at * groups) * 4 + piece / 2, k = kb * 16 + (piece & 1) * 8;
     if (kb >= j.kblocks) continue;
     u4v *dst = j.dst + (tile * j.kblocks + kb) * 64 + (piece & 1) * 32 + lane / 8;
     float val[4][8];
+    int e[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int64_t row = tile * 32 + q * 8 + lane / 8;
+      e[q] = j.exps ? j.exps[row] : 0;
       const bool live = row < j.m.rows && k < j.m.cols && !(j.labels && j.labels[row] == j.ignore);
 #pragma unroll
       for (int i = 0; i < 8; ++i) val[q][i] = 0.f;
@@ -295,15 +294,15 @@ __global__ void __launch_bounds__(256) vce_pack_kernel(PackJob w, PackJob x, con
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      h8v hi, lo;
+      E8 hi, lo;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float f = ldexpf(val[q][i], e) * j.sign;
-        hi[i] = (_Float16)f;
-        if (NP == 2) lo[i] = (_Float16)(f - (float)hi[i]);
+        const float f = ldexpf(val[q][i], e[q]) * j.sign;
+        hi[i] = (typename F::E)f;
+        if (F::NA == 2) lo[i] = (typename F::E)(f - (float)hi[i]);
       }
       dst[q * 8] = __builtin_bit_cast(u4v, hi);
-      if (NP == 2) dst[q * 8 + j.plane] = __builtin_bit_cast(u4v, lo);
+      if (F::NA == 2) dst[q * 8 + j.plane] = __builtin_bit_cast(u4v, lo);
     }
   }
 }
@@ -317,20 +316,24 @@ struct TransposeJob {
   u4v *dst;           // [32-column tile][row block], contraction over the rows, in slot order
   int64_t plane;      // of both: they hold the same number of blocks
   int64_t row_tiles, col_tiles;
+  const int *exps, *exp;   // of the rows and of the copy (exps NULL: as they are)
 };
 
 // The packed copies for the contraction over rows, from those over columns: one 32x32 tile per wavefront, every plane as two
 // products with the identity.  Each value passes the matrix core as itself times one and its planes add up to it: exact.
+// Here rows have to share an exponent, the largest row's; the pieces have room for what that takes from the others.
 template <typename T>
 __device__ __forceinline__ void transpose_tiles(const TransposeJob &w, const TransposeJob &x, int64_t u, int64_t step) {
-  constexpr int FROM = Types<T>::Logits::NA, TO = Types<T>::Grads::NA;
+  typedef typename Types<T>::Logits F;
+  typedef typename F::E8 E8;
+  constexpr int FROM = F::NA, TO = Types<T>::Grads::NA;
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const int64_t nw = w.row_tiles * w.col_tiles, nx = x.row_tiles * x.col_tiles;
-  h8v ident[2];
+  E8 ident[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ident[s][i] = 16 * s + 8 * h + i == (lane & 31) ? (_Float16)1.f : (_Float16)0.f;
+    for (int i = 0; i < 8; ++i) ident[s][i] = 16 * s + 8 * h + i == (lane & 31) ? (typename F::E)1.f : (typename F::E)0.f;
   for (; u < nw + nx; u += step) {
     const bool first = u < nw;
     const TransposeJob &j = first ? w : x;
@@ -343,7 +346,7 @@ __device__ __forceinline__ void transpose_tiles(const TransposeJob &w, const Tra
 #pragma unroll
     for (int pl = 0; pl < FROM; ++pl)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) tr = mfma(__builtin_bit_cast(h8v, src[pl * j.plane + s * 64]), ident[s], tr);
+      for (int s = 0; s < 2; ++s) tr = mfma(__builtin_bit_cast(E8, src[pl * j.plane + s * 64]), ident[s], tr);
     u4v *dst = j.dst + (ct * j.row_tiles + rt) * 128 + lane;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -351,6 +354,10 @@ __device__ __forceinline__ void transpose_tiles(const TransposeJob &w, const Tra
       b8v o[TO];
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = tr[8 * s + k];
+      if constexpr (FROM == 2) {   // every row to the copy's scale
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], *j.exp - j.exps[rt * 32 + slot_place(s, h, k)]);
+      }
       bf16_pieces<TO>(v, o);
 #pragma unroll
       for (int pl = 0; pl < TO; ++pl) dst[pl * j.plane + s * 64] = __builtin_bit_cast(u4v, o[pl]);
@@ -442,7 +449,10 @@ struct GemmArgs {
   const Scalars *scal;
   const int *exp_g;            // DW: packed gradient = G * 2^exp_g
   float scale;
-  // STATS, GRAD
+  // STATS, GRAD: logit in the log2 domain = accumulator * 2^(exp_c - exps_a[word] - exps_b[row]) * c
+  const int *exps_a, *exps_b;  // float32 input: from the first word of the piece on, and of the rows
+  int exp_c;
+  float c;
   int64_t P, V, v0;            // v0: first word of the piece
   const int64_t *labels;
   float2 *partial;             // STATS: [pair][Pp]
@@ -503,6 +513,8 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
   const bool late = wave >= WAVES / 2;
+  constexpr bool SCALED = (MODE == STATS || MODE == GRAD) && NA == 2;
+  __shared__ __attribute__((aligned(16))) int word_exp[SCALED ? 2 : 1][SCALED ? 64 * MT : 1];   // of this tile and the next
 
   // Workgroups go to the eight XCDs in turn: each XCD takes a run of consecutive tiles, ordered as bands of eight
   // M tiles walked along N, so that its L2 holds the operands of the tiles it works on together.
@@ -590,7 +602,7 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
   place(tile);
   fill(0);
   if (stages > 1) fill(1);
-  for (;;) {
+  for (int turn = 0;; turn ^= 1) {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -604,6 +616,13 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
     // what the epilogue needs of its rows, ahead of the loads that it would wait for otherwise
     int place_of[NT];             // the label's place among this wavefront's words, or something out of their range
     float top2[NT], coef_a[NT], coef_b[NT];
+    int row_exp[NT];
+    if constexpr (SCALED) {
+      // (the other half is still being read by wavefronts that are an epilogue behind; they are done before the next write)
+      if ((int)threadIdx.x < 64 * MT) word_exp[turn][threadIdx.x] = g.exps_a[min(m_tile * 64 * MT + (int)threadIdx.x, g.a_tiles * 32 - 1)];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) row_exp[n] = g.exp_c - g.exps_b[n0 + 32 * n];
+    }
     if constexpr (MODE == STATS || MODE == GRAD) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -648,13 +667,25 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
     // accumulator register r of tile (i, n): row m0 + 32 i + (r & 3) + 8 (r >> 2) + 4 h of A, row n0 + 32 n of B
 
     if constexpr (MODE == STATS || MODE == GRAD) {
-      const float c = ldexpf(fabsf(g.scale) * LOG2E, -(g.scal->exp_x + g.scal->exp_w));
+      const float c = g.c;
       // words of this wavefront that exist, from this lane's first one on: compared with constants below
       const int left = (int)min(g.V - (g.v0 + m0), (int64_t)(32 * MT)) - 4 * h;
       const bool whole = g.V - (g.v0 + m0) >= 32 * MT;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int64_t p = n0 + 32 * n;
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int4 e = *reinterpret_cast<const int4 *>(&word_exp[turn][wm * 32 * MT + 32 * i + 8 * q + 4 * h]);
+              acc[i][n][4 * q] = ldexpf(acc[i][n][4 * q], row_exp[n] - e.x);
+              acc[i][n][4 * q + 1] = ldexpf(acc[i][n][4 * q + 1], row_exp[n] - e.y);
+              acc[i][n][4 * q + 2] = ldexpf(acc[i][n][4 * q + 2], row_exp[n] - e.z);
+              acc[i][n][4 * q + 3] = ldexpf(acc[i][n][4 * q + 3], row_exp[n] - e.w);
+            }
+        }
         const bool mine = place_of[n] >= 0;
         const int at = place_of[n] - 4 * h;    // from this lane's first word on; the other half's places match no constant
         const bool here = __any(mine);
@@ -1699,11 +1730,19 @@ struct Kept {  // what the forward pass leaves for the backward pass
   Scalars *scal;
   float2 *stat;
   u4v *xf, *wf;
+  int *ex, *ew;   // float32: exponents of the packed rows
   Kept(Carve &c, const Shape &s) {
     scal = c.take<Scalars>(1);
     stat = c.take<float2>(s.Pp);
     xf = c.take<u4v>(s.np * s.plane(s.Pp));
     wf = c.take<u4v>(s.np * s.plane(s.Vp));
+    ex = c.take<int>(s.np == 2 ? s.Pp : 0);
+    ew = c.take<int>(s.np == 2 ? s.Vp : 0);
+  }
+  // what the logits' products need besides the operands; words from v0 on
+  void scales(const Shape &s, float scale, int64_t v0, GemmArgs &g) const {
+    g.c = fabsf(scale) * LOG2E, g.exp_c = 0;
+    if (s.np == 2) g.exps_a = ew + v0, g.exps_b = ex, g.c = frexpf(g.c, &g.exp_c);
   }
 };
 
@@ -1813,11 +1852,11 @@ double tile_time(int products, int64_t tiles, int mt) {
   return ((double)(tiles / CUS) + (tiles % CUS ? 0.75 : 0.)) * (mt * products + (products == 1 ? 1.5 : 1.8));
 }
 
-// Words per workgroup of STATS and GRAD, in units of 64.
+// Words per workgroup of STATS and GRAD, in units of 64: up to five, four with two planes, whose exponents take the registers.
 int word_units(int planes, int64_t words, int64_t rows) {
-  const int products = planes == 1 ? 1 : 3;
+  const int products = planes == 1 ? 1 : 3, most = planes == 1 ? 5 : 4;
   int best = 1;
-  for (int mt = 2; mt <= 5; ++mt) {
+  for (int mt = 2; mt <= most; ++mt) {
     auto time = [&](int m) { return tile_time(products, (words + 64 * m - 1) / (64 * m) * ((rows + 255) / 256), m); };
     if (time(mt) < time(best)) best = mt;
   }
@@ -1831,7 +1870,9 @@ int launch_words(const GemmArgs &g, int64_t words, int64_t rows, hipStream_t st)
     case 2: return launch_tiles<T, 2, MODE>(p, nullptr, st);
     case 3: return launch_tiles<T, 3, MODE>(p, nullptr, st);
     case 4: return launch_tiles<T, 4, MODE>(p, nullptr, st);
-    default: return launch_tiles<T, 5, MODE>(p, nullptr, st);
+    default:
+      if constexpr (Types<T>::Logits::NA == 1) return launch_tiles<T, 5, MODE>(p, nullptr, st);
+      return PR_EUNSUPPORTED;   // (no choice of word_units)
   }
 }
 
@@ -1866,27 +1907,30 @@ struct Call {
 template <typename T>
 int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, float *lse, float *loss, hipStream_t st) {
   const Shape s(c.dtype, c.P, c.V, c.D);
-  const bool scaled = c.dtype != PR_F16;
-  // 64 elements a thread, or four rows a wavefront, until the chip is full
-  auto amax_blocks = [&](int64_t n) { return scaled ? (int)std::min<int64_t>(AMAX_BLOCKS, n) : 0; };
-  const AmaxJob aw{c.w, nullptr, 0, amax_blocks((c.V * ((c.D + 7) / 8) + 2047) / 2048)};
-  const AmaxJob ax{c.x, c.labels, c.ignore, amax_blocks((c.P + 15) / 16)};
-  if (scaled) {
-    hipLaunchKernelGGL((vce_amax_kernel<T>), dim3(aw.blocks + ax.blocks), dim3(256), 0, st, aw, ax, f.amax);
+  const int kb = (int)(s.Dk / 16);
+  int w_blocks = 0, x_blocks = 0;
+  if (s.np == 2) {
+    int lanes = 1;
+    while (lanes < 64 && lanes * 8 < c.D) lanes *= 2;
+    const int rows = 16 * (64 / lanes);   // of a workgroup at a time
+    auto blocks = [&](int64_t padded) { return (int)std::min<int64_t>(AMAX_BLOCKS, (padded + rows - 1) / rows); };
+    w_blocks = blocks(s.Vp), x_blocks = blocks(s.Pp);
+    const AmaxJob aw{c.w, nullptr, 0, w_blocks, s.Vp, k.ew}, ax{c.x, c.labels, c.ignore, x_blocks, s.Pp, k.ex};
+    hipLaunchKernelGGL((vce_amax_kernel<T>), dim3(w_blocks + x_blocks), dim3(256), 0, st, aw, ax, lanes, f.amax);
     PR_TRY(check_launch("pr_vocab_ce"));
   }
-  const int kb = (int)(s.Dk / 16);
-  const PackJob jw{c.w, nullptr, 0, k.wf, s.plane(s.Vp), s.Vp / 32 * ((kb + 3) / 4), kb, aw.blocks, 1.f};
-  const PackJob jx{c.x, c.labels, c.ignore, k.xf, s.plane(s.Pp), s.Pp / 32 * ((kb + 3) / 4), kb, ax.blocks,
-                   c.scale < 0.f ? -1.f : 1.f};
+  const PackJob jw{c.w, nullptr, 0, k.wf, s.plane(s.Vp), s.Vp / 32 * ((kb + 3) / 4), kb, w_blocks, s.np == 2 ? k.ew : nullptr, 1.f};
+  const PackJob jx{c.x, c.labels, c.ignore, k.xf, s.plane(s.Pp), s.Pp / 32 * ((kb + 3) / 4), kb, x_blocks,
+                   s.np == 2 ? k.ex : nullptr, c.scale < 0.f ? -1.f : 1.f};
   const int64_t pack_blocks = std::min<int64_t>(2048, (jw.units + jx.units + 3) / 4);
-  hipLaunchKernelGGL((vce_pack_kernel<T, Types<T>::Logits::NA>), dim3((unsigned)pack_blocks), dim3(256), 0, st, jw, jx, f.amax, k.scal);
+  hipLaunchKernelGGL((vce_pack_kernel<T>), dim3((unsigned)pack_blocks), dim3(256), 0, st, jw, jx, f.amax, k.scal);
   PR_TRY(check_launch("pr_vocab_ce"));
   GemmArgs g{};
   g.A = k.wf, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
   g.kblocks = g.k_split = kb, g.splits = 1;
   g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.labels = c.labels;
   g.partial = f.partial, g.target = f.target, g.Pp = s.Pp;
+  k.scales(s, c.scale, 0, g);
   PR_TRY((launch_words<T, STATS>(g, s.Vp, s.Pp, st)));
   const RowsOut rows{c.P, c.V, c.ignore, c.labels, f.target, k.stat, lse, row_loss};
   hipLaunchKernelGGL(vce_join_kernel, dim3((unsigned)(s.Pp / 8)), dim3(256), 0, st, rows, s.Pp, f.pairs, f.partial);
@@ -2046,8 +2090,8 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
   const Shape s(c.dtype, c.P, c.V, c.D);
   const int kb = (int)(s.Dk / 16), kv = (int)(s.Vp / 16), kp = (int)(s.Pp / 16);
   const CoefJob coef{c.P, s.Pp, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, k.stat, b.exp_g, b.coef_a, b.coef_b};
-  const TransposeJob tw{k.wf, b.wt, s.plane(s.Vp), dx ? s.Vp / 32 : 0, s.Dk / 32};
-  const TransposeJob tx{k.xf, b.xt, s.plane(s.Pp), dw ? s.Pp / 32 : 0, s.Dk / 32};
+  const TransposeJob tw{k.wf, b.wt, s.plane(s.Vp), dx ? s.Vp / 32 : 0, s.Dk / 32, k.ew, &k.scal->exp_w};
+  const TransposeJob tx{k.xf, b.xt, s.plane(s.Pp), dw ? s.Pp / 32 : 0, s.Dk / 32, k.ex, &k.scal->exp_x};
   const int64_t turns = ((tw.row_tiles + tx.row_tiles) * (s.Dk / 32) + 15) / 16;
   hipLaunchKernelGGL(vce_prepare_kernel<T>, dim3((unsigned)((s.Pp + COEF_ROWS - 1) / COEF_ROWS + std::min<int64_t>(1024, turns))),
                      dim3(1024), 0, st, coef, tw, tx);
@@ -2058,6 +2102,7 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
     g.A = k.wf + v0 / 32 * kb * 64, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
     g.kblocks = g.k_split = kb, g.splits = 1, g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.v0 = v0, g.labels = c.labels, g.Pp = s.Pp;
     g.stat = k.stat, g.coef_a = b.coef_a, g.coef_b = b.coef_b;
+    k.scales(s, c.scale, v0, g);
     g.gx = dx ? b.gx : nullptr, g.gw = dw ? b.gw : nullptr;
     g.plane_gx = g.plane_gw = s.Pp * b.piece / 8, g.ld_gx = b.piece / 16, g.ld_gw = kp;
     PR_TRY((launch_words<T, GRAD>(g, words, s.Pp, st)));

@@ -5,8 +5,11 @@ are trained and scored on when every pixel has a label in a table of phrase embe
 ``torch.nn.functional.cross_entropy(scale * features @ vocabulary.T, labels)``, without the ``[rows, words]`` logits: the
 forward pass keeps one maximum and sum a row, the backward pass makes the products again for one piece of the vocabulary
 at a time.  (Up to 128 rows of a large vocabulary do keep them for it, 4 bytes each, and read the vocabulary as it is.)
-Products take 16-bit operands and add in float32; float32 inputs are split into two float16 planes or three bfloat16 pieces
-(2^-21 of a product at most is left out), so float32 stays float32 in accuracy.  Results do not depend on the order in
+Products take 16-bit operands and add in float32.  Of float32 input 2^-21 of a product at most is left out: few rows take it
+in three bfloat16 pieces, all 24 bits; otherwise the logits take every row and every word by a power of two of its own, in 22
+bits (a value below 2^-15 of its row's largest to 2^-38 of that).  The gradients' products are made of bfloat16 pieces, which
+hold each softmax entry to 2^-24 (float32 input) or 2^-16, whatever the other rows' and words' sizes and weights are.
+Results do not depend on the order in
 which workgroups run.  HIP kernels only (``pr_vocab_ce_fwd``, ``pr_vocab_ce_bwd``); there is no CPU path.
 """
 from __future__ import annotations

@@ -166,3 +166,45 @@ def test_logits_far_beyond_the_differences_that_float32_holds(P, V, D, exponent,
         v = scale * torch.mm(gr, m.double())
         bound = scale * torch.mm(gr.abs(), m.double().abs()) * held + HALF[dtype] * 1.01 * v.abs() + 2.0 ** -80
         close(got[k], (v, bound), k, tight=0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("P,V,D", [(300, 1000, 64), (257, 333, 136), (140, 700, 512), (100, 9000, 64)])
+@pytest.mark.parametrize("exponent", [40, -40, 90])
+@pytest.mark.parametrize("which", ["row", "word"])
+def test_one_row_or_word_of_another_magnitude(P, V, D, exponent, which, dtype):
+    """A row (or word) 2^40 or 2^90 times as large as the others, or as small, counts as one row (word): the others keep
+    their values."""
+    x, w, y, g = inputs(P, V, D, dtype, seed=P + exponent)
+    odd = 37
+    t = x if which == "row" else w
+    t[odd] = (t[odd].double() * 2.0 ** exponent).to(dtype)
+    up = torch.randn(P, generator=g).cuda()
+    ref = reference(x, w, y, 2.0, up)
+    got = run(x, w, y, 2.0, up)
+    z = 2.0 * torch.mm(x.double(), w.double().t().contiguous())
+    others = (z.abs() < 1e4).all(dim=1) if which == "row" else z[:, odd] < 1e3    # rows that do not take the odd word alone
+    assert others.sum() > P // 3
+    for k in ("loss", "lse", "dx"):
+        close(got[k], ref[k], k, rows=others if got[k].dim() == 1 else others[:, None])
+    words = torch.ones(V, dtype=torch.bool, device="cuda")
+    if exponent > 0 and which == "row":           # the words that the odd row moves hold its gradient, of its size
+        words[y[odd]] = words[z[odd].argmax()] = False
+    elif exponent > 0:
+        words[odd] = False
+    close(got["dw"], ref["dw"], "dw", rows=words[:, None], tight=0.3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("P,V,D", [(300, 1000, 64), (130, 500, 33), (1025, 400, 8)])
+@pytest.mark.parametrize("which", ["rows", "words"])
+def test_rows_or_words_over_many_powers_of_two(P, V, D, which):
+    x, w, y, g = inputs(P, V, D, torch.float32, seed=P)
+    t = x if which == "rows" else w
+    t *= (2.0 ** torch.randint(-60, 1, (len(t),), generator=g).double()).float().cuda()[:, None]
+    up = torch.ones(P, device="cuda")
+    ref = reference(x, w, y, 3.0, up)
+    got = run(x, w, y, 3.0, up)
+    for k in ("loss", "lse", "dx", "dw"):
+        close(got[k], ref[k], k)
