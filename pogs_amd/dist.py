@@ -334,10 +334,12 @@ class ShardedExchange:
         return fire
 
     def finish_step(self) -> None:
-        """After ``backward()``: starts the buckets whose hooks did not all fire (a parameter no gradient reached)."""
+        """After ``backward()``: starts the buckets whose hooks did not all fire (a parameter no gradient reached), and
+        tells autograd that the parameters have been written, so that a graph that saved one is refused."""
         for b in self.buckets:
             if not b.launched:
                 self._launch(b)
+        torch.autograd.graph.increment_version(list(self.params.values()))
 
     @torch.no_grad()
     def _launch(self, b: _Bucket) -> None:

@@ -250,7 +250,7 @@ class Optimizers:
                 raise ValueError("a max_norm over all groups and a max_norm of a group's own exclude each other")
         if max_norm is not None or any(m is not None for m in limits):
             limits = self._check_clipped(param_groups, limits)       # before any state is touched
-        entries, rules, keep = [], [], []        # rules: (group or None for all together, its limit or None)
+        entries, rules, keep, stepped = [], [], [], []     # rules: (group or None for all together, its limit or None)
         for name, limit in zip(param_groups, limits):
             cfg = self.config[name]
             b1, b2 = cfg.get("betas", (0.9, 0.999))
@@ -268,6 +268,7 @@ class Optimizers:
                 st["step"] += 1
                 rules.append((None, max_norm) if max_norm is not None else (name, limit))
                 keep.append(g)
+                stepped.append(p)
                 entries.append(_ADAM_GROUP.pack(p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(),
                                                 st["exp_avg_sq"].data_ptr(), p.numel(), st["step"], lr, b1, b2, eps))
         self._norms, self._norm_of = [], None
@@ -282,6 +283,7 @@ class Optimizers:
                     _call("pr_adam_step", b"".join(part), len(part), _raw_stream(dev.index))
             else:
                 self._step_clipped(entries, rules, param_groups, dev, _raw_stream(dev.index))
+        torch.autograd.graph.increment_version(stepped)     # written in place: a graph that saved one is refused
         del keep
 
     def _check_clipped(self, param_groups: List[str], limits: list) -> List[Optional[float]]:

@@ -326,3 +326,21 @@ def test_sharded_exchange_single_process_is_plain_adam():
             o.step()
     for k in p:
         assert torch.allclose(p[k], q[k], rtol=1e-12, atol=1e-14), k
+
+
+def test_a_graph_that_saved_a_parameter_is_refused_after_the_exchange_has_stepped_it():
+    from pogs_amd.dist import ShardedExchange
+
+    p = {k: v.clone().requires_grad_(True) for k, v in _toy_params(50).items()}
+    ex = ShardedExchange(p, _TorchAdamShards(_LRS), big_bytes=1 << 30)
+    old = _toy_loss(p, 0, 0)
+    ex.begin_step()
+    _toy_loss(p, 0, 1).backward()
+    ex.finish_step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        old.backward()
+    for t in p.values():
+        t.grad = None
+    ex.begin_step()
+    _toy_loss(p, 0, 2).backward()       # a new graph is not
+    ex.finish_step()

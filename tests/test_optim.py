@@ -131,3 +131,27 @@ def test_ragged_sizes_and_many_tensors():
         opt.optimizer_step_all()
     for p, q in zip(ref_p, dev_p):
         assert (q.detach().cpu() - p.detach()).abs().max().item() <= 2e-6 * max(p.detach().abs().max().item(), 1e-3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [None, 1e-3])
+def test_a_graph_that_saved_a_parameter_is_refused_after_its_step(gpu, max_norm):
+    """A loss of few rows reads the vocabulary again in its backward pass: after a step of the vocabulary that would mix its
+    old logits with new words."""
+    from pogs_amd.optim import Optimizers
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    g = torch.Generator().manual_seed(3)
+    words = torch.randn(9000, 64, generator=g).cuda().requires_grad_(True)
+    x = torch.randn(20, 64, generator=g).cuda().requires_grad_(True)
+    y = torch.randint(0, 9000, (20,), generator=g).cuda()
+    opt = Optimizers({"words": {"lr": 1e-2, "max_norm": max_norm}}, {"words": [words]})
+    first, second = vocabulary_cross_entropy(x, words, y), (words * words).sum()
+    vocabulary_cross_entropy(x, words, y).backward()
+    before = words._version
+    opt.optimizer_step_all()
+    assert words._version > before
+    for old in (first, second):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            old.backward()
+    vocabulary_cross_entropy(x, words, y).backward()
