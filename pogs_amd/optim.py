@@ -26,7 +26,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .rendering import _call, _on, _raw_stream
+from .rendering import _call, _on, _raw_stream, _refuse_dual
 
 
 _ADAM_GROUP = struct.Struct("=4Q2q4d")     # pr_adam_group
@@ -100,11 +100,13 @@ def grad_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) 
     """Norm over all elements of all ``tensors`` (gradients; float32, float16 or bfloat16 in any mix and layout) as a
     0-d float32 tensor on their device.  Counterpart of ``torch.nn.utils.get_total_norm`` for ``norm_type`` 1, 2 and inf.
     Sums are kept in float64, in an order that depends on the sizes alone: equal inputs give equal bits.  No host
-    synchronisation; safe in a captured graph.  An empty list has norm 0 (on the CPU, as in torch)."""
+    synchronisation; safe in a captured graph.  A plain number to autograd, as in torch; forward-mode tensors are refused.
+    An empty list has norm 0 (on the CPU, as in torch)."""
     kind = _norm_kind(norm_type)
     grads = [tensors] if isinstance(tensors, Tensor) else list(tensors)
     if not grads:
         return torch.tensor(0.0)
+    _refuse_dual("grad_norm", grads)
     dev = _check_grads(grads)
     lib = _lib.load()
     with _on(dev):

@@ -22,6 +22,7 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from .dist import pending, wait_ready
@@ -45,6 +46,13 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch
 def _on(device: torch.device):
     """Context in which ``device`` is the current one: nothing to do where it already is (the change costs 3 us)."""
     return _HERE if _raw_device() == device.index else torch.cuda.device(device)
+
+
+def _refuse_dual(what: str, tensors) -> None:
+    """Raises if forward-mode differentiation is on and reaches one of the tensors: a kernel that is not behind an autograd
+    function would drop the tangent, which reads as a derivative of zero."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 class StageTimer:

@@ -22,7 +22,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .rendering import _call, _on, _ptr, _raw_stream
+from .rendering import _call, _on, _ptr, _raw_stream, _refuse_dual
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # PR_F32, PR_F16, PR_BF16
 _REDUCTIONS = ("none", "sum", "mean")
@@ -124,6 +124,7 @@ def _check(features: Tensor, vocabulary: Tensor, labels: Tensor, scale: float, r
         raise ValueError(f"scale must be finite (within 1e38), got {scale}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
+    _refuse_dual("vocabulary_cross_entropy", (features, vocabulary))
     if not features.is_cuda:
         raise RuntimeError("pogs_amd.vocabulary runs on a HIP device only (no CPU fallback)")
     if not features.device == vocabulary.device == labels.device:
@@ -141,7 +142,7 @@ def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tenso
     (NaN if there are none, as in torch), their ``"sum"``, or with ``"none"`` one value a row (0 for an ignored one);
     with ``return_lse`` also every row's ``log sum_v exp(scale <x, w_v>)`` (0 for an ignored row).  Differentiable in
     features and vocabulary, through the loss and the log-sum (gradients in the inputs' type, from the formula; not
-    twice).  Ignored rows contribute nothing, even if their features are not finite.  A label that is neither in
+    twice, and not in forward mode, which is refused).  Ignored rows contribute nothing, even if their features are not finite.  A label that is neither in
     ``0..V-1`` nor ``ignore_index`` makes its row's loss NaN and the gradients with it: nothing is read out of range,
     and the host does not wait to look.  Features may be changed in place before the backward pass, labels may not, and
     neither may the vocabulary where it is large and the rows are at most 128 (autograd refuses).  Safe in a captured

@@ -208,3 +208,23 @@ def test_rows_or_words_over_many_powers_of_two(P, V, D, which):
     got = run(x, w, y, 3.0, up)
     for k in ("loss", "lse", "dx", "dw"):
         close(got[k], ref[k], k)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    """A tangent would be dropped, and read as a derivative of zero."""
+    import torch.autograd.forward_ad as fwd
+
+    from pogs_amd.optim import grad_norm
+    from pogs_amd.vocabulary import vocabulary_cross_entropy
+
+    x, w, y = torch.randn(4, 8), torch.randn(5, 8), torch.zeros(4, dtype=torch.int64)
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for args in ((dual, w, y), (dual * 2, w, y), (x, fwd.make_dual(w, w), y)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                vocabulary_cross_entropy(*args)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            grad_norm([x, dual])
+        with pytest.raises(RuntimeError, match="HIP device"):     # a level that no tensor takes part in is none
+            vocabulary_cross_entropy(x, w, y)
