@@ -133,6 +133,19 @@ __device__ __forceinline__ void bf16_pieces(const float (&v)[8], b8v (&out)[N]) 
   for (int i = 0; i < 8; ++i) out[N - 1][i] = (__bf16)r[i];
 }
 
+// A factor as mantissa and exponent: applied together with a power of two that brings a result back, so that neither their
+// product with the other comes near the ends of float32.
+struct Scale {
+  float m;
+  int e;
+  __host__ static Scale of(float v) {
+    Scale s;
+    s.m = frexpf(v, &s.e);
+    return s;
+  }
+  __device__ __forceinline__ float times(float v, int exponent) const { return ldexpf(v * m, e + exponent); }
+};
+
 struct Scalars {  // per call, on the device
   int exp_x, exp_w;  // the transposed copies are value * 2^exp
   float n_valid;     // rows whose label is not the ignored one
@@ -448,7 +461,7 @@ struct GemmArgs {
   int m_tiles, n_tiles, splits;
   const Scalars *scal;
   const int *exp_g;            // DW: packed gradient = G * 2^exp_g
-  float scale;
+  Scale scale;
   // STATS, GRAD: logit in the log2 domain = accumulator * 2^(exp_c - exps_a[word] - exps_b[row]) * c
   const int *exps_a, *exps_b;  // float32 input: from the first word of the piece on, and of the rows
   int exp_c;
@@ -812,7 +825,7 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
             const int d = m0 + 32 * i + 8 * q + 4 * h;
             float x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = ldexpf(acc[i][n][4 * q + k] * fabsf(g.scale), e);  // X's copy has its sign
+            for (int k = 0; k < 4; ++k) x[k] = g.scale.times(acc[i][n][4 * q + k], e);
             T *dst = (T *)g.out + v * g.D + d;
             if ((g.D & 3) == 0) {
               if (d < g.D) store4<T>(dst, x[0], x[1], x[2], x[3]);
@@ -1651,7 +1664,7 @@ __global__ void __launch_bounds__(1024) vce_join_reduce_kernel(RowsOut o, int pa
 struct FinishJob {
   int64_t rows, D, plane, ld;  // rows of the result; rows of a split and their stride in `acc`
   int splits;
-  float scale;
+  Scale scale;
   const float *acc;
   const int *exp_other, *exp_g;
   void *out;
@@ -1675,7 +1688,7 @@ __global__ void __launch_bounds__(256) vce_finish_kernel(const FinishJob a, cons
       const float4 q = *reinterpret_cast<const float4 *>(src + k * j.plane * j.ld);
       v.x += q.x, v.y += q.y, v.z += q.z, v.w += q.w;
     }
-    const float x[4] = {ldexpf(v.x * j.scale, e), ldexpf(v.y * j.scale, e), ldexpf(v.z * j.scale, e), ldexpf(v.w * j.scale, e)};
+    const float x[4] = {j.scale.times(v.x, e), j.scale.times(v.y, e), j.scale.times(v.z, e), j.scale.times(v.w, e)};
     T *dst = (T *)j.out + p * j.D + d;
     if ((j.D & 3) == 0) {
       store4<T>(dst, x[0], x[1], x[2], x[3]);
@@ -1928,7 +1941,7 @@ int forward(const Call &c, int mean, Kept &k, FwdScratch &f, float *row_loss, fl
   GemmArgs g{};
   g.A = k.wf, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
   g.kblocks = g.k_split = kb, g.splits = 1;
-  g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.labels = c.labels;
+  g.P = c.P, g.V = c.V, g.labels = c.labels;
   g.partial = f.partial, g.target = f.target, g.Pp = s.Pp;
   k.scales(s, c.scale, 0, g);
   PR_TRY((launch_words<T, STATS>(g, s.Vp, s.Pp, st)));
@@ -2096,11 +2109,12 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
   hipLaunchKernelGGL(vce_prepare_kernel<T>, dim3((unsigned)((s.Pp + COEF_ROWS - 1) / COEF_ROWS + std::min<int64_t>(1024, turns))),
                      dim3(1024), 0, st, coef, tw, tx);
   PR_TRY(check_launch("pr_vocab_ce"));
+  const Scale abs_scale = Scale::of(fabsf(c.scale));   // X's copy has the sign
   for (int64_t v0 = 0; v0 < s.Vp; v0 += b.piece) {
     const int64_t words = std::min(b.piece, s.Vp - v0);
     GemmArgs g{};
     g.A = k.wf + v0 / 32 * kb * 64, g.B = k.xf, g.plane_a = s.plane(s.Vp), g.plane_b = s.plane(s.Pp), g.ld_a = g.ld_b = kb;
-    g.kblocks = g.k_split = kb, g.splits = 1, g.scal = k.scal, g.scale = c.scale, g.P = c.P, g.V = c.V, g.v0 = v0, g.labels = c.labels, g.Pp = s.Pp;
+    g.kblocks = g.k_split = kb, g.splits = 1, g.P = c.P, g.V = c.V, g.v0 = v0, g.labels = c.labels, g.Pp = s.Pp;
     g.stat = k.stat, g.coef_a = b.coef_a, g.coef_b = b.coef_b;
     k.scales(s, c.scale, v0, g);
     g.gx = dx ? b.gx : nullptr, g.gw = dw ? b.gw : nullptr;
@@ -2110,21 +2124,21 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
     Product px{{}, s.Dk, s.Pp}, pw{{}, s.Dk, words};
     GemmArgs &x = px.g, &w = pw.g;
     x.A = b.wt + v0 / 16 * 64, x.B = b.gx, x.plane_a = s.plane(s.Vp), x.plane_b = g.plane_gx, x.ld_a = kv, x.ld_b = g.ld_gx;
-    x.scal = k.scal, x.acc = b.acc, x.Pp = s.Pp, x.ld_acc = s.Dk, x.add = v0 > 0;
+    x.acc = b.acc, x.Pp = s.Pp, x.ld_acc = s.Dk, x.add = v0 > 0;
     // the splits of a full piece; a shorter last piece leaves the rest of them as they are
     x.kblocks = (int)(words / 16), x.k_split = b.split_words.blocks, x.splits = (x.kblocks + x.k_split - 1) / x.k_split;
     w.A = b.xt, w.B = b.gw, w.plane_a = s.plane(s.Pp), w.plane_b = g.plane_gw, w.ld_a = w.ld_b = kp;
     w.kblocks = kp, w.k_split = b.split_rows.blocks, w.splits = b.split_rows.n;
-    w.scal = k.scal, w.exp_g = b.exp_g, w.scale = c.scale, w.V = c.V, w.v0 = v0, w.out = dw, w.D = c.D;
+    w.scal = k.scal, w.exp_g = b.exp_g, w.scale = abs_scale, w.V = c.V, w.v0 = v0, w.out = dw, w.D = c.D;
     w.acc = b.acc_w, w.Pp = words, w.ld_acc = s.Dk;
     if (dx || split_dw)
       PR_TRY((launch_features<T, DX>(dx ? px : pw, dx && split_dw ? &pw : nullptr, st)));
     if (dw && !split_dw) PR_TRY((launch_features<T, DW>(pw, nullptr, st)));
     FinishJob jobs[2] = {};
     int n = 0;
-    if (dx && last) jobs[n++] = FinishJob{c.P, c.D, s.Pp, s.Dk, b.split_words.n, c.scale, b.acc, &k.scal->exp_w, b.exp_g, dx};
+    if (dx && last) jobs[n++] = FinishJob{c.P, c.D, s.Pp, s.Dk, b.split_words.n, Scale::of(c.scale), b.acc, &k.scal->exp_w, b.exp_g, dx};
     if (split_dw)
-      jobs[n++] = FinishJob{std::min(words, c.V - v0), c.D, words, s.Dk, w.splits, fabsf(c.scale), b.acc_w, &k.scal->exp_x,
+      jobs[n++] = FinishJob{std::min(words, c.V - v0), c.D, words, s.Dk, w.splits, abs_scale, b.acc_w, &k.scal->exp_x,
                             b.exp_g, dw + v0 * c.D};
     if (n) {
       hipLaunchKernelGGL((vce_finish_kernel<T>), dim3((unsigned)((jobs[0].rows + jobs[1].rows + 3) / 4)), dim3(256), 0, st,

@@ -228,3 +228,21 @@ def test_forward_mode_is_refused(grad):
             grad_norm([x, dual])
         with pytest.raises(RuntimeError, match="HIP device"):     # a level that no tensor takes part in is none
             vocabulary_cross_entropy(x, w, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("P,V,D,exp_x,exp_w", [(P, V, D, *e) for P, V, D in ((200, 300, 64), (300, 5000, 64))
+                                               for e in ((-60, -60), (0, -100), (-100, 0), (-100, 4), (40, 60))]
+                         + [(40, 20_000, 32, *e) for e in ((-40, -40), (0, -80), (-80, 0), (40, 60))])
+def test_a_scale_near_the_ends_of_float32(P, V, D, exp_x, exp_w, dtype):
+    """Powers of two that cancel in the logits: the same bits as without them, in the gradients too."""
+    x, w, y, g = inputs(P, V, D, dtype, seed=P)
+    up = torch.randn(P, generator=g).cuda()
+    base = run(x, w, y, 1.0, up)
+    got = run(x * 2.0 ** exp_x, w * 2.0 ** exp_w, y, 2.0 ** -(exp_x + exp_w), up)
+    for k, e in (("loss", 0), ("lse", 0), ("dx", exp_x), ("dw", exp_w)):
+        # (values that the scale takes below the smallest float32 are left out)
+        want, have = base[k].double(), got[k].double() * 2.0 ** e
+        held = (base[k].double() * 2.0 ** -e).abs() > 2.0 ** -125
+        assert torch.isfinite(got[k]).all() and torch.equal(have[held], want[held]), k
