@@ -387,6 +387,8 @@ struct CoefJob {
   const float2 *stat;
   int *exp_g;
   float *a, *b;
+  const float *tops;   // largest factors of parts of the rows, or NULL: every workgroup looks for the largest itself
+  int n_tops;
   // G = ra exp2(logit - maximum) - rb at the label: the sum of the exponentials goes into ra
   __device__ __forceinline__ void row(int64_t p, float one, float &ra, float &rb) const {
     ra = rb = 0.f;
@@ -412,13 +414,29 @@ __device__ __forceinline__ int coef_exponent(float top) { return top > 0.f ? TOP
 
 constexpr int COEF_ROWS = 4096;  // rows whose factors one workgroup writes
 
-// Row factors of G, scaled by coef_exponent.  Every workgroup looks for the largest itself; with one gradient for all rows
-// there is nothing to look for.
+// The largest row factors of many rows, one a workgroup.
+__global__ void __launch_bounds__(1024) vce_largest_kernel(CoefJob c, float *__restrict__ tops) {
+  const float one = c.one();
+  float top = 0.f;
+  for (int64_t p = (int64_t)blockIdx.x * 1024 + threadIdx.x; p < c.P; p += (int64_t)gridDim.x * 1024) c.largest(p, one, top);
+  __shared__ float part[16];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, part[i]);
+  tops[blockIdx.x] = top;
+}
+
+// Row factors of G, scaled by coef_exponent.  With one gradient for all rows there is no largest to look for.
 __device__ __forceinline__ void row_factors(const CoefJob &c, int block) {
   const float one = c.one();
   float top = fabsf(one) < INFINITY ? fabsf(one) : 0.f;
   if (c.per_row || c.g_lse) {
-    for (int64_t p = threadIdx.x; p < c.P; p += 1024) c.largest(p, one, top);
+    if (c.tops) top = (int)threadIdx.x < c.n_tops ? fmaxf(top, c.tops[threadIdx.x]) : top;
+    else
+      for (int64_t p = threadIdx.x; p < c.P; p += 1024) c.largest(p, one, top);
     __shared__ float part[16];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -1794,7 +1812,7 @@ Splits choose_splits(int64_t Dk, int64_t n_rows, int64_t k) {
 
 struct BwdScratch {
   int *exp_g;
-  float *coef_a, *coef_b, *acc, *acc_w;
+  float *tops, *coef_a, *coef_b, *acc, *acc_w;
   u4v *xt, *wt, *gx, *gw;
   int64_t piece;  // words
   Splits split_words, split_rows;  // of the contractions of dX (a full piece's words) and of dW
@@ -1806,6 +1824,7 @@ struct BwdScratch {
     split_words = choose_splits(s.Dk, s.Pp, piece / 16);
     split_rows = choose_splits(s.Dk, piece, s.Pp / 16);
     exp_g = c.take<int>(1);
+    tops = c.take<float>(CUS);
     coef_a = c.take<float>(s.Pp);
     coef_b = c.take<float>(s.Pp);
     acc = c.take<float>(dx ? split_words.n * s.Pp * s.Dk : 0);
@@ -2090,7 +2109,7 @@ template <typename T>
 int few_backward(const Call &c, int per_row, int mean, const FewKept &k, const FewBwdScratch &b, const float *g_loss,
                  const float *g_lse, T *dx, T *dw, hipStream_t st) {
   const FewShape s(c.dtype, c.P, c.V, c.D);
-  const FewGrad f{{c.P, s.R, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, k.stat, nullptr, nullptr, nullptr},
+  const FewGrad f{{c.P, s.R, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, k.stat, nullptr, nullptr, nullptr, nullptr, 0},
                   c.D, s.Dk, k.logits};
   if (s.nb == 1) return few_gradients<T, 1>(c, s, k, b, f, dx, dw, st);
   if (s.nb == 2) return few_gradients<T, 2>(c, s, k, b, f, dx, dw, st);
@@ -2102,7 +2121,15 @@ int backward(const Call &c, int per_row, int mean, const Kept &k, BwdScratch &b,
              T *dw, hipStream_t st) {
   const Shape s(c.dtype, c.P, c.V, c.D);
   const int kb = (int)(s.Dk / 16), kv = (int)(s.Vp / 16), kp = (int)(s.Pp / 16);
-  const CoefJob coef{c.P, s.Pp, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, k.stat, b.exp_g, b.coef_a, b.coef_b};
+  // above one workgroup's rows the largest factor has a launch of its own (2 M rows of 100 words x 512 dims: 29.1 ms without,
+  // when 507 workgroups each look through all rows)
+  const bool search = (per_row || g_lse) && s.Pp > COEF_ROWS;
+  const CoefJob coef{c.P, s.Pp, c.V, c.ignore, c.labels, g_loss, g_lse, per_row, mean, k.scal, k.stat, b.exp_g, b.coef_a, b.coef_b, search ? b.tops : nullptr,
+                     (int)std::min<int64_t>(CUS, (c.P + 1023) / 1024)};
+  if (search) {
+    hipLaunchKernelGGL(vce_largest_kernel, dim3(coef.n_tops), dim3(1024), 0, st, coef, b.tops);
+    PR_TRY(check_launch("pr_vocab_ce"));
+  }
   const TransposeJob tw{k.wf, b.wt, s.plane(s.Vp), dx ? s.Vp / 32 : 0, s.Dk / 32, k.ew, &k.scal->exp_w};
   const TransposeJob tx{k.xf, b.xt, s.plane(s.Pp), dw ? s.Pp / 32 : 0, s.Dk / 32, k.ex, &k.scal->exp_x};
   const int64_t turns = ((tw.row_tiles + tx.row_tiles) * (s.Dk / 32) + 15) / 16;

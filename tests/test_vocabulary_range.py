@@ -246,3 +246,16 @@ def test_a_scale_near_the_ends_of_float32(P, V, D, exp_x, exp_w, dtype):
         want, have = base[k].double(), got[k].double() * 2.0 ** e
         held = (base[k].double() * 2.0 ** -e).abs() > 2.0 ** -125
         assert torch.isfinite(got[k]).all() and torch.equal(have[held], want[held]), k
+
+
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("P", [4096, 4097, 9001])
+def test_many_rows_of_very_different_weight(P, dtype):
+    """More rows than one workgroup makes the factors of; the largest is in the last one's."""
+    x, w, y, g = inputs(P, 300, 32, dtype, seed=P)
+    weight = torch.logspace(-4, 3, P).cuda() * (1e-4 if dtype == torch.float32 else 1.0)
+    ref = reference(x, w, y, 2.0, weight)
+    got = run(x, w, y, 2.0, weight)
+    for k in ("loss", "lse", "dx", "dw"):
+        close(got[k], ref[k], k, tight=0.2 if k == "dw" else 0.5)
