@@ -25,8 +25,9 @@ PASSES = 6
 IGN = -100
 
 
-def reference(x, w, labels, scale, up, ignore=IGN):
-    """Values and bounds in float64: loss, lse, dx and dw; up: the rows' upstream gradients of the loss."""
+def reference(x, w, labels, scale, up, ignore=IGN, exact=False):
+    """Values and bounds in float64: loss, lse, dx and dw; up: the rows' upstream gradients of the loss.  exact: every sum of
+    a logit is a float32 number, so that only the scale rounds it."""
     dtype, (P, D), V = x.dtype, x.shape, w.shape[0]
     tau = 3 * 2.0 ** -22 if dtype == torch.float32 else 0.0
     held = 2.0 ** -21 if dtype == torch.float32 else 2.0 ** -15
@@ -39,6 +40,8 @@ def reference(x, w, labels, scale, up, ignore=IGN):
     xmax, wmax = x.abs().amax(1), w.abs().amax(1)
     dz = abs(scale) * (torch.mm(x.abs(), w.abs().t().contiguous()) * (tau + (PASSES * D / 16 + 16) * U)
                        + planes * D * xmax[:, None] * wmax)
+    if exact:
+        dz = 4 * U * z.abs()
     lse = torch.logsumexp(z, 1)
     p = (z - lse[:, None]).exp()
     # a word's logit counts in the log-sum as far as it is probable
@@ -259,3 +262,32 @@ def test_many_rows_of_very_different_weight(P, dtype):
     got = run(x, w, y, 2.0, weight)
     for k in ("loss", "lse", "dx", "dw"):
         close(got[k], ref[k], k, tight=0.2 if k == "dw" else 0.5)
+
+
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("P,V,D", [(17, 3, 700_001), (2, 3, 1_040_000), (129, 5, 60_003)])
+@pytest.mark.parametrize("sparse", ["features", "vocabulary"])
+def test_many_features(P, V, D, sparse, dtype):
+    """Eighths of small whole numbers, and zeros but for some 300 columns in one of the factors: logits are exact in any
+    order of their sum, so the width of the rows leaves no room in the bounds, and the other factor fills every column of
+    the gradient that is made of it."""
+    g = torch.Generator().manual_seed(P)
+    x, w = (torch.randint(1, 4, (n, D), generator=g) * (2 * torch.randint(0, 2, (n, D), generator=g) - 1) / 8.0 for n in (P, V))
+    edges = [0, 1, 7, 8, 31, 32, 63, 64, 255, 256, 511, 512, 4095, 4096, 65535 % D, D // 2, D - 257, D - 65, D - 33, D - 9, D - 2, D - 1]
+    keep = torch.zeros(D)
+    keep[torch.cat([torch.tensor(edges), torch.randint(0, D, (280,), generator=g)])] = 1.0
+    if sparse == "features":
+        x = x * keep
+    else:
+        w = w * keep
+    x, w = x.to(dtype).cuda(), w.to(dtype).cuda()
+    y = torch.randint(0, V, (P,), generator=g).cuda()
+    up = torch.randn(P, generator=g).cuda()
+    ref = reference(x, w, y, 0.25, up, exact=True)
+    got = run(x, w, y, 0.25, up)
+    for k in ("loss", "lse", "dx", "dw"):
+        close(got[k], ref[k], k, tight=0.0 if sparse == {"dx": "vocabulary", "dw": "features"}.get(k) else 0.9)
+    # nothing reaches a column in which the other factor is zero
+    none = keep.cuda() == 0
+    assert (got["dw" if sparse == "features" else "dx"][:, none] == 0).all()
