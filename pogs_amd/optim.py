@@ -240,11 +240,12 @@ class Optimizers:
     def optimizer_step_all(self, max_norm: Optional[float] = None) -> None:
         self.optimizer_step_some(list(self.parameters), max_norm)
 
-    def optimizer_step_some(self, param_groups: List[str], max_norm: Optional[float] = None) -> None:
+    def optimizer_step_some(self, param_groups: Iterable[str], max_norm: Optional[float] = None) -> None:
         """One Adam update of every parameter (that has a gradient) of the named groups, in one launch per
         ``pr_adam_max_groups()`` tensors.  Groups with a ``max_norm`` of their own are clipped one by one; ``max_norm``
         given here clips the gradient of all the named groups together to one norm instead, and then none of them may
         have its own."""
+        param_groups = list(param_groups)        # gone through more than once
         limits = [self.config[name].get("max_norm") for name in param_groups]
         if max_norm is not None:
             max_norm = _max_norm(max_norm)

@@ -458,3 +458,12 @@ def test_matches_torch_clip_grad_norm():
     assert abs(n.item() - m.item()) <= 1e-6 * m.item()
     for x, y in zip(a, b):
         assert ((x.grad - y.grad).abs() <= 2e-6 * y.grad.abs()).all()
+
+
+def test_clipped_steps_of_an_iterator_are_refused_before_they_begin():
+    from pogs_amd.optim import Optimizers
+
+    p = _OnADevice(0)
+    free = Optimizers({"a": {"lr": 1e-3}}, {"a": [p, p]})
+    with pytest.raises(ValueError, match="twice"):
+        free.optimizer_step_some(iter(["a"]), max_norm=1.0)

@@ -155,3 +155,17 @@ def test_a_graph_that_saved_a_parameter_is_refused_after_its_step(gpu, max_norm)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             old.backward()
     vocabulary_cross_entropy(x, words, y).backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [None, 1e-3])
+def test_groups_named_by_an_iterator_are_stepped(gpu, max_norm):
+    from pogs_amd.optim import Optimizers
+
+    p = torch.ones(8, device=gpu, requires_grad=True)
+    p.grad = torch.ones_like(p)
+    opt = Optimizers({"a": {"lr": 1e-2}, "b": {"lr": 1e-2}}, {"a": [p], "b": []})
+    opt.optimizer_step_some((n for n in ("a", "b")), max_norm)
+    assert opt.state("a")["step"] == 1 and (p < 1).all()
+    opt.optimizer_step_some(filter(None, ["a"]))
+    assert opt.state("a")["step"] == 2
