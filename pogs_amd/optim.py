@@ -127,7 +127,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
 
     Gradients may be float32, float16 or bfloat16, of any layout, all on one device and in memory of their own: two that
     begin at the same place (a parameter listed twice) or whose blocks overlap are refused, as scaling them at once is a
-    race.  Each value is rounded once, to its own type.  Where the norm is within bounds no gradient is written.  A norm that is not finite
+    race, and so is an expanded one; then nothing has been scaled.  Each value is rounded once, to its own type.  Where the norm is within bounds no gradient is written.  A norm that is not finite
     gives what torch gives: factor 0 for an infinite norm, NaN for a NaN one; ``error_if_nonfinite`` raises instead, and
     only then does the host wait for the device."""
     kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
@@ -146,6 +146,8 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
             starts = [g.data_ptr() for g in grads if g.numel()]
             if len(set(starts)) < len(starts):
                 raise RuntimeError("clip_grad_norm_: two gradients share memory")
+            if any([0 in g.stride() and any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)) for g in grads]):
+                raise RuntimeError("clip_grad_norm_: an expanded gradient cannot be scaled in place")
         table, limit = _grad_table(flat), ctypes.c_double(max_norm)
         at, n = _address(table), len(flat)
         nbytes = lib.pr_grad_norm_scratch_bytes(at, n, 1)

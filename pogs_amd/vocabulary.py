@@ -9,8 +9,8 @@ Products take 16-bit operands and add in float32.  Of float32 input 2^-21 of a p
 in three bfloat16 pieces, all 24 bits; otherwise the logits take every row and every word by a power of two of its own, in 22
 bits (a value below 2^-15 of its row's largest to 2^-38 of that).  The gradients' products are made of bfloat16 pieces, which
 hold each softmax entry to 2^-24 (float32 input) or 2^-16, whatever the other rows' and words' sizes and weights are.
-Results do not depend on the order in
-which workgroups run.  HIP kernels only (``pr_vocab_ce_fwd``, ``pr_vocab_ce_bwd``); there is no CPU path.
+Results do not depend on the order in which workgroups run; a call with gradients to come and one without may take different
+kernels and differ in the last bits.  HIP kernels only (``pr_vocab_ce_fwd``, ``pr_vocab_ce_bwd``); there is no CPU path.
 """
 from __future__ import annotations
 
@@ -142,7 +142,8 @@ def vocabulary_cross_entropy(features: Tensor, vocabulary: Tensor, labels: Tenso
     (NaN if there are none, as in torch), their ``"sum"``, or with ``"none"`` one value a row (0 for an ignored one);
     with ``return_lse`` also every row's ``log sum_v exp(scale <x, w_v>)`` (0 for an ignored row).  Differentiable in
     features and vocabulary, through the loss and the log-sum (gradients in the inputs' type, from the formula; not
-    twice, and not in forward mode, which is refused).  Ignored rows contribute nothing, even if their features are not finite.  A label that is neither in
+    twice, and not in forward mode, which is refused).  Ignored rows contribute nothing, even if their features are not finite; the loss and log-sum of a row with an
+    infinite logit are NaN.  A label that is neither in
     ``0..V-1`` nor ``ignore_index`` makes its row's loss NaN and the gradients with it: nothing is read out of range,
     and the host does not wait to look.  Features may be changed in place before the backward pass, labels may not, and
     neither may the vocabulary where it is large and the rows are at most 128 (autograd refuses).  Safe in a captured

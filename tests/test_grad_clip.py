@@ -467,3 +467,19 @@ def test_clipped_steps_of_an_iterator_are_refused_before_they_begin():
     free = Optimizers({"a": {"lr": 1e-3}}, {"a": [p, p]})
     with pytest.raises(ValueError, match="twice"):
         free.optimizer_step_some(iter(["a"]), max_norm=1.0)
+
+
+@pytest.mark.gpu
+def test_an_expanded_gradient_is_refused_before_anything_is_scaled(gpu):
+    from pogs_amd.optim import clip_grad_norm_, grad_norm
+
+    p, q = torch.zeros(64, device=gpu, requires_grad=True), torch.zeros(8, 4, device=gpu, requires_grad=True)
+    p.grad, q.grad = torch.ones(64, device=gpu), torch.ones(8, 1, device=gpu).expand(8, 4)
+    with pytest.raises(RuntimeError, match="expanded"):
+        clip_grad_norm_([p, q], 0.5)
+    assert (p.grad == 1).all() and (q.grad == 1).all()
+    assert grad_norm([p.grad, q.grad]).item() == pytest.approx(96 ** 0.5, rel=1e-6)
+    one = torch.zeros(1, 6, device=gpu, requires_grad=True)       # of one row only: nothing is written twice
+    one.grad = torch.ones(12, device=gpu).as_strided((1, 6), (0, 2))
+    assert clip_grad_norm_([p, one], 0.5).item() == pytest.approx(70 ** 0.5, rel=1e-6)
+    assert torch.equal(one.grad[0], p.grad[:6]) and (p.grad < 0.1).all()
