@@ -37,9 +37,9 @@
 // G of one piece of the vocabulary is all that is ever held of the P x V logits.
 //
 // Bound: the matrix cores, at the clock that the chip's power allows (1.75 to 1.8 GHz under these kernels, of 2.4).
-// 8192 rows x 131072 words x 1024 dims, bfloat16, loss and both gradients, 11.0 ms: STATS 1.76 ms (1250 TFLOP/s), and for
-// each of eight pieces GRAD 0.39 (700, with 1 GB of G to write), DX 0.40 and DW 0.38 (1380 and 1460, two products each);
-// largest magnitude 0.07, packing 0.11, transposing 0.09.  A library product of 8192^3 bfloat16 runs at 1290 on the same card.
+// 8192 rows x 131072 words x 1024 dims, bfloat16, loss and both gradients, 11.1 ms: STATS 1.75 ms (1260 TFLOP/s), and for
+// each of eight pieces GRAD 0.39 (710, with 1 GB of G to write), DX 0.40 and DW 0.38 (1390 and 1450, two products each);
+// packing 0.10, transposing 0.09.  A library product of 8192^3 bfloat16 runs at 1290 on the same card.
 #include <math.h>
 
 #include <algorithm>
@@ -63,20 +63,21 @@ constexpr float MAX_FLOOR = -3.0e38f;  // a maximum over nothing: exp2 of anythi
 constexpr float LN2F = 0.69314718055994531f;
 // The kernels for few rows read the vocabulary once for the scores and once for dX, where the packed path reads it three
 // times and writes it twice before its products; they multiply 32, 64 or 128 rows, whatever there are.  131072 words x 1024
-// dims, loss and both gradients: 1 row 465 against 1355 us (bfloat16 223 against 720), 128 rows 660 against 1398 (322
-// against 739); loss alone, 128 rows: 203 against 466 (71 against 252).  256 rows would be two such passes, which is what
-// the packed path takes for them (1419 and 728 us with gradients).
+// dims, loss and both gradients: 1 row 453 against 1589 us (bfloat16 212 against 817, float16 228 against 902), 128 rows 686
+// against 1658 (333 against 839, 409 against 936); loss alone, 128 rows: 220 against 495 (74 against 175).  256 rows have no
+// kernel here; two such passes would still take less than packing (1703 and 862 us with gradients).
 constexpr int FEW_ROWS = 128;
 // Below so many elements of the vocabulary there is little to gain (2000 words x 256 dims: 42 against 64 us on the GPU,
 // less than the host takes), and the packed path's backward pass has its own copy of the vocabulary.
 // Narrow tables gain more (both gradients, 1 M words x 16 dims: 8 rows 0.22 against 3.40 ms, 128 rows 0.57 against 3.41;
 // bfloat16 0.16 and 0.43 against 2.63): their logits are wider than they are, 512 bytes a word for 128 rows, but so is what
-// packing holds, 320 bytes (bfloat16 128) for 32 dims or fewer and 2 GB of G.
+// packing holds, 320 bytes (bfloat16 128) for 32 dims or fewer and 1 GB of G.
 constexpr int64_t FEW_VOCABULARY = 1 << 19;
 constexpr int SCORE_ROWS = 64;      // rows that they take from any vocabulary where no backward pass follows
 constexpr int SCORE_BLOCKS = 1024;  // workgroups of the score kernel: four per CU
 // Workgroups of the others, where there is work for so many: two per CU.  (One row to 128 of 131072 words x 1024 dims,
-// bfloat16, loss and gradients: 223 to 322 us; 256 workgroups 267 to 386, 1024 workgroups 223 to 359.)
+// bfloat16, loss and gradients, G's second piece cut off: 223 to 322 us; 256 workgroups 267 to 386, 1024 workgroups 223 to
+// 359.)
 constexpr int FEW_BLOCKS = 512;
 constexpr int AMAX_BLOCKS = 1024;  // partial maxima per tensor at most
 
@@ -237,11 +238,15 @@ __global__ void __launch_bounds__(256) vce_amax_kernel(AmaxJob w, AmaxJob x, int
     }
     for (int64_t k = lane * 8; k < j.m.cols; k += lanes * 8) {
       float v[4][8];
+      if (j.m.ld_col == 1 && (j.m.cols & 7) == 0) {   // four loads under way
+        Eight<T> e[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 4; ++q) e[q].load((const T *)j.m.data + min(r0 + q * groups, j.m.rows - 1) * j.m.ld_row + k);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[q][i] = 0.f;
-        if (live[q]) load8<T>(j.m, r0 + q * groups, k, v[q]);
+        for (int q = 0; q < 4; ++q) e[q].get(v[q]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) load8<T>(j.m, min(r0 + q * groups, j.m.rows - 1), k, v[q]);
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q)
@@ -250,6 +255,7 @@ __global__ void __launch_bounds__(256) vce_amax_kernel(AmaxJob w, AmaxJob x, int
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
+      if (!live[q]) top[q] = 0.f;
       for (int d = lanes / 2; d > 0; d >>= 1) top[q] = fmaxf(top[q], __shfl_xor(top[q], d));
       if (lane == 0 && r0 + q * groups < j.padded) j.exps[r0 + q * groups] = top[q] > 0.f ? TOP_EXP - ilogbf(top[q]) : OF_ZEROS;
       all = fmaxf(all, top[q]);
@@ -873,10 +879,11 @@ __global__ void __launch_bounds__(512, 2) vce_gemm_kernel(const GemmArgs g, cons
 //           together; reads the vocabulary once.  Partials per run of words, added by FINISH.
 //   DW      32 words a wavefront: G of all rows is made from the logits in registers and multiplies the features, a 32- or
 //           64-wide chunk at a time, which the workgroup shares through LDS, three stages deep.  Writes dW once.
-// Bound: HBM for the fewest rows (131072 words x 1024 dims, one row: float32 SCORE 140 us, DX 111, DW 119 for 537 MB each,
-// 3.8 to 4.8 TB/s; bfloat16 53, 65 and 53 for 268 MB), the matrix cores and the conversions more and more from 64 rows on
-// (128 rows: float32 205, 262 and 258 us; bfloat16 70, 129 and 109).  After a DW its lines are still on their way out of
-// the cache, which a SCORE waits for (float32 213 us instead of 140).
+// Bound: HBM for the fewest rows (131072 words x 1024 dims, one row: float32 SCORE 140 us, DX 112, DW 120 for 537 MB each,
+// 3.8 to 4.8 TB/s; bfloat16 53, 65 and 54 for 268 MB, float16 80 and 56 for the gradients), the matrix cores and the
+// conversions more and more from 64 rows on (128 rows: float32 205, 259 and 252 us; bfloat16 70, 134 and 114; float16, whose
+// features take two pieces and DW so much LDS that a CU holds one workgroup, 154 and 203 for the gradients).  After a DW its
+// lines are still on their way out of the cache, which a SCORE waits for (float32 210 us instead of 140).
 template <typename T>
 struct Operand;  // the pieces of eight consecutive values, ready for the matrix cores
 template <>
@@ -1802,7 +1809,7 @@ constexpr int64_t PIECE_BYTES = 1024ll << 20;
 
 // Splits of a contraction of `k` blocks, where its tiles alone are fewer than the CUs: as many, up to 16, as give each CU
 // a tile at most, of at least four blocks each.  Every split writes and reads a partial result of its own, which costs
-// more than CUs without work where there is a round of tiles already (50021 words x 768 dims: 1441 against 745 us).
+// more than CUs without work where there is a round of tiles already (50021 words x 768 dims, G in one piece: 1441 against 745 us).
 struct Splits {
   int n, blocks;  // blocks of each but the last
 };
@@ -1879,12 +1886,14 @@ int launch_tiles(const Product &a, const Product *b, hipStream_t st) {
 }
 
 // Time of so many tiles of 64 mt by 256, in arbitrary units.  A tile costs its products and the operand rows that it does
-// not share: 1.5 of one plane's products (256 features by 256 words against 128 by 256: 178 and 219 us for the same product),
-// 1.8 where there are three (320 words by 256 rows against 256 by 256: 233 and 222 us).
+// not share, in units of one product of 64 rows: 1.5 with one plane each (256 features by 256 words against 128 by 256: 178 and
+// 219 us for the same product), 1.8 with two and three of each (320 words by 256 rows against 256 by 256: 233 and 222 us), 6
+// with one and two, where two thirds of what is loaded is not shared (the same as above: 390 and 560 us).
 // The chip is bound by its power, so a last round that leaves CUs without work runs at a higher clock: three quarters of a
 // full one.
 double tile_time(int products, int64_t tiles, int mt) {
-  return ((double)(tiles / CUS) + (tiles % CUS ? 0.75 : 0.)) * (mt * products + (products == 1 ? 1.5 : 1.8));
+  const double own = products == 1 ? 1.5 : products == 2 ? 6. : 1.8;
+  return ((double)(tiles / CUS) + (tiles % CUS ? 0.75 : 0.)) * (mt * products + own);
 }
 
 // Words per workgroup of STATS and GRAD, in units of 64: up to five, four with two planes, whose exponents take the registers.
