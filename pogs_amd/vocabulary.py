@@ -8,7 +8,7 @@ at a time.  (Up to 128 rows of a large vocabulary do keep them for it, 4 bytes e
 Products take 16-bit operands and add in float32.  Of float32 input 2^-21 of a product at most is left out: few rows take it
 in three bfloat16 pieces, all 24 bits; otherwise the logits take every row and every word by a power of two of its own, in 22
 bits (a value below 2^-15 of its row's largest to 2^-38 of that).  The gradients' products are made of bfloat16 pieces, which
-hold each softmax entry to 2^-24 (float32 input) or 2^-16, whatever the other rows' and words' sizes and weights are.
+hold each softmax entry to 2^-24 (float32 input) or 2^-16, beside rows, words and weights up to 2^130 times as large.
 Results do not depend on the order in which workgroups run; a call with gradients to come and one without may take different
 kernels and differ in the last bits.  HIP kernels only (``pr_vocab_ce_fwd``, ``pr_vocab_ce_bwd``); there is no CPU path.
 """
